@@ -161,6 +161,25 @@ class LinkProfile(ctypes.Structure):
                 ("propagation_ns", ctypes.c_uint64), ("consume_delay_ns", ctypes.c_uint64 * 2)]
 
 
+class KvCacheArrays(ctypes.Structure):
+    _fields_ = [("struct_size", ctypes.c_uint32), ("blocks", ctypes.c_uint32),
+                ("kv_heads", ctypes.c_uint32), ("head_dim", ctypes.c_uint32),
+                ("block_tokens", ctypes.c_uint32), ("reserved0", ctypes.c_uint32)] + [
+                   (name, ctypes.c_void_p) for name in (
+                       "d_keys", "d_values", "d_key_scale", "d_value_scale", "d_bounds",
+                       "d_weight")]
+
+
+class KvBatch(ctypes.Structure):
+    _fields_ = [("struct_size", ctypes.c_uint32), ("seqs", ctypes.c_uint32),
+                ("table_width", ctypes.c_uint32), ("table_stride", ctypes.c_uint32),
+                ("tokens", ctypes.c_uint32), ("reserved0", ctypes.c_uint32),
+                ("d_table", ctypes.c_void_p), ("d_lens", ctypes.c_void_p),
+                ("d_first", ctypes.c_void_p)]
+
+
+KV_BF16, KV_F16, KV_F32 = 0, 1, 2
+
 LINK_COUNTER_FIELDS = ("flits", "wire_bytes", "ucie_header_bytes", "crc_position_bytes",
                        "aou_header_bytes", "aou_message_bytes", "unused_message_bytes",
                        "credit_only_flits", "accounting_saturated")
@@ -181,6 +200,7 @@ LINK_FLIT_DTYPE = np.dtype([("start_ns", np.uint64), ("delivered_ns", np.uint64)
 _P = ctypes.c_void_p
 _U32 = ctypes.c_uint32
 _U64 = ctypes.c_uint64
+_I64 = ctypes.c_int64
 _SZ = ctypes.c_size_t
 _INT = ctypes.c_int
 
@@ -251,6 +271,16 @@ SIGNATURES = {
     "hbfsim_amd_probe_bandwidth": (_INT, [_P, _SZ, ctypes.c_uint, _P,
                                           ctypes.POINTER(ctypes.c_float),
                                           ctypes.POINTER(ctypes.c_float)]),
+    "hbfsim_amd_kv_append": (_INT, [_P, _P, _P, _P, _U32, _P, _P]),
+    "hbfsim_amd_kv_read": (_INT, [_P, _P, _SZ, _U32, _P, _P, _P, _P, _P]),
+    "hbfsim_amd_kv_attend_workspace": (_INT, [_P, _P, _U32, _U32, _U32, ctypes.POINTER(_SZ)]),
+    "hbfsim_amd_kv_attend": (_INT, [_P, _P, _P, _U32, _U32, _I64, _I64, ctypes.c_float, _P, _U32,
+                                    _U32, _P, _P, _SZ, _P]),
+    "hbfsim_amd_kv_select_workspace": (_INT, [_P, _P, ctypes.POINTER(_SZ)]),
+    "hbfsim_amd_kv_select": (_INT, [_P, _P, _P, _U32, _U32, _I64, _I64, _U32, _U32, _U32, _P, _P,
+                                    _SZ, _P]),
+    "hbfsim_amd_kv_evict": (_INT, [_P, _U32, _U32, _U32, _P, _P, _U32, _U32, _U32, _U32, _U32,
+                                   _U32, _P, _P, _P, _P, _P, _SZ, _P]),
 }
 
 _lib = None

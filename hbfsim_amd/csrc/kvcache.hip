@@ -1,0 +1,1396 @@
+// kvcache.hip -- a paged key/value cache held in 8 bits, and the operators of
+// a decode or prompt step on it: append, read, select, attend, evict.
+//
+// No counterpart in the reference.  The timing engine prices the reads and
+// writes of a paged cache (the paged-KV record streams of workloads.py); these
+// operators are the step itself, so that a study knows which blocks a step
+// reads, which may leave for the flash tier, and what the tokens become.
+//
+// Layout.  A block holds t tokens (16, 32, 64 or 128) of every kv head; P is
+// the head dimension rounded up to 64.  Per (block, kv head) the codes are
+// t/16 tiles of 16 tokens x P dims, and a tile's 1-KiB pieces (16 tokens x 64
+// dims) are stored in the order in which a wave's lanes feed them to the
+// matrix units, so one 16-byte load per lane fetches a whole piece from one
+// contiguous KiB and nothing is transposed in LDS or registers:
+//   keys   lane (c, t): token t, dims 16 c .. 16 c + 15 of the piece
+//   values lane (c, n): tokens 4 c .. 4 c + 3 of dims n, 16 + n, 32 + n, 48 + n
+// with lane = 16 c + t.  Scores are computed as S^T = K Q^T (a lane holds one
+// query row's scores of tokens 4 c .. 4 c + 3), which is already the operand
+// layout in which O^T = V^T P^T wants the probabilities.
+//
+// Codes are widened to f16 (exact) and multiplied in f16 with f32 sums: a
+// query row is first scaled by a power of two so that its largest element
+// lies in [2^14, 2^15), where a bf16 or f16 value keeps every bit down to
+// 2^-28 of the row's largest.  A block's value scale joins the exponent: with
+//   t = score + log2(value_scale),  w = 2^(t - m)
+// the row's output is sum(w code) / sum(w / value_scale), so one set of
+// accumulators serves blocks of different scales.  Sums, maxima and
+// denominators are f32; w is rounded to f16 (11 bits) for the matrix units,
+// finer than the output types' own rounding of bf16 and equal to f16's.
+#include <hip/hip_runtime.h>
+#include <hip/hip_bf16.h>
+#include <hip/hip_fp16.h>
+
+#include "../../include/hbfsim_amd.h"
+
+#include <cstddef>
+#include <cstdint>
+
+namespace {
+
+constexpr int kWave = 64;
+constexpr float kInv127 = 1.0f / 127.0f;
+constexpr float kScaleMin = 0x1p-40f;
+constexpr float kScaleMax = 0x1p40f;
+constexpr float kQueryScaleMin = 0x1p-100f;
+constexpr float kLog2e = 1.44269504088896340736f;
+constexpr float kInf = __builtin_inff();
+
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef std::uint32_t u32x4 __attribute__((ext_vector_type(4)));
+
+struct Bf16 {
+    std::uint16_t bits;
+};
+struct F16 {
+    std::uint16_t bits;
+};
+
+__device__ inline float to_float(Bf16 x)
+{
+    return __uint_as_float(static_cast<std::uint32_t>(x.bits) << 16);
+}
+__device__ inline float to_float(F16 x) { return static_cast<float>(__builtin_bit_cast(_Float16, x.bits)); }
+__device__ inline float to_float(float x) { return x; }
+
+template <typename T>
+__device__ inline T from_float(float x);
+template <>
+__device__ inline Bf16 from_float<Bf16>(float x)
+{
+    const std::uint32_t u = __float_as_uint(x);
+    if ((u & 0x7fffffffu) > 0x7f800000u) {
+        return Bf16{static_cast<std::uint16_t>((u >> 16) | 0x40u)};
+    }
+    return Bf16{static_cast<std::uint16_t>((u + 0x7fffu + ((u >> 16) & 1u)) >> 16)};
+}
+template <>
+__device__ inline F16 from_float<F16>(float x)
+{
+    return F16{__builtin_bit_cast(std::uint16_t, static_cast<_Float16>(x))};
+}
+template <>
+__device__ inline float from_float<float>(float x)
+{
+    return x;
+}
+
+// One call's view of the cache and the batch.
+struct Cache {
+    std::int8_t* keys;
+    std::int8_t* values;
+    float* key_scale;
+    float* value_scale;
+    std::int8_t* bounds;
+    unsigned long long* weight;
+    std::uint32_t blocks, kv_heads, dim, dims;  // dims: dim rounded up to 64
+    std::uint32_t tokens, tile_shift;           // a block's tokens; log2 of its 16-token tiles
+};
+struct Batch {
+    const std::int32_t* table;
+    const std::int32_t* lens;
+    const std::int32_t* first;  // null: one token of the batch per sequence
+    std::uint32_t seqs, width, stride, tokens;
+};
+
+// A group of consecutive tokens of one sequence of the batch.  Sequence s owns
+// the slots from floor(first[s] / per) + s on, at least one and at least
+// ceil(its tokens / per); the host launches floor(tokens / per) + seqs.
+struct Group {
+    std::uint32_t seq;
+    std::int32_t from, count;  // tokens of the sequence's part of the batch
+    std::int32_t row;          // batch row of token `from`
+    std::int64_t seen;         // tokens of the cache that token `from` attends to
+};
+__device__ inline std::uint32_t slot_base(const Batch& b, std::uint32_t s, std::uint32_t per)
+{
+    return static_cast<std::uint32_t>(b.first[s]) / per + s;
+}
+__device__ inline bool find_group(const Batch& b, std::uint32_t slot, std::uint32_t per, Group* g)
+{
+    std::uint32_t s = slot;
+    std::int32_t begin, total;
+    if (b.first == nullptr) {
+        begin = static_cast<std::int32_t>(slot);
+        total = 1;
+        g->from = 0;
+    } else {
+        std::uint32_t lo = 0, hi = b.seqs;  // the last sequence whose base is not above slot
+        while (hi - lo > 1) {
+            const std::uint32_t mid = (lo + hi) / 2;
+            if (slot_base(b, mid, per) <= slot) {
+                lo = mid;
+            } else {
+                hi = mid;
+            }
+        }
+        s = lo;
+        begin = b.first[s];
+        total = b.first[s + 1] - begin;
+        const std::uint32_t base = slot_base(b, s, per);
+        if (slot < base) {
+            return false;
+        }
+        const std::uint64_t from = static_cast<std::uint64_t>(slot - base) * per;
+        if (total <= 0 || from >= static_cast<std::uint64_t>(total)) {
+            return false;
+        }
+        g->from = static_cast<std::int32_t>(from);
+    }
+    // offsets that do not describe the batch leave their rows out
+    if (begin < 0 || static_cast<std::uint64_t>(begin) + total > b.tokens) {
+        return false;
+    }
+    g->seq = s;
+    g->count = total - g->from < static_cast<std::int32_t>(per) ? total - g->from
+                                                                : static_cast<std::int32_t>(per);
+    g->row = begin + g->from;
+    g->seen = static_cast<std::int64_t>(b.lens[s]) - total + g->from + 1;
+    return true;
+}
+
+// A physical block, or -1 for an entry that names none of the pool's.
+__device__ inline std::int32_t block_at(const Cache& c, const Batch& b, std::uint32_t seq,
+                                        std::int64_t logical)
+{
+    if (logical < 0 || logical >= static_cast<std::int64_t>(b.width)) {
+        return -1;
+    }
+    const std::int32_t id = b.table[static_cast<std::size_t>(seq) * b.stride + logical];
+    return static_cast<std::uint32_t>(id) < c.blocks ? id : -1;
+}
+
+// 4 codes -> 4 f16, exactly: 0x6400 | (code + 128) is 1024 + 128 + code.
+__device__ inline f16x4 widen(std::uint32_t codes)
+{
+    const std::uint32_t u = codes ^ 0x80808080u;
+    const std::uint32_t a = __builtin_amdgcn_perm(0x64646464u, u, 0x04010400u);
+    const std::uint32_t b = __builtin_amdgcn_perm(0x64646464u, u, 0x04030402u);
+    const f16x2 bias = {static_cast<_Float16>(1152.0f), static_cast<_Float16>(1152.0f)};
+    const f16x2 x = __builtin_bit_cast(f16x2, a) - bias, y = __builtin_bit_cast(f16x2, b) - bias;
+    return __builtin_shufflevector(x, y, 0, 1, 2, 3);
+}
+__device__ inline f16x8 widen8(std::uint32_t lo, std::uint32_t hi)
+{
+    return __builtin_shufflevector(widen(lo), widen(hi), 0, 1, 2, 3, 4, 5, 6, 7);
+}
+
+__device__ inline float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// ---- attend ---------------------------------------------------------------
+
+struct Attend {
+    Cache c;
+    Batch b;
+    const void* q;
+    std::int64_t q_token, q_head;  // strides in elements
+    std::uint32_t q_vector;        // rows may be loaded 16 bytes at a time
+    std::uint32_t heads, group;    // query heads; query heads per kv head
+    std::uint32_t per;             // tokens per unit
+    std::uint32_t row_tiles;       // 16-row tiles per unit (1 unless group > 16)
+    float scale;                   // softmax scale times log2(e)
+    const std::int32_t* selected;
+    std::uint32_t count;
+    std::uint32_t split, splits;   // tokens per split, splits launched
+    void* out;
+    float* partial;                // [unit, kv head, row tile, split][16][dims]
+    float* stats;                  // [...][16][2]: reference exponent, denominator
+    float* lse;                    // [tokens, heads], log2 of the row's denominator, or null
+};
+
+// Splits that hold work for a unit whose last token sees `seen` tokens.
+__device__ inline std::uint32_t live_splits(const Attend& a, std::int64_t seen)
+{
+    const std::int64_t n = a.selected != nullptr
+                               ? static_cast<std::int64_t>(a.count) * a.c.tokens
+                               : seen;
+    return seen <= 0 ? 0u : static_cast<std::uint32_t>((n + a.split - 1) / a.split);
+}
+
+__device__ inline std::int64_t visible(const Attend& a, std::int64_t seen)
+{
+    const std::int64_t most = static_cast<std::int64_t>(a.b.width) * a.c.tokens;
+    return seen < most ? seen : most;
+}
+
+// A workgroup of kWaves waves takes one (unit, kv head, row tile, split); its
+// waves take pairs of 16-token tiles in turn and join through LDS.
+template <typename T, int CH, int kWaves>
+__global__ __launch_bounds__(kWaves * kWave) void k_kv_attend(Attend a)
+{
+    constexpr int P = CH * 64;
+    __shared__ float s_out[kWaves][16][P];
+    __shared__ float s_ref[kWaves][16], s_den[kWaves][16];
+
+    const std::uint32_t unit = blockIdx.x;
+    const std::uint32_t head = blockIdx.y % a.c.kv_heads, row_tile = blockIdx.y / a.c.kv_heads;
+    const std::uint32_t split = blockIdx.z;
+    const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
+    const int m = lane & 15, quarter = lane >> 4;
+
+    Group g;
+    if (!find_group(a.b, unit, a.per, &g)) {
+        return;
+    }
+    const std::int64_t seen = visible(a, g.seen + g.count - 1);
+    const std::uint32_t live = live_splits(a, seen);
+    if (split >= live && !(split == 0 && a.splits == 1)) {
+        return;
+    }
+
+    // this lane's query row
+    const std::uint32_t r = row_tile * 16 + m;
+    const std::uint32_t row_token = r / a.group, row_head = r % a.group;
+    const bool row_live = row_token < static_cast<std::uint32_t>(g.count);
+    std::int64_t limit64 = row_live ? visible(a, g.seen + row_token) : 0;
+    const int limit = limit64 > 0 ? static_cast<int>(limit64) : 0;
+    const std::int64_t token_row = g.row + static_cast<std::int64_t>(row_token);
+    const std::uint32_t q_head = head * a.group + row_head;
+
+    f16x8 query[CH * 2];
+    float factor = 0.0f;
+    {
+        const T* q = static_cast<const T*>(a.q) + token_row * a.q_token + q_head * a.q_head;
+        float x[CH * 16];
+        float top = 0.0f;
+#pragma unroll
+        for (int i = 0; i < CH * 2; ++i) {
+            const int d0 = (i / 2) * 64 + quarter * 16 + (i & 1) * 8;
+            if (row_live && a.q_vector != 0 && d0 + 8 <= static_cast<int>(a.c.dim)) {
+                union {
+                    u32x4 v;
+                    T e[8];
+                } u;
+                u.v = *reinterpret_cast<const u32x4*>(q + d0);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) x[i * 8 + j] = to_float(u.e[j]);
+            } else {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    x[i * 8 + j] = row_live && d0 + j < static_cast<int>(a.c.dim) ? to_float(q[d0 + j]) : 0.0f;
+                }
+            }
+#pragma unroll
+            for (int j = 0; j < 8; ++j) top = fmaxf(top, fabsf(x[i * 8 + j]));
+        }
+        top = fmaxf(top, __shfl_xor(top, 16));
+        top = fmaxf(top, __shfl_xor(top, 32));
+        const int k = top > 0.0f && top < kInf ? 14 - ilogbf(top) : 0;
+        factor = ldexpf(a.scale, -k);
+#pragma unroll
+        for (int i = 0; i < CH * 2; ++i) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) query[i][j] = static_cast<_Float16>(ldexpf(x[i * 8 + j], k));
+        }
+    }
+
+    f32x4 acc[CH * 4];
+#pragma unroll
+    for (int i = 0; i < CH * 4; ++i) acc[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    float ref = -kInf, den = 0.0f;
+
+    const std::int64_t total = a.selected != nullptr
+                                   ? static_cast<std::int64_t>(a.count) * a.c.tokens
+                                   : seen;
+    const std::int64_t begin = static_cast<std::int64_t>(split) * a.split;
+    const std::int64_t end = begin + a.split < total ? begin + a.split : total;
+    const std::int32_t* list =
+        a.selected == nullptr
+            ? nullptr
+            : a.selected + (static_cast<std::int64_t>(g.row) * a.c.kv_heads + head) * a.count;
+    const std::uint32_t tile_mask = (1u << a.c.tile_shift) - 1;
+    const std::size_t head_bytes = static_cast<std::size_t>(a.c.tokens) * P;
+
+    for (std::int64_t at = begin + wave * 32; at < end; at += kWaves * 32) {
+        u32x4 kc[2][CH], vc[2][CH];
+        float ks[2], vs[2];
+        int pos[2];
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            const std::int64_t tile = at / 16 + u;
+            const std::int64_t entry = tile >> a.c.tile_shift;
+            std::int64_t logical = -1;
+            if (tile * 16 < end) {
+                logical = list == nullptr ? entry : list[entry];
+            }
+            const std::uint32_t sub = static_cast<std::uint32_t>(tile) & tile_mask;
+            std::int32_t id = block_at(a.c, a.b, g.seq, logical);
+            pos[u] = id >= 0 && logical * a.c.tokens + sub * 16 < seen
+                         ? static_cast<int>(logical * a.c.tokens + sub * 16)
+                         : 0x7fffffff - 15;
+            id = id < 0 ? 0 : id;
+            const std::size_t bh = static_cast<std::size_t>(id) * a.c.kv_heads + head;
+            const std::int8_t* kp = a.c.keys + bh * head_bytes + static_cast<std::size_t>(sub) * 16 * P;
+            const std::int8_t* vp = a.c.values + bh * head_bytes + static_cast<std::size_t>(sub) * 16 * P;
+#pragma unroll
+            for (int i = 0; i < CH; ++i) {
+                kc[u][i] = reinterpret_cast<const u32x4*>(kp)[i * kWave + lane];
+                vc[u][i] = reinterpret_cast<const u32x4*>(vp)[i * kWave + lane];
+            }
+            ks[u] = a.c.key_scale[bh];
+            vs[u] = a.c.value_scale[bh];
+        }
+        float t[2][4];
+        float top = -kInf;
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            f32x4 s = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int i = 0; i < CH; ++i) {
+                s = __builtin_amdgcn_mfma_f32_16x16x32_f16(widen8(kc[u][i].x, kc[u][i].y), query[2 * i], s, 0, 0, 0);
+                s = __builtin_amdgcn_mfma_f32_16x16x32_f16(widen8(kc[u][i].z, kc[u][i].w), query[2 * i + 1], s, 0, 0, 0);
+            }
+            const float f = factor * ks[u], e = log2f(vs[u]);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float x = fmaf(s[i], f, e);
+                t[u][i] = pos[u] + quarter * 4 + i < limit ? x : -kInf;
+                top = fmaxf(top, t[u][i]);
+            }
+        }
+        // The row's reference exponent stays 2^7 to 2^15 below its largest
+        // weight (the f16 range), so it moves only now and then.
+        if (__any(top > ref + 15.0f)) {
+            top = fmaxf(top, __shfl_xor(top, 16));
+            top = fmaxf(top, __shfl_xor(top, 32));
+            const float next = fmaxf(ref, top - 7.0f);
+            const float shrink = next == -kInf ? 1.0f : exp2_fast(ref - next);
+            ref = next;
+            den *= shrink;
+#pragma unroll
+            for (int i = 0; i < CH * 4; ++i) acc[i] *= shrink;
+        }
+        f16x8 w;
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            const float inv = 1.0f / vs[u];
+            float sum = 0.0f;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float x = pos[u] + quarter * 4 + i < limit ? exp2_fast(t[u][i] - ref) : 0.0f;
+                sum += x;
+                w[u * 4 + i] = static_cast<_Float16>(x);
+            }
+            den = sum != 0.0f ? fmaf(sum, inv, den) : den;
+        }
+#pragma unroll
+        for (int i = 0; i < CH; ++i) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                acc[i * 4 + j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+                    widen8(vc[0][i][j], vc[1][i][j]), w, acc[i * 4 + j], 0, 0, 0);
+            }
+        }
+    }
+    den += __shfl_xor(den, 16);
+    den += __shfl_xor(den, 32);
+
+    if (quarter == 0) {
+        s_ref[wave][m] = ref;
+        s_den[wave][m] = den;
+    }
+    __syncthreads();
+    float top = s_ref[0][m];
+#pragma unroll
+    for (int i = 1; i < kWaves; ++i) top = fmaxf(top, s_ref[i][m]);
+    const float mine = ref == -kInf ? 0.0f : exp2_fast(ref - top);
+#pragma unroll
+    for (int i = 0; i < CH * 4; ++i) {
+        const f32x4 x = acc[i] * mine;
+        *reinterpret_cast<f32x4*>(&s_out[wave][m][i * 16 + quarter * 4]) = x;
+    }
+    __syncthreads();
+
+    const std::uint32_t rows = g.count * a.group;  // rows of the unit
+    for (int i = threadIdx.x; i < 16 * P; i += kWaves * kWave) {
+        const int row = i / P, d = i % P;
+        const std::uint32_t rr = row_tile * 16 + row;
+        if (rr >= rows || (a.per == 1 && rr >= a.group)) {
+            continue;
+        }
+        float top_row = s_ref[0][row];
+#pragma unroll
+        for (int k = 1; k < kWaves; ++k) top_row = fmaxf(top_row, s_ref[k][row]);
+        float o = 0.0f, l = 0.0f;
+#pragma unroll
+        for (int k = 0; k < kWaves; ++k) {
+            o += s_out[k][row][d];
+            l += s_ref[k][row] == -kInf ? s_den[k][row] : s_den[k][row] * exp2_fast(s_ref[k][row] - top_row);
+        }
+        if (a.splits == 1) {
+            const std::int64_t tok = g.row + static_cast<std::int64_t>(rr / a.group);
+            const std::uint32_t h = head * a.group + rr % a.group;
+            if (d < static_cast<int>(a.c.dim)) {
+                static_cast<T*>(a.out)[(tok * a.heads + h) * a.c.dim + d] =
+                    from_float<T>(l == 0.0f ? 0.0f : o / l);
+            }
+            if (d == 0 && a.lse != nullptr) {
+                a.lse[tok * a.heads + h] = l == 0.0f ? kInf : top_row + log2f(l);
+            }
+        } else {
+            const std::size_t cell =
+                ((static_cast<std::size_t>(unit) * gridDim.y + blockIdx.y) * a.splits + split) * 16 + row;
+            a.partial[cell * P + d] = o;
+            if (d == 0) {
+                a.stats[cell * 2] = top_row;
+                a.stats[cell * 2 + 1] = l;
+            }
+        }
+    }
+}
+
+// Joins a unit's splits: one workgroup per (unit, kv head, row tile).
+template <typename T>
+__global__ __launch_bounds__(256) void k_kv_merge(Attend a)
+{
+    const std::uint32_t unit = blockIdx.x;
+    const std::uint32_t head = blockIdx.y % a.c.kv_heads, row_tile = blockIdx.y / a.c.kv_heads;
+    const int P = static_cast<int>(a.c.dims);
+    Group g;
+    if (!find_group(a.b, unit, a.per, &g)) {
+        return;
+    }
+    const std::uint32_t live = live_splits(a, visible(a, g.seen + g.count - 1));
+    const std::size_t cell0 = (static_cast<std::size_t>(unit) * gridDim.y + blockIdx.y) * a.splits * 16;
+    for (int i = threadIdx.x; i < 16 * P; i += 256) {
+        const int row = i / P, d = i % P;
+        const std::uint32_t rr = row_tile * 16 + row;
+        if (rr >= g.count * a.group || (a.per == 1 && rr >= a.group)) {
+            continue;
+        }
+        float top = -kInf;
+        for (std::uint32_t s = 0; s < live; ++s) {
+            top = fmaxf(top, a.stats[(cell0 + s * 16 + row) * 2]);
+        }
+        float o = 0.0f, l = 0.0f;
+        for (std::uint32_t s = 0; s < live; ++s) {
+            const std::size_t cell = cell0 + s * 16 + row;
+            const float ref = a.stats[cell * 2];
+            const float f = ref == -kInf ? 1.0f : exp2_fast(ref - top);
+            o = fmaf(a.partial[cell * P + d], f, o);
+            l = fmaf(a.stats[cell * 2 + 1], f, l);
+        }
+        const std::int64_t tok = g.row + static_cast<std::int64_t>(rr / a.group);
+        const std::uint32_t h = head * a.group + rr % a.group;
+        if (d < static_cast<int>(a.c.dim)) {
+            static_cast<T*>(a.out)[(tok * a.heads + h) * a.c.dim + d] =
+                from_float<T>(l == 0.0f ? 0.0f : o / l);
+        }
+        if (d == 0 && a.lse != nullptr) {
+            a.lse[tok * a.heads + h] = l == 0.0f ? kInf : top + log2f(l);
+        }
+    }
+}
+
+// weight[block, head] += the probabilities of the unit's rows over the block.
+// One wave per block of the sequence; sums are f32 within a block and joined
+// as integers, so the order in which blocks of shared prefixes are reached
+// does not change them.
+template <typename T, int CH>
+__global__ __launch_bounds__(256) void k_kv_weigh(Attend a)
+{
+    constexpr int P = CH * 64;
+    const std::uint32_t head = blockIdx.y % a.c.kv_heads, row_tile = blockIdx.y / a.c.kv_heads;
+    const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
+    const int m = lane & 15, quarter = lane >> 4;
+    Group g;
+    if (!find_group(a.b, blockIdx.x, a.per, &g)) {
+        return;
+    }
+    const std::int64_t seen = visible(a, g.seen + g.count - 1);
+    if (seen <= 0) {
+        return;
+    }
+    const std::uint32_t r = row_tile * 16 + m;
+    const std::uint32_t row_token = r / a.group, row_head = r % a.group;
+    const bool row_live = row_token < static_cast<std::uint32_t>(g.count) && (a.per > 1 || r < a.group);
+    const std::int64_t limit64 = row_live ? visible(a, g.seen + row_token) : 0;
+    const int limit = limit64 > 0 ? static_cast<int>(limit64) : 0;
+    const std::int64_t token_row = g.row + static_cast<std::int64_t>(row_token);
+    const std::uint32_t q_head = head * a.group + row_head;
+    f16x8 query[CH * 2];
+    float factor, lse = kInf;
+    {
+        const T* q = static_cast<const T*>(a.q) + token_row * a.q_token + q_head * a.q_head;
+        float x[CH * 16];
+        float top = 0.0f;
+#pragma unroll
+        for (int i = 0; i < CH * 16; ++i) {
+            const int d = (i / 16) * 64 + quarter * 16 + (i & 15);
+            x[i] = row_live && d < static_cast<int>(a.c.dim) ? to_float(q[d]) : 0.0f;
+            top = fmaxf(top, fabsf(x[i]));
+        }
+        top = fmaxf(top, __shfl_xor(top, 16));
+        top = fmaxf(top, __shfl_xor(top, 32));
+        const int k = top > 0.0f && top < kInf ? 14 - ilogbf(top) : 0;
+        factor = ldexpf(a.scale, -k);
+#pragma unroll
+        for (int i = 0; i < CH * 16; ++i) query[i / 8][i % 8] = static_cast<_Float16>(ldexpf(x[i], k));
+        if (row_live) {
+            lse = a.lse[token_row * a.heads + q_head];
+        }
+    }
+    const std::size_t head_bytes = static_cast<std::size_t>(a.c.tokens) * P;
+    const std::uint32_t nb = static_cast<std::uint32_t>((seen + a.c.tokens - 1) / a.c.tokens);
+    for (std::uint32_t blk = blockIdx.z * 4 + wave; blk < nb; blk += gridDim.z * 4) {
+        const std::int32_t id = block_at(a.c, a.b, g.seq, blk);
+        if (id < 0) {
+            continue;
+        }
+        const std::size_t bh = static_cast<std::size_t>(id) * a.c.kv_heads + head;
+        const float f = factor * a.c.key_scale[bh];
+        float sum = 0.0f;
+        for (std::uint32_t sub = 0; sub < a.c.tokens / 16; ++sub) {
+            const u32x4* kp = reinterpret_cast<const u32x4*>(a.c.keys + bh * head_bytes +
+                                                             static_cast<std::size_t>(sub) * 16 * P);
+            f32x4 s = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int i = 0; i < CH; ++i) {
+                const u32x4 k = kp[i * kWave + lane];
+                s = __builtin_amdgcn_mfma_f32_16x16x32_f16(widen8(k.x, k.y), query[2 * i], s, 0, 0, 0);
+                s = __builtin_amdgcn_mfma_f32_16x16x32_f16(widen8(k.z, k.w), query[2 * i + 1], s, 0, 0, 0);
+            }
+            const std::int64_t pos = static_cast<std::int64_t>(blk) * a.c.tokens + sub * 16 + quarter * 4;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                sum += pos + i < limit ? exp2_fast(fmaf(s[i], f, -lse)) : 0.0f;
+            }
+        }
+#pragma unroll
+        for (int x = 1; x < kWave; x *= 2) sum += __shfl_xor(sum, x);
+        if (lane == 0 && sum < 1e9f) {  // a sum that is not a number adds nothing
+            atomicAdd(a.c.weight + bh, static_cast<unsigned long long>(__double2ull_rn(static_cast<double>(sum) * 0x1p32)));
+        }
+    }
+}
+
+// ---- append and read ------------------------------------------------------
+
+struct Append {
+    Cache c;
+    Batch b;
+    const void* x[2];                       // keys, values
+    std::int64_t token_stride[2], head_stride[2];
+};
+
+__device__ inline float quantise(float x, float inv)
+{
+    const float r = rintf(x * inv);
+    return r != r ? 0.0f : fminf(fmaxf(r, -127.0f), 127.0f);
+}
+
+// The block `slot` of the batch's writes and the new tokens in it.
+struct Write {
+    std::int32_t id;
+    int begin, end;       // the block's slots that get new tokens
+    std::int64_t row;     // batch row of slot `begin`
+};
+__device__ inline bool find_write(const Append& a, std::uint32_t slot, Write* w)
+{
+    const std::uint32_t t = a.c.tokens;
+    std::uint32_t s = slot;
+    std::int32_t begin = static_cast<std::int32_t>(slot), total = 1;
+    std::uint64_t nth = 0;
+    if (a.b.first != nullptr) {
+        // sequence s owns the slots from floor(first[s] / t) + 2 s on
+        const auto base = [&](std::uint32_t i) {
+            return static_cast<std::uint32_t>(a.b.first[i]) / t + 2 * i;
+        };
+        std::uint32_t lo = 0, hi = a.b.seqs;
+        while (hi - lo > 1) {
+            const std::uint32_t mid = (lo + hi) / 2;
+            if (base(mid) <= slot) {
+                lo = mid;
+            } else {
+                hi = mid;
+            }
+        }
+        s = lo;
+        if (slot < base(s)) {
+            return false;
+        }
+        begin = a.b.first[s];
+        total = a.b.first[s + 1] - begin;
+        nth = slot - base(s);
+    }
+    if (total <= 0 || begin < 0 || static_cast<std::uint64_t>(begin) + total > a.b.tokens) {
+        return false;
+    }
+    const std::int64_t from = static_cast<std::int64_t>(a.b.lens[s]) - total, to = from + total;
+    if (from < 0) {
+        return false;
+    }
+    const std::int64_t blk = from / t + static_cast<std::int64_t>(nth);
+    if (blk * t >= to) {
+        return false;
+    }
+    w->id = block_at(a.c, a.b, s, blk);
+    if (w->id < 0) {
+        return false;
+    }
+    w->begin = from > blk * t ? static_cast<int>(from - blk * t) : 0;
+    w->end = to < (blk + 1) * t ? static_cast<int>(to - blk * t) : static_cast<int>(t);
+    w->row = begin + (blk * t + w->begin - from);
+    return true;
+}
+
+// One wave per (slot, kv head, keys or values).
+template <typename T>
+__global__ __launch_bounds__(kWave) void k_kv_append(Append a)
+{
+    Write w;
+    if (!find_write(a, blockIdx.x, &w)) {
+        return;
+    }
+    const std::uint32_t head = blockIdx.y, which = blockIdx.z;
+    const int lane = threadIdx.x;
+    const int P = static_cast<int>(a.c.dims), D = static_cast<int>(a.c.dim);
+    const int count = w.end - w.begin;
+    const bool begun = w.begin > 0;
+    const std::size_t bh = static_cast<std::size_t>(w.id) * a.c.kv_heads + head;
+    const T* x = static_cast<const T*>(a.x[which]) + w.row * a.token_stride[which] + head * a.head_stride[which];
+    const std::int64_t row = a.token_stride[which];
+
+    float top = 0.0f;
+    bool bad = false;
+    for (int i = 0; i < count; ++i) {
+        for (int d = lane; d < D; d += kWave) {
+            const float v = fabsf(to_float(x[i * row + d]));
+            bad |= !(v < kInf);
+            top = fmaxf(top, v);
+        }
+    }
+#pragma unroll
+    for (int k = 1; k < kWave; k *= 2) top = fmaxf(top, __shfl_xor(top, k));
+    float* scales = which == 0 ? a.c.key_scale : a.c.value_scale;
+    float scale = top * kInv127;
+    scale = __any(bad) || !(scale <= kScaleMax) ? __builtin_nanf("") : fmaxf(scale, kScaleMin);
+    float ratio = 0.0f;
+    if (begun) {
+        const float before = scales[bh];
+        scale = before != before || scale != scale ? __builtin_nanf("") : fmaxf(before, scale);
+        ratio = before / scale;
+    }
+    const float inv = 1.0f / scale;
+    if (lane == 0) {
+        scales[bh] = scale;
+        if (which == 0 && !begun) {
+            a.c.weight[bh] = 0;
+        }
+    }
+
+    // codes: every 16-byte piece that holds a new token or changes
+    std::int8_t* pool = (which == 0 ? a.c.keys : a.c.values) + bh * (static_cast<std::size_t>(a.c.tokens) * P);
+    const int tiles = static_cast<int>(a.c.tokens) / 16;
+    const int c = lane >> 4, n = lane & 15;
+    for (int tile = 0; tile < tiles; ++tile) {
+        for (int chunk = 0; chunk < P / 64; ++chunk) {
+            u32x4* piece = reinterpret_cast<u32x4*>(pool + (static_cast<std::size_t>(tile) * (P / 64) + chunk) * 1024) + lane;
+            const int lo = tile * 16 + (which == 0 ? n : 4 * c), hi = lo + (which == 0 ? 1 : 4);
+            const bool holds_new = lo < w.end && hi > w.begin;
+            if (!holds_new && begun && ratio == 1.0f) {
+                continue;
+            }
+            union {
+                u32x4 v;
+                std::int8_t e[16];
+            } u;
+            u.v = begun ? *piece : u32x4{0u, 0u, 0u, 0u};
+#pragma unroll
+            for (int k = 0; k < 16; ++k) {
+                const int token = which == 0 ? lo : lo + (k & 3);
+                const int d = chunk * 64 + (which == 0 ? 16 * c + k : 16 * (k >> 2) + n);
+                float q;
+                if (token >= w.begin && token < w.end) {
+                    q = d < D ? quantise(to_float(x[(token - w.begin) * row + d]), inv) : 0.0f;
+                } else {
+                    q = quantise(static_cast<float>(u.e[k]), ratio);
+                }
+                u.e[k] = static_cast<std::int8_t>(q);
+            }
+            *piece = u.v;
+        }
+    }
+    if (which == 0) {
+        std::int8_t* bounds = a.c.bounds + bh * 2 * P;
+        for (int d = lane; d < P; d += kWave) {
+            float lo = 127.0f, hi = -127.0f;
+            if (begun) {
+                lo = quantise(static_cast<float>(bounds[d]), ratio);
+                hi = quantise(static_cast<float>(bounds[P + d]), ratio);
+            }
+            for (int i = 0; i < count; ++i) {
+                const float q = d < D ? quantise(to_float(x[i * row + d]), inv) : 0.0f;
+                lo = fminf(lo, q);
+                hi = fmaxf(hi, q);
+            }
+            bounds[d] = static_cast<std::int8_t>(lo);
+            bounds[P + d] = static_cast<std::int8_t>(hi);
+        }
+    }
+}
+
+// Blocks back as values: one workgroup per (entry, kv head).
+template <typename T>
+__global__ __launch_bounds__(256) void k_kv_read(Cache c, const std::int32_t* ids, T* k_out, T* v_out, T* low, T* high)
+{
+    const std::uint32_t head = blockIdx.y;
+    const std::int32_t id = ids[blockIdx.x];
+    const bool inside = static_cast<std::uint32_t>(id) < c.blocks;
+    const int P = static_cast<int>(c.dims), D = static_cast<int>(c.dim), t = static_cast<int>(c.tokens);
+    const std::size_t bh = inside ? static_cast<std::size_t>(id) * c.kv_heads + head : 0;
+    const std::size_t to = static_cast<std::size_t>(blockIdx.x) * c.kv_heads + head;
+    const float ks = inside ? c.key_scale[bh] : 0.0f, vs = inside ? c.value_scale[bh] : 0.0f;
+    const std::int8_t* kp = c.keys + bh * (static_cast<std::size_t>(t) * P);
+    const std::int8_t* vp = c.values + bh * (static_cast<std::size_t>(t) * P);
+    for (int i = threadIdx.x; i < t * D; i += 256) {
+        const int token = i / D, d = i % D;
+        const std::size_t piece = (static_cast<std::size_t>(token / 16) * (P / 64) + d / 64) * 1024;
+        const int n = token % 16, e = d % 64;
+        const float kq = kp[piece + ((e / 16) * 16 + n) * 16 + e % 16];
+        const float vq = vp[piece + ((n / 4) * 16 + e % 16) * 16 + (e / 16) * 4 + n % 4];
+        k_out[to * t * D + i] = from_float<T>(kq * ks);
+        v_out[to * t * D + i] = from_float<T>(vq * vs);
+    }
+    for (int d = threadIdx.x; d < D; d += 256) {
+        low[to * D + d] = from_float<T>(static_cast<float>(c.bounds[bh * 2 * P + d]) * ks);
+        high[to * D + d] = from_float<T>(static_cast<float>(c.bounds[bh * 2 * P + P + d]) * ks);
+    }
+}
+
+// ---- select and evict -----------------------------------------------------
+
+// The keys of the `want` largest of n (want < n; ties to the lower index):
+// *threshold is the smallest of them, and the call returns how many of those
+// equal to it are taken.  A workgroup's threads all call it; `key(i)` is read
+// once per digit.
+template <typename K, int kThreads, typename F>
+__device__ std::uint32_t radix_threshold(F key, std::uint32_t n, std::uint32_t want, K* threshold)
+{
+    __shared__ std::uint32_t bins[256];
+    __shared__ std::uint32_t s_digit, s_left;
+    constexpr int kBits = sizeof(K) * 8;
+    K prefix = 0, mask = 0;
+    std::uint32_t left = want;
+    for (int shift = kBits - 8; shift >= 0; shift -= 8) {
+        for (int i = threadIdx.x; i < 256; i += kThreads) bins[i] = 0;
+        __syncthreads();
+        for (std::uint32_t i = threadIdx.x; i < n; i += kThreads) {
+            const K k = key(i);
+            if ((k & mask) == prefix) {
+                atomicAdd(&bins[(k >> shift) & 255], 1u);
+            }
+        }
+        __syncthreads();
+        if (threadIdx.x == 0) {
+            std::uint32_t above = 0;
+            int digit = 255;
+            for (; digit > 0 && above + bins[digit] < left; --digit) above += bins[digit];
+            s_digit = digit;
+            s_left = left - above;
+        }
+        __syncthreads();
+        prefix |= static_cast<K>(s_digit) << shift;
+        mask |= static_cast<K>(255) << shift;
+        left = s_left;
+        __syncthreads();
+    }
+    *threshold = prefix;
+    return left;
+}
+
+// Exclusive rank of this thread's flag among the workgroup's, and their sum.
+template <int kThreads>
+__device__ std::uint32_t flag_rank(bool flag, std::uint32_t* total)
+{
+    __shared__ std::uint32_t waves[kThreads / kWave];
+    const unsigned long long votes = __ballot(flag);
+    const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
+    if (lane == 0) waves[wave] = __popcll(votes);
+    __syncthreads();
+    std::uint32_t before = 0, sum = 0;
+#pragma unroll
+    for (int i = 0; i < kThreads / kWave; ++i) {
+        before += i < wave ? waves[i] : 0;
+        sum += waves[i];
+    }
+    __syncthreads();
+    *total = sum;
+    return before + __popcll(votes & ((1ull << lane) - 1));
+}
+
+struct Select {
+    Cache c;
+    Batch b;
+    const void* q;
+    std::int64_t q_token, q_head;
+    std::uint32_t group, count, keep_first, keep_last;
+    std::uint32_t* keys;      // [tokens, kv heads, width]
+    std::int32_t* selected;   // [tokens, kv heads, count]
+};
+
+// Blocks that a query token sees, and its sequence.
+__device__ inline std::uint32_t select_blocks(const Select& a, std::uint32_t token, std::uint32_t* seq)
+{
+    Group g;
+    std::uint32_t slot = token;
+    if (a.b.first != nullptr) {
+        std::uint32_t lo = 0, hi = a.b.seqs;
+        while (hi - lo > 1) {
+            const std::uint32_t mid = (lo + hi) / 2;
+            if (static_cast<std::uint32_t>(a.b.first[mid]) <= token) {
+                lo = mid;
+            } else {
+                hi = mid;
+            }
+        }
+        slot = token + lo;  // slot_base with one token per slot
+    }
+    if (!find_group(a.b, slot, 1, &g) || g.seen <= 0) {
+        *seq = 0;
+        return 0;
+    }
+    *seq = g.seq;
+    const std::int64_t nb = (g.seen + a.c.tokens - 1) / a.c.tokens;
+    return nb < static_cast<std::int64_t>(a.b.width) ? static_cast<std::uint32_t>(nb) : a.b.width;
+}
+
+__device__ inline std::uint32_t ordered(float x)
+{
+    const std::uint32_t u = __float_as_uint(x);
+    return (u & 0x80000000u) != 0 ? ~u : u | 0x80000000u;
+}
+
+// Scores of a query token and kv head against every block it sees.
+template <typename T>
+__global__ __launch_bounds__(256) void k_kv_score(Select a)
+{
+    __shared__ std::int32_t s_code[512];  // group sums: parts that meet `low`, then `high`
+    __shared__ float s_top[4];
+    const std::uint32_t token = blockIdx.x, head = blockIdx.y;
+    const int P = static_cast<int>(a.c.dims), D = static_cast<int>(a.c.dim);
+    std::uint32_t seq;
+    const std::uint32_t nb = select_blocks(a, token, &seq);
+    const T* q = static_cast<const T*>(a.q) + token * a.q_token +
+                 static_cast<std::int64_t>(head) * a.group * a.q_head;
+    float top = 0.0f;
+    for (int i = threadIdx.x; i < static_cast<int>(a.group) * D; i += 256) {
+        top = fmaxf(top, fabsf(to_float(q[(i / D) * a.q_head + i % D])));
+    }
+    for (int k = 1; k < kWave; k *= 2) top = fmaxf(top, __shfl_xor(top, k));
+    if (threadIdx.x % kWave == 0) s_top[threadIdx.x / kWave] = top;
+    __syncthreads();
+    top = fmaxf(fmaxf(s_top[0], s_top[1]), fmaxf(s_top[2], s_top[3]));
+    const float inv = 1.0f / fmaxf(top * kInv127, kQueryScaleMin);
+    for (int d = threadIdx.x; d < P; d += 256) {
+        std::int32_t lo = 0, hi = 0;
+        for (std::uint32_t g = 0; g < a.group; ++g) {
+            const std::int32_t code = d < D ? static_cast<std::int32_t>(quantise(to_float(q[g * a.q_head + d]), inv)) : 0;
+            lo += code < 0 ? code : 0;
+            hi += code > 0 ? code : 0;
+        }
+        s_code[d] = lo;
+        s_code[P + d] = hi;
+    }
+    __syncthreads();
+    std::uint32_t* keys = a.keys + (static_cast<std::size_t>(token) * a.c.kv_heads + head) * a.b.width;
+    for (std::uint32_t blk = blockIdx.z * 256 + threadIdx.x; blk < nb; blk += gridDim.z * 256) {
+        const std::int32_t id = block_at(a.c, a.b, seq, blk);
+        std::uint32_t key = 0;
+        if (id >= 0) {
+            const std::size_t bh = static_cast<std::size_t>(id) * a.c.kv_heads + head;
+            const u32x4* bounds = reinterpret_cast<const u32x4*>(a.c.bounds + bh * 2 * P);
+            std::int32_t sum = 0;
+            for (int i = 0; i < 2 * P / 16; ++i) {
+                union {
+                    u32x4 v;
+                    std::int8_t e[16];
+                } u;
+                u.v = bounds[i];
+#pragma unroll
+                for (int k = 0; k < 16; ++k) sum += u.e[k] * s_code[i * 16 + k];
+            }
+            float score = static_cast<float>(sum) * a.c.key_scale[bh];
+            if (score != score || blk < a.keep_first || blk + a.keep_last >= nb) score = kInf;
+            key = ordered(score);
+        }
+        keys[blk] = key;
+    }
+}
+
+// Picks the `count` best of a row's keys; blocks that are not there have key 0.
+__global__ __launch_bounds__(256) void k_kv_pick(Select a)
+{
+    const std::uint32_t token = blockIdx.x, head = blockIdx.y;
+    const std::size_t cell = static_cast<std::size_t>(token) * a.c.kv_heads + head;
+    const std::uint32_t* keys = a.keys + cell * a.b.width;
+    std::int32_t* out = a.selected + cell * a.count;
+    std::uint32_t seq;
+    const std::uint32_t nb = select_blocks(a, token, &seq);
+    std::uint32_t threshold = 1, equal = 0xffffffffu;
+    if (nb > a.count) {
+        equal = radix_threshold<std::uint32_t, 256>([&](std::uint32_t i) { return keys[i]; }, nb, a.count, &threshold);
+    }
+    std::uint32_t done = 0, ties = 0;
+    for (std::uint32_t base = 0; base < nb; base += 256) {
+        const std::uint32_t i = base + threadIdx.x;
+        const std::uint32_t k = i < nb ? keys[i] : 0;
+        std::uint32_t total;
+        const std::uint32_t rank = flag_rank<256>(k == threshold, &total);
+        const bool take = k != 0 && (k > threshold || (k == threshold && ties + rank < equal));
+        ties += total;
+        const std::uint32_t at = flag_rank<256>(take, &total);
+        if (take) out[done + at] = static_cast<std::int32_t>(i);
+        done += total;
+    }
+    for (std::uint32_t i = done + threadIdx.x; i < a.count; i += 256) out[i] = -1;
+}
+
+struct Evict {
+    const unsigned long long* weight;
+    std::uint32_t blocks, kv_heads, tokens;
+    const std::int32_t* table;
+    const std::int32_t* lens;
+    std::uint32_t seqs, width, stride, keep, keep_first, keep_last;
+    unsigned long long* keys;  // [seqs, width]
+    std::int32_t* out_table;   // [seqs, width]
+    std::int32_t* out_lens;
+    std::int32_t* freed;       // [seqs, width]
+    std::int32_t* freed_count;
+};
+
+// One workgroup per sequence.  A block's key is its summed weight plus 1; a
+// table entry that names no block has key 0 and goes first.
+__global__ __launch_bounds__(256) void k_kv_evict(Evict a)
+{
+    const std::uint32_t s = blockIdx.x;
+    const std::int64_t len = a.lens[s];
+    const std::int64_t nb64 = len <= 0 ? 0 : (len + a.tokens - 1) / a.tokens;
+    const std::uint32_t nb = nb64 < static_cast<std::int64_t>(a.width) ? static_cast<std::uint32_t>(nb64) : a.width;
+    const std::int32_t* table = a.table + static_cast<std::size_t>(s) * a.stride;
+    unsigned long long* keys = a.keys + static_cast<std::size_t>(s) * a.width;
+    unsigned long long threshold = 0;
+    std::uint32_t equal = 0xffffffffu;
+    if (nb > a.keep) {
+        for (std::uint32_t i = threadIdx.x; i < nb; i += 256) {
+            const std::uint32_t id = static_cast<std::uint32_t>(table[i]);
+            unsigned long long key = 0;
+            if (id < a.blocks) {
+                for (std::uint32_t h = 0; h < a.kv_heads; ++h) key += a.weight[static_cast<std::size_t>(id) * a.kv_heads + h];
+                key += 1;
+            }
+            if (i < a.keep_first || i + a.keep_last >= nb) key = ~0ull;
+            keys[i] = key;
+        }
+        __syncthreads();
+        equal = radix_threshold<unsigned long long, 256>([&](std::uint32_t i) { return keys[i]; }, nb, a.keep, &threshold);
+    }
+    std::int32_t* kept = a.out_table + static_cast<std::size_t>(s) * a.width;
+    std::int32_t* freed = a.freed + static_cast<std::size_t>(s) * a.width;
+    std::uint32_t done = 0, ties = 0;
+    for (std::uint32_t base = 0; base < nb; base += 256) {
+        const std::uint32_t i = base + threadIdx.x;
+        const bool in = i < nb;
+        const unsigned long long k = !in ? 0 : nb > a.keep ? keys[i] : 0;
+        std::uint32_t total;
+        const std::uint32_t rank = flag_rank<256>(in && k == threshold, &total);
+        const bool take = in && (k > threshold || (k == threshold && ties + rank < equal));
+        ties += total;
+        const std::uint32_t at = flag_rank<256>(take, &total);
+        if (take) {
+            kept[done + at] = table[i];
+        } else if (in) {
+            freed[i - (done + at)] = table[i];
+        }
+        done += total;
+    }
+    for (std::uint32_t i = done + threadIdx.x; i < a.width; i += 256) kept[i] = -1;
+    for (std::uint32_t i = nb - done + threadIdx.x; i < a.width; i += 256) freed[i] = -1;
+    if (threadIdx.x == 0) {
+        a.out_lens[s] = static_cast<std::int32_t>(len - static_cast<std::int64_t>(nb - done) * a.tokens);
+        a.freed_count[s] = static_cast<std::int32_t>(nb - done);
+    }
+}
+
+// ---- host -----------------------------------------------------------------
+
+// A launch dimension holds fewer than 2^32 threads.
+constexpr std::size_t kMostGroups = std::size_t{1} << 23;
+
+bool aligned16(const void* p) { return (reinterpret_cast<std::uintptr_t>(p) & 15u) == 0; }
+
+int checked(hipError_t e) { return e == hipSuccess ? HBFSIM_OK : HBFSIM_CUDA_ERROR; }
+
+// The cache's own fields; pools may be asked for or not.
+int take_cache(const hbfsim_amd_kv_cache* in, Cache* out)
+{
+    if (in == nullptr || in->struct_size != sizeof(*in)) {
+        return HBFSIM_INVALID_ARGUMENT;
+    }
+    const bool tokens_ok = in->block_tokens == 16 || in->block_tokens == 32 ||
+                           in->block_tokens == 64 || in->block_tokens == 128;
+    if (in->blocks == 0 || in->blocks > 0x7fffffffu || in->kv_heads == 0 || in->kv_heads > 1024 ||
+        in->head_dim == 0 || in->head_dim > 256 || !tokens_ok) {
+        return HBFSIM_INVALID_ARGUMENT;
+    }
+    if (in->d_keys == nullptr || in->d_values == nullptr || in->d_key_scale == nullptr ||
+        in->d_value_scale == nullptr || in->d_bounds == nullptr || in->d_weight == nullptr ||
+        !aligned16(in->d_keys) || !aligned16(in->d_values) || !aligned16(in->d_bounds)) {
+        return HBFSIM_INVALID_ARGUMENT;
+    }
+    out->keys = in->d_keys;
+    out->values = in->d_values;
+    out->key_scale = in->d_key_scale;
+    out->value_scale = in->d_value_scale;
+    out->bounds = in->d_bounds;
+    out->weight = reinterpret_cast<unsigned long long*>(in->d_weight);
+    out->blocks = in->blocks;
+    out->kv_heads = in->kv_heads;
+    out->dim = in->head_dim;
+    out->dims = (in->head_dim + 63) / 64 * 64;
+    out->tokens = in->block_tokens;
+    out->tile_shift = in->block_tokens == 16 ? 0 : in->block_tokens == 32 ? 1 : in->block_tokens == 64 ? 2 : 3;
+    return HBFSIM_OK;
+}
+
+int take_batch(const hbfsim_amd_kv_batch* in, const Cache& c, Batch* out)
+{
+    if (in == nullptr || in->struct_size != sizeof(*in) || in->table_stride < in->table_width) {
+        return HBFSIM_INVALID_ARGUMENT;
+    }
+    // positions are 32-bit signed, with room for a tile beyond the last
+    if (static_cast<std::uint64_t>(in->table_width) * c.tokens > 0x7fffff00u ||
+        in->tokens > 0x7fffff00u || in->seqs > 0x7fffff00u) {
+        return HBFSIM_INVALID_ARGUMENT;
+    }
+    if (in->d_first == nullptr && in->tokens != in->seqs) {
+        return HBFSIM_INVALID_ARGUMENT;
+    }
+    if (in->seqs != 0 && in->tokens != 0 && (in->d_lens == nullptr || (in->table_width != 0 && in->d_table == nullptr))) {
+        return HBFSIM_INVALID_ARGUMENT;
+    }
+    out->table = in->d_table;
+    out->lens = in->d_lens;
+    out->first = in->d_first;
+    out->seqs = in->seqs;
+    out->width = in->table_width;
+    out->stride = in->table_stride;
+    out->tokens = in->tokens;
+    return HBFSIM_OK;
+}
+
+bool two_byte(std::uint32_t type) { return type == HBFSIM_AMD_KV_BF16 || type == HBFSIM_AMD_KV_F16; }
+
+// How attend cuts its work: from the call's host-side sizes alone.
+struct Cut {
+    std::uint32_t per, row_tiles, units, split, splits;
+    std::size_t partial, stats, lse, bytes;
+};
+
+std::size_t up256(std::size_t x) { return (x + 255) & ~std::size_t{255}; }
+
+Cut cut_attend(const Cache& c, const Batch& b, std::uint32_t heads, std::uint32_t count, bool accumulate)
+{
+    Cut k{};
+    const std::uint32_t group = heads / c.kv_heads;
+    k.per = b.first == nullptr || count != 0 || group > 8 ? 1 : 16 / group;
+    k.row_tiles = group > 16 ? (group + 15) / 16 : 1;
+    k.units = b.first == nullptr ? b.seqs : b.tokens / k.per + b.seqs;
+    const std::uint64_t longest = static_cast<std::uint64_t>(count != 0 ? count : b.width) * c.tokens;
+    const std::uint64_t pairs = static_cast<std::uint64_t>(k.units) * c.kv_heads * k.row_tiles;
+    std::uint64_t split = 2048;
+    while (split > 256 && pairs * ((longest + split - 1) / split) < 1024) split /= 2;
+    k.split = static_cast<std::uint32_t>(split);
+    k.splits = longest == 0 ? 1 : static_cast<std::uint32_t>((longest + split - 1) / split);
+    if (k.splits > 1) {
+        const std::size_t cells = static_cast<std::size_t>(pairs) * k.splits * 16;
+        k.stats = up256(cells * c.dims * sizeof(float));
+        k.lse = k.stats + up256(cells * 2 * sizeof(float));
+    }
+    k.bytes = k.lse + (accumulate ? up256(static_cast<std::size_t>(b.tokens) * heads * sizeof(float)) : 0);
+    return k;
+}
+
+template <typename T, int CH>
+void launch_attend(const Attend& a, const Cut& k, bool accumulate, hipStream_t stream)
+{
+    const dim3 grid(k.units, a.c.kv_heads * k.row_tiles, k.splits);
+    hipLaunchKernelGGL((k_kv_attend<T, CH, 4>), grid, dim3(256), 0, stream, a);
+    if (k.splits > 1) {
+        hipLaunchKernelGGL((k_kv_merge<T>), dim3(k.units, grid.y), dim3(256), 0, stream, a);
+    }
+    if (accumulate && a.b.width != 0) {
+        const std::uint32_t z = a.b.width / 64 < 65535 ? (a.b.width + 63) / 64 : 65535;
+        hipLaunchKernelGGL((k_kv_weigh<T, CH>), dim3(k.units, grid.y, z), dim3(256), 0, stream, a);
+    }
+}
+
+template <typename T>
+int run_attend(const Attend& a, const Cut& k, bool accumulate, hipStream_t stream)
+{
+    switch (a.c.dims / 64) {
+    case 1: launch_attend<T, 1>(a, k, accumulate, stream); break;
+    case 2: launch_attend<T, 2>(a, k, accumulate, stream); break;
+    case 3: launch_attend<T, 3>(a, k, accumulate, stream); break;
+    default: launch_attend<T, 4>(a, k, accumulate, stream); break;
+    }
+    return checked(hipGetLastError());
+}
+
+}  // namespace
+
+#define HBF_API extern "C" __attribute__((visibility("default")))
+
+HBF_API int hbfsim_amd_kv_append(const hbfsim_amd_kv_cache* cache, const hbfsim_amd_kv_batch* batch,
+                                 const void* d_k, const void* d_v, uint32_t type,
+                                 const int64_t strides[4], void* stream)
+{
+    Append a{};
+    int rc = take_cache(cache, &a.c);
+    if (rc == HBFSIM_OK) rc = take_batch(batch, a.c, &a.b);
+    if (rc != HBFSIM_OK) {
+        return rc;
+    }
+    if (type > HBFSIM_AMD_KV_F32 || strides == nullptr) {
+        return HBFSIM_INVALID_ARGUMENT;
+    }
+    if (a.b.tokens == 0 || a.b.seqs == 0 || a.b.width == 0) {
+        return HBFSIM_OK;
+    }
+    if (d_k == nullptr || d_v == nullptr) {
+        return HBFSIM_INVALID_ARGUMENT;
+    }
+    a.x[0] = d_k;
+    a.x[1] = d_v;
+    for (int i = 0; i < 2; ++i) {
+        a.token_stride[i] = strides[2 * i];
+        a.head_stride[i] = strides[2 * i + 1];
+    }
+    const std::uint32_t slots = a.b.first == nullptr ? a.b.seqs : a.b.tokens / a.c.tokens + 2 * a.b.seqs;
+    if (slots > kMostGroups) {
+        return HBFSIM_UNSUPPORTED;
+    }
+    const dim3 grid(slots, a.c.kv_heads, 2);
+    const hipStream_t s = static_cast<hipStream_t>(stream);
+    if (type == HBFSIM_AMD_KV_BF16) {
+        hipLaunchKernelGGL(k_kv_append<Bf16>, grid, dim3(kWave), 0, s, a);
+    } else if (type == HBFSIM_AMD_KV_F16) {
+        hipLaunchKernelGGL(k_kv_append<F16>, grid, dim3(kWave), 0, s, a);
+    } else {
+        hipLaunchKernelGGL(k_kv_append<float>, grid, dim3(kWave), 0, s, a);
+    }
+    return checked(hipGetLastError());
+}
+
+HBF_API int hbfsim_amd_kv_read(const hbfsim_amd_kv_cache* cache, const int32_t* d_blocks, size_t n,
+                               uint32_t type, void* d_k, void* d_v, void* d_low, void* d_high,
+                               void* stream)
+{
+    Cache c{};
+    const int rc = take_cache(cache, &c);
+    if (rc != HBFSIM_OK) {
+        return rc;
+    }
+    if (type > HBFSIM_AMD_KV_F32) {
+        return HBFSIM_INVALID_ARGUMENT;
+    }
+    if (n > kMostGroups) {
+        return HBFSIM_UNSUPPORTED;
+    }
+    if (n == 0) {
+        return HBFSIM_OK;
+    }
+    if (d_blocks == nullptr || d_k == nullptr || d_v == nullptr || d_low == nullptr || d_high == nullptr) {
+        return HBFSIM_INVALID_ARGUMENT;
+    }
+    const dim3 grid(static_cast<unsigned>(n), c.kv_heads);
+    const hipStream_t s = static_cast<hipStream_t>(stream);
+    if (type == HBFSIM_AMD_KV_BF16) {
+        hipLaunchKernelGGL(k_kv_read<Bf16>, grid, dim3(256), 0, s, c, d_blocks, static_cast<Bf16*>(d_k),
+                           static_cast<Bf16*>(d_v), static_cast<Bf16*>(d_low), static_cast<Bf16*>(d_high));
+    } else if (type == HBFSIM_AMD_KV_F16) {
+        hipLaunchKernelGGL(k_kv_read<F16>, grid, dim3(256), 0, s, c, d_blocks, static_cast<F16*>(d_k),
+                           static_cast<F16*>(d_v), static_cast<F16*>(d_low), static_cast<F16*>(d_high));
+    } else {
+        hipLaunchKernelGGL(k_kv_read<float>, grid, dim3(256), 0, s, c, d_blocks, static_cast<float*>(d_k),
+                           static_cast<float*>(d_v), static_cast<float*>(d_low), static_cast<float*>(d_high));
+    }
+    return checked(hipGetLastError());
+}
+
+HBF_API int hbfsim_amd_kv_attend_workspace(const hbfsim_amd_kv_cache* cache, const hbfsim_amd_kv_batch* batch,
+                                           uint32_t heads, uint32_t count, uint32_t accumulate, size_t* bytes)
+{
+    Cache c{};
+    Batch b{};
+    int rc = take_cache(cache, &c);
+    if (rc == HBFSIM_OK) rc = take_batch(batch, c, &b);
+    if (rc != HBFSIM_OK) {
+        return rc;
+    }
+    if (bytes == nullptr || heads == 0 || heads % c.kv_heads != 0) {
+        return HBFSIM_INVALID_ARGUMENT;
+    }
+    *bytes = b.tokens == 0 || b.seqs == 0 ? 0 : cut_attend(c, b, heads, count, accumulate != 0).bytes;
+    return HBFSIM_OK;
+}
+
+HBF_API int hbfsim_amd_kv_attend(const hbfsim_amd_kv_cache* cache, const hbfsim_amd_kv_batch* batch,
+                                 const void* d_q, uint32_t type, uint32_t heads, int64_t token_stride,
+                                 int64_t head_stride, float scale, const int32_t* d_selected, uint32_t count,
+                                 uint32_t accumulate, void* d_out, void* d_workspace, size_t workspace_bytes,
+                                 void* stream)
+{
+    Attend a{};
+    int rc = take_cache(cache, &a.c);
+    if (rc == HBFSIM_OK) rc = take_batch(batch, a.c, &a.b);
+    if (rc != HBFSIM_OK) {
+        return rc;
+    }
+    if (!two_byte(type) || heads == 0 || heads % a.c.kv_heads != 0 || !(scale == scale) ||
+        scale == kInf || scale == -kInf || (d_selected == nullptr) != (count == 0) ||
+        (accumulate != 0 && count != 0) || static_cast<std::uint64_t>(count) * a.c.tokens > 0x7fffff00u) {
+        return HBFSIM_INVALID_ARGUMENT;
+    }
+    if (a.b.tokens == 0 || a.b.seqs == 0) {
+        return HBFSIM_OK;
+    }
+    const Cut k = cut_attend(a.c, a.b, heads, count, accumulate != 0);
+    if (d_q == nullptr || d_out == nullptr || workspace_bytes < k.bytes ||
+        (k.bytes != 0 && (d_workspace == nullptr || !aligned16(d_workspace)))) {
+        return HBFSIM_INVALID_ARGUMENT;
+    }
+    if (k.units > kMostGroups || k.splits > 65535 || a.c.kv_heads * k.row_tiles > 65535) {
+        return HBFSIM_UNSUPPORTED;
+    }
+    a.q = d_q;
+    a.q_token = token_stride;
+    a.q_head = head_stride;
+    a.q_vector = aligned16(d_q) && token_stride % 8 == 0 && head_stride % 8 == 0 ? 1 : 0;
+    a.heads = heads;
+    a.group = heads / a.c.kv_heads;
+    a.per = k.per;
+    a.row_tiles = k.row_tiles;
+    a.scale = scale * kLog2e;
+    a.selected = d_selected;
+    a.count = count;
+    a.split = k.split;
+    a.splits = k.splits;
+    a.out = d_out;
+    unsigned char* ws = static_cast<unsigned char*>(d_workspace);
+    a.partial = k.splits > 1 ? reinterpret_cast<float*>(ws + k.partial) : nullptr;
+    a.stats = k.splits > 1 ? reinterpret_cast<float*>(ws + k.stats) : nullptr;
+    a.lse = accumulate != 0 ? reinterpret_cast<float*>(ws + k.lse) : nullptr;
+    const hipStream_t s = static_cast<hipStream_t>(stream);
+    return type == HBFSIM_AMD_KV_BF16 ? run_attend<Bf16>(a, k, accumulate != 0, s)
+                                      : run_attend<F16>(a, k, accumulate != 0, s);
+}
+
+HBF_API int hbfsim_amd_kv_select_workspace(const hbfsim_amd_kv_cache* cache, const hbfsim_amd_kv_batch* batch,
+                                           size_t* bytes)
+{
+    Cache c{};
+    Batch b{};
+    int rc = take_cache(cache, &c);
+    if (rc == HBFSIM_OK) rc = take_batch(batch, c, &b);
+    if (rc != HBFSIM_OK) {
+        return rc;
+    }
+    if (bytes == nullptr) {
+        return HBFSIM_INVALID_ARGUMENT;
+    }
+    *bytes = static_cast<std::size_t>(b.tokens) * c.kv_heads * b.width * sizeof(std::uint32_t);
+    return HBFSIM_OK;
+}
+
+HBF_API int hbfsim_amd_kv_select(const hbfsim_amd_kv_cache* cache, const hbfsim_amd_kv_batch* batch,
+                                 const void* d_q, uint32_t type, uint32_t heads, int64_t token_stride,
+                                 int64_t head_stride, uint32_t count, uint32_t keep_first, uint32_t keep_last,
+                                 int32_t* d_selected, void* d_workspace, size_t workspace_bytes, void* stream)
+{
+    Select a{};
+    int rc = take_cache(cache, &a.c);
+    if (rc == HBFSIM_OK) rc = take_batch(batch, a.c, &a.b);
+    if (rc != HBFSIM_OK) {
+        return rc;
+    }
+    if (!two_byte(type) || heads == 0 || heads % a.c.kv_heads != 0 || heads / a.c.kv_heads > 64 || count == 0 ||
+        count > 0x7fffffffu || static_cast<std::uint64_t>(keep_first) + keep_last > count) {
+        return HBFSIM_INVALID_ARGUMENT;
+    }
+    if (a.b.tokens == 0 || a.b.seqs == 0) {
+        return HBFSIM_OK;
+    }
+    const std::size_t need = static_cast<std::size_t>(a.b.tokens) * a.c.kv_heads * a.b.width * sizeof(std::uint32_t);
+    if (d_q == nullptr || d_selected == nullptr || workspace_bytes < need || (need != 0 && d_workspace == nullptr)) {
+        return HBFSIM_INVALID_ARGUMENT;
+    }
+    if (a.b.tokens > kMostGroups || a.b.width > 1024 * 65535u) {
+        return HBFSIM_UNSUPPORTED;
+    }
+    a.q = d_q;
+    a.q_token = token_stride;
+    a.q_head = head_stride;
+    a.group = heads / a.c.kv_heads;
+    a.count = count;
+    a.keep_first = keep_first;
+    a.keep_last = keep_last;
+    a.keys = static_cast<std::uint32_t*>(d_workspace);
+    a.selected = d_selected;
+    const hipStream_t s = static_cast<hipStream_t>(stream);
+    if (a.b.width != 0) {
+        const std::uint32_t z = (a.b.width + 1023) / 1024;
+        const dim3 grid(a.b.tokens, a.c.kv_heads, z);
+        if (type == HBFSIM_AMD_KV_BF16) {
+            hipLaunchKernelGGL(k_kv_score<Bf16>, grid, dim3(256), 0, s, a);
+        } else {
+            hipLaunchKernelGGL(k_kv_score<F16>, grid, dim3(256), 0, s, a);
+        }
+    }
+    hipLaunchKernelGGL(k_kv_pick, dim3(a.b.tokens, a.c.kv_heads), dim3(256), 0, s, a);
+    return checked(hipGetLastError());
+}
+
+HBF_API int hbfsim_amd_kv_evict(const int64_t* d_weight, uint32_t blocks, uint32_t kv_heads, uint32_t block_tokens,
+                                const int32_t* d_table, const int32_t* d_lens, uint32_t seqs, uint32_t width,
+                                uint32_t stride, uint32_t keep, uint32_t keep_first, uint32_t keep_last,
+                                int32_t* d_out_table, int32_t* d_out_lens, int32_t* d_freed,
+                                int32_t* d_freed_count, void* d_workspace, size_t workspace_bytes, void* stream)
+{
+    const bool tokens_ok = block_tokens == 16 || block_tokens == 32 || block_tokens == 64 || block_tokens == 128;
+    if (blocks == 0 || blocks > 0x7fffffffu || kv_heads == 0 || kv_heads > 1024 || !tokens_ok || keep == 0 ||
+        keep_last == 0 || static_cast<std::uint64_t>(keep_first) + keep_last > keep || stride < width ||
+        seqs > 0x7fffff00u || static_cast<std::uint64_t>(width) * block_tokens > 0x7fffff00u) {
+        return HBFSIM_INVALID_ARGUMENT;
+    }
+    if (seqs == 0) {
+        return HBFSIM_OK;
+    }
+    if (seqs > kMostGroups) {
+        return HBFSIM_UNSUPPORTED;
+    }
+    const std::size_t need = static_cast<std::size_t>(seqs) * width * sizeof(unsigned long long);
+    if (d_weight == nullptr || d_lens == nullptr || d_out_lens == nullptr || d_freed_count == nullptr ||
+        workspace_bytes < need || (need != 0 && (d_table == nullptr || d_out_table == nullptr || d_freed == nullptr ||
+                                                 d_workspace == nullptr || !aligned16(d_workspace)))) {
+        return HBFSIM_INVALID_ARGUMENT;
+    }
+    Evict a{reinterpret_cast<const unsigned long long*>(d_weight), blocks, kv_heads, block_tokens, d_table, d_lens,
+            seqs, width, stride, keep, keep_first, keep_last, static_cast<unsigned long long*>(d_workspace),
+            d_out_table, d_out_lens, d_freed, d_freed_count};
+    hipLaunchKernelGGL(k_kv_evict, dim3(seqs), dim3(256), 0, static_cast<hipStream_t>(stream), a);
+    return checked(hipGetLastError());
+}

@@ -801,6 +801,137 @@ int hbfsim_amd_validate_profile(const char* path, char* error,
 int hbfsim_amd_probe_bandwidth(void* d_buffer, size_t bytes, unsigned reps, void* stream,
                                float* read_ms, float* write_ms);
 
+/* ===== 7. Paged key/value cache in 8 bits ==============================
+ *
+ * No counterpart in the reference: the decode or prompt step whose reads and
+ * appends the paged-KV record streams stand for.  A cache is a pool of
+ * blocks of `block_tokens` tokens of every kv head, its keys and values held
+ * as signed 8-bit codes with one float scale per (block, kv head) each; a
+ * sequence is a row of a block table.  With dims = head_dim rounded up to 64
+ * (zeros beyond head_dim) the device arrays are, innermost last:
+ *   d_keys   int8 [blocks][kv_heads][block_tokens / 16][dims / 64][4][16][16]
+ *            token 16 * tile + [5], dim 64 * chunk + 16 * [4] + [6]
+ *   d_values int8 [blocks][kv_heads][block_tokens / 16][dims / 64][4][16][4][4]
+ *            token 16 * tile + 4 * [4] + [7], dim 64 * chunk + 16 * [6] + [5]
+ *   d_key_scale, d_value_scale float [blocks][kv_heads]
+ *   d_bounds int8 [blocks][kv_heads][2][dims]: the lowest, then the highest
+ *            key code of the block's tokens in each dim
+ *   d_weight int64 [blocks][kv_heads]: accumulated attention probability in
+ *            units of 2^-32
+ * keys, values and bounds are 16-byte aligned.  No call allocates,
+ * synchronises or copies to the host: work is queued on `stream`, and a
+ * workspace must stay untouched until it is done. */
+#define HBFSIM_AMD_KV_BF16 0u
+#define HBFSIM_AMD_KV_F16 1u
+#define HBFSIM_AMD_KV_F32 2u
+
+typedef struct hbfsim_amd_kv_cache {
+    uint32_t struct_size;       /* sizeof(hbfsim_amd_kv_cache) */
+    uint32_t blocks;            /* in the pool, at most 2^31 - 1 */
+    uint32_t kv_heads;          /* 1..1024 */
+    uint32_t head_dim;          /* 1..256 */
+    uint32_t block_tokens;      /* 16, 32, 64 or 128 */
+    uint32_t reserved0;
+    int8_t* d_keys;
+    int8_t* d_values;
+    float* d_key_scale;
+    float* d_value_scale;
+    int8_t* d_bounds;
+    int64_t* d_weight;
+} hbfsim_amd_kv_cache;
+
+/* The sequences of a step.  Sequence s holds d_lens[s] tokens once the
+ * step's own are stored, in the blocks d_table[s * table_stride + i]; the
+ * step's tokens are its last ones, rows [d_first[s], d_first[s + 1]) of the
+ * batch (d_first NULL: one token each, tokens == seqs).  Token i of them
+ * sees the sequence up to itself.  Table entries outside [0, blocks) are
+ * blocks that are not there: nothing is stored in them and nothing attends
+ * to them; so are positions past table_width blocks. */
+typedef struct hbfsim_amd_kv_batch {
+    uint32_t struct_size;       /* sizeof(hbfsim_amd_kv_batch) */
+    uint32_t seqs;
+    uint32_t table_width;       /* blocks per row */
+    uint32_t table_stride;      /* entries from one row to the next, >= table_width */
+    uint32_t tokens;            /* of the step, all sequences together */
+    uint32_t reserved0;
+    const int32_t* d_table;
+    const int32_t* d_lens;      /* [seqs] */
+    const int32_t* d_first;     /* [seqs + 1], or NULL */
+} hbfsim_amd_kv_batch;
+
+/* Stores the step's keys and values, [tokens][kv_heads][head_dim] with the
+ * token and head strides strides[0..1] (keys) and strides[2..3] (values) in
+ * elements.  Per (block, kv head) and tensor: s = max|x| / 127 over the new
+ * tokens (at least 2^-40), a block begun before keeps the larger of its scale
+ * and s and has its codes and bounds requantised to it, code = x / s rounded
+ * to nearest even.  A value that is not finite, or a scale above 2^40, makes
+ * the scale NaN, so that what reads the block is NaN until it is begun anew.
+ * Beginning a block zeroes its other slots and its weight.
+ * HBFSIM_INVALID_ARGUMENT for sizes outside the limits above. */
+int hbfsim_amd_kv_append(const hbfsim_amd_kv_cache* cache, const hbfsim_amd_kv_batch* batch,
+                         const void* d_k, const void* d_v, uint32_t type,
+                         const int64_t strides[4], void* stream);
+
+/* Blocks back as values: entry i of d_blocks gives d_k and d_v
+ * [i][kv_heads][block_tokens][head_dim] and the bounds d_low and d_high
+ * [i][kv_heads][head_dim], code * scale in `type`; zeros for an id outside
+ * the pool. */
+int hbfsim_amd_kv_read(const hbfsim_amd_kv_cache* cache, const int32_t* d_blocks, size_t n,
+                       uint32_t type, void* d_k, void* d_v, void* d_low, void* d_high,
+                       void* stream);
+
+/* Attention of the step's queries [tokens][heads][head_dim] (bf16 or f16,
+ * strides in elements; query heads h * heads / kv_heads .. share kv head h)
+ * over the cache: d_out [tokens][heads][head_dim], contiguous, is the
+ * softmax of scale * q k over the tokens that the query sees, times v; zeros
+ * where it sees none.  With d_selected [tokens][kv_heads][count] (logical
+ * blocks, distinct, anything below 0 for none) a query sees those blocks
+ * alone.  With `accumulate` (not together with d_selected) d_weight of each
+ * block and kv head gains the probabilities of its tokens, summed over the
+ * queries and the heads that share it; a sum that is not a number adds
+ * nothing.  The workspace call gives the bytes needed for the same sizes. */
+int hbfsim_amd_kv_attend_workspace(const hbfsim_amd_kv_cache* cache,
+                                   const hbfsim_amd_kv_batch* batch, uint32_t heads,
+                                   uint32_t count, uint32_t accumulate, size_t* bytes);
+int hbfsim_amd_kv_attend(const hbfsim_amd_kv_cache* cache, const hbfsim_amd_kv_batch* batch,
+                         const void* d_q, uint32_t type, uint32_t heads, int64_t token_stride,
+                         int64_t head_stride, float scale, const int32_t* d_selected,
+                         uint32_t count, uint32_t accumulate, void* d_out, void* d_workspace,
+                         size_t workspace_bytes, void* stream);
+
+/* For each query token and kv head, the `count` blocks to attend to:
+ * d_selected [tokens][kv_heads][count], ascending, -1 beyond.  The first
+ * keep_first and the last keep_last blocks that the token sees are always
+ * among them (keep_first + keep_last <= count), the others are the best by
+ *   score = key_scale * sum over the group's heads and dims of
+ *           max(c * low, c * high)
+ * with the block's bounds and the group's queries as 8-bit codes c of one
+ * scale (max|q| / 127): whole numbers, so scores do not depend on an order
+ * of sums.  Equal scores go to the lower index; a NaN scale counts as the
+ * best; query elements that are not numbers count as 0.  At most 64 query
+ * heads per kv head. */
+int hbfsim_amd_kv_select_workspace(const hbfsim_amd_kv_cache* cache,
+                                   const hbfsim_amd_kv_batch* batch, size_t* bytes);
+int hbfsim_amd_kv_select(const hbfsim_amd_kv_cache* cache, const hbfsim_amd_kv_batch* batch,
+                         const void* d_q, uint32_t type, uint32_t heads, int64_t token_stride,
+                         int64_t head_stride, uint32_t count, uint32_t keep_first,
+                         uint32_t keep_last, int32_t* d_selected, void* d_workspace,
+                         size_t workspace_bytes, void* stream);
+
+/* Blocks that leave: every sequence of more than `keep` blocks keeps its
+ * first keep_first, its last keep_last (at least 1) and the others of the
+ * largest weight summed over kv heads (ties to the lower index; entries that
+ * name no block go first).  d_out_table [seqs][width] holds the kept blocks
+ * in order and d_freed [seqs][width] those that left, -1 beyond; d_out_lens
+ * the remaining tokens, d_freed_count the number that left.  The inputs are
+ * not changed.  Workspace: seqs * width * 8 bytes. */
+int hbfsim_amd_kv_evict(const int64_t* d_weight, uint32_t blocks, uint32_t kv_heads,
+                        uint32_t block_tokens, const int32_t* d_table, const int32_t* d_lens,
+                        uint32_t seqs, uint32_t width, uint32_t stride, uint32_t keep,
+                        uint32_t keep_first, uint32_t keep_last, int32_t* d_out_table,
+                        int32_t* d_out_lens, int32_t* d_freed, int32_t* d_freed_count,
+                        void* d_workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
