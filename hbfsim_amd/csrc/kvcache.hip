@@ -45,6 +45,8 @@ constexpr float kScaleMax = 0x1p40f;
 constexpr float kQueryScaleMin = 0x1p-100f;
 constexpr float kLog2e = 1.44269504088896340736f;
 constexpr float kInf = __builtin_inff();
+constexpr float kLowest = -3.0e38f;            // a row's reference exponent before its first score
+constexpr std::int32_t kNowhere = 0x7fffffff - 127;  // a position that no row sees
 
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
@@ -201,13 +203,15 @@ struct Attend {
     std::uint32_t heads, group;    // query heads; query heads per kv head
     std::uint32_t per;             // tokens per unit
     std::uint32_t row_tiles;       // 16-row tiles per unit (1 unless group > 16)
+    std::uint32_t pairs;           // kv heads times row tiles: a unit's workgroups, heads first
+    std::uint32_t rows;            // rows of a tile that any unit uses
     float scale;                   // softmax scale times log2(e)
     const std::int32_t* selected;
     std::uint32_t count;
     std::uint32_t split, splits;   // tokens per split, splits launched
     void* out;
-    float* partial;                // [unit, kv head, row tile, split][16][dims]
-    float* stats;                  // [...][16][2]: reference exponent, denominator
+    float* partial;                // [unit, row tile, kv head, split][rows][dims]
+    float* stats;                  // [...][rows][2]: reference exponent, denominator
     float* lse;                    // [tokens, heads], log2 of the row's denominator, or null
 };
 
@@ -226,19 +230,109 @@ __device__ inline std::int64_t visible(const Attend& a, std::int64_t seen)
     return seen < most ? seen : most;
 }
 
-// A workgroup of kWaves waves takes one (unit, kv head, row tile, split); its
-// waves take pairs of 16-token tiles in turn and join through LDS.
+// Four dims of a finished row: sums `o` and denominator `l` at exponent `ref`.
+template <typename T>
+__device__ inline void finish_row(const Attend& a, std::int64_t token, std::uint32_t head, int d, f32x4 o, float l,
+                                  float ref)
+{
+    T* out = static_cast<T*>(a.out) + (token * a.heads + head) * a.c.dim + d;
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        if (d + i < static_cast<int>(a.c.dim)) out[i] = from_float<T>(l == 0.0f ? 0.0f : o[i] * inv);
+    }
+    if (d == 0 && a.lse != nullptr) {
+        a.lse[token * a.heads + head] = l == 0.0f ? kInf : ref + log2f(l);
+    }
+}
+
+// The query rows of a wave as the matrix units take them: lane (quarter, m)
+// holds row m's dims 16 quarter .. 16 quarter + 15 of every 64, scaled by a
+// power of two; *factor undoes it and applies the softmax scale.
+template <typename T, int CH>
+__device__ inline void load_query(const Attend& a, const T* q, bool live, int quarter, f16x8 (&query)[CH * 2],
+                                  float* factor)
+{
+    float x[CH * 16];
+    float top = 0.0f;
+#pragma unroll
+    for (int i = 0; i < CH * 2; ++i) {
+        const int d0 = (i / 2) * 64 + quarter * 16 + (i & 1) * 8;
+        if (live && a.q_vector != 0 && d0 + 8 <= static_cast<int>(a.c.dim)) {
+            union {
+                u32x4 v;
+                T e[8];
+            } u;
+            u.v = *reinterpret_cast<const u32x4*>(q + d0);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) x[i * 8 + j] = to_float(u.e[j]);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                x[i * 8 + j] = live && d0 + j < static_cast<int>(a.c.dim) ? to_float(q[d0 + j]) : 0.0f;
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) top = fmaxf(top, fabsf(x[i * 8 + j]));
+    }
+    top = fmaxf(top, __shfl_xor(top, 16));
+    top = fmaxf(top, __shfl_xor(top, 32));
+    const int k = top > 0.0f && top < kInf ? 14 - ilogbf(top) : 0;
+    *factor = ldexpf(a.scale, -k);
+#pragma unroll
+    for (int i = 0; i < CH * 2; ++i) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) query[i][j] = static_cast<_Float16>(ldexpf(x[i * 8 + j], k));
+    }
+}
+
+// What a wave knows of up to 64 consecutive tiles, one per lane.
+struct Tiles {
+    std::int32_t id, sub, pos;          // block, tile within it, first token's position
+    float key_scale, log_scale, inv_scale;
+};
+
+__device__ inline Tiles load_tiles(const Attend& a, std::uint32_t seq, std::uint32_t head, const std::int32_t* list,
+                                   std::int64_t tile, bool inside, std::int64_t seen)
+{
+    Tiles t{0, 0, kNowhere, 0.0f, 0.0f, 1.0f};
+    if (inside) {
+        const std::int64_t entry = tile >> a.c.tile_shift;
+        const std::int64_t logical = list == nullptr ? entry : list[entry];
+        const std::int32_t sub = static_cast<std::int32_t>(tile) & ((1 << a.c.tile_shift) - 1);
+        const std::int32_t id = block_at(a.c, a.b, seq, logical);
+        const std::int64_t pos = logical * a.c.tokens + sub * 16;
+        if (id >= 0 && pos < seen) {
+            const std::size_t bh = static_cast<std::size_t>(id) * a.c.kv_heads + head;
+            const float vs = a.c.value_scale[bh];
+            t = Tiles{id, sub, static_cast<std::int32_t>(pos), a.c.key_scale[bh], log2f(vs), 1.0f / vs};
+        }
+    }
+    return t;
+}
+
+__device__ inline std::int32_t lane_int(std::int32_t x, int lane) { return __builtin_amdgcn_readlane(x, lane); }
+__device__ inline float lane_float(float x, int lane)
+{
+    return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(x), lane));
+}
+
+// A workgroup of kWaves waves takes one (kv head, row tile, unit; split); its
+// waves take a run of 16-token tiles each and join through LDS.  A lane looks
+// up one tile of the wave's next 64 (block, scales), so the loop itself has no
+// dependent loads; the keys of the pair of tiles after this one are on their
+// way while its softmax runs, the values while the next scores do.
 template <typename T, int CH, int kWaves>
 __global__ __launch_bounds__(kWaves * kWave) void k_kv_attend(Attend a)
 {
-    constexpr int P = CH * 64;
-    __shared__ float s_out[kWaves][16][P];
+    constexpr int P = CH * 64, kRow = P + 4;
+    extern __shared__ float s_out[];  // [kWaves][rows][kRow]
     __shared__ float s_ref[kWaves][16], s_den[kWaves][16];
 
-    const std::uint32_t unit = blockIdx.x;
-    const std::uint32_t head = blockIdx.y % a.c.kv_heads, row_tile = blockIdx.y / a.c.kv_heads;
-    const std::uint32_t split = blockIdx.z;
-    const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
+    const std::uint32_t unit = blockIdx.x / a.pairs, pair = blockIdx.x % a.pairs;
+    const std::uint32_t head = pair % a.c.kv_heads, row_tile = pair / a.c.kv_heads;
+    const std::uint32_t split = blockIdx.y;
+    const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     const int m = lane & 15, quarter = lane >> 4;
 
     Group g;
@@ -255,145 +349,113 @@ __global__ __launch_bounds__(kWaves * kWave) void k_kv_attend(Attend a)
     const std::uint32_t r = row_tile * 16 + m;
     const std::uint32_t row_token = r / a.group, row_head = r % a.group;
     const bool row_live = row_token < static_cast<std::uint32_t>(g.count);
-    std::int64_t limit64 = row_live ? visible(a, g.seen + row_token) : 0;
+    const std::int64_t limit64 = row_live ? visible(a, g.seen + row_token) : 0;
     const int limit = limit64 > 0 ? static_cast<int>(limit64) : 0;
     const std::int64_t token_row = g.row + static_cast<std::int64_t>(row_token);
-    const std::uint32_t q_head = head * a.group + row_head;
 
     f16x8 query[CH * 2];
-    float factor = 0.0f;
-    {
-        const T* q = static_cast<const T*>(a.q) + token_row * a.q_token + q_head * a.q_head;
-        float x[CH * 16];
-        float top = 0.0f;
-#pragma unroll
-        for (int i = 0; i < CH * 2; ++i) {
-            const int d0 = (i / 2) * 64 + quarter * 16 + (i & 1) * 8;
-            if (row_live && a.q_vector != 0 && d0 + 8 <= static_cast<int>(a.c.dim)) {
-                union {
-                    u32x4 v;
-                    T e[8];
-                } u;
-                u.v = *reinterpret_cast<const u32x4*>(q + d0);
-#pragma unroll
-                for (int j = 0; j < 8; ++j) x[i * 8 + j] = to_float(u.e[j]);
-            } else {
-#pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    x[i * 8 + j] = row_live && d0 + j < static_cast<int>(a.c.dim) ? to_float(q[d0 + j]) : 0.0f;
-                }
-            }
-#pragma unroll
-            for (int j = 0; j < 8; ++j) top = fmaxf(top, fabsf(x[i * 8 + j]));
-        }
-        top = fmaxf(top, __shfl_xor(top, 16));
-        top = fmaxf(top, __shfl_xor(top, 32));
-        const int k = top > 0.0f && top < kInf ? 14 - ilogbf(top) : 0;
-        factor = ldexpf(a.scale, -k);
-#pragma unroll
-        for (int i = 0; i < CH * 2; ++i) {
-#pragma unroll
-            for (int j = 0; j < 8; ++j) query[i][j] = static_cast<_Float16>(ldexpf(x[i * 8 + j], k));
-        }
-    }
+    float factor;
+    load_query<T, CH>(a, static_cast<const T*>(a.q) + token_row * a.q_token + (head * a.group + row_head) * a.q_head,
+                      row_live, quarter, query, &factor);
 
     f32x4 acc[CH * 4];
 #pragma unroll
     for (int i = 0; i < CH * 4; ++i) acc[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-    float ref = -kInf, den = 0.0f;
+    float ref = kLowest, den = 0.0f;
 
-    const std::int64_t total = a.selected != nullptr
-                                   ? static_cast<std::int64_t>(a.count) * a.c.tokens
-                                   : seen;
+    const std::int64_t total = a.selected != nullptr ? static_cast<std::int64_t>(a.count) * a.c.tokens : seen;
     const std::int64_t begin = static_cast<std::int64_t>(split) * a.split;
     const std::int64_t end = begin + a.split < total ? begin + a.split : total;
     const std::int32_t* list =
-        a.selected == nullptr
-            ? nullptr
-            : a.selected + (static_cast<std::int64_t>(g.row) * a.c.kv_heads + head) * a.count;
-    const std::uint32_t tile_mask = (1u << a.c.tile_shift) - 1;
+        a.selected == nullptr ? nullptr
+                              : a.selected + (static_cast<std::int64_t>(g.row) * a.c.kv_heads + head) * a.count;
     const std::size_t head_bytes = static_cast<std::size_t>(a.c.tokens) * P;
+    const std::int64_t tiles = end > begin ? (end - begin + 15) / 16 : 0;
+    const std::int64_t per_wave = (tiles + 2 * kWaves - 1) / (2 * kWaves) * 2;
+    const std::int64_t tile0 = wave * per_wave;
+    const std::int64_t tile1 = tile0 + per_wave < tiles ? tile0 + per_wave : tiles;
 
-    for (std::int64_t at = begin + wave * 32; at < end; at += kWaves * 32) {
+    for (std::int64_t at = tile0; at < tile1; at += kWave) {
+        const int n = static_cast<int>(tile1 - at < kWave ? tile1 - at : kWave);
+        const Tiles info = load_tiles(a, g.seq, head, list, begin / 16 + at + lane, lane < n, seen);
         u32x4 kc[2][CH], vc[2][CH];
-        float ks[2], vs[2];
-        int pos[2];
+        const auto tile_at = [&](const std::int8_t* pool, int tile) {
+            const std::size_t bh = static_cast<std::size_t>(lane_int(info.id, tile)) * a.c.kv_heads + head;
+            return reinterpret_cast<const u32x4*>(pool + bh * head_bytes +
+                                                  static_cast<std::size_t>(lane_int(info.sub, tile)) * 16 * P);
+        };
+        const auto load = [&](u32x4 (&to)[2][CH], const std::int8_t* pool, int tile) {
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-            const std::int64_t tile = at / 16 + u;
-            const std::int64_t entry = tile >> a.c.tile_shift;
-            std::int64_t logical = -1;
-            if (tile * 16 < end) {
-                logical = list == nullptr ? entry : list[entry];
+            for (int u = 0; u < 2; ++u) {
+                const u32x4* p = tile_at(pool, tile + u);
+#pragma unroll
+                for (int i = 0; i < CH; ++i) to[u][i] = p[i * kWave + lane];
             }
-            const std::uint32_t sub = static_cast<std::uint32_t>(tile) & tile_mask;
-            std::int32_t id = block_at(a.c, a.b, g.seq, logical);
-            pos[u] = id >= 0 && logical * a.c.tokens + sub * 16 < seen
-                         ? static_cast<int>(logical * a.c.tokens + sub * 16)
-                         : 0x7fffffff - 15;
-            id = id < 0 ? 0 : id;
-            const std::size_t bh = static_cast<std::size_t>(id) * a.c.kv_heads + head;
-            const std::int8_t* kp = a.c.keys + bh * head_bytes + static_cast<std::size_t>(sub) * 16 * P;
-            const std::int8_t* vp = a.c.values + bh * head_bytes + static_cast<std::size_t>(sub) * 16 * P;
+        };
+        const auto step = [&](int tile, bool more) __attribute__((always_inline)) {
+            f32x4 s[2];
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                s[u] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int i = 0; i < CH; ++i) {
+                    s[u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(widen8(kc[u][i].x, kc[u][i].y), query[2 * i], s[u], 0, 0, 0);
+                    s[u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(widen8(kc[u][i].z, kc[u][i].w), query[2 * i + 1], s[u], 0, 0, 0);
+                }
+            }
+            if (more) load(kc, a.c.keys, tile + 2);
+            float t[2][4];
+            float top = -kInf;
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                const float f = factor * lane_float(info.key_scale, tile + u), e = lane_float(info.log_scale, tile + u);
+                const int left = limit - lane_int(info.pos, tile + u) - quarter * 4;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    t[u][i] = i < left ? fmaf(s[u][i], f, e) : -kInf;
+                    top = fmaxf(top, t[u][i]);
+                }
+            }
+            // The row's reference exponent stays 2^7 to 2^15 below its largest
+            // weight (the f16 range), so it moves only now and then.
+            if (__any(top > ref + 15.0f)) {
+                top = fmaxf(top, __shfl_xor(top, 16));
+                top = fmaxf(top, __shfl_xor(top, 32));
+                const float next = fmaxf(ref, top - 7.0f);
+                const float shrink = exp2_fast(ref - next);
+                ref = next;
+                den *= shrink;
+#pragma unroll
+                for (int i = 0; i < CH * 4; ++i) acc[i] *= shrink;
+            }
+            f16x8 w;
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                float sum = 0.0f;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float x = exp2_fast(t[u][i] - ref);
+                    sum += x;
+                    w[u * 4 + i] = static_cast<_Float16>(x);
+                }
+                // a block of NaN scale reaches only the rows that see some of it
+                den = sum != 0.0f ? fmaf(sum, lane_float(info.inv_scale, tile + u), den) : den;
+            }
 #pragma unroll
             for (int i = 0; i < CH; ++i) {
-                kc[u][i] = reinterpret_cast<const u32x4*>(kp)[i * kWave + lane];
-                vc[u][i] = reinterpret_cast<const u32x4*>(vp)[i * kWave + lane];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    acc[i * 4 + j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(widen8(vc[0][i][j], vc[1][i][j]), w,
+                                                                            acc[i * 4 + j], 0, 0, 0);
+                }
             }
-            ks[u] = a.c.key_scale[bh];
-            vs[u] = a.c.value_scale[bh];
-        }
-        float t[2][4];
-        float top = -kInf;
-#pragma unroll
-        for (int u = 0; u < 2; ++u) {
-            f32x4 s = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-            for (int i = 0; i < CH; ++i) {
-                s = __builtin_amdgcn_mfma_f32_16x16x32_f16(widen8(kc[u][i].x, kc[u][i].y), query[2 * i], s, 0, 0, 0);
-                s = __builtin_amdgcn_mfma_f32_16x16x32_f16(widen8(kc[u][i].z, kc[u][i].w), query[2 * i + 1], s, 0, 0, 0);
-            }
-            const float f = factor * ks[u], e = log2f(vs[u]);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const float x = fmaf(s[i], f, e);
-                t[u][i] = pos[u] + quarter * 4 + i < limit ? x : -kInf;
-                top = fmaxf(top, t[u][i]);
-            }
-        }
-        // The row's reference exponent stays 2^7 to 2^15 below its largest
-        // weight (the f16 range), so it moves only now and then.
-        if (__any(top > ref + 15.0f)) {
-            top = fmaxf(top, __shfl_xor(top, 16));
-            top = fmaxf(top, __shfl_xor(top, 32));
-            const float next = fmaxf(ref, top - 7.0f);
-            const float shrink = next == -kInf ? 1.0f : exp2_fast(ref - next);
-            ref = next;
-            den *= shrink;
-#pragma unroll
-            for (int i = 0; i < CH * 4; ++i) acc[i] *= shrink;
-        }
-        f16x8 w;
-#pragma unroll
-        for (int u = 0; u < 2; ++u) {
-            const float inv = 1.0f / vs[u];
-            float sum = 0.0f;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const float x = pos[u] + quarter * 4 + i < limit ? exp2_fast(t[u][i] - ref) : 0.0f;
-                sum += x;
-                w[u * 4 + i] = static_cast<_Float16>(x);
-            }
-            den = sum != 0.0f ? fmaf(sum, inv, den) : den;
-        }
-#pragma unroll
-        for (int i = 0; i < CH; ++i) {
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                acc[i * 4 + j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
-                    widen8(vc[0][i][j], vc[1][i][j]), w, acc[i * 4 + j], 0, 0, 0);
-            }
-        }
+            if (more) load(vc, a.c.values, tile + 2);
+        };
+        load(kc, a.c.keys, 0);
+        load(vc, a.c.values, 0);
+        int tile = 0;
+        for (; tile + 2 < n; tile += 2) step(tile, true);
+        step(tile, false);
     }
     den += __shfl_xor(den, 16);
     den += __shfl_xor(den, 32);
@@ -406,44 +468,40 @@ __global__ __launch_bounds__(kWaves * kWave) void k_kv_attend(Attend a)
     float top = s_ref[0][m];
 #pragma unroll
     for (int i = 1; i < kWaves; ++i) top = fmaxf(top, s_ref[i][m]);
-    const float mine = ref == -kInf ? 0.0f : exp2_fast(ref - top);
+    const float mine = exp2_fast(ref - top);
+    const int rows = static_cast<int>(a.rows);
+    if (m < rows) {
 #pragma unroll
-    for (int i = 0; i < CH * 4; ++i) {
-        const f32x4 x = acc[i] * mine;
-        *reinterpret_cast<f32x4*>(&s_out[wave][m][i * 16 + quarter * 4]) = x;
+        for (int i = 0; i < CH * 4; ++i) {
+            *reinterpret_cast<f32x4*>(&s_out[(wave * rows + m) * kRow + i * 16 + quarter * 4]) = acc[i] * mine;
+        }
     }
     __syncthreads();
 
-    const std::uint32_t rows = g.count * a.group;  // rows of the unit
-    for (int i = threadIdx.x; i < 16 * P; i += kWaves * kWave) {
-        const int row = i / P, d = i % P;
+    const std::uint32_t unit_rows = g.count * a.group;
+    for (int i = threadIdx.x; i < rows * (P / 4); i += kWaves * kWave) {
+        const int row = i / (P / 4), d = i % (P / 4) * 4;
         const std::uint32_t rr = row_tile * 16 + row;
-        if (rr >= rows || (a.per == 1 && rr >= a.group)) {
+        if (rr >= unit_rows) {
             continue;
         }
         float top_row = s_ref[0][row];
 #pragma unroll
         for (int k = 1; k < kWaves; ++k) top_row = fmaxf(top_row, s_ref[k][row]);
-        float o = 0.0f, l = 0.0f;
+        f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
+        float l = 0.0f;
 #pragma unroll
         for (int k = 0; k < kWaves; ++k) {
-            o += s_out[k][row][d];
-            l += s_ref[k][row] == -kInf ? s_den[k][row] : s_den[k][row] * exp2_fast(s_ref[k][row] - top_row);
+            o += *reinterpret_cast<const f32x4*>(&s_out[(k * rows + row) * kRow + d]);
+            l = fmaf(s_den[k][row], exp2_fast(s_ref[k][row] - top_row), l);
         }
         if (a.splits == 1) {
-            const std::int64_t tok = g.row + static_cast<std::int64_t>(rr / a.group);
-            const std::uint32_t h = head * a.group + rr % a.group;
-            if (d < static_cast<int>(a.c.dim)) {
-                static_cast<T*>(a.out)[(tok * a.heads + h) * a.c.dim + d] =
-                    from_float<T>(l == 0.0f ? 0.0f : o / l);
-            }
-            if (d == 0 && a.lse != nullptr) {
-                a.lse[tok * a.heads + h] = l == 0.0f ? kInf : top_row + log2f(l);
-            }
+            finish_row<T>(a, g.row + static_cast<std::int64_t>(rr / a.group), head * a.group + rr % a.group, d, o, l,
+                          top_row);
         } else {
             const std::size_t cell =
-                ((static_cast<std::size_t>(unit) * gridDim.y + blockIdx.y) * a.splits + split) * 16 + row;
-            a.partial[cell * P + d] = o;
+                (static_cast<std::size_t>(blockIdx.x) * a.splits + split) * rows + row;
+            *reinterpret_cast<f32x4*>(&a.partial[cell * P + d]) = o;
             if (d == 0) {
                 a.stats[cell * 2] = top_row;
                 a.stats[cell * 2 + 1] = l;
@@ -452,46 +510,69 @@ __global__ __launch_bounds__(kWaves * kWave) void k_kv_attend(Attend a)
     }
 }
 
-// Joins a unit's splits: one workgroup per (unit, kv head, row tile).
+// Joins a unit's splits: one workgroup per (kv head, row tile; unit; row).
+// Its threads first turn the splits' reference exponents into factors, then
+// take dims in fours and the splits in turn.
 template <typename T>
 __global__ __launch_bounds__(256) void k_kv_merge(Attend a)
 {
-    const std::uint32_t unit = blockIdx.x;
-    const std::uint32_t head = blockIdx.y % a.c.kv_heads, row_tile = blockIdx.y / a.c.kv_heads;
-    const int P = static_cast<int>(a.c.dims);
+    constexpr int kChunk = 256;
+    __shared__ float s_factor[kChunk], s_wave[4], s_sum[4];
+    __shared__ f32x4 s_part[256];
+    const std::uint32_t unit = blockIdx.x / a.pairs, pair = blockIdx.x % a.pairs, row = blockIdx.y;
+    const std::uint32_t head = pair % a.c.kv_heads, row_tile = pair / a.c.kv_heads;
+    const int P = static_cast<int>(a.c.dims), lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
     Group g;
     if (!find_group(a.b, unit, a.per, &g)) {
         return;
     }
-    const std::uint32_t live = live_splits(a, visible(a, g.seen + g.count - 1));
-    const std::size_t cell0 = (static_cast<std::size_t>(unit) * gridDim.y + blockIdx.y) * a.splits * 16;
-    for (int i = threadIdx.x; i < 16 * P; i += 256) {
-        const int row = i / P, d = i % P;
-        const std::uint32_t rr = row_tile * 16 + row;
-        if (rr >= g.count * a.group || (a.per == 1 && rr >= a.group)) {
-            continue;
+    const std::uint32_t rr = row_tile * 16 + row;
+    if (rr >= g.count * a.group) {
+        return;
+    }
+    const int live = static_cast<int>(live_splits(a, visible(a, g.seen + g.count - 1)));
+    const std::size_t cell0 = static_cast<std::size_t>(blockIdx.x) * a.splits * a.rows + row;
+    const float2* stats = reinterpret_cast<const float2*>(a.stats);
+    float top = kLowest;
+    for (int s = threadIdx.x; s < live; s += 256) top = fmaxf(top, stats[cell0 + static_cast<std::size_t>(s) * a.rows].x);
+    for (int k = 1; k < kWave; k *= 2) top = fmaxf(top, __shfl_xor(top, k));
+    if (lane == 0) s_wave[wave] = top;
+    __syncthreads();
+    top = fmaxf(fmaxf(s_wave[0], s_wave[1]), fmaxf(s_wave[2], s_wave[3]));
+
+    const int quads = P / 4, groups = 256 / quads;  // threads that share a quad of dims
+    const int d = threadIdx.x % quads * 4, part = threadIdx.x / quads;
+    f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
+    float l = 0.0f;
+    for (int s0 = 0; s0 < live; s0 += kChunk) {
+        const int s = s0 + static_cast<int>(threadIdx.x);
+        float f = 0.0f;
+        if (s < live) {
+            const float2 x = stats[cell0 + static_cast<std::size_t>(s) * a.rows];
+            f = exp2_fast(x.x - top);
+            l = fmaf(x.y, f, l);
         }
-        float top = -kInf;
-        for (std::uint32_t s = 0; s < live; ++s) {
-            top = fmaxf(top, a.stats[(cell0 + s * 16 + row) * 2]);
+        __syncthreads();
+        s_factor[threadIdx.x] = f;
+        __syncthreads();
+        if (part < groups) {
+            const int n = live - s0 < kChunk ? live - s0 : kChunk;
+#pragma unroll 4
+            for (int k = part; k < n; k += groups) {
+                const f32x4 x = *reinterpret_cast<const f32x4*>(
+                    &a.partial[(cell0 + static_cast<std::size_t>(s0 + k) * a.rows) * P + d]);
+                o += x * s_factor[k];
+            }
         }
-        float o = 0.0f, l = 0.0f;
-        for (std::uint32_t s = 0; s < live; ++s) {
-            const std::size_t cell = cell0 + s * 16 + row;
-            const float ref = a.stats[cell * 2];
-            const float f = ref == -kInf ? 1.0f : exp2_fast(ref - top);
-            o = fmaf(a.partial[cell * P + d], f, o);
-            l = fmaf(a.stats[cell * 2 + 1], f, l);
-        }
-        const std::int64_t tok = g.row + static_cast<std::int64_t>(rr / a.group);
-        const std::uint32_t h = head * a.group + rr % a.group;
-        if (d < static_cast<int>(a.c.dim)) {
-            static_cast<T*>(a.out)[(tok * a.heads + h) * a.c.dim + d] =
-                from_float<T>(l == 0.0f ? 0.0f : o / l);
-        }
-        if (d == 0 && a.lse != nullptr) {
-            a.lse[tok * a.heads + h] = l == 0.0f ? kInf : top + log2f(l);
-        }
+    }
+    for (int k = 1; k < kWave; k *= 2) l += __shfl_xor(l, k);
+    if (lane == 0) s_sum[wave] = l;
+    s_part[threadIdx.x] = o;
+    __syncthreads();
+    if (static_cast<int>(threadIdx.x) < quads) {
+        for (int k = 1; k < groups; ++k) o += s_part[threadIdx.x + k * quads];
+        finish_row<T>(a, g.row + static_cast<std::int64_t>(rr / a.group), head * a.group + rr % a.group, d, o,
+                      s_sum[0] + s_sum[1] + s_sum[2] + s_sum[3], top);
     }
 }
 
@@ -503,11 +584,12 @@ template <typename T, int CH>
 __global__ __launch_bounds__(256) void k_kv_weigh(Attend a)
 {
     constexpr int P = CH * 64;
-    const std::uint32_t head = blockIdx.y % a.c.kv_heads, row_tile = blockIdx.y / a.c.kv_heads;
+    const std::uint32_t unit = blockIdx.x / a.pairs, pair = blockIdx.x % a.pairs;
+    const std::uint32_t head = pair % a.c.kv_heads, row_tile = pair / a.c.kv_heads;
     const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
     const int m = lane & 15, quarter = lane >> 4;
     Group g;
-    if (!find_group(a.b, blockIdx.x, a.per, &g)) {
+    if (!find_group(a.b, unit, a.per, &g)) {
         return;
     }
     const std::int64_t seen = visible(a, g.seen + g.count - 1);
@@ -522,30 +604,13 @@ __global__ __launch_bounds__(256) void k_kv_weigh(Attend a)
     const std::int64_t token_row = g.row + static_cast<std::int64_t>(row_token);
     const std::uint32_t q_head = head * a.group + row_head;
     f16x8 query[CH * 2];
-    float factor, lse = kInf;
-    {
-        const T* q = static_cast<const T*>(a.q) + token_row * a.q_token + q_head * a.q_head;
-        float x[CH * 16];
-        float top = 0.0f;
-#pragma unroll
-        for (int i = 0; i < CH * 16; ++i) {
-            const int d = (i / 16) * 64 + quarter * 16 + (i & 15);
-            x[i] = row_live && d < static_cast<int>(a.c.dim) ? to_float(q[d]) : 0.0f;
-            top = fmaxf(top, fabsf(x[i]));
-        }
-        top = fmaxf(top, __shfl_xor(top, 16));
-        top = fmaxf(top, __shfl_xor(top, 32));
-        const int k = top > 0.0f && top < kInf ? 14 - ilogbf(top) : 0;
-        factor = ldexpf(a.scale, -k);
-#pragma unroll
-        for (int i = 0; i < CH * 16; ++i) query[i / 8][i % 8] = static_cast<_Float16>(ldexpf(x[i], k));
-        if (row_live) {
-            lse = a.lse[token_row * a.heads + q_head];
-        }
-    }
+    float factor;
+    load_query<T, CH>(a, static_cast<const T*>(a.q) + token_row * a.q_token + q_head * a.q_head, row_live, quarter,
+                      query, &factor);
+    const float lse = row_live ? a.lse[token_row * a.heads + q_head] : kInf;
     const std::size_t head_bytes = static_cast<std::size_t>(a.c.tokens) * P;
     const std::uint32_t nb = static_cast<std::uint32_t>((seen + a.c.tokens - 1) / a.c.tokens);
-    for (std::uint32_t blk = blockIdx.z * 4 + wave; blk < nb; blk += gridDim.z * 4) {
+    for (std::uint32_t blk = blockIdx.y * 4 + wave; blk < nb; blk += gridDim.y * 4) {
         const std::int32_t id = block_at(a.c, a.b, g.seq, blk);
         if (id < 0) {
             continue;
@@ -1096,7 +1161,7 @@ bool two_byte(std::uint32_t type) { return type == HBFSIM_AMD_KV_BF16 || type ==
 
 // How attend cuts its work: from the call's host-side sizes alone.
 struct Cut {
-    std::uint32_t per, row_tiles, units, split, splits;
+    std::uint32_t per, row_tiles, rows, units, split, splits;
     std::size_t partial, stats, lse, bytes;
 };
 
@@ -1108,6 +1173,7 @@ Cut cut_attend(const Cache& c, const Batch& b, std::uint32_t heads, std::uint32_
     const std::uint32_t group = heads / c.kv_heads;
     k.per = b.first == nullptr || count != 0 || group > 8 ? 1 : 16 / group;
     k.row_tiles = group > 16 ? (group + 15) / 16 : 1;
+    k.rows = k.per * group < 16 ? k.per * group : 16;
     k.units = b.first == nullptr ? b.seqs : b.tokens / k.per + b.seqs;
     const std::uint64_t longest = static_cast<std::uint64_t>(count != 0 ? count : b.width) * c.tokens;
     const std::uint64_t pairs = static_cast<std::uint64_t>(k.units) * c.kv_heads * k.row_tiles;
@@ -1116,7 +1182,7 @@ Cut cut_attend(const Cache& c, const Batch& b, std::uint32_t heads, std::uint32_
     k.split = static_cast<std::uint32_t>(split);
     k.splits = longest == 0 ? 1 : static_cast<std::uint32_t>((longest + split - 1) / split);
     if (k.splits > 1) {
-        const std::size_t cells = static_cast<std::size_t>(pairs) * k.splits * 16;
+        const std::size_t cells = static_cast<std::size_t>(pairs) * k.splits * k.rows;
         k.stats = up256(cells * c.dims * sizeof(float));
         k.lse = k.stats + up256(cells * 2 * sizeof(float));
     }
@@ -1127,14 +1193,15 @@ Cut cut_attend(const Cache& c, const Batch& b, std::uint32_t heads, std::uint32_
 template <typename T, int CH>
 void launch_attend(const Attend& a, const Cut& k, bool accumulate, hipStream_t stream)
 {
-    const dim3 grid(k.units, a.c.kv_heads * k.row_tiles, k.splits);
-    hipLaunchKernelGGL((k_kv_attend<T, CH, 4>), grid, dim3(256), 0, stream, a);
+    const std::uint32_t groups = k.units * a.pairs;
+    const std::size_t lds = 4 * k.rows * (CH * 64 + 4) * sizeof(float);
+    hipLaunchKernelGGL((k_kv_attend<T, CH, 4>), dim3(groups, k.splits), dim3(256), lds, stream, a);
     if (k.splits > 1) {
-        hipLaunchKernelGGL((k_kv_merge<T>), dim3(k.units, grid.y), dim3(256), 0, stream, a);
+        hipLaunchKernelGGL((k_kv_merge<T>), dim3(groups, k.rows), dim3(256), 0, stream, a);
     }
     if (accumulate && a.b.width != 0) {
         const std::uint32_t z = a.b.width / 64 < 65535 ? (a.b.width + 63) / 64 : 65535;
-        hipLaunchKernelGGL((k_kv_weigh<T, CH>), dim3(k.units, grid.y, z), dim3(256), 0, stream, a);
+        hipLaunchKernelGGL((k_kv_weigh<T, CH>), dim3(groups, z), dim3(256), 0, stream, a);
     }
 }
 
@@ -1273,7 +1340,7 @@ HBF_API int hbfsim_amd_kv_attend(const hbfsim_amd_kv_cache* cache, const hbfsim_
         (k.bytes != 0 && (d_workspace == nullptr || !aligned16(d_workspace)))) {
         return HBFSIM_INVALID_ARGUMENT;
     }
-    if (k.units > kMostGroups || k.splits > 65535 || a.c.kv_heads * k.row_tiles > 65535) {
+    if (static_cast<std::uint64_t>(k.units) * a.c.kv_heads * k.row_tiles > kMostGroups || k.splits > 65535) {
         return HBFSIM_UNSUPPORTED;
     }
     a.q = d_q;
@@ -1284,6 +1351,8 @@ HBF_API int hbfsim_amd_kv_attend(const hbfsim_amd_kv_cache* cache, const hbfsim_
     a.group = heads / a.c.kv_heads;
     a.per = k.per;
     a.row_tiles = k.row_tiles;
+    a.rows = k.rows;
+    a.pairs = a.c.kv_heads * k.row_tiles;
     a.scale = scale * kLog2e;
     a.selected = d_selected;
     a.count = count;
