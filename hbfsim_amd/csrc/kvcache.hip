@@ -35,6 +35,7 @@
 
 #include <cstddef>
 #include <cstdint>
+#include <type_traits>
 
 namespace {
 
@@ -200,6 +201,7 @@ struct Attend {
     const void* q;
     std::int64_t q_token, q_head;  // strides in elements
     std::uint32_t q_vector;        // rows may be loaded 16 bytes at a time
+    std::uint32_t out_vector;      // and stored 8 at a time
     std::uint32_t heads, group;    // query heads; query heads per kv head
     std::uint32_t per;             // tokens per unit
     std::uint32_t row_tiles;       // 16-row tiles per unit (1 unless group > 16)
@@ -237,9 +239,19 @@ __device__ inline void finish_row(const Attend& a, std::int64_t token, std::uint
 {
     T* out = static_cast<T*>(a.out) + (token * a.heads + head) * a.c.dim + d;
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    union {
+        uint2 v;
+        T e[4];
+    } u;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        if (d + i < static_cast<int>(a.c.dim)) out[i] = from_float<T>(l == 0.0f ? 0.0f : o[i] * inv);
+    for (int i = 0; i < 4; ++i) u.e[i] = from_float<T>(l == 0.0f ? 0.0f : o[i] * inv);
+    if ((a.c.dim & 3) == 0 && a.out_vector != 0) {
+        if (d < static_cast<int>(a.c.dim)) *reinterpret_cast<uint2*>(out) = u.v;
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if (d + i < static_cast<int>(a.c.dim)) out[i] = u.e[i];
+        }
     }
     if (d == 0 && a.lse != nullptr) {
         a.lse[token * a.heads + head] = l == 0.0f ? kInf : ref + log2f(l);
@@ -250,26 +262,29 @@ __device__ inline void finish_row(const Attend& a, std::int64_t token, std::uint
 // holds row m's dims 16 quarter .. 16 quarter + 15 of every 64, scaled by a
 // power of two; *factor undoes it and applies the softmax scale.
 template <typename T, int CH>
-__device__ inline void load_query(const Attend& a, const T* q, bool live, int quarter, f16x8 (&query)[CH * 2],
-                                  float* factor)
+__device__ inline void load_query(const Attend& a, std::int64_t token, std::uint32_t head, bool live, int quarter,
+                                  f16x8 (&query)[CH * 2], float* factor)
 {
+    // rows that are not there read the batch's first one and take zeros
+    const T* q = static_cast<const T*>(a.q) + (live ? token * a.q_token + head * a.q_head : 0);
     float x[CH * 16];
     float top = 0.0f;
 #pragma unroll
     for (int i = 0; i < CH * 2; ++i) {
-        const int d0 = (i / 2) * 64 + quarter * 16 + (i & 1) * 8;
-        if (live && a.q_vector != 0 && d0 + 8 <= static_cast<int>(a.c.dim)) {
+        const int d0 = (i / 2) * 64 + quarter * 16 + (i & 1) * 8, dim = static_cast<int>(a.c.dim);
+        if (a.q_vector != 0 && dim % 8 == 0) {
             union {
                 u32x4 v;
                 T e[8];
             } u;
-            u.v = *reinterpret_cast<const u32x4*>(q + d0);
+            u.v = *reinterpret_cast<const u32x4*>(q + (d0 < dim ? d0 : 0));
 #pragma unroll
-            for (int j = 0; j < 8; ++j) x[i * 8 + j] = to_float(u.e[j]);
+            for (int j = 0; j < 8; ++j) x[i * 8 + j] = live && d0 < dim ? to_float(u.e[j]) : 0.0f;
         } else {
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                x[i * 8 + j] = live && d0 + j < static_cast<int>(a.c.dim) ? to_float(q[d0 + j]) : 0.0f;
+                const float e = to_float(q[d0 + j < dim ? d0 + j : 0]);
+                x[i * 8 + j] = live && d0 + j < dim ? e : 0.0f;
             }
         }
 #pragma unroll
@@ -277,12 +292,16 @@ __device__ inline void load_query(const Attend& a, const T* q, bool live, int qu
     }
     top = fmaxf(top, __shfl_xor(top, 16));
     top = fmaxf(top, __shfl_xor(top, 32));
-    const int k = top > 0.0f && top < kInf ? 14 - ilogbf(top) : 0;
-    *factor = ldexpf(a.scale, -k);
+    // below 2^-46 a row's scores are nothing beside one another's rounding
+    int k = top > 0.0f && top < kInf ? 14 - ilogbf(top) : 0;
+    k = k > 60 ? 60 : k;
+    // the softmax scale's sign goes to the rows, so that the factor is positive
+    const float sign = a.scale < 0.0f ? -1.0f : a.scale == 0.0f ? 0.0f : 1.0f;
+    *factor = fmaxf(ldexpf(fabsf(a.scale), -k), 0x1p-80f);
 #pragma unroll
     for (int i = 0; i < CH * 2; ++i) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) query[i][j] = static_cast<_Float16>(ldexpf(x[i * 8 + j], k));
+        for (int j = 0; j < 8; ++j) query[i][j] = static_cast<_Float16>(ldexpf(sign * x[i * 8 + j], k));
     }
 }
 
@@ -305,7 +324,11 @@ __device__ inline Tiles load_tiles(const Attend& a, std::uint32_t seq, std::uint
         if (id >= 0 && pos < seen) {
             const std::size_t bh = static_cast<std::size_t>(id) * a.c.kv_heads + head;
             const float vs = a.c.value_scale[bh];
-            t = Tiles{id, sub, static_cast<std::int32_t>(pos), a.c.key_scale[bh], log2f(vs), 1.0f / vs};
+            const float ks = a.c.key_scale[bh];
+            // a NaN value scale shows through its logarithm in the rows that
+            // see the block, and through nothing in those that do not
+            t = Tiles{id, sub, static_cast<std::int32_t>(pos), ks < kScaleMin ? kScaleMin : ks, log2f(vs),
+                      vs == vs ? 1.0f / vs : 1.0f};
         }
     }
     return t;
@@ -355,8 +378,7 @@ __global__ __launch_bounds__(kWaves * kWave) void k_kv_attend(Attend a)
 
     f16x8 query[CH * 2];
     float factor;
-    load_query<T, CH>(a, static_cast<const T*>(a.q) + token_row * a.q_token + (head * a.group + row_head) * a.q_head,
-                      row_live, quarter, query, &factor);
+    load_query<T, CH>(a, token_row, head * a.group + row_head, row_live, quarter, query, &factor);
 
     f32x4 acc[CH * 4];
 #pragma unroll
@@ -438,8 +460,7 @@ __global__ __launch_bounds__(kWaves * kWave) void k_kv_attend(Attend a)
                     sum += x;
                     w[u * 4 + i] = static_cast<_Float16>(x);
                 }
-                // a block of NaN scale reaches only the rows that see some of it
-                den = sum != 0.0f ? fmaf(sum, lane_float(info.inv_scale, tile + u), den) : den;
+                den = fmaf(sum, lane_float(info.inv_scale, tile + u), den);
             }
 #pragma unroll
             for (int i = 0; i < CH; ++i) {
@@ -510,6 +531,304 @@ __global__ __launch_bounds__(kWaves * kWave) void k_kv_attend(Attend a)
     }
 }
 
+// attend for chunks of many tokens, where the matrix units and the softmax's
+// vector work bound it and not memory.  A workgroup of four waves takes
+// 4 * RT * 16 query rows of one kv head (consecutive tokens, every head of the
+// group) and one split; the waves share the cache's tiles, which they widen to
+// f16 once for all of them and keep in LDS in lane order (a 16-byte read per
+// lane per operand, free of conflicts, two buffers), and each keeps RT tiles of
+// 16 rows in registers, so that an operand read serves RT products.
+template <typename T, int CH, int RT>
+__global__ __launch_bounds__(256, 2) void k_kv_attend_many(Attend a)
+{
+    constexpr int P = CH * 64;
+    constexpr int kTiles = CH <= 2 ? 4 : 2;            // 16-token tiles per stage
+    constexpr int kKeys = kTiles * CH, kValues = kTiles / 2 * CH;
+    constexpr int kKeysEach = (kKeys + 3) / 4, kValuesEach = (kValues + 3) / 4;
+    constexpr int kKeyBytes = kTiles * CH * 2048, kStage = 2 * kKeyBytes;
+    extern __shared__ unsigned char s_stage[];        // [2][kStage]: keys, then values
+
+    const std::uint32_t split = blockIdx.y;
+    // the last tokens of a chunk see the most: they start first
+    const std::uint32_t block = gridDim.x - 1 - blockIdx.x;
+    const std::uint32_t unit = block / a.pairs, head = block % a.pairs;
+    const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    const int m = lane & 15, quarter = lane >> 4;
+
+    Group g;
+    if (!find_group(a.b, unit, a.per, &g)) {
+        return;
+    }
+    const std::int64_t seen = visible(a, g.seen + g.count - 1);
+    const std::uint32_t live = live_splits(a, seen);
+    if (split >= live && !(split == 0 && a.splits == 1)) {
+        return;
+    }
+
+    f16x8 query[RT][CH * 2];
+    float factor[RT], ref[RT], den[RT];
+    int limit[RT];
+    int least = 0x7fffffff, most = 0;
+    f32x4 acc[RT][CH * 4];
+#pragma unroll
+    for (int k = 0; k < RT; ++k) {
+        const std::uint32_t r = (wave * RT + k) * 16 + m;
+        const std::uint32_t row_token = r / a.group, row_head = r % a.group;
+        const bool row_live = row_token < static_cast<std::uint32_t>(g.count);
+        const std::int64_t limit64 = row_live ? visible(a, g.seen + row_token) : 0;
+        limit[k] = limit64 > 0 ? static_cast<int>(limit64) : 0;
+        least = row_live && limit[k] < least ? limit[k] : least;
+        most = limit[k] > most ? limit[k] : most;
+        load_query<T, CH>(a, g.row + static_cast<std::int64_t>(row_token), head * a.group + row_head, row_live, quarter,
+                          query[k], &factor[k]);
+        ref[k] = kLowest;
+        den[k] = 0.0f;
+#pragma unroll
+        for (int i = 0; i < CH * 4; ++i) acc[k][i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    }
+#pragma unroll
+    for (int k = 1; k < kWave; k *= 2) {
+        const int x = __shfl_xor(least, k), y = __shfl_xor(most, k);
+        least = x < least ? x : least;
+        most = y > most ? y : most;
+    }
+    least = __builtin_amdgcn_readfirstlane(least);
+    most = __builtin_amdgcn_readfirstlane(most);
+
+    const std::int64_t begin = static_cast<std::int64_t>(split) * a.split;
+    const std::int64_t end = begin + a.split < seen ? begin + a.split : seen;
+    const std::int64_t tiles = end > begin ? (end - begin + 15) / 16 : 0;
+    const std::int64_t stages = (tiles + kTiles - 1) / kTiles;
+    const std::size_t head_bytes = static_cast<std::size_t>(a.c.tokens) * P;
+
+    Tiles info, seen_info;  // of the stages being fetched, and of those being computed
+    u32x4 kreg[kKeysEach], vreg[kValuesEach][2];
+    const auto look_up = [&](std::int64_t stage) {  // the 64 tiles from this stage on
+        const std::int64_t at = stage * kTiles + lane;
+        info = load_tiles(a, g.seq, head, nullptr, begin / 16 + at, at < tiles, seen);
+    };
+    const auto tile_at = [&](const std::int8_t* pool, int tile) {
+        const std::size_t bh = static_cast<std::size_t>(lane_int(info.id, tile)) * a.c.kv_heads + head;
+        return reinterpret_cast<const u32x4*>(pool + bh * head_bytes +
+                                              static_cast<std::size_t>(lane_int(info.sub, tile)) * 16 * P);
+    };
+    const auto fetch = [&](std::int64_t stage) {
+        const int t0 = static_cast<int>(stage % (kWave / kTiles)) * kTiles;
+#pragma unroll
+        for (int k = 0; k < kKeysEach; ++k) {
+            const int u = wave + 4 * k;
+            if (u < kKeys) kreg[k] = tile_at(a.c.keys, t0 + u / CH)[u % CH * kWave + lane];
+        }
+#pragma unroll
+        for (int k = 0; k < kValuesEach; ++k) {
+            const int u = wave + 4 * k;
+            if (u < kValues) {
+                vreg[k][0] = tile_at(a.c.values, t0 + u / CH * 2)[u % CH * kWave + lane];
+                vreg[k][1] = tile_at(a.c.values, t0 + u / CH * 2 + 1)[u % CH * kWave + lane];
+            }
+        }
+    };
+    const auto put = [&](std::int64_t stage) {
+        f16x8* keys = reinterpret_cast<f16x8*>(s_stage + (stage & 1) * kStage);
+        f16x8* values = keys + kKeyBytes / 16;
+#pragma unroll
+        for (int k = 0; k < kKeysEach; ++k) {
+            const int u = wave + 4 * k;
+            if (u < kKeys) {
+                keys[(2 * u) * kWave + lane] = widen8(kreg[k].x, kreg[k].y);
+                keys[(2 * u + 1) * kWave + lane] = widen8(kreg[k].z, kreg[k].w);
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < kValuesEach; ++k) {
+            const int u = wave + 4 * k;
+            if (u < kValues) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) values[(4 * u + j) * kWave + lane] = widen8(vreg[k][0][j], vreg[k][1][j]);
+            }
+        }
+    };
+    const auto compute = [&](std::int64_t stage) __attribute__((always_inline)) {
+        const int t0 = static_cast<int>(stage % (kWave / kTiles)) * kTiles;
+        const f16x8* keys = reinterpret_cast<const f16x8*>(s_stage + (stage & 1) * kStage) + lane;
+        const f16x8* values = keys + kKeyBytes / 16;
+#pragma unroll 1
+        for (int tile = t0; tile < t0 + kTiles; tile += 2) {
+            f32x4 s[2][RT];
+            float f[2], e[2];
+            int pos[2];
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                pos[u] = lane_int(seen_info.pos, tile + u);
+                f[u] = lane_float(seen_info.key_scale, tile + u);
+                e[u] = lane_float(seen_info.log_scale, tile + u);
+#pragma unroll
+                for (int k = 0; k < RT; ++k) s[u][k] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int i = 0; i < CH * 2; ++i) {
+                    const f16x8 key = keys[(u * CH * 2 + i) * kWave];
+#pragma unroll
+                    for (int k = 0; k < RT; ++k) s[u][k] = __builtin_amdgcn_mfma_f32_16x16x32_f16(key, query[k][i], s[u][k], 0, 0, 0);
+                }
+            }
+            const bool whole = (pos[0] > pos[1] ? pos[0] : pos[1]) + 16 <= least;
+            float scale[2][RT], shift[2][RT];
+#pragma unroll
+            for (int k = 0; k < RT; ++k) {
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    scale[u][k] = factor[k] * f[u];
+                    shift[u][k] = e[u];
+                }
+            }
+            // Scores of tokens that a row does not see become -inf; a tile of
+            // NaN scales does not reach the rows that see none of it.
+            if (!whole) {
+#pragma unroll
+                for (int k = 0; k < RT; ++k) {
+#pragma unroll
+                    for (int u = 0; u < 2; ++u) {
+                        const int left = limit[k] - pos[u] - quarter * 4;
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) s[u][k][i] = i < left ? s[u][k][i] : -kInf;
+                        scale[u][k] = pos[u] < limit[k] ? scale[u][k] : 1.0f;
+                        shift[u][k] = pos[u] < limit[k] ? shift[u][k] : 0.0f;
+                    }
+                }
+            }
+            float top[RT];
+            bool move = false;
+#pragma unroll
+            for (int k = 0; k < RT; ++k) {
+                float x[2];
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    x[u] = fmaf(fmaxf(fmaxf(s[u][k][0], s[u][k][1]), fmaxf(s[u][k][2], s[u][k][3])), scale[u][k], shift[u][k]);
+                }
+                top[k] = fmaxf(x[0], x[1]);
+                move |= top[k] > ref[k] + 15.0f;
+            }
+            if (__any(move)) {
+#pragma unroll
+                for (int k = 0; k < RT; ++k) {
+                    float t = fmaxf(top[k], __shfl_xor(top[k], 16));
+                    t = fmaxf(t, __shfl_xor(t, 32));
+                    const float next = fmaxf(ref[k], t - 7.0f);
+                    const float shrink = exp2_fast(ref[k] - next);
+                    ref[k] = next;
+                    den[k] *= shrink;
+#pragma unroll
+                    for (int i = 0; i < CH * 4; ++i) acc[k][i] *= shrink;
+                }
+            }
+            f16x8 w[RT];
+#pragma unroll
+            for (int k = 0; k < RT; ++k) {
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    const float from = shift[u][k] - ref[k];
+                    float x[4];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        x[i] = exp2_fast(fmaf(s[u][k][i], scale[u][k], from));
+                        w[k][u * 4 + i] = static_cast<_Float16>(x[i]);
+                    }
+                    const float sum = (x[0] + x[1]) + (x[2] + x[3]);
+                    den[k] = fmaf(sum, lane_float(seen_info.inv_scale, tile + u), den[k]);
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < CH * 4; ++i) {
+                const f16x8 value = values[i * kWave];
+#pragma unroll
+                for (int k = 0; k < RT; ++k) acc[k][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(value, w[k], acc[k][i], 0, 0, 0);
+            }
+            keys += CH * 4 * kWave;
+            values += CH * 4 * kWave;
+        }
+    };
+    if (stages > 0) {
+        look_up(0);
+        fetch(0);
+        put(0);
+        if (stages > 1) fetch(1);
+        seen_info = info;
+    }
+    __syncthreads();
+    for (std::int64_t stage = 0; stage < stages; ++stage) {
+        if (stage % (kWave / kTiles) == 0) seen_info = info;
+        if (stage + 1 < stages) put(stage + 1);
+        if (stage + 2 < stages) {
+            if ((stage + 2) % (kWave / kTiles) == 0) look_up(stage + 2);
+            fetch(stage + 2);
+        }
+        compute(stage);
+        __syncthreads();
+    }
+
+#pragma unroll
+    for (int k = 0; k < RT; ++k) {
+        den[k] += __shfl_xor(den[k], 16);
+        den[k] += __shfl_xor(den[k], 32);
+        const std::uint32_t r = (wave * RT + k) * 16 + m;
+        if (r >= g.count * a.group) {
+            continue;
+        }
+        if (a.splits == 1) {
+            const std::int64_t token = g.row + static_cast<std::int64_t>(r / a.group);
+            const std::uint32_t h = head * a.group + r % a.group;
+#pragma unroll
+            for (int i = 0; i < CH * 4; ++i) finish_row<T>(a, token, h, i * 16 + quarter * 4, acc[k][i], den[k], ref[k]);
+        } else {
+            const std::size_t cell = (static_cast<std::size_t>(block) * a.splits + split) * a.rows + r;
+#pragma unroll
+            for (int i = 0; i < CH * 4; ++i) {
+                *reinterpret_cast<f32x4*>(&a.partial[cell * P + i * 16 + quarter * 4]) = acc[k][i];
+            }
+            if (quarter == 0) {
+                a.stats[cell * 2] = ref[k];
+                a.stats[cell * 2 + 1] = den[k];
+            }
+        }
+    }
+}
+
+// Joins a unit's splits where there are few of them: a thread takes four dims
+// of a row and goes through the splits, a workgroup as many rows as fit.
+template <typename T>
+__global__ __launch_bounds__(256) void k_kv_merge_few(Attend a)
+{
+    const std::uint32_t unit = blockIdx.x / a.pairs, pair = blockIdx.x % a.pairs;
+    const std::uint32_t head = pair % a.c.kv_heads, row_tile = pair / a.c.kv_heads;
+    const std::uint32_t quads = a.c.dims / 4, groups = 256 / quads;
+    const std::uint32_t row = blockIdx.y * groups + threadIdx.x / quads, d = threadIdx.x % quads * 4;
+    Group g;
+    if (!find_group(a.b, unit, a.per, &g)) {
+        return;
+    }
+    const std::uint32_t rr = row_tile * 16 + row;
+    if (threadIdx.x >= groups * quads || row >= a.rows || rr >= g.count * a.group) {
+        return;
+    }
+    const int live = static_cast<int>(live_splits(a, visible(a, g.seen + g.count - 1)));
+    const std::size_t cell0 = static_cast<std::size_t>(blockIdx.x) * a.splits * a.rows + row;
+    const float2* stats = reinterpret_cast<const float2*>(a.stats) + cell0;
+    const float* partial = a.partial + cell0 * a.c.dims + d;
+    float top = kLowest;
+    for (int s = 0; s < live; ++s) top = fmaxf(top, stats[static_cast<std::size_t>(s) * a.rows].x);
+    f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
+    float l = 0.0f;
+#pragma unroll 4
+    for (int s = 0; s < live; ++s) {
+        const float2 x = stats[static_cast<std::size_t>(s) * a.rows];
+        const float f = exp2_fast(x.x - top);
+        o += *reinterpret_cast<const f32x4*>(partial + static_cast<std::size_t>(s) * a.rows * a.c.dims) * f;
+        l = fmaf(x.y, f, l);
+    }
+    finish_row<T>(a, g.row + static_cast<std::int64_t>(rr / a.group), head * a.group + rr % a.group, static_cast<int>(d),
+                  o, l, top);
+}
+
 // Joins a unit's splits: one workgroup per (kv head, row tile; unit; row).
 // Its threads first turn the splits' reference exponents into factors, then
 // take dims in fours and the splits in turn.
@@ -526,7 +845,7 @@ __global__ __launch_bounds__(256) void k_kv_merge(Attend a)
     if (!find_group(a.b, unit, a.per, &g)) {
         return;
     }
-    const std::uint32_t rr = row_tile * 16 + row;
+    const std::uint32_t rr = row_tile * 16 + row;  // row tiles are whole where there are several
     if (rr >= g.count * a.group) {
         return;
     }
@@ -605,8 +924,7 @@ __global__ __launch_bounds__(256) void k_kv_weigh(Attend a)
     const std::uint32_t q_head = head * a.group + row_head;
     f16x8 query[CH * 2];
     float factor;
-    load_query<T, CH>(a, static_cast<const T*>(a.q) + token_row * a.q_token + q_head * a.q_head, row_live, quarter,
-                      query, &factor);
+    load_query<T, CH>(a, token_row, q_head, row_live, quarter, query, &factor);
     const float lse = row_live ? a.lse[token_row * a.heads + q_head] : kInf;
     const std::size_t head_bytes = static_cast<std::size_t>(a.c.tokens) * P;
     const std::uint32_t nb = static_cast<std::uint32_t>((seen + a.c.tokens - 1) / a.c.tokens);
@@ -1161,13 +1479,17 @@ bool two_byte(std::uint32_t type) { return type == HBFSIM_AMD_KV_BF16 || type ==
 
 // How attend cuts its work: from the call's host-side sizes alone.
 struct Cut {
+    std::uint32_t many;  // row tiles per wave of the many-row form, or 0
     std::uint32_t per, row_tiles, rows, units, split, splits;
     std::size_t partial, stats, lse, bytes;
 };
 
 std::size_t up256(std::size_t x) { return (x + 255) & ~std::size_t{255}; }
 
-Cut cut_attend(const Cache& c, const Batch& b, std::uint32_t heads, std::uint32_t count, bool accumulate)
+// Row tiles per wave that fit the registers of two waves per SIMD.
+std::uint32_t many_tiles(std::uint32_t dims) { return dims <= 64 ? 3 : dims <= 128 ? 3 : 1; }
+
+Cut cut_few(const Cache& c, const Batch& b, std::uint32_t heads, std::uint32_t count)
 {
     Cut k{};
     const std::uint32_t group = heads / c.kv_heads;
@@ -1181,8 +1503,50 @@ Cut cut_attend(const Cache& c, const Batch& b, std::uint32_t heads, std::uint32_
     while (split > 256 && pairs * ((longest + split - 1) / split) < 1024) split /= 2;
     k.split = static_cast<std::uint32_t>(split);
     k.splits = longest == 0 ? 1 : static_cast<std::uint32_t>((longest + split - 1) / split);
+    return k;
+}
+
+Cut cut_many(const Cache& c, const Batch& b, std::uint32_t heads)
+{
+    Cut k{};
+    const std::uint32_t group = heads / c.kv_heads;
+    k.many = many_tiles(c.dims);
+    const std::uint32_t room = 4 * k.many * 16;
+    k.per = room / group;
+    k.row_tiles = 1;
+    k.rows = k.per * group;
+    k.units = b.tokens / k.per + b.seqs;
+    const std::uint64_t longest = static_cast<std::uint64_t>(b.width) * c.tokens;
+    const std::uint64_t groups = static_cast<std::uint64_t>(k.units) * c.kv_heads;
+    // Two workgroups fit a CU; splits fill the last round of them, each at
+    // the price of its partial sums' round trip.
+    std::uint64_t best = 1;
+    double score = 0.0;
+    for (std::uint64_t s = 1; s <= 8 && (s == 1 || longest / s >= 512); ++s) {
+        const double rounds = static_cast<double>(groups * s) / 512.0;
+        const double whole = static_cast<double>(static_cast<std::uint64_t>((groups * s + 511) / 512));
+        const double got = rounds / whole / (1.0 + 0.03 * static_cast<double>(s - 1));
+        if (got > score * 1.02) {
+            score = got;
+            best = s;
+        }
+    }
+    const std::uint64_t split = longest == 0 ? 64 : ((longest + best - 1) / best + 63) / 64 * 64;
+    k.split = static_cast<std::uint32_t>(split);
+    k.splits = longest == 0 ? 1 : static_cast<std::uint32_t>((longest + split - 1) / split);
+    return k;
+}
+
+Cut cut_attend(const Cache& c, const Batch& b, std::uint32_t heads, std::uint32_t count, bool accumulate)
+{
+    const std::uint32_t group = heads / c.kv_heads;
+    // Many rows once a sequence's share of the step fills half a workgroup's.
+    const std::uint64_t room = 4 * many_tiles(c.dims) * 16;
+    const bool many = b.first != nullptr && count == 0 && group <= room &&
+                      static_cast<std::uint64_t>(b.tokens) * group * 2 >= room * b.seqs;
+    Cut k = many ? cut_many(c, b, heads) : cut_few(c, b, heads, count);
     if (k.splits > 1) {
-        const std::size_t cells = static_cast<std::size_t>(pairs) * k.splits * k.rows;
+        const std::size_t cells = static_cast<std::size_t>(k.units) * c.kv_heads * k.row_tiles * k.splits * k.rows;
         k.stats = up256(cells * c.dims * sizeof(float));
         k.lse = k.stats + up256(cells * 2 * sizeof(float));
     }
@@ -1191,17 +1555,30 @@ Cut cut_attend(const Cache& c, const Batch& b, std::uint32_t heads, std::uint32_
 }
 
 template <typename T, int CH>
-void launch_attend(const Attend& a, const Cut& k, bool accumulate, hipStream_t stream)
+void launch_attend(Attend a, const Cut& k, bool accumulate, hipStream_t stream)
 {
+    constexpr int RT = CH == 1 ? 3 : CH == 2 ? 3 : 1;
     const std::uint32_t groups = k.units * a.pairs;
-    const std::size_t lds = 4 * k.rows * (CH * 64 + 4) * sizeof(float);
-    hipLaunchKernelGGL((k_kv_attend<T, CH, 4>), dim3(groups, k.splits), dim3(256), lds, stream, a);
-    if (k.splits > 1) {
+    if (k.many != 0) {
+        const std::size_t lds = (CH <= 2 ? 32 : 16) * 1024 * CH;
+        hipLaunchKernelGGL((k_kv_attend_many<T, CH, RT>), dim3(groups, k.splits), dim3(256), lds, stream, a);
+    } else {
+        const std::size_t lds = 4 * k.rows * (CH * 64 + 4) * sizeof(float);
+        hipLaunchKernelGGL((k_kv_attend<T, CH, 4>), dim3(groups, k.splits), dim3(256), lds, stream, a);
+    }
+    if (k.splits > 16) {
         hipLaunchKernelGGL((k_kv_merge<T>), dim3(groups, k.rows), dim3(256), 0, stream, a);
+    } else if (k.splits > 1) {
+        const std::uint32_t at_once = 1024 / a.c.dims;
+        hipLaunchKernelGGL((k_kv_merge_few<T>), dim3(groups, (k.rows + at_once - 1) / at_once), dim3(256), 0, stream, a);
     }
     if (accumulate && a.b.width != 0) {
+        const Cut few = cut_few(a.c, a.b, a.heads, 0);
+        a.per = few.per;
+        a.row_tiles = few.row_tiles;
+        a.pairs = a.c.kv_heads * few.row_tiles;
         const std::uint32_t z = a.b.width / 64 < 65535 ? (a.b.width + 63) / 64 : 65535;
-        hipLaunchKernelGGL((k_kv_weigh<T, CH>), dim3(groups, z), dim3(256), 0, stream, a);
+        hipLaunchKernelGGL((k_kv_weigh<T, CH>), dim3(few.units * a.pairs, z), dim3(256), 0, stream, a);
     }
 }
 
@@ -1340,13 +1717,16 @@ HBF_API int hbfsim_amd_kv_attend(const hbfsim_amd_kv_cache* cache, const hbfsim_
         (k.bytes != 0 && (d_workspace == nullptr || !aligned16(d_workspace)))) {
         return HBFSIM_INVALID_ARGUMENT;
     }
-    if (static_cast<std::uint64_t>(k.units) * a.c.kv_heads * k.row_tiles > kMostGroups || k.splits > 65535) {
+    const Cut few = cut_few(a.c, a.b, heads, count);
+    if (static_cast<std::uint64_t>(k.units) * a.c.kv_heads * k.row_tiles > kMostGroups || k.splits > 65535 ||
+        (accumulate != 0 && static_cast<std::uint64_t>(few.units) * a.c.kv_heads * few.row_tiles > kMostGroups)) {
         return HBFSIM_UNSUPPORTED;
     }
     a.q = d_q;
     a.q_token = token_stride;
     a.q_head = head_stride;
     a.q_vector = aligned16(d_q) && token_stride % 8 == 0 && head_stride % 8 == 0 ? 1 : 0;
+    a.out_vector = (reinterpret_cast<std::uintptr_t>(d_out) & 7u) == 0 ? 1 : 0;
     a.heads = heads;
     a.group = heads / a.c.kv_heads;
     a.per = k.per;
