@@ -40,6 +40,7 @@
 namespace {
 
 constexpr int kWave = 64;
+constexpr int kPickThreads = 1024;  // of a workgroup that chooses blocks
 constexpr float kInv127 = 1.0f / 127.0f;
 constexpr float kScaleMin = 0x1p-40f;
 constexpr float kScaleMax = 0x1p40f;
@@ -53,6 +54,7 @@ typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef std::int32_t i32x4 __attribute__((ext_vector_type(4)));
 typedef std::uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
 struct Bf16 {
@@ -1156,63 +1158,128 @@ __global__ __launch_bounds__(256) void k_kv_read(Cache c, const std::int32_t* id
 
 // ---- select and evict -----------------------------------------------------
 
-// The keys of the `want` largest of n (want < n; ties to the lower index):
-// *threshold is the smallest of them, and the call returns how many of those
-// equal to it are taken.  A workgroup's threads all call it; `key(i)` is read
-// once per digit.
-template <typename K, int kThreads, typename F>
-__device__ std::uint32_t radix_threshold(F key, std::uint32_t n, std::uint32_t want, K* threshold)
+// The `want` largest of the n keys of a workgroup (want <= n; ties to the
+// lower index): those above *threshold, and as many equal to it as the call
+// returns.  All threads call it after a barrier behind the keys' stores.
+// Digits of 8 bits from the highest bit in which two keys differ, a histogram
+// of the keys that still match each, its suffix sums by one wave; it ends as
+// soon as a digit's keys are all taken.
+template <typename K, int kThreads>
+__device__ std::uint32_t pick_threshold(const K* keys, std::uint32_t n, std::uint32_t want, K* threshold)
 {
     __shared__ std::uint32_t bins[256];
-    __shared__ std::uint32_t s_digit, s_left;
-    constexpr int kBits = sizeof(K) * 8;
-    K prefix = 0, mask = 0;
+    __shared__ K s_differ[kThreads / kWave];
+    __shared__ std::uint32_t s_found[2];
+    const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
+    if (want == 0) {
+        *threshold = ~K{0};
+        return 0;
+    }
+    const K sample = keys[0];
+    K differ = 0;
+    for (std::uint32_t i = threadIdx.x; i < n; i += kThreads) differ |= keys[i] ^ sample;
+#pragma unroll
+    for (int k = 1; k < kWave; k *= 2) differ |= __shfl_xor(differ, k);
+    if (lane == 0) s_differ[wave] = differ;
+    __syncthreads();
+    differ = 0;
+#pragma unroll
+    for (int i = 0; i < kThreads / kWave; ++i) differ |= s_differ[i];
+    int top = differ == 0 ? 0 : 64 - __clzll(static_cast<long long>(differ));  // bits in which keys differ
+    K mask = top >= static_cast<int>(sizeof(K) * 8) ? K{0} : static_cast<K>(~K{0} << top);
+    K prefix = sample & mask;
     std::uint32_t left = want;
-    for (int shift = kBits - 8; shift >= 0; shift -= 8) {
+    while (top > 0) {
+        const int shift = top > 8 ? top - 8 : 0;
+        const std::uint32_t digits = (1u << (top - shift)) - 1;
         for (int i = threadIdx.x; i < 256; i += kThreads) bins[i] = 0;
         __syncthreads();
         for (std::uint32_t i = threadIdx.x; i < n; i += kThreads) {
-            const K k = key(i);
-            if ((k & mask) == prefix) {
-                atomicAdd(&bins[(k >> shift) & 255], 1u);
+            const K k = keys[i];
+            if ((k & mask) == prefix) atomicAdd(&bins[static_cast<std::uint32_t>(k >> shift) & digits], 1u);
+        }
+        __syncthreads();
+        if (wave == 0) {
+            std::uint32_t mine[4], sum = 0;  // lane 0 holds the highest digits
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                mine[i] = bins[255 - lane * 4 - i];
+                sum += mine[i];
+            }
+            std::uint32_t upto = sum;
+#pragma unroll
+            for (int k = 1; k < kWave; k *= 2) {
+                const std::uint32_t x = __shfl_up(upto, k);
+                upto += lane >= k ? x : 0;
+            }
+            std::uint32_t above = upto - sum;
+            if (above < left && upto >= left) {
+                int i = 0;
+                for (; i < 3 && above + mine[i] < left; ++i) above += mine[i];
+                s_found[0] = 255 - lane * 4 - i;
+                s_found[1] = left - above;
             }
         }
         __syncthreads();
-        if (threadIdx.x == 0) {
-            std::uint32_t above = 0;
-            int digit = 255;
-            for (; digit > 0 && above + bins[digit] < left; --digit) above += bins[digit];
-            s_digit = digit;
-            s_left = left - above;
+        const std::uint32_t digit = s_found[0];
+        left = s_found[1];
+        prefix |= static_cast<K>(digit) << shift;
+        mask |= static_cast<K>(digits) << shift;
+        top = shift;
+        if (bins[digit] == left) {  // every key of this digit is taken
+            *threshold = prefix == 0 ? prefix : prefix - 1;
+            return prefix == 0 ? left : 0;
         }
-        __syncthreads();
-        prefix |= static_cast<K>(s_digit) << shift;
-        mask |= static_cast<K>(255) << shift;
-        left = s_left;
         __syncthreads();
     }
     *threshold = prefix;
     return left;
 }
 
-// Exclusive rank of this thread's flag among the workgroup's, and their sum.
-template <int kThreads>
-__device__ std::uint32_t flag_rank(bool flag, std::uint32_t* total)
+// Places in order of the n items of a workgroup that `above` or, for the
+// first `equal` of them, `ties` names: calls put(i, place) for an item taken
+// and skip(i, items taken before it) for one not.  Returns how many are taken.
+template <int kThreads, typename A, typename P, typename S>
+__device__ std::uint32_t place_in_order(std::uint32_t n, std::uint32_t equal, A about, P put, S skip)
 {
-    __shared__ std::uint32_t waves[kThreads / kWave];
-    const unsigned long long votes = __ballot(flag);
+    __shared__ unsigned long long s_wave[kThreads / kWave];
     const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
-    if (lane == 0) waves[wave] = __popcll(votes);
+    const std::uint32_t each = (n + kThreads - 1) / kThreads;
+    const std::uint32_t begin = threadIdx.x * each < n ? threadIdx.x * each : n;
+    const std::uint32_t end = begin + each < n ? begin + each : n;
+    unsigned long long mine = 0;  // above in the low half, ties in the high one
+    for (std::uint32_t i = begin; i < end; ++i) {
+        const int x = about(i);
+        mine += x > 0 ? 1ull : x == 0 ? 1ull << 32 : 0ull;
+    }
+    unsigned long long upto = mine;
+#pragma unroll
+    for (int k = 1; k < kWave; k *= 2) {
+        const unsigned long long x = __shfl_up(upto, k);
+        upto += lane >= k ? x : 0ull;
+    }
+    if (lane == kWave - 1) s_wave[wave] = upto;
     __syncthreads();
-    std::uint32_t before = 0, sum = 0;
+    unsigned long long before = upto - mine, all = 0;
 #pragma unroll
     for (int i = 0; i < kThreads / kWave; ++i) {
-        before += i < wave ? waves[i] : 0;
-        sum += waves[i];
+        before += i < wave ? s_wave[i] : 0ull;
+        all += s_wave[i];
     }
-    __syncthreads();
-    *total = sum;
-    return before + __popcll(votes & ((1ull << lane) - 1));
+    std::uint32_t over = static_cast<std::uint32_t>(before), tied = static_cast<std::uint32_t>(before >> 32);
+    for (std::uint32_t i = begin; i < end; ++i) {
+        const int x = about(i);
+        const std::uint32_t place = over + (tied < equal ? tied : equal);
+        if (x > 0 || (x == 0 && tied < equal)) {
+            put(i, place);
+        } else {
+            skip(i, place);
+        }
+        over += x > 0;
+        tied += x == 0;
+    }
+    const std::uint32_t ties = static_cast<std::uint32_t>(all >> 32);
+    return static_cast<std::uint32_t>(all) + (ties < equal ? ties : equal);
 }
 
 struct Select {
@@ -1221,14 +1288,197 @@ struct Select {
     const void* q;
     std::int64_t q_token, q_head;
     std::uint32_t group, count, keep_first, keep_last;
+    std::uint32_t per, share; // tokens per group of the scoring pass, blocks per workgroup
+    std::uint32_t staged;     // the choice reads its keys from LDS
     std::uint32_t* keys;      // [tokens, kv heads, width]
     std::int32_t* selected;   // [tokens, kv heads, count]
 };
 
-// Blocks that a query token sees, and its sequence.
-__device__ inline std::uint32_t select_blocks(const Select& a, std::uint32_t token, std::uint32_t* seq)
+__device__ inline std::uint32_t ordered(float x)
 {
+    const std::uint32_t u = __float_as_uint(x);
+    return (u & 0x80000000u) != 0 ? ~u : u | 0x80000000u;
+}
+
+// Blocks that a token that sees `seen` tokens sees.
+__device__ inline std::uint32_t select_blocks(const Select& a, std::int64_t seen)
+{
+    const std::int64_t nb = seen <= 0 ? 0 : (seen + a.c.tokens - 1) / a.c.tokens;
+    return nb < static_cast<std::int64_t>(a.b.width) ? static_cast<std::uint32_t>(nb) : a.b.width;
+}
+
+// The group's queries of a token as codes of one scale, summed over the heads
+// by sign (what meets the low bounds, then what meets the high ones), each sum
+// as 128 * [0] + [1] of two signed bytes.  One wave; [2][2 * dims] bytes.
+template <typename T>
+__device__ void query_codes(const Select& a, std::int64_t row, std::uint32_t head, int lane, std::int8_t* to)
+{
+    const int P = static_cast<int>(a.c.dims), D = static_cast<int>(a.c.dim), G = static_cast<int>(a.group);
+    const T* q = static_cast<const T*>(a.q) + row * a.q_token + static_cast<std::int64_t>(head) * G * a.q_head;
+    float top = 0.0f;
+    for (int g = 0; g < G; ++g) {
+        for (int d = lane; d < D; d += kWave) top = fmaxf(top, fabsf(to_float(q[g * a.q_head + d])));
+    }
+#pragma unroll
+    for (int k = 1; k < kWave; k *= 2) top = fmaxf(top, __shfl_xor(top, k));
+    const float inv = 1.0f / fmaxf(top * kInv127, kQueryScaleMin);
+    for (int d = lane; d < P; d += kWave) {
+        std::int32_t sum[2] = {0, 0};
+        for (int g = 0; g < G && d < D; ++g) {
+            const std::int32_t code = static_cast<std::int32_t>(quantise(to_float(q[g * a.q_head + d]), inv));
+            sum[code > 0] += code;
+        }
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const std::int32_t hi = (sum[i] + 64) >> 7;
+            to[i * P + d] = static_cast<std::int8_t>(hi);
+            to[2 * P + i * P + d] = static_cast<std::int8_t>(sum[i] - hi * 128);
+        }
+    }
+}
+
+// Scores of a wave's 16 blocks for up to 8 query tokens: bounds are the
+// matrix units' second operand (a lane's block is lane % 16), the tokens'
+// codes the first (rows 2 t and 2 t + 1 are token t's two bytes), so that a
+// lane ends with its block's scores of tokens 2 (lane / 16) and the next.
+template <int CH>
+__device__ inline void block_scores(const Cache& c, std::int32_t id, std::uint32_t head, int quarter,
+                                    const i32x4 (&codes)[CH * 2], float (&score)[2])
+{
+    const std::size_t bh = static_cast<std::size_t>(id < 0 ? 0 : id) * c.kv_heads + head;
+    const i32x4* bounds = reinterpret_cast<const i32x4*>(c.bounds + bh * (CH * 128));
+    i32x4 x[CH * 2];
+#pragma unroll
+    for (int i = 0; i < CH * 2; ++i) x[i] = bounds[i * 4 + quarter];
+    const float scale = c.key_scale[bh];
+    i32x4 s = {0, 0, 0, 0};
+#pragma unroll
+    for (int i = 0; i < CH * 2; ++i) s = __builtin_amdgcn_mfma_i32_16x16x64_i8(codes[i], x[i], s, 0, 0, 0);
+    score[0] = static_cast<float>(s[0] * 128 + s[1]) * scale;
+    score[1] = static_cast<float>(s[2] * 128 + s[3]) * scale;
+}
+
+template <int CH>
+__device__ inline void load_codes(const std::int8_t* from, int token, int part, int quarter, i32x4 (&codes)[CH * 2])
+{
+    const i32x4* p = reinterpret_cast<const i32x4*>(from + (token * 2 + part) * (CH * 128));
+#pragma unroll
+    for (int i = 0; i < CH * 2; ++i) codes[i] = p[i * 4 + quarter];
+}
+
+// A block's key: 0 for one that is not there, and above every score's for a
+// scale that is not a number.
+__device__ inline std::uint32_t score_key(std::int32_t id, float score)
+{
+    return id < 0 ? 0u : ordered(score != score ? kInf : score);
+}
+
+// Writes a row's choice of its nb keys: the first and last that are always
+// in, the best of the others.
+template <int kThreads>
+__device__ void write_choice(const Select& a, const std::uint32_t* keys, std::uint32_t nb, std::int32_t* out)
+{
+    std::uint32_t threshold = 0, equal = 0, lo = 0, hi = 0;  // lo..hi: those that compete
+    if (nb > a.count) {
+        lo = a.keep_first;
+        hi = nb - a.keep_last;
+        std::uint32_t sure = 0;  // of those always in, the ones that are there
+        const std::uint32_t always = a.keep_first + a.keep_last;
+        for (std::uint32_t base = 0; base < always; base += kThreads) {
+            const std::uint32_t i = base + threadIdx.x;
+            sure += __syncthreads_count(i < always && keys[i < lo ? i : hi + i - lo] != 0);
+        }
+        const std::uint32_t want = a.count - sure < hi - lo ? a.count - sure : hi - lo;
+        equal = pick_threshold<std::uint32_t, kThreads>(keys + lo, hi - lo, want, &threshold);
+    }
+    // keys of 0, blocks that are not there, are never taken
+    const auto about = [&](std::uint32_t i) {
+        const std::uint32_t k = keys[i];
+        if (k == 0) return -1;
+        return i < lo || i >= hi || k > threshold ? 1 : k == threshold ? 0 : -1;
+    };
+    const std::uint32_t done = place_in_order<kThreads>(
+        nb, equal, about, [&](std::uint32_t i, std::uint32_t at) { out[at] = static_cast<std::int32_t>(i); },
+        [](std::uint32_t, std::uint32_t) {});
+    for (std::uint32_t i = done + threadIdx.x; i < a.count; i += kThreads) out[i] = -1;
+}
+
+// Scores and choice of one query token and kv head in one workgroup, the keys
+// in LDS.
+template <typename T, int CH>
+__global__ __launch_bounds__(kPickThreads) void k_kv_select(Select a)
+{
+    extern __shared__ std::uint32_t s_keys[];
+    __shared__ i32x4 s_codes[CH * 16];
+    const std::uint32_t token = blockIdx.x / a.c.kv_heads, head = blockIdx.x % a.c.kv_heads;
+    const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
     Group g;
+    std::uint32_t nb = 0;
+    if (find_group(a.b, token, 1, &g)) nb = select_blocks(a, g.seen);
+    std::int8_t* codes_at = reinterpret_cast<std::int8_t*>(s_codes);
+    if (wave == 0 && nb > a.count) query_codes<T>(a, token, head, lane, codes_at);
+    __syncthreads();
+    const int quarter = lane >> 4;
+    i32x4 codes[CH * 2];
+    // rows past the token's two are not looked at: they repeat them
+    load_codes<CH>(codes_at, 0, lane & 1, quarter, codes);
+    for (std::uint32_t at = wave * 16; at < nb; at += kPickThreads / kWave * 16) {
+        const std::uint32_t blk = at + (lane & 15);
+        const std::int32_t id = blk < nb ? block_at(a.c, a.b, g.seq, blk) : -1;
+        std::uint32_t key = id < 0 ? 0u : 1u;
+        if (nb > a.count) {
+            float score[2];
+            block_scores<CH>(a.c, id, head, quarter, codes, score);
+            key = score_key(id, score[0]);
+        }
+        if (blk < nb && quarter == 0) s_keys[blk] = key;
+    }
+    __syncthreads();
+    write_choice<kPickThreads>(a, s_keys, nb, a.selected + static_cast<std::size_t>(blockIdx.x) * a.count);
+}
+
+// Scores of groups of up to 8 tokens of a sequence, to global memory.
+template <typename T, int CH>
+__global__ __launch_bounds__(256) void k_kv_score(Select a)
+{
+    __shared__ i32x4 s_codes[8 * CH * 16];
+    const std::uint32_t slot = blockIdx.x / a.c.kv_heads, head = blockIdx.x % a.c.kv_heads;
+    const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave, quarter = lane >> 4;
+    Group g;
+    if (!find_group(a.b, slot, a.per, &g)) {
+        return;
+    }
+    const std::uint32_t nb = select_blocks(a, g.seen + g.count - 1);
+    if (blockIdx.y * a.share >= nb) {
+        return;
+    }
+    std::int8_t* codes_at = reinterpret_cast<std::int8_t*>(s_codes);
+    for (int t = wave; t < g.count; t += 4) query_codes<T>(a, g.row + t, head, lane, codes_at + t * (CH * 256));
+    __syncthreads();
+    i32x4 codes[CH * 2];
+    const int t = (lane & 15) / 2 < g.count ? (lane & 15) / 2 : 0;
+    load_codes<CH>(codes_at, t, lane & 1, quarter, codes);
+    const std::uint32_t end = (blockIdx.y + 1) * a.share < nb ? (blockIdx.y + 1) * a.share : nb;
+    for (std::uint32_t at = blockIdx.y * a.share + wave * 16; at < end; at += 64) {
+        const std::uint32_t blk = at + (lane & 15);
+        const std::int32_t id = blk < end ? block_at(a.c, a.b, g.seq, blk) : -1;
+        float score[2];
+        block_scores<CH>(a.c, id, head, quarter, codes, score);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const int token = quarter * 2 + i;
+            if (token < g.count && blk < end) {
+                a.keys[(static_cast<std::size_t>(g.row + token) * a.c.kv_heads + head) * a.b.width + blk] = score_key(id, score[i]);
+            }
+        }
+    }
+}
+
+// The choice of each row of those keys.
+__global__ __launch_bounds__(256) void k_kv_pick(Select a)
+{
+    extern __shared__ std::uint32_t s_keys[];
+    const std::uint32_t token = blockIdx.x / a.c.kv_heads;
     std::uint32_t slot = token;
     if (a.b.first != nullptr) {
         std::uint32_t lo = 0, hi = a.b.seqs;
@@ -1242,104 +1492,15 @@ __device__ inline std::uint32_t select_blocks(const Select& a, std::uint32_t tok
         }
         slot = token + lo;  // slot_base with one token per slot
     }
-    if (!find_group(a.b, slot, 1, &g) || g.seen <= 0) {
-        *seq = 0;
-        return 0;
+    Group g;
+    const std::uint32_t nb = find_group(a.b, slot, 1, &g) ? select_blocks(a, g.seen) : 0;
+    const std::uint32_t* keys = a.keys + static_cast<std::size_t>(blockIdx.x) * a.b.width;
+    if (a.staged != 0) {
+        for (std::uint32_t i = threadIdx.x; i < nb; i += 256) s_keys[i] = keys[i];
+        __syncthreads();
+        keys = s_keys;
     }
-    *seq = g.seq;
-    const std::int64_t nb = (g.seen + a.c.tokens - 1) / a.c.tokens;
-    return nb < static_cast<std::int64_t>(a.b.width) ? static_cast<std::uint32_t>(nb) : a.b.width;
-}
-
-__device__ inline std::uint32_t ordered(float x)
-{
-    const std::uint32_t u = __float_as_uint(x);
-    return (u & 0x80000000u) != 0 ? ~u : u | 0x80000000u;
-}
-
-// Scores of a query token and kv head against every block it sees.
-template <typename T>
-__global__ __launch_bounds__(256) void k_kv_score(Select a)
-{
-    __shared__ std::int32_t s_code[512];  // group sums: parts that meet `low`, then `high`
-    __shared__ float s_top[4];
-    const std::uint32_t token = blockIdx.x, head = blockIdx.y;
-    const int P = static_cast<int>(a.c.dims), D = static_cast<int>(a.c.dim);
-    std::uint32_t seq;
-    const std::uint32_t nb = select_blocks(a, token, &seq);
-    const T* q = static_cast<const T*>(a.q) + token * a.q_token +
-                 static_cast<std::int64_t>(head) * a.group * a.q_head;
-    float top = 0.0f;
-    for (int i = threadIdx.x; i < static_cast<int>(a.group) * D; i += 256) {
-        top = fmaxf(top, fabsf(to_float(q[(i / D) * a.q_head + i % D])));
-    }
-    for (int k = 1; k < kWave; k *= 2) top = fmaxf(top, __shfl_xor(top, k));
-    if (threadIdx.x % kWave == 0) s_top[threadIdx.x / kWave] = top;
-    __syncthreads();
-    top = fmaxf(fmaxf(s_top[0], s_top[1]), fmaxf(s_top[2], s_top[3]));
-    const float inv = 1.0f / fmaxf(top * kInv127, kQueryScaleMin);
-    for (int d = threadIdx.x; d < P; d += 256) {
-        std::int32_t lo = 0, hi = 0;
-        for (std::uint32_t g = 0; g < a.group; ++g) {
-            const std::int32_t code = d < D ? static_cast<std::int32_t>(quantise(to_float(q[g * a.q_head + d]), inv)) : 0;
-            lo += code < 0 ? code : 0;
-            hi += code > 0 ? code : 0;
-        }
-        s_code[d] = lo;
-        s_code[P + d] = hi;
-    }
-    __syncthreads();
-    std::uint32_t* keys = a.keys + (static_cast<std::size_t>(token) * a.c.kv_heads + head) * a.b.width;
-    for (std::uint32_t blk = blockIdx.z * 256 + threadIdx.x; blk < nb; blk += gridDim.z * 256) {
-        const std::int32_t id = block_at(a.c, a.b, seq, blk);
-        std::uint32_t key = 0;
-        if (id >= 0) {
-            const std::size_t bh = static_cast<std::size_t>(id) * a.c.kv_heads + head;
-            const u32x4* bounds = reinterpret_cast<const u32x4*>(a.c.bounds + bh * 2 * P);
-            std::int32_t sum = 0;
-            for (int i = 0; i < 2 * P / 16; ++i) {
-                union {
-                    u32x4 v;
-                    std::int8_t e[16];
-                } u;
-                u.v = bounds[i];
-#pragma unroll
-                for (int k = 0; k < 16; ++k) sum += u.e[k] * s_code[i * 16 + k];
-            }
-            float score = static_cast<float>(sum) * a.c.key_scale[bh];
-            if (score != score || blk < a.keep_first || blk + a.keep_last >= nb) score = kInf;
-            key = ordered(score);
-        }
-        keys[blk] = key;
-    }
-}
-
-// Picks the `count` best of a row's keys; blocks that are not there have key 0.
-__global__ __launch_bounds__(256) void k_kv_pick(Select a)
-{
-    const std::uint32_t token = blockIdx.x, head = blockIdx.y;
-    const std::size_t cell = static_cast<std::size_t>(token) * a.c.kv_heads + head;
-    const std::uint32_t* keys = a.keys + cell * a.b.width;
-    std::int32_t* out = a.selected + cell * a.count;
-    std::uint32_t seq;
-    const std::uint32_t nb = select_blocks(a, token, &seq);
-    std::uint32_t threshold = 1, equal = 0xffffffffu;
-    if (nb > a.count) {
-        equal = radix_threshold<std::uint32_t, 256>([&](std::uint32_t i) { return keys[i]; }, nb, a.count, &threshold);
-    }
-    std::uint32_t done = 0, ties = 0;
-    for (std::uint32_t base = 0; base < nb; base += 256) {
-        const std::uint32_t i = base + threadIdx.x;
-        const std::uint32_t k = i < nb ? keys[i] : 0;
-        std::uint32_t total;
-        const std::uint32_t rank = flag_rank<256>(k == threshold, &total);
-        const bool take = k != 0 && (k > threshold || (k == threshold && ties + rank < equal));
-        ties += total;
-        const std::uint32_t at = flag_rank<256>(take, &total);
-        if (take) out[done + at] = static_cast<std::int32_t>(i);
-        done += total;
-    }
-    for (std::uint32_t i = done + threadIdx.x; i < a.count; i += 256) out[i] = -1;
+    write_choice<256>(a, keys, nb, a.selected + static_cast<std::size_t>(blockIdx.x) * a.count);
 }
 
 struct Evict {
@@ -1355,53 +1516,50 @@ struct Evict {
     std::int32_t* freed_count;
 };
 
-// One workgroup per sequence.  A block's key is its summed weight plus 1; a
-// table entry that names no block has key 0 and goes first.
-__global__ __launch_bounds__(256) void k_kv_evict(Evict a)
+// One workgroup per sequence, the keys in LDS if they fit (kStaged).  A
+// block's key is its summed weight plus 1; a table entry that names no block
+// has key 0 and goes first.
+template <bool kStaged>
+__global__ __launch_bounds__(kPickThreads) void k_kv_evict(Evict a)
 {
+    extern __shared__ unsigned long long s_weights[];
     const std::uint32_t s = blockIdx.x;
     const std::int64_t len = a.lens[s];
     const std::int64_t nb64 = len <= 0 ? 0 : (len + a.tokens - 1) / a.tokens;
     const std::uint32_t nb = nb64 < static_cast<std::int64_t>(a.width) ? static_cast<std::uint32_t>(nb64) : a.width;
     const std::int32_t* table = a.table + static_cast<std::size_t>(s) * a.stride;
-    unsigned long long* keys = a.keys + static_cast<std::size_t>(s) * a.width;
+    unsigned long long* keys = kStaged ? s_weights : a.keys + static_cast<std::size_t>(s) * a.width;
     unsigned long long threshold = 0;
-    std::uint32_t equal = 0xffffffffu;
+    std::uint32_t equal = 0, lo = 0, hi = 0;
     if (nb > a.keep) {
-        for (std::uint32_t i = threadIdx.x; i < nb; i += 256) {
+        lo = a.keep_first;
+        hi = nb - a.keep_last;
+        for (std::uint32_t i = threadIdx.x; i < nb; i += kPickThreads) {
             const std::uint32_t id = static_cast<std::uint32_t>(table[i]);
             unsigned long long key = 0;
             if (id < a.blocks) {
-                for (std::uint32_t h = 0; h < a.kv_heads; ++h) key += a.weight[static_cast<std::size_t>(id) * a.kv_heads + h];
-                key += 1;
+                const unsigned long long* w = a.weight + static_cast<std::size_t>(id) * a.kv_heads;
+                key = 1;
+#pragma unroll 8
+                for (std::uint32_t h = 0; h < a.kv_heads; ++h) key += w[h];
             }
-            if (i < a.keep_first || i + a.keep_last >= nb) key = ~0ull;
             keys[i] = key;
         }
         __syncthreads();
-        equal = radix_threshold<unsigned long long, 256>([&](std::uint32_t i) { return keys[i]; }, nb, a.keep, &threshold);
+        equal = pick_threshold<unsigned long long, kPickThreads>(keys + lo, hi - lo, a.keep - a.keep_first - a.keep_last, &threshold);
     }
     std::int32_t* kept = a.out_table + static_cast<std::size_t>(s) * a.width;
     std::int32_t* freed = a.freed + static_cast<std::size_t>(s) * a.width;
-    std::uint32_t done = 0, ties = 0;
-    for (std::uint32_t base = 0; base < nb; base += 256) {
-        const std::uint32_t i = base + threadIdx.x;
-        const bool in = i < nb;
-        const unsigned long long k = !in ? 0 : nb > a.keep ? keys[i] : 0;
-        std::uint32_t total;
-        const std::uint32_t rank = flag_rank<256>(in && k == threshold, &total);
-        const bool take = in && (k > threshold || (k == threshold && ties + rank < equal));
-        ties += total;
-        const std::uint32_t at = flag_rank<256>(take, &total);
-        if (take) {
-            kept[done + at] = table[i];
-        } else if (in) {
-            freed[i - (done + at)] = table[i];
-        }
-        done += total;
-    }
-    for (std::uint32_t i = done + threadIdx.x; i < a.width; i += 256) kept[i] = -1;
-    for (std::uint32_t i = nb - done + threadIdx.x; i < a.width; i += 256) freed[i] = -1;
+    const auto about = [&](std::uint32_t i) {
+        if (i < lo || i >= hi) return 1;
+        const unsigned long long k = keys[i];
+        return k > threshold ? 1 : k == threshold ? 0 : -1;
+    };
+    const std::uint32_t done = place_in_order<kPickThreads>(
+        nb, equal, about, [&](std::uint32_t i, std::uint32_t at) { kept[at] = table[i]; },
+        [&](std::uint32_t i, std::uint32_t before) { freed[i - before] = table[i]; });
+    for (std::uint32_t i = done + threadIdx.x; i < a.width; i += kPickThreads) kept[i] = -1;
+    for (std::uint32_t i = nb - done + threadIdx.x; i < a.width; i += kPickThreads) freed[i] = -1;
     if (threadIdx.x == 0) {
         a.out_lens[s] = static_cast<std::int32_t>(len - static_cast<std::int64_t>(nb - done) * a.tokens);
         a.freed_count[s] = static_cast<std::int32_t>(nb - done);
@@ -1487,7 +1645,7 @@ struct Cut {
 std::size_t up256(std::size_t x) { return (x + 255) & ~std::size_t{255}; }
 
 // Row tiles per wave that fit the registers of two waves per SIMD.
-std::uint32_t many_tiles(std::uint32_t dims) { return dims <= 64 ? 3 : dims <= 128 ? 3 : 1; }
+std::uint32_t many_tiles(std::uint32_t dims) { return dims <= 64 ? 4 : dims <= 128 ? 3 : 2; }
 
 Cut cut_few(const Cache& c, const Batch& b, std::uint32_t heads, std::uint32_t count)
 {
@@ -1554,10 +1712,75 @@ Cut cut_attend(const Cache& c, const Batch& b, std::uint32_t heads, std::uint32_
     return k;
 }
 
+// Keys of a row that a choosing workgroup holds in LDS.
+constexpr std::size_t kMostStaged = std::size_t{128} << 10;
+
+// A kernel asks for more LDS than the 64 KiB that it has unasked, its own
+// arrays among them.
+bool lds_allowed(const void* kernel, std::size_t bytes)
+{
+    return bytes <= (std::size_t{48} << 10) ||
+           hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes)) == hipSuccess;
+}
+
+// One workgroup per row does it all where there are rows enough to fill the
+// card and no other token reads the same bounds.
+bool select_in_one(const Cache& c, const Batch& b)
+{
+    return b.first == nullptr && static_cast<std::uint64_t>(b.tokens) * c.kv_heads >= 128 &&
+           static_cast<std::size_t>(b.width) * sizeof(std::uint32_t) <= kMostStaged;
+}
+
+std::size_t select_bytes(const Cache& c, const Batch& b)
+{
+    return select_in_one(c, b) ? 0
+                               : static_cast<std::size_t>(b.tokens) * c.kv_heads * b.width * sizeof(std::uint32_t);
+}
+
+template <typename T, int CH>
+bool launch_select(Select& a, bool one, hipStream_t stream)
+{
+    const std::size_t keys = static_cast<std::size_t>(a.b.width) * sizeof(std::uint32_t);
+    const std::uint32_t rows = a.b.tokens * a.c.kv_heads;
+    if (one) {
+        if (!lds_allowed(reinterpret_cast<const void*>(&k_kv_select<T, CH>), keys)) {
+            return false;
+        }
+        hipLaunchKernelGGL((k_kv_select<T, CH>), dim3(rows), dim3(kPickThreads), keys, stream, a);
+        return true;
+    }
+    if (a.b.width != 0) {
+        a.per = a.b.first == nullptr ? 1 : 8;
+        const std::uint32_t slots = a.b.first == nullptr ? a.b.seqs : a.b.tokens / 8 + a.b.seqs;
+        a.share = 256;
+        while (a.share < 4096 && static_cast<std::uint64_t>(slots) * a.c.kv_heads * (a.b.width / a.share) > 4096) a.share *= 2;
+        while (a.b.width / a.share > 65534) a.share *= 2;
+        hipLaunchKernelGGL((k_kv_score<T, CH>), dim3(slots * a.c.kv_heads, (a.b.width + a.share - 1) / a.share), dim3(256), 0,
+                           stream, a);
+    }
+    a.staged = keys <= kMostStaged ? 1 : 0;
+    if (a.staged != 0 && !lds_allowed(reinterpret_cast<const void*>(&k_kv_pick), keys)) {
+        return false;
+    }
+    hipLaunchKernelGGL(k_kv_pick, dim3(rows), dim3(256), a.staged != 0 ? keys : 0, stream, a);
+    return true;
+}
+
+template <typename T>
+bool run_select(Select& a, bool one, hipStream_t stream)
+{
+    switch (a.c.dims / 64) {
+    case 1: return launch_select<T, 1>(a, one, stream);
+    case 2: return launch_select<T, 2>(a, one, stream);
+    case 3: return launch_select<T, 3>(a, one, stream);
+    default: return launch_select<T, 4>(a, one, stream);
+    }
+}
+
 template <typename T, int CH>
 void launch_attend(Attend a, const Cut& k, bool accumulate, hipStream_t stream)
 {
-    constexpr int RT = CH == 1 ? 3 : CH == 2 ? 3 : 1;
+    constexpr int RT = CH == 1 ? 4 : CH == 2 ? 3 : 2;
     const std::uint32_t groups = k.units * a.pairs;
     if (k.many != 0) {
         const std::size_t lds = (CH <= 2 ? 32 : 16) * 1024 * CH;
@@ -1761,7 +1984,7 @@ HBF_API int hbfsim_amd_kv_select_workspace(const hbfsim_amd_kv_cache* cache, con
     if (bytes == nullptr) {
         return HBFSIM_INVALID_ARGUMENT;
     }
-    *bytes = static_cast<std::size_t>(b.tokens) * c.kv_heads * b.width * sizeof(std::uint32_t);
+    *bytes = select_bytes(c, b);
     return HBFSIM_OK;
 }
 
@@ -1783,11 +2006,13 @@ HBF_API int hbfsim_amd_kv_select(const hbfsim_amd_kv_cache* cache, const hbfsim_
     if (a.b.tokens == 0 || a.b.seqs == 0) {
         return HBFSIM_OK;
     }
-    const std::size_t need = static_cast<std::size_t>(a.b.tokens) * a.c.kv_heads * a.b.width * sizeof(std::uint32_t);
-    if (d_q == nullptr || d_selected == nullptr || workspace_bytes < need || (need != 0 && d_workspace == nullptr)) {
+    const bool one = select_in_one(a.c, a.b);
+    const std::size_t need = select_bytes(a.c, a.b);
+    if (d_q == nullptr || d_selected == nullptr || workspace_bytes < need ||
+        (need != 0 && (d_workspace == nullptr || !aligned16(d_workspace)))) {
         return HBFSIM_INVALID_ARGUMENT;
     }
-    if (a.b.tokens > kMostGroups || a.b.width > 1024 * 65535u) {
+    if (static_cast<std::uint64_t>(a.b.tokens) * a.c.kv_heads > kMostGroups / 2) {
         return HBFSIM_UNSUPPORTED;
     }
     a.q = d_q;
@@ -1800,17 +2025,13 @@ HBF_API int hbfsim_amd_kv_select(const hbfsim_amd_kv_cache* cache, const hbfsim_
     a.keys = static_cast<std::uint32_t*>(d_workspace);
     a.selected = d_selected;
     const hipStream_t s = static_cast<hipStream_t>(stream);
-    if (a.b.width != 0) {
-        const std::uint32_t z = (a.b.width + 1023) / 1024;
-        const dim3 grid(a.b.tokens, a.c.kv_heads, z);
-        if (type == HBFSIM_AMD_KV_BF16) {
-            hipLaunchKernelGGL(k_kv_score<Bf16>, grid, dim3(256), 0, s, a);
-        } else {
-            hipLaunchKernelGGL(k_kv_score<F16>, grid, dim3(256), 0, s, a);
-        }
+    bool ok = true;
+    if (type == HBFSIM_AMD_KV_BF16) {
+        ok = run_select<Bf16>(a, one, s);
+    } else {
+        ok = run_select<F16>(a, one, s);
     }
-    hipLaunchKernelGGL(k_kv_pick, dim3(a.b.tokens, a.c.kv_heads), dim3(256), 0, s, a);
-    return checked(hipGetLastError());
+    return ok ? checked(hipGetLastError()) : HBFSIM_CUDA_ERROR;
 }
 
 HBF_API int hbfsim_amd_kv_evict(const int64_t* d_weight, uint32_t blocks, uint32_t kv_heads, uint32_t block_tokens,
@@ -1828,7 +2049,7 @@ HBF_API int hbfsim_amd_kv_evict(const int64_t* d_weight, uint32_t blocks, uint32
     if (seqs == 0) {
         return HBFSIM_OK;
     }
-    if (seqs > kMostGroups) {
+    if (seqs > kMostGroups / 2) {
         return HBFSIM_UNSUPPORTED;
     }
     const std::size_t need = static_cast<std::size_t>(seqs) * width * sizeof(unsigned long long);
@@ -1840,6 +2061,15 @@ HBF_API int hbfsim_amd_kv_evict(const int64_t* d_weight, uint32_t blocks, uint32
     Evict a{reinterpret_cast<const unsigned long long*>(d_weight), blocks, kv_heads, block_tokens, d_table, d_lens,
             seqs, width, stride, keep, keep_first, keep_last, static_cast<unsigned long long*>(d_workspace),
             d_out_table, d_out_lens, d_freed, d_freed_count};
-    hipLaunchKernelGGL(k_kv_evict, dim3(seqs), dim3(256), 0, static_cast<hipStream_t>(stream), a);
+    const hipStream_t s = static_cast<hipStream_t>(stream);
+    const std::size_t lds = static_cast<std::size_t>(width) * sizeof(unsigned long long);
+    if (lds <= kMostStaged) {
+        if (!lds_allowed(reinterpret_cast<const void*>(&k_kv_evict<true>), lds)) {
+            return HBFSIM_CUDA_ERROR;
+        }
+        hipLaunchKernelGGL(k_kv_evict<true>, dim3(seqs), dim3(kPickThreads), lds, s, a);
+    } else {
+        hipLaunchKernelGGL(k_kv_evict<false>, dim3(seqs), dim3(kPickThreads), 0, s, a);
+    }
     return checked(hipGetLastError());
 }

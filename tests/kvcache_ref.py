@@ -96,8 +96,9 @@ class RefCache:
                     score = whole.astype(F) * self.scale[0][np.where(live, ids, 0), h]
                     score = np.where(np.isnan(score), np.inf, score)
                     at = np.arange(nb)
-                    score = np.where((at < keep_first) | (at + keep_last >= nb), np.inf, score)
-                    order = [j for j in sorted(at, key=lambda j: (-score[j], j)) if live[j]]
+                    always = (at < keep_first) | (at + keep_last >= nb)
+                    order = [j for j in sorted(at, key=lambda j: (not always[j], -score[j], j))
+                             if live[j]]
                     got = sorted(order[:count])
                     out[first[s] + i, h, :len(got)] = got
         return out
