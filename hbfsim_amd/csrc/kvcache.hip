@@ -969,6 +969,7 @@ struct Append {
     Batch b;
     const void* x[2];                       // keys, values
     std::int64_t token_stride[2], head_stride[2];
+    std::uint32_t vector[2];                // rows may be loaded 16 bytes at a time
 };
 
 __device__ inline float quantise(float x, float inv)
@@ -1032,127 +1033,291 @@ __device__ inline bool find_write(const Append& a, std::uint32_t slot, Write* w)
     return true;
 }
 
-// One wave per (slot, kv head, keys or values).
+// 16 consecutive elements of a row from d0 on, zeros past its dim.
 template <typename T>
-__global__ __launch_bounds__(kWave) void k_kv_append(Append a)
+__device__ inline void load_16(const T* row, int d0, int dim, bool vector, float (&x)[16])
 {
+    constexpr int kEach = 16 / sizeof(T);
+    if (vector && dim % kEach == 0) {
+#pragma unroll
+        for (int i = 0; i < 16; i += kEach) {
+            union {
+                u32x4 v;
+                T e[kEach];
+            } u;
+            u.v = *reinterpret_cast<const u32x4*>(row + (d0 + i < dim ? d0 + i : 0));
+#pragma unroll
+            for (int j = 0; j < kEach; ++j) x[i + j] = d0 + i < dim ? to_float(u.e[j]) : 0.0f;
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            const float e = to_float(row[d0 + i < dim ? d0 + i : 0]);
+            x[i] = d0 + i < dim ? e : 0.0f;
+        }
+    }
+}
+
+// rint(x * inv) of four values as bytes.  Adding 1.5 * 2^23 leaves the whole
+// number nearest to the rounded product in the low bits, so the two must not
+// become one fused step; it needs no limit, as |x| is at most the largest from
+// which the scale came.
+__device__ inline std::uint32_t codes_of(float x0, float x1, float x2, float x3, float inv)
+{
+#pragma clang fp contract(off)
+    constexpr float kWhole = 12582912.0f;
+    const float p0 = x0 * inv, p1 = x1 * inv, p2 = x2 * inv, p3 = x3 * inv;
+    const std::uint32_t a = __float_as_uint(p0 + kWhole), b = __float_as_uint(p1 + kWhole);
+    const std::uint32_t c = __float_as_uint(p2 + kWhole), d = __float_as_uint(p3 + kWhole);
+    return __builtin_amdgcn_perm(__builtin_amdgcn_perm(d, c, 0x0c0c0400u), __builtin_amdgcn_perm(b, a, 0x0c0c0400u), 0x05040100u);
+}
+
+// Old codes at a new scale.
+__device__ inline std::uint32_t rescaled(std::uint32_t codes, float ratio)
+{
+    std::uint32_t out = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float q = quantise(static_cast<float>(static_cast<std::int8_t>(codes >> (8 * i))), ratio);
+        out |= static_cast<std::uint32_t>(static_cast<std::uint8_t>(static_cast<std::int8_t>(q))) << (8 * i);
+    }
+    return out;
+}
+
+template <int kLane>
+__device__ inline std::uint32_t from_quad(std::uint32_t x)  // lane kLane's of each four lanes
+{
+    return static_cast<std::uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(x), kLane * 0x55, 0xf, 0xf, true));
+}
+
+// One workgroup per (slot, kv head, keys or values), one wave per 16 tokens of
+// the block: a lane holds token lane % 16's dims 16 (lane / 16) .. + 15 of
+// every 64 in registers from the one read of the input to its codes.  That is
+// the keys' layout already; values are transposed four tokens by four dims
+// within four lanes.
+template <typename T, int CH>
+__global__ __launch_bounds__(512) void k_kv_append(Append a)
+{
+    constexpr int P = CH * 64, kRow = P + 4;
+    extern __shared__ std::uint8_t s_codes[];  // keys: [block tokens][kRow]
+    __shared__ float s_top[8];
+    __shared__ int s_bad[8];
     Write w;
     if (!find_write(a, blockIdx.x, &w)) {
         return;
     }
     const std::uint32_t head = blockIdx.y, which = blockIdx.z;
-    const int lane = threadIdx.x;
-    const int P = static_cast<int>(a.c.dims), D = static_cast<int>(a.c.dim);
-    const int count = w.end - w.begin;
+    const int lane = threadIdx.x % kWave, tile = threadIdx.x / kWave, waves = static_cast<int>(a.c.tokens) / 16;
+    const int n = lane & 15, c = lane >> 4, D = static_cast<int>(a.c.dim);
     const bool begun = w.begin > 0;
     const std::size_t bh = static_cast<std::size_t>(w.id) * a.c.kv_heads + head;
-    const T* x = static_cast<const T*>(a.x[which]) + w.row * a.token_stride[which] + head * a.head_stride[which];
-    const std::int64_t row = a.token_stride[which];
+    float* scales = which == 0 ? a.c.key_scale : a.c.value_scale;
+    const float before = begun ? scales[bh] : 0.0f;
+    const int token = tile * 16 + n;
+    const bool fresh = token >= w.begin && token < w.end;
+    const T* row = static_cast<const T*>(a.x[which]) + (w.row + (fresh ? token - w.begin : 0)) * a.token_stride[which] +
+                   head * a.head_stride[which];
 
+    float x[CH][16];
     float top = 0.0f;
     bool bad = false;
-    for (int i = 0; i < count; ++i) {
-        for (int d = lane; d < D; d += kWave) {
-            const float v = fabsf(to_float(x[i * row + d]));
-            bad |= !(v < kInf);
-            top = fmaxf(top, v);
+#pragma unroll
+    for (int i = 0; i < CH; ++i) {
+        load_16<T>(row, i * 64 + c * 16, D, a.vector[which] != 0, x[i]);
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+            x[i][j] = fresh ? x[i][j] : 0.0f;
+            bad |= !(fabsf(x[i][j]) < kInf);
+            top = fmaxf(top, fabsf(x[i][j]));
         }
     }
 #pragma unroll
     for (int k = 1; k < kWave; k *= 2) top = fmaxf(top, __shfl_xor(top, k));
-    float* scales = which == 0 ? a.c.key_scale : a.c.value_scale;
+    const bool any_bad = __any(bad);
+    if (lane == 0) {
+        s_top[tile] = top;
+        s_bad[tile] = any_bad;
+    }
+    __syncthreads();
+    bad = any_bad;
+    for (int i = 0; i < waves; ++i) {
+        top = fmaxf(top, s_top[i]);
+        bad |= s_bad[i] != 0;
+    }
     float scale = top * kInv127;
-    scale = __any(bad) || !(scale <= kScaleMax) ? __builtin_nanf("") : fmaxf(scale, kScaleMin);
+    scale = bad || !(scale <= kScaleMax) ? __builtin_nanf("") : fmaxf(scale, kScaleMin);
     float ratio = 0.0f;
     if (begun) {
-        const float before = scales[bh];
         scale = before != before || scale != scale ? __builtin_nanf("") : fmaxf(before, scale);
         ratio = before / scale;
     }
-    const float inv = 1.0f / scale;
-    if (lane == 0) {
+    const bool lost = scale != scale;  // no codes but zeros
+    const float inv = lost ? 0.0f : 1.0f / scale;
+    if (threadIdx.x == 0) {
         scales[bh] = scale;
         if (which == 0 && !begun) {
             a.c.weight[bh] = 0;
         }
     }
 
-    // codes: every 16-byte piece that holds a new token or changes
-    std::int8_t* pool = (which == 0 ? a.c.keys : a.c.values) + bh * (static_cast<std::size_t>(a.c.tokens) * P);
-    const int tiles = static_cast<int>(a.c.tokens) / 16;
-    const int c = lane >> 4, n = lane & 15;
-    for (int tile = 0; tile < tiles; ++tile) {
-        for (int chunk = 0; chunk < P / 64; ++chunk) {
-            u32x4* piece = reinterpret_cast<u32x4*>(pool + (static_cast<std::size_t>(tile) * (P / 64) + chunk) * 1024) + lane;
-            const int lo = tile * 16 + (which == 0 ? n : 4 * c), hi = lo + (which == 0 ? 1 : 4);
-            const bool holds_new = lo < w.end && hi > w.begin;
-            if (!holds_new && begun && ratio == 1.0f) {
-                continue;
-            }
-            union {
-                u32x4 v;
-                std::int8_t e[16];
-            } u;
-            u.v = begun ? *piece : u32x4{0u, 0u, 0u, 0u};
+    std::int8_t* pool = (which == 0 ? a.c.keys : a.c.values) + bh * (static_cast<std::size_t>(a.c.tokens) * P) +
+                        static_cast<std::size_t>(tile) * 16 * P;
+    const bool keep = begun && ratio == 1.0f;  // old codes stay as they are
 #pragma unroll
-            for (int k = 0; k < 16; ++k) {
-                const int token = which == 0 ? lo : lo + (k & 3);
-                const int d = chunk * 64 + (which == 0 ? 16 * c + k : 16 * (k >> 2) + n);
-                float q;
-                if (token >= w.begin && token < w.end) {
-                    q = d < D ? quantise(to_float(x[(token - w.begin) * row + d]), inv) : 0.0f;
-                } else {
-                    q = quantise(static_cast<float>(u.e[k]), ratio);
-                }
-                u.e[k] = static_cast<std::int8_t>(q);
+    for (int i = 0; i < CH; ++i) {
+        u32x4 q = {0u, 0u, 0u, 0u};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const std::uint32_t y = codes_of(x[i][4 * j], x[i][4 * j + 1], x[i][4 * j + 2], x[i][4 * j + 3], inv);
+            q[j] = lost ? 0u : y;
+        }
+        if (which == 0) {
+            u32x4* piece = reinterpret_cast<u32x4*>(pool + i * 1024) + lane;
+            if (begun && !fresh && !keep) {
+                const u32x4 old = *piece;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) q[j] = rescaled(old[j], ratio);
             }
-            *piece = u.v;
+            if (fresh || !keep) {
+                *piece = q;
+            }
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                *reinterpret_cast<std::uint32_t*>(s_codes + token * kRow + i * 64 + c * 16 + j * 4) = q[j];
+            }
+        } else {
+            // lane r of four holds, for each j, byte r of the four lanes' words: the codes of
+            // dim 16 c + 4 j + r of tokens 4 (n / 4) .. + 3
+            const int r = n & 3, first = tile * 16 + (n & 12);
+            const std::uint32_t pick = (static_cast<std::uint32_t>(r + 4) << 8) | static_cast<std::uint32_t>(r);
+            std::uint32_t mask = 0;  // bytes of new tokens
+#pragma unroll
+            for (int k = 0; k < 4; ++k) mask |= first + k >= w.begin && first + k < w.end ? 0xffu << (8 * k) : 0u;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const std::uint32_t lo = __builtin_amdgcn_perm(from_quad<1>(q[j]), from_quad<0>(q[j]), pick);
+                const std::uint32_t hi = __builtin_amdgcn_perm(from_quad<3>(q[j]), from_quad<2>(q[j]), pick);
+                std::uint32_t y = __builtin_amdgcn_perm(hi, lo, 0x05040100u);
+                std::uint32_t* at = reinterpret_cast<std::uint32_t*>(pool + i * 1024 + ((n >> 2) * 16 + 4 * j + r) * 16 + c * 4);
+                if (mask == 0 && keep) {
+                    continue;
+                }
+                if (begun && mask != 0xffffffffu) {
+                    const std::uint32_t old = *at;
+                    y = (y & mask) | ((keep ? old : rescaled(old, ratio)) & ~mask);
+                }
+                *at = y;
+            }
         }
     }
-    if (which == 0) {
-        std::int8_t* bounds = a.c.bounds + bh * 2 * P;
-        for (int d = lane; d < P; d += kWave) {
-            float lo = 127.0f, hi = -127.0f;
-            if (begun) {
-                lo = quantise(static_cast<float>(bounds[d]), ratio);
-                hi = quantise(static_cast<float>(bounds[P + d]), ratio);
+    if (which != 0) {
+        return;
+    }
+    __syncthreads();
+    std::int8_t* bounds = a.c.bounds + bh * 2 * P;
+    for (int d = threadIdx.x * 2; d < P; d += static_cast<int>(blockDim.x) * 2) {
+        int lo[2] = {127, 127}, hi[2] = {-127, -127};
+        if (begun) {
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                lo[u] = static_cast<int>(quantise(static_cast<float>(bounds[d + u]), ratio));
+                hi[u] = static_cast<int>(quantise(static_cast<float>(bounds[P + d + u]), ratio));
             }
-            for (int i = 0; i < count; ++i) {
-                const float q = d < D ? quantise(to_float(x[i * row + d]), inv) : 0.0f;
-                lo = fminf(lo, q);
-                hi = fmaxf(hi, q);
+        }
+#pragma unroll 4
+        for (int k = w.begin; k < w.end; ++k) {
+            const std::uint16_t two = *reinterpret_cast<const std::uint16_t*>(s_codes + k * kRow + d);
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                const int q = static_cast<std::int8_t>(two >> (8 * u));
+                lo[u] = q < lo[u] ? q : lo[u];
+                hi[u] = q > hi[u] ? q : hi[u];
             }
-            bounds[d] = static_cast<std::int8_t>(lo);
-            bounds[P + d] = static_cast<std::int8_t>(hi);
+        }
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            bounds[d + u] = static_cast<std::int8_t>(lo[u]);
+            bounds[P + d + u] = static_cast<std::int8_t>(hi[u]);
         }
     }
 }
 
-// Blocks back as values: one workgroup per (entry, kv head).
+// Blocks back as values: one wave per (entry, kv head, 16 tokens, keys or
+// values).  Keys: a lane widens a token's 16 dims of every 64 and stores them
+// as they are.  Values: four lanes transpose four tokens by four dims first,
+// as append does.
 template <typename T>
-__global__ __launch_bounds__(256) void k_kv_read(Cache c, const std::int32_t* ids, T* k_out, T* v_out, T* low, T* high)
+__device__ inline void store_16(T* row, int d0, int dim, bool vector, std::uint32_t w0, std::uint32_t w1, std::uint32_t w2,
+                                std::uint32_t w3, float scale)
 {
-    const std::uint32_t head = blockIdx.y;
+    constexpr int kEach = 16 / sizeof(T);
+    const std::uint32_t word[4] = {w0, w1, w2, w3};
+    union {
+        u32x4 v[sizeof(T)];
+        T e[16];
+    } u;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+        u.e[i] = from_float<T>(static_cast<float>(static_cast<std::int8_t>(word[i / 4] >> (8 * (i % 4)))) * scale);
+    }
+    if (vector && dim % kEach == 0) {
+#pragma unroll
+        for (int i = 0; i < 16; i += kEach) {
+            if (d0 + i < dim) *reinterpret_cast<u32x4*>(row + d0 + i) = u.v[i / kEach];
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            if (d0 + i < dim) row[d0 + i] = u.e[i];
+        }
+    }
+}
+
+template <typename T, int CH>
+__global__ __launch_bounds__(512) void k_kv_read(Cache c, const std::int32_t* ids, T* k_out, T* v_out, T* low, T* high,
+                                                 std::uint32_t vector)
+{
+    constexpr int P = CH * 64;
+    const std::uint32_t head = blockIdx.y, which = blockIdx.z;
     const std::int32_t id = ids[blockIdx.x];
     const bool inside = static_cast<std::uint32_t>(id) < c.blocks;
-    const int P = static_cast<int>(c.dims), D = static_cast<int>(c.dim), t = static_cast<int>(c.tokens);
+    const int D = static_cast<int>(c.dim), t = static_cast<int>(c.tokens);
+    const int lane = threadIdx.x % kWave, tile = threadIdx.x / kWave, n = lane & 15, quarter = lane >> 4;
     const std::size_t bh = inside ? static_cast<std::size_t>(id) * c.kv_heads + head : 0;
     const std::size_t to = static_cast<std::size_t>(blockIdx.x) * c.kv_heads + head;
-    const float ks = inside ? c.key_scale[bh] : 0.0f, vs = inside ? c.value_scale[bh] : 0.0f;
-    const std::int8_t* kp = c.keys + bh * (static_cast<std::size_t>(t) * P);
-    const std::int8_t* vp = c.values + bh * (static_cast<std::size_t>(t) * P);
-    for (int i = threadIdx.x; i < t * D; i += 256) {
-        const int token = i / D, d = i % D;
-        const std::size_t piece = (static_cast<std::size_t>(token / 16) * (P / 64) + d / 64) * 1024;
-        const int n = token % 16, e = d % 64;
-        const float kq = kp[piece + ((e / 16) * 16 + n) * 16 + e % 16];
-        const float vq = vp[piece + ((n / 4) * 16 + e % 16) * 16 + (e / 16) * 4 + n % 4];
-        k_out[to * t * D + i] = from_float<T>(kq * ks);
-        v_out[to * t * D + i] = from_float<T>(vq * vs);
+    const float scale = inside ? (which == 0 ? c.key_scale : c.value_scale)[bh] : 0.0f;
+    const std::int8_t* pool = (which == 0 ? c.keys : c.values) + bh * (static_cast<std::size_t>(t) * P) +
+                              static_cast<std::size_t>(tile) * 16 * P;
+    T* row = (which == 0 ? k_out : v_out) + (to * t + tile * 16 + n) * D;
+#pragma unroll
+    for (int i = 0; i < CH; ++i) {
+        std::uint32_t w[4];
+        if (which == 0) {
+            const u32x4 x = reinterpret_cast<const u32x4*>(pool + i * 1024)[lane];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) w[j] = x[j];
+        } else {
+            const int r = n & 3;
+            const std::uint32_t pick = (static_cast<std::uint32_t>(r + 4) << 8) | static_cast<std::uint32_t>(r);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const std::uint32_t x = *reinterpret_cast<const std::uint32_t*>(
+                    pool + i * 1024 + ((n >> 2) * 16 + 4 * j + r) * 16 + quarter * 4);
+                const std::uint32_t lo = __builtin_amdgcn_perm(from_quad<1>(x), from_quad<0>(x), pick);
+                const std::uint32_t hi = __builtin_amdgcn_perm(from_quad<3>(x), from_quad<2>(x), pick);
+                w[j] = __builtin_amdgcn_perm(hi, lo, 0x05040100u);
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) w[j] = inside ? w[j] : 0u;
+        store_16<T>(row, i * 64 + quarter * 16, D, vector != 0, w[0], w[1], w[2], w[3], scale);
     }
-    for (int d = threadIdx.x; d < D; d += 256) {
-        low[to * D + d] = from_float<T>(static_cast<float>(c.bounds[bh * 2 * P + d]) * ks);
-        high[to * D + d] = from_float<T>(static_cast<float>(c.bounds[bh * 2 * P + P + d]) * ks);
+    if (which == 0) {
+        for (int d = threadIdx.x; d < D; d += static_cast<int>(blockDim.x)) {
+            const std::int8_t* b = c.bounds + bh * 2 * P + d;
+            low[to * D + d] = from_float<T>(inside ? static_cast<float>(b[0]) * scale : 0.0f);
+            high[to * D + d] = from_float<T>(inside ? static_cast<float>(b[P]) * scale : 0.0f);
+        }
     }
 }
 
@@ -1337,25 +1502,32 @@ __device__ void query_codes(const Select& a, std::int64_t row, std::uint32_t hea
     }
 }
 
-// Scores of a wave's 16 blocks for up to 8 query tokens: bounds are the
+// Scores of a wave's 32 blocks for up to 8 query tokens, 16 at a time: bounds are the
 // matrix units' second operand (a lane's block is lane % 16), the tokens'
 // codes the first (rows 2 t and 2 t + 1 are token t's two bytes), so that a
 // lane ends with its block's scores of tokens 2 (lane / 16) and the next.
 template <int CH>
-__device__ inline void block_scores(const Cache& c, std::int32_t id, std::uint32_t head, int quarter,
-                                    const i32x4 (&codes)[CH * 2], float (&score)[2])
+__device__ inline void block_scores(const Cache& c, const std::int32_t (&id)[2], std::uint32_t head, int quarter,
+                                    const i32x4 (&codes)[CH * 2], float (&score)[2][2])
 {
-    const std::size_t bh = static_cast<std::size_t>(id < 0 ? 0 : id) * c.kv_heads + head;
-    const i32x4* bounds = reinterpret_cast<const i32x4*>(c.bounds + bh * (CH * 128));
-    i32x4 x[CH * 2];
+    i32x4 x[2][CH * 2];
+    float scale[2];
 #pragma unroll
-    for (int i = 0; i < CH * 2; ++i) x[i] = bounds[i * 4 + quarter];
-    const float scale = c.key_scale[bh];
-    i32x4 s = {0, 0, 0, 0};
+    for (int u = 0; u < 2; ++u) {
+        const std::size_t bh = static_cast<std::size_t>(id[u] < 0 ? 0 : id[u]) * c.kv_heads + head;
+        const i32x4* bounds = reinterpret_cast<const i32x4*>(c.bounds + bh * (CH * 128));
 #pragma unroll
-    for (int i = 0; i < CH * 2; ++i) s = __builtin_amdgcn_mfma_i32_16x16x64_i8(codes[i], x[i], s, 0, 0, 0);
-    score[0] = static_cast<float>(s[0] * 128 + s[1]) * scale;
-    score[1] = static_cast<float>(s[2] * 128 + s[3]) * scale;
+        for (int i = 0; i < CH * 2; ++i) x[u][i] = bounds[i * 4 + quarter];
+        scale[u] = c.key_scale[bh];
+    }
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+        i32x4 s = {0, 0, 0, 0};
+#pragma unroll
+        for (int i = 0; i < CH * 2; ++i) s = __builtin_amdgcn_mfma_i32_16x16x64_i8(codes[i], x[u][i], s, 0, 0, 0);
+        score[u][0] = static_cast<float>(s[0] * 128 + s[1]) * scale[u];
+        score[u][1] = static_cast<float>(s[2] * 128 + s[3]) * scale[u];
+    }
 }
 
 template <int CH>
@@ -1422,16 +1594,28 @@ __global__ __launch_bounds__(kPickThreads) void k_kv_select(Select a)
     i32x4 codes[CH * 2];
     // rows past the token's two are not looked at: they repeat them
     load_codes<CH>(codes_at, 0, lane & 1, quarter, codes);
-    for (std::uint32_t at = wave * 16; at < nb; at += kPickThreads / kWave * 16) {
-        const std::uint32_t blk = at + (lane & 15);
-        const std::int32_t id = blk < nb ? block_at(a.c, a.b, g.seq, blk) : -1;
-        std::uint32_t key = id < 0 ? 0u : 1u;
-        if (nb > a.count) {
-            float score[2];
-            block_scores<CH>(a.c, id, head, quarter, codes, score);
-            key = score_key(id, score[0]);
+    const auto look_up = [&](std::uint32_t at, std::int32_t (&id)[2]) {
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            const std::uint32_t blk = at + u * 16 + (lane & 15);
+            id[u] = blk < nb ? block_at(a.c, a.b, g.seq, blk) : -1;
         }
-        if (blk < nb && quarter == 0) s_keys[blk] = key;
+    };
+    std::int32_t next[2];
+    look_up(wave * 32, next);
+    for (std::uint32_t at = wave * 32; at < nb; at += kPickThreads / kWave * 32) {
+        const std::int32_t id[2] = {next[0], next[1]};
+        look_up(at + kPickThreads / kWave * 32, next);
+        std::uint32_t key[2] = {id[0] < 0 ? 0u : 1u, id[1] < 0 ? 0u : 1u};
+        if (nb > a.count) {
+            float score[2][2];
+            block_scores<CH>(a.c, id, head, quarter, codes, score);
+            key[0] = score_key(id[0], score[0][0]);
+            key[1] = score_key(id[1], score[1][0]);
+        }
+        // quarter u stores tile u's keys
+        const std::uint32_t blk = at + (lane & 31);
+        if (blk < nb && lane < 32) s_keys[blk] = quarter == 0 ? key[0] : key[1];
     }
     __syncthreads();
     write_choice<kPickThreads>(a, s_keys, nb, a.selected + static_cast<std::size_t>(blockIdx.x) * a.count);
@@ -1459,16 +1643,30 @@ __global__ __launch_bounds__(256) void k_kv_score(Select a)
     const int t = (lane & 15) / 2 < g.count ? (lane & 15) / 2 : 0;
     load_codes<CH>(codes_at, t, lane & 1, quarter, codes);
     const std::uint32_t end = (blockIdx.y + 1) * a.share < nb ? (blockIdx.y + 1) * a.share : nb;
-    for (std::uint32_t at = blockIdx.y * a.share + wave * 16; at < end; at += 64) {
-        const std::uint32_t blk = at + (lane & 15);
-        const std::int32_t id = blk < end ? block_at(a.c, a.b, g.seq, blk) : -1;
-        float score[2];
+    const auto look_up = [&](std::uint32_t at, std::int32_t (&id)[2]) {
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            const std::uint32_t blk = at + u * 16 + (lane & 15);
+            id[u] = blk < end ? block_at(a.c, a.b, g.seq, blk) : -1;
+        }
+    };
+    std::int32_t next[2];
+    look_up(blockIdx.y * a.share + wave * 32, next);
+    for (std::uint32_t at = blockIdx.y * a.share + wave * 32; at < end; at += 128) {
+        const std::int32_t id[2] = {next[0], next[1]};
+        look_up(at + 128, next);
+        float score[2][2];
         block_scores<CH>(a.c, id, head, quarter, codes, score);
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const int token = quarter * 2 + i;
-            if (token < g.count && blk < end) {
-                a.keys[(static_cast<std::size_t>(g.row + token) * a.c.kv_heads + head) * a.b.width + blk] = score_key(id, score[i]);
+        for (int u = 0; u < 2; ++u) {
+            const std::uint32_t blk = at + u * 16 + (lane & 15);
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const int token = quarter * 2 + i;
+                if (token < g.count && blk < end) {
+                    a.keys[(static_cast<std::size_t>(g.row + token) * a.c.kv_heads + head) * a.b.width + blk] =
+                        score_key(id[u], score[u][i]);
+                }
             }
         }
     }
@@ -1712,6 +1910,44 @@ Cut cut_attend(const Cache& c, const Batch& b, std::uint32_t heads, std::uint32_
     return k;
 }
 
+template <typename T, int CH>
+void launch_append(const Append& a, std::uint32_t slots, hipStream_t stream)
+{
+    const std::size_t lds = static_cast<std::size_t>(a.c.tokens) * (CH * 64 + 4);
+    hipLaunchKernelGGL((k_kv_append<T, CH>), dim3(slots, a.c.kv_heads, 2), dim3(a.c.tokens * 4), lds, stream, a);
+}
+
+template <typename T>
+void run_append(const Append& a, std::uint32_t slots, hipStream_t stream)
+{
+    switch (a.c.dims / 64) {
+    case 1: launch_append<T, 1>(a, slots, stream); break;
+    case 2: launch_append<T, 2>(a, slots, stream); break;
+    case 3: launch_append<T, 3>(a, slots, stream); break;
+    default: launch_append<T, 4>(a, slots, stream); break;
+    }
+}
+
+template <typename T, int CH>
+void launch_read(const Cache& c, const std::int32_t* ids, std::uint32_t n, void* k, void* v, void* low, void* high,
+                 std::uint32_t vector, hipStream_t stream)
+{
+    hipLaunchKernelGGL((k_kv_read<T, CH>), dim3(n, c.kv_heads, 2), dim3(c.tokens * 4), 0, stream, c, ids, static_cast<T*>(k),
+                       static_cast<T*>(v), static_cast<T*>(low), static_cast<T*>(high), vector);
+}
+
+template <typename T>
+void run_read(const Cache& c, const std::int32_t* ids, std::uint32_t n, void* k, void* v, void* low, void* high,
+              std::uint32_t vector, hipStream_t stream)
+{
+    switch (c.dims / 64) {
+    case 1: launch_read<T, 1>(c, ids, n, k, v, low, high, vector, stream); break;
+    case 2: launch_read<T, 2>(c, ids, n, k, v, low, high, vector, stream); break;
+    case 3: launch_read<T, 3>(c, ids, n, k, v, low, high, vector, stream); break;
+    default: launch_read<T, 4>(c, ids, n, k, v, low, high, vector, stream); break;
+    }
+}
+
 // Keys of a row that a choosing workgroup holds in LDS.
 constexpr std::size_t kMostStaged = std::size_t{128} << 10;
 
@@ -1850,14 +2086,20 @@ HBF_API int hbfsim_amd_kv_append(const hbfsim_amd_kv_cache* cache, const hbfsim_
     if (slots > kMostGroups) {
         return HBFSIM_UNSUPPORTED;
     }
-    const dim3 grid(slots, a.c.kv_heads, 2);
+    const std::size_t each = type == HBFSIM_AMD_KV_F32 ? 4 : 8;  // elements of 16 bytes
+    for (int i = 0; i < 2; ++i) {
+        a.vector[i] = aligned16(a.x[i]) && a.token_stride[i] % static_cast<std::int64_t>(each) == 0 &&
+                              a.head_stride[i] % static_cast<std::int64_t>(each) == 0
+                          ? 1
+                          : 0;
+    }
     const hipStream_t s = static_cast<hipStream_t>(stream);
     if (type == HBFSIM_AMD_KV_BF16) {
-        hipLaunchKernelGGL(k_kv_append<Bf16>, grid, dim3(kWave), 0, s, a);
+        run_append<Bf16>(a, slots, s);
     } else if (type == HBFSIM_AMD_KV_F16) {
-        hipLaunchKernelGGL(k_kv_append<F16>, grid, dim3(kWave), 0, s, a);
+        run_append<F16>(a, slots, s);
     } else {
-        hipLaunchKernelGGL(k_kv_append<float>, grid, dim3(kWave), 0, s, a);
+        run_append<float>(a, slots, s);
     }
     return checked(hipGetLastError());
 }
@@ -1883,17 +2125,14 @@ HBF_API int hbfsim_amd_kv_read(const hbfsim_amd_kv_cache* cache, const int32_t* 
     if (d_blocks == nullptr || d_k == nullptr || d_v == nullptr || d_low == nullptr || d_high == nullptr) {
         return HBFSIM_INVALID_ARGUMENT;
     }
-    const dim3 grid(static_cast<unsigned>(n), c.kv_heads);
     const hipStream_t s = static_cast<hipStream_t>(stream);
+    const std::uint32_t vector = aligned16(d_k) && aligned16(d_v) ? 1 : 0, count = static_cast<std::uint32_t>(n);
     if (type == HBFSIM_AMD_KV_BF16) {
-        hipLaunchKernelGGL(k_kv_read<Bf16>, grid, dim3(256), 0, s, c, d_blocks, static_cast<Bf16*>(d_k),
-                           static_cast<Bf16*>(d_v), static_cast<Bf16*>(d_low), static_cast<Bf16*>(d_high));
+        run_read<Bf16>(c, d_blocks, count, d_k, d_v, d_low, d_high, vector, s);
     } else if (type == HBFSIM_AMD_KV_F16) {
-        hipLaunchKernelGGL(k_kv_read<F16>, grid, dim3(256), 0, s, c, d_blocks, static_cast<F16*>(d_k),
-                           static_cast<F16*>(d_v), static_cast<F16*>(d_low), static_cast<F16*>(d_high));
+        run_read<F16>(c, d_blocks, count, d_k, d_v, d_low, d_high, vector, s);
     } else {
-        hipLaunchKernelGGL(k_kv_read<float>, grid, dim3(256), 0, s, c, d_blocks, static_cast<float*>(d_k),
-                           static_cast<float*>(d_v), static_cast<float*>(d_low), static_cast<float*>(d_high));
+        run_read<float>(c, d_blocks, count, d_k, d_v, d_low, d_high, vector, s);
     }
     return checked(hipGetLastError());
 }
