@@ -217,6 +217,7 @@ struct Attend {
     float* partial;                // [unit, row tile, kv head, split][rows][dims]
     float* stats;                  // [...][rows][2]: reference exponent, denominator
     float* lse;                    // [tokens, heads], log2 of the row's denominator, or null
+    float* tile_sums;              // [unit, row tile, kv head, tile][rows], log2 of a row's sum over a tile
 };
 
 // Splits that hold work for a unit whose last token sees `seen` tokens.
@@ -347,7 +348,9 @@ __device__ inline float lane_float(float x, int lane)
 // up one tile of the wave's next 64 (block, scales), so the loop itself has no
 // dependent loads; the keys of the pair of tiles after this one are on their
 // way while its softmax runs, the values while the next scores do.
-template <typename T, int CH, int kWaves>
+// kWeigh: each tile's sum of a row's weights is left behind as one logarithm,
+// from which k_kv_weigh makes probabilities once the row's denominator is known.
+template <typename T, int CH, int kWaves, bool kWeigh>
 __global__ __launch_bounds__(kWaves * kWave) void k_kv_attend(Attend a)
 {
     constexpr int P = CH * 64, kRow = P + 4;
@@ -394,6 +397,8 @@ __global__ __launch_bounds__(kWaves * kWave) void k_kv_attend(Attend a)
         a.selected == nullptr ? nullptr
                               : a.selected + (static_cast<std::int64_t>(g.row) * a.c.kv_heads + head) * a.count;
     const std::size_t head_bytes = static_cast<std::size_t>(a.c.tokens) * P;
+    float* sums = kWeigh ? a.tile_sums + (static_cast<std::size_t>(blockIdx.x) * a.c.tokens / 16 * a.b.width + begin / 16) * a.rows
+                         : nullptr;
     const std::int64_t tiles = end > begin ? (end - begin + 15) / 16 : 0;
     const std::int64_t per_wave = (tiles + 2 * kWaves - 1) / (2 * kWaves) * 2;
     const std::int64_t tile0 = wave * per_wave;
@@ -462,7 +467,15 @@ __global__ __launch_bounds__(kWaves * kWave) void k_kv_attend(Attend a)
                     sum += x;
                     w[u * 4 + i] = static_cast<_Float16>(x);
                 }
-                den = fmaf(sum, lane_float(info.inv_scale, tile + u), den);
+                const float part = sum * lane_float(info.inv_scale, tile + u);
+                den += part;
+                if (kWeigh) {
+                    float all = part + __shfl_xor(part, 16);
+                    all += __shfl_xor(all, 32);
+                    if (quarter == 0 && m < static_cast<int>(a.rows) && tile + u < n) {
+                        sums[(at + tile + u) * a.rows + m] = __builtin_amdgcn_logf(all) + ref;
+                    }
+                }
             }
 #pragma unroll
             for (int i = 0; i < CH; ++i) {
@@ -897,12 +910,58 @@ __global__ __launch_bounds__(256) void k_kv_merge(Attend a)
     }
 }
 
-// weight[block, head] += the probabilities of the unit's rows over the block.
-// One wave per block of the sequence; sums are f32 within a block and joined
-// as integers, so the order in which blocks of shared prefixes are reached
-// does not change them.
-template <typename T, int CH>
+// weight[block, head] += the probabilities of the unit's rows over the block,
+// from the tiles' sums: one thread per block.  Sums are f32 within a block and
+// joined as integers, so the order in which blocks of shared prefixes are
+// reached does not change them.
+__device__ inline void add_weight(const Attend& a, std::size_t bh, float sum)
+{
+    if (sum < 1e9f) {  // a sum that is not a number adds nothing
+        atomicAdd(a.c.weight + bh, static_cast<unsigned long long>(__double2ull_rn(static_cast<double>(sum) * 0x1p32)));
+    }
+}
+
 __global__ __launch_bounds__(256) void k_kv_weigh(Attend a)
+{
+    __shared__ float s_lse[16];
+    const std::uint32_t unit = blockIdx.x / a.pairs, pair = blockIdx.x % a.pairs;
+    const std::uint32_t head = pair % a.c.kv_heads, row_tile = pair / a.c.kv_heads;
+    Group g;
+    if (!find_group(a.b, unit, a.per, &g)) {
+        return;
+    }
+    const std::int64_t seen = visible(a, g.seen + g.count - 1);
+    if (seen <= 0 || static_cast<std::int64_t>(blockIdx.y) * 256 * a.c.tokens >= seen) {
+        return;
+    }
+    const std::uint32_t r = row_tile * 16 + threadIdx.x;
+    if (threadIdx.x < a.rows) {
+        s_lse[threadIdx.x] = r < g.count * a.group
+                                 ? a.lse[(g.row + static_cast<std::int64_t>(r / a.group)) * a.heads + head * a.group + r % a.group]
+                                 : kInf;
+    }
+    __syncthreads();
+    const std::uint32_t blk = blockIdx.y * 256 + threadIdx.x;
+    const std::int32_t id = static_cast<std::int64_t>(blk) * a.c.tokens < seen ? block_at(a.c, a.b, g.seq, blk) : -1;
+    if (id < 0) {
+        return;
+    }
+    const std::uint32_t per_block = a.c.tokens / 16;
+    const float* sums = a.tile_sums + (static_cast<std::size_t>(blockIdx.x) * a.b.width + blk) * per_block * a.rows;
+    float sum = 0.0f;
+    for (std::uint32_t tile = 0; tile < per_block && (static_cast<std::int64_t>(blk) * per_block + tile) * 16 < seen; ++tile) {
+        for (std::uint32_t k = 0; k < a.rows; ++k) {
+            const float l = s_lse[k];
+            sum += l == kInf ? 0.0f : exp2_fast(sums[tile * a.rows + k] - l);
+        }
+    }
+    add_weight(a, static_cast<std::size_t>(id) * a.c.kv_heads + head, sum);
+}
+
+// The same where the many-row form ran, from the keys again: one wave per
+// block of the sequence; 16 query rows at a time.
+template <typename T, int CH>
+__global__ __launch_bounds__(256) void k_kv_weigh_again(Attend a)
 {
     constexpr int P = CH * 64;
     const std::uint32_t unit = blockIdx.x / a.pairs, pair = blockIdx.x % a.pairs;
@@ -956,8 +1015,8 @@ __global__ __launch_bounds__(256) void k_kv_weigh(Attend a)
         }
 #pragma unroll
         for (int x = 1; x < kWave; x *= 2) sum += __shfl_xor(sum, x);
-        if (lane == 0 && sum < 1e9f) {  // a sum that is not a number adds nothing
-            atomicAdd(a.c.weight + bh, static_cast<unsigned long long>(__double2ull_rn(static_cast<double>(sum) * 0x1p32)));
+        if (lane == 0) {
+            add_weight(a, bh, sum);
         }
     }
 }
@@ -1837,7 +1896,7 @@ bool two_byte(std::uint32_t type) { return type == HBFSIM_AMD_KV_BF16 || type ==
 struct Cut {
     std::uint32_t many;  // row tiles per wave of the many-row form, or 0
     std::uint32_t per, row_tiles, rows, units, split, splits;
-    std::size_t partial, stats, lse, bytes;
+    std::size_t partial, stats, lse, tile_sums, bytes;
 };
 
 std::size_t up256(std::size_t x) { return (x + 255) & ~std::size_t{255}; }
@@ -1855,8 +1914,10 @@ Cut cut_few(const Cache& c, const Batch& b, std::uint32_t heads, std::uint32_t c
     k.units = b.first == nullptr ? b.seqs : b.tokens / k.per + b.seqs;
     const std::uint64_t longest = static_cast<std::uint64_t>(count != 0 ? count : b.width) * c.tokens;
     const std::uint64_t pairs = static_cast<std::uint64_t>(k.units) * c.kv_heads * k.row_tiles;
+    // Splits of 2048 tokens, shorter where they would not fill the card; up to
+    // 768 tokens take one, whose few microseconds a second launch would cost.
     std::uint64_t split = 2048;
-    while (split > 256 && pairs * ((longest + split - 1) / split) < 1024) split /= 2;
+    while (longest > 768 && split > 256 && pairs * ((longest + split - 1) / split) < 1024) split /= 2;
     k.split = static_cast<std::uint32_t>(split);
     k.splits = longest == 0 ? 1 : static_cast<std::uint32_t>((longest + split - 1) / split);
     return k;
@@ -1906,7 +1967,11 @@ Cut cut_attend(const Cache& c, const Batch& b, std::uint32_t heads, std::uint32_
         k.stats = up256(cells * c.dims * sizeof(float));
         k.lse = k.stats + up256(cells * 2 * sizeof(float));
     }
-    k.bytes = k.lse + (accumulate ? up256(static_cast<std::size_t>(b.tokens) * heads * sizeof(float)) : 0);
+    k.tile_sums = k.lse + (accumulate ? up256(static_cast<std::size_t>(b.tokens) * heads * sizeof(float)) : 0);
+    k.bytes = k.tile_sums;
+    if (accumulate && k.many == 0) {
+        k.bytes += up256(static_cast<std::size_t>(k.units) * c.kv_heads * k.row_tiles * b.width * (c.tokens / 16) * k.rows * sizeof(float));
+    }
     return k;
 }
 
@@ -2023,7 +2088,11 @@ void launch_attend(Attend a, const Cut& k, bool accumulate, hipStream_t stream)
         hipLaunchKernelGGL((k_kv_attend_many<T, CH, RT>), dim3(groups, k.splits), dim3(256), lds, stream, a);
     } else {
         const std::size_t lds = 4 * k.rows * (CH * 64 + 4) * sizeof(float);
-        hipLaunchKernelGGL((k_kv_attend<T, CH, 4>), dim3(groups, k.splits), dim3(256), lds, stream, a);
+        if (accumulate) {
+            hipLaunchKernelGGL((k_kv_attend<T, CH, 4, true>), dim3(groups, k.splits), dim3(256), lds, stream, a);
+        } else {
+            hipLaunchKernelGGL((k_kv_attend<T, CH, 4, false>), dim3(groups, k.splits), dim3(256), lds, stream, a);
+        }
     }
     if (k.splits > 16) {
         hipLaunchKernelGGL((k_kv_merge<T>), dim3(groups, k.rows), dim3(256), 0, stream, a);
@@ -2031,13 +2100,16 @@ void launch_attend(Attend a, const Cut& k, bool accumulate, hipStream_t stream)
         const std::uint32_t at_once = 1024 / a.c.dims;
         hipLaunchKernelGGL((k_kv_merge_few<T>), dim3(groups, (k.rows + at_once - 1) / at_once), dim3(256), 0, stream, a);
     }
-    if (accumulate && a.b.width != 0) {
+    if (!accumulate || a.b.width == 0) {
+    } else if (k.many == 0) {
+        hipLaunchKernelGGL(k_kv_weigh, dim3(groups, (a.b.width + 255) / 256), dim3(256), 0, stream, a);
+    } else {
         const Cut few = cut_few(a.c, a.b, a.heads, 0);
         a.per = few.per;
         a.row_tiles = few.row_tiles;
         a.pairs = a.c.kv_heads * few.row_tiles;
         const std::uint32_t z = a.b.width / 64 < 65535 ? (a.b.width + 63) / 64 : 65535;
-        hipLaunchKernelGGL((k_kv_weigh<T, CH>), dim3(few.units * a.pairs, z), dim3(256), 0, stream, a);
+        hipLaunchKernelGGL((k_kv_weigh_again<T, CH>), dim3(few.units * a.pairs, z), dim3(256), 0, stream, a);
     }
 }
 
@@ -2205,6 +2277,7 @@ HBF_API int hbfsim_amd_kv_attend(const hbfsim_amd_kv_cache* cache, const hbfsim_
     a.partial = k.splits > 1 ? reinterpret_cast<float*>(ws + k.partial) : nullptr;
     a.stats = k.splits > 1 ? reinterpret_cast<float*>(ws + k.stats) : nullptr;
     a.lse = accumulate != 0 ? reinterpret_cast<float*>(ws + k.lse) : nullptr;
+    a.tile_sums = accumulate != 0 && k.many == 0 ? reinterpret_cast<float*>(ws + k.tile_sums) : nullptr;
     const hipStream_t s = static_cast<hipStream_t>(stream);
     return type == HBFSIM_AMD_KV_BF16 ? run_attend<Bf16>(a, k, accumulate != 0, s)
                                       : run_attend<F16>(a, k, accumulate != 0, s);

@@ -26,7 +26,6 @@ from typing import Any
 import torch
 
 from . import _native as nat
-from .engine import _stream_handle
 
 BLOCK_TOKENS = (16, 32, 64, 128)
 WEIGHT_UNIT = 2.0 ** -32
@@ -44,21 +43,28 @@ def _refuse(rc: int, what: str) -> None:
     nat.check(rc, what)
 
 
+def _handle(stream: Any, device: Any) -> int:
+    """The stream's handle: the device's current one, a torch stream's, or a
+    handle already.  (The raw accessor costs a tenth of building a Stream.)"""
+    if stream is None:
+        return torch._C._cuda_getCurrentRawStream(device.index)
+    return stream.cuda_stream if hasattr(stream, "cuda_stream") else stream
+
+
 def _workspace(nbytes: int, device: Any, stream: Any) -> Any:
     """Scratch of one call, handed back to torch's allocator after it: work
     queued later on the same stream is ordered behind the call."""
     if nbytes == 0:
         return None
     ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
-    _used_on(stream, ws)
+    if stream is not None:
+        _used_on(stream, ws)
     return ws
 
 
 def _used_on(stream: Any, *tensors: Any) -> None:
     """Tells torch's allocator that a stream other than the current one uses
     the tensors, so that none of them is handed out again before it has."""
-    if stream is None:
-        return
     if not hasattr(stream, "cuda_stream"):
         stream = torch.cuda.ExternalStream(stream, device=tensors[0].device)
     for t in tensors:
@@ -112,15 +118,16 @@ def evict(weight: Any, table: Any, lens: Any, keep: int, block_tokens: int = 16,
     if min(keep, keep_first, keep_last) < 0:
         raise ValueError("keep, keep_first and keep_last must not be negative")
     stride = table.stride(0) if seqs > 1 else width
-    out_table, freed = torch.empty((2, seqs, width), dtype=torch.int32, device=device)
-    out_lens, count = torch.empty((2, seqs), dtype=torch.int32, device=device)
+    out_table, freed = torch.empty((2, seqs, width), dtype=torch.int32, device=device).unbind()
+    out_lens, count = torch.empty((2, seqs), dtype=torch.int32, device=device).unbind()
     ws = _workspace(seqs * width * 8, device, stream)
-    _used_on(stream, out_table, out_lens)
+    if stream is not None:
+        _used_on(stream, out_table, out_lens)
     _refuse(nat.load().hbfsim_amd_kv_evict(
         weight.data_ptr(), weight.shape[0], weight.shape[1], block_tokens, table.data_ptr(),
         lens.data_ptr(), seqs, width, stride, keep, keep_first, keep_last, out_table.data_ptr(),
         out_lens.data_ptr(), freed.data_ptr(), count.data_ptr(),
-        ws.data_ptr() if ws is not None else None, seqs * width * 8, _stream_handle(stream)),
+        ws.data_ptr() if ws is not None else None, seqs * width * 8, _handle(stream, device)),
         "evict")
     return out_table, out_lens, freed, count
 
@@ -184,6 +191,7 @@ class KvCache:
                                     key_scale.data_ptr(), value_scale.data_ptr(),
                                     bounds.data_ptr(), weight.data_ptr())
         self._ref = ctypes.byref(self._c)
+        self._need: dict = {}  # workspace bytes by a call's sizes
 
     # -- checks -----------------------------------------------------------
     def _rows(self, x: Any, heads: int | None, name: str) -> tuple[int, int, int]:
@@ -206,6 +214,12 @@ class KvCache:
             raise ValueError(f"{heads} query heads do not divide among {self.kv_heads} kv heads")
         return tokens, heads, kind
 
+    def _remember(self, sizes: tuple, nbytes: int) -> int:
+        if len(self._need) >= 4096:
+            self._need.clear()
+        self._need[sizes] = nbytes
+        return nbytes
+
     # -- operators --------------------------------------------------------
     def append(self, k: Any, v: Any, table: Any, lens: Any, first: Any = None,
                stream: Any = None) -> None:
@@ -219,7 +233,7 @@ class KvCache:
         strides = (ctypes.c_int64 * 4)(k.stride(0), k.stride(1), v.stride(0), v.stride(1))
         _refuse(self._lib.hbfsim_amd_kv_append(self._ref, ctypes.byref(b), k.data_ptr(),
                                                v.data_ptr(), kind, strides,
-                                               _stream_handle(stream)), "append")
+                                               _handle(stream, self.device)), "append")
 
     def read(self, blocks: Any, dtype: Any = torch.bfloat16, stream: Any = None) -> tuple:
         """The values that the blocks (int32 ids) stand for: keys and values
@@ -232,12 +246,13 @@ class KvCache:
         kv = torch.empty((2, n, self.kv_heads, self.block_tokens, self.head_dim), dtype=dtype,
                          device=self.device)
         ends = torch.empty((2, n, self.kv_heads, self.head_dim), dtype=dtype, device=self.device)
-        k, v = kv
-        low, high = ends
-        _used_on(stream, kv, ends)
+        k, v = kv.unbind()
+        low, high = ends.unbind()
+        if stream is not None:
+            _used_on(stream, kv, ends)
         _refuse(self._lib.hbfsim_amd_kv_read(self._ref, blocks.data_ptr(), n, _TYPES[dtype],
                                              k.data_ptr(), v.data_ptr(), low.data_ptr(),
-                                             high.data_ptr(), _stream_handle(stream)), "read")
+                                             high.data_ptr(), _handle(stream, self.device)), "read")
         return k, v, low, high
 
     def attend(self, q: Any, table: Any, lens: Any, first: Any = None, selected: Any = None,
@@ -264,21 +279,26 @@ class KvCache:
             chosen = selected.data_ptr()
         if out is None:
             out = torch.empty((tokens, heads, self.head_dim), dtype=q.dtype, device=self.device)
-            _used_on(stream, out)
+            if stream is not None:
+                _used_on(stream, out)
         elif tuple(out.shape) != tuple(q.shape) or out.dtype != q.dtype \
                 or out.device != self.device or not out.is_contiguous():
             raise ValueError("out must be a contiguous tensor of q's shape and type")
         ref = ctypes.byref(b)
-        need = ctypes.c_size_t()
-        _refuse(self._lib.hbfsim_amd_kv_attend_workspace(self._ref, ref, heads, count,
-                                                         int(accumulate), ctypes.byref(need)),
-                "attend")
-        ws = _workspace(need.value, self.device, stream)
+        sizes = (b.seqs, b.table_width, tokens, first is None, heads, count, accumulate)
+        need = self._need.get(sizes)
+        if need is None:
+            got = ctypes.c_size_t()
+            _refuse(self._lib.hbfsim_amd_kv_attend_workspace(self._ref, ref, heads, count,
+                                                             int(accumulate), ctypes.byref(got)),
+                    "attend")
+            need = self._remember(sizes, got.value)
+        ws = _workspace(need, self.device, stream)
         _refuse(self._lib.hbfsim_amd_kv_attend(
             self._ref, ref, q.data_ptr(), kind, heads, q.stride(0), q.stride(1),
             1.0 / math.sqrt(self.head_dim) if scale is None else scale, chosen, count,
             int(accumulate), out.data_ptr(), ws.data_ptr() if ws is not None else None,
-            need.value, _stream_handle(stream)), "attend")
+            need, _handle(stream, self.device)), "attend")
         return out
 
     def select(self, q: Any, table: Any, lens: Any, count: int, first: Any = None,
@@ -293,15 +313,20 @@ class KvCache:
         b = _batch(table, lens, first, tokens, self.device)
         ref = ctypes.byref(b)
         out = torch.empty((tokens, self.kv_heads, count), dtype=torch.int32, device=self.device)
-        _used_on(stream, out)
-        need = ctypes.c_size_t()
-        _refuse(self._lib.hbfsim_amd_kv_select_workspace(self._ref, ref, ctypes.byref(need)),
-                "select")
-        ws = _workspace(need.value, self.device, stream)
+        if stream is not None:
+            _used_on(stream, out)
+        sizes = (b.seqs, b.table_width, tokens, first is None)
+        need = self._need.get(sizes)
+        if need is None:
+            got = ctypes.c_size_t()
+            _refuse(self._lib.hbfsim_amd_kv_select_workspace(self._ref, ref, ctypes.byref(got)),
+                    "select")
+            need = self._remember(sizes, got.value)
+        ws = _workspace(need, self.device, stream)
         _refuse(self._lib.hbfsim_amd_kv_select(
             self._ref, ref, q.data_ptr(), kind, heads, q.stride(0), q.stride(1), count, keep_first,
-            keep_last, out.data_ptr(), ws.data_ptr() if ws is not None else None, need.value,
-            _stream_handle(stream)), "select")
+            keep_last, out.data_ptr(), ws.data_ptr() if ws is not None else None, need,
+            _handle(stream, self.device)), "select")
         return out
 
     def evict(self, table: Any, lens: Any, keep: int, keep_first: int = 1, keep_last: int = 1,
