@@ -579,3 +579,36 @@ def trace_event_spans(events, shard_base: dict[str, int], page_bytes: int, line_
     if not parts:
         raise ValueError("trace contains no expert accesses")
     return _spans(parts)
+
+
+# ---------------------------------------------------------------------------
+# A paged cache held in 8 bits (hbfsim_amd.kvcache) on flash: what a step reads
+# and writes of it.  A block's codes of one kv head are one run of bytes in the
+# key pool and one in the value pool; a block is written, whole, when its last
+# token fills it, and until then it is in HBM.
+
+
+def kv_cache_spans(key_base: int, value_base: int, head_bytes: int, kv_heads: int,
+                   reads: np.ndarray, writes: np.ndarray,
+                   line: int = 128) -> tuple[np.ndarray, np.ndarray, np.ndarray]:
+    """Spans (base, first, op) of a step: the blocks of `writes` (ids) into
+    both pools, then keys and values of every (block, kv head) of `reads`
+    [n, 2], in their order.  ValueError where a head's run is not whole lines
+    of both pools."""
+    if head_bytes <= 0 or head_bytes % line or key_base % line or value_base % line:
+        raise ValueError("a head's codes and the pools must be whole lines")
+    reads = np.asarray(reads, np.int64).reshape(-1, 2)
+    writes = np.asarray(writes, np.int64).reshape(-1)
+    if (reads < 0).any() or (reads[:, 1] >= kv_heads).any() or (writes < 0).any():
+        raise ValueError("block ids must not be negative, kv heads below kv_heads")
+    pools = np.array([key_base, value_base], np.uint64)
+    at = writes.astype(np.uint64) * np.uint64(kv_heads * head_bytes)
+    wb = (pools[None] + at[:, None]).reshape(-1)
+    at = (reads[:, 0] * kv_heads + reads[:, 1]).astype(np.uint64) * np.uint64(head_bytes)
+    rb = (pools[None] + at[:, None]).reshape(-1)
+    lines = np.concatenate([np.full(len(wb), kv_heads * head_bytes // line, np.uint64),
+                            np.full(len(rb), head_bytes // line, np.uint64)])
+    first = np.zeros(len(lines) + 1, np.uint64)
+    np.cumsum(lines, out=first[1:])
+    op = np.concatenate([np.ones(len(wb), np.uint32), np.zeros(len(rb), np.uint32)])
+    return np.concatenate([wb, rb]), first, op
