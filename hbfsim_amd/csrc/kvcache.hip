@@ -193,6 +193,15 @@ __device__ inline f16x8 widen8(std::uint32_t lo, std::uint32_t hi)
     return __builtin_shufflevector(widen(lo), widen(hi), 0, 1, 2, 3, 4, 5, 6, 7);
 }
 
+// The larger of three, without the quieting of NaNs that the compiler puts
+// before each fmaxf of a value that came through a branch.
+__device__ inline float max_of_3(float x, float y, float z)
+{
+    float r;
+    asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(x), "v"(y), "v"(z));
+    return r;
+}
+
 __device__ inline float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 
 // ---- attend ---------------------------------------------------------------
@@ -581,7 +590,7 @@ __global__ __launch_bounds__(256, 2) void k_kv_attend_many(Attend a)
     }
 
     f16x8 query[RT][CH * 2];
-    float factor[RT], ref[RT], den[RT];
+    float factor[RT], ref[RT], den[RT], over[RT];  // over: how far a score may pass ref
     int limit[RT];
     int least = 0x7fffffff, most = 0;
     f32x4 acc[RT][CH * 4];
@@ -596,8 +605,9 @@ __global__ __launch_bounds__(256, 2) void k_kv_attend_many(Attend a)
         most = limit[k] > most ? limit[k] : most;
         load_query<T, CH>(a, g.row + static_cast<std::int64_t>(row_token), head * a.group + row_head, row_live, quarter,
                           query[k], &factor[k]);
-        ref[k] = kLowest;
+        ref[k] = 0.0f;
         den[k] = 0.0f;
+        over[k] = kLowest;
 #pragma unroll
         for (int i = 0; i < CH * 4; ++i) acc[k][i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     }
@@ -687,17 +697,16 @@ __global__ __launch_bounds__(256, 2) void k_kv_attend_many(Attend a)
                 }
             }
             const bool whole = (pos[0] > pos[1] ? pos[0] : pos[1]) + 16 <= least;
-            float scale[2][RT], shift[2][RT];
+            // scores as exponents above the row's reference
 #pragma unroll
             for (int k = 0; k < RT; ++k) {
 #pragma unroll
                 for (int u = 0; u < 2; ++u) {
-                    scale[u][k] = factor[k] * f[u];
-                    shift[u][k] = e[u];
+                    const float scale = factor[k] * f[u], shift = e[u] - ref[k];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) s[u][k][i] = fmaf(s[u][k][i], scale, shift);
                 }
             }
-            // Scores of tokens that a row does not see become -inf; a tile of
-            // NaN scales does not reach the rows that see none of it.
             if (!whole) {
 #pragma unroll
                 for (int k = 0; k < RT; ++k) {
@@ -706,8 +715,6 @@ __global__ __launch_bounds__(256, 2) void k_kv_attend_many(Attend a)
                         const int left = limit[k] - pos[u] - quarter * 4;
 #pragma unroll
                         for (int i = 0; i < 4; ++i) s[u][k][i] = i < left ? s[u][k][i] : -kInf;
-                        scale[u][k] = pos[u] < limit[k] ? scale[u][k] : 1.0f;
-                        shift[u][k] = pos[u] < limit[k] ? shift[u][k] : 0.0f;
                     }
                 }
             }
@@ -715,23 +722,25 @@ __global__ __launch_bounds__(256, 2) void k_kv_attend_many(Attend a)
             bool move = false;
 #pragma unroll
             for (int k = 0; k < RT; ++k) {
-                float x[2];
-#pragma unroll
-                for (int u = 0; u < 2; ++u) {
-                    x[u] = fmaf(fmaxf(fmaxf(s[u][k][0], s[u][k][1]), fmaxf(s[u][k][2], s[u][k][3])), scale[u][k], shift[u][k]);
-                }
-                top[k] = fmaxf(x[0], x[1]);
-                move |= top[k] > ref[k] + 15.0f;
+                top[k] = max_of_3(s[0][k][0], s[0][k][1], max_of_3(s[0][k][2], s[0][k][3], max_of_3(s[1][k][0], s[1][k][1], max_of_3(s[1][k][2], s[1][k][3], s[1][k][3]))));
+                move |= top[k] > over[k];
             }
             if (__any(move)) {
 #pragma unroll
                 for (int k = 0; k < RT; ++k) {
                     float t = fmaxf(top[k], __shfl_xor(top[k], 16));
                     t = fmaxf(t, __shfl_xor(t, 32));
-                    const float next = fmaxf(ref[k], t - 7.0f);
-                    const float shrink = exp2_fast(ref[k] - next);
-                    ref[k] = next;
+                    // up for a row that has sums, either way for one that has none
+                    const float up = t > over[k] ? t - 7.0f : 0.0f;
+                    const float shrink = over[k] == kLowest ? 0.0f : exp2_fast(-up);
+                    over[k] = t > over[k] ? 15.0f : over[k];
+                    ref[k] += up;
                     den[k] *= shrink;
+#pragma unroll
+                    for (int u = 0; u < 2; ++u) {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) s[u][k][i] -= up;
+                    }
 #pragma unroll
                     for (int i = 0; i < CH * 4; ++i) acc[k][i] *= shrink;
                 }
@@ -741,11 +750,10 @@ __global__ __launch_bounds__(256, 2) void k_kv_attend_many(Attend a)
             for (int k = 0; k < RT; ++k) {
 #pragma unroll
                 for (int u = 0; u < 2; ++u) {
-                    const float from = shift[u][k] - ref[k];
                     float x[4];
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
-                        x[i] = exp2_fast(fmaf(s[u][k][i], scale[u][k], from));
+                        x[i] = exp2_fast(s[u][k][i]);
                         w[k][u * 4 + i] = static_cast<_Float16>(x[i]);
                     }
                     const float sum = (x[0] + x[1]) + (x[2] + x[3]);
@@ -801,7 +809,7 @@ __global__ __launch_bounds__(256, 2) void k_kv_attend_many(Attend a)
                 *reinterpret_cast<f32x4*>(&a.partial[cell * P + i * 16 + quarter * 4]) = acc[k][i];
             }
             if (quarter == 0) {
-                a.stats[cell * 2] = ref[k];
+                a.stats[cell * 2] = over[k] == kLowest ? kLowest : ref[k];
                 a.stats[cell * 2 + 1] = den[k];
             }
         }
@@ -2079,15 +2087,23 @@ bool run_select(Select& a, bool one, hipStream_t stream)
 }
 
 template <typename T, int CH>
-void launch_attend(Attend a, const Cut& k, bool accumulate, hipStream_t stream)
+bool launch_attend(Attend a, const Cut& k, bool accumulate, hipStream_t stream)
 {
     constexpr int RT = CH == 1 ? 4 : CH == 2 ? 3 : 2;
     const std::uint32_t groups = k.units * a.pairs;
     if (k.many != 0) {
         const std::size_t lds = (CH <= 2 ? 32 : 16) * 1024 * CH;
+        if (!lds_allowed(reinterpret_cast<const void*>(&k_kv_attend_many<T, CH, RT>), lds)) {
+            return false;
+        }
         hipLaunchKernelGGL((k_kv_attend_many<T, CH, RT>), dim3(groups, k.splits), dim3(256), lds, stream, a);
     } else {
         const std::size_t lds = 4 * k.rows * (CH * 64 + 4) * sizeof(float);
+        const void* kernel = accumulate ? reinterpret_cast<const void*>(&k_kv_attend<T, CH, 4, true>)
+                                        : reinterpret_cast<const void*>(&k_kv_attend<T, CH, 4, false>);
+        if (!lds_allowed(kernel, lds)) {
+            return false;
+        }
         if (accumulate) {
             hipLaunchKernelGGL((k_kv_attend<T, CH, 4, true>), dim3(groups, k.splits), dim3(256), lds, stream, a);
         } else {
@@ -2111,18 +2127,20 @@ void launch_attend(Attend a, const Cut& k, bool accumulate, hipStream_t stream)
         const std::uint32_t z = a.b.width / 64 < 65535 ? (a.b.width + 63) / 64 : 65535;
         hipLaunchKernelGGL((k_kv_weigh_again<T, CH>), dim3(few.units * a.pairs, z), dim3(256), 0, stream, a);
     }
+    return true;
 }
 
 template <typename T>
 int run_attend(const Attend& a, const Cut& k, bool accumulate, hipStream_t stream)
 {
+    bool ok = false;
     switch (a.c.dims / 64) {
-    case 1: launch_attend<T, 1>(a, k, accumulate, stream); break;
-    case 2: launch_attend<T, 2>(a, k, accumulate, stream); break;
-    case 3: launch_attend<T, 3>(a, k, accumulate, stream); break;
-    default: launch_attend<T, 4>(a, k, accumulate, stream); break;
+    case 1: ok = launch_attend<T, 1>(a, k, accumulate, stream); break;
+    case 2: ok = launch_attend<T, 2>(a, k, accumulate, stream); break;
+    case 3: ok = launch_attend<T, 3>(a, k, accumulate, stream); break;
+    default: ok = launch_attend<T, 4>(a, k, accumulate, stream); break;
     }
-    return checked(hipGetLastError());
+    return ok ? checked(hipGetLastError()) : HBFSIM_CUDA_ERROR;
 }
 
 }  // namespace
