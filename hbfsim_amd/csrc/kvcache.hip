@@ -120,6 +120,24 @@ struct Group {
     std::int32_t row;          // batch row of token `from`
     std::int64_t seen;         // tokens of the cache that token `from` attends to
 };
+// The last of n indices whose base (not decreasing) is not above `value`, 0 if
+// there is none.  A wave compares 64 of them at a time, so that up to 64
+// sequences cost one trip to memory and 4096 two; all lanes take part.
+template <typename F>
+__device__ inline std::uint32_t last_not_above(std::uint32_t n, std::uint32_t value, F base)
+{
+    const std::uint32_t lane = threadIdx.x % kWave;
+    std::uint32_t lo = 0;
+    while (n > 1) {
+        const std::uint32_t step = (n + kWave - 1) / kWave;
+        const unsigned long long votes = __ballot(lane * step < n && base(lo + lane * step) <= value);
+        const std::uint32_t at = votes == 0 ? 0 : (63 - static_cast<std::uint32_t>(__clzll(static_cast<long long>(votes)))) * step;
+        lo += at;
+        n = n - at < step ? n - at : step;
+        if (votes == 0) break;
+    }
+    return __builtin_amdgcn_readfirstlane(lo);
+}
 __device__ inline std::uint32_t slot_base(const Batch& b, std::uint32_t s, std::uint32_t per)
 {
     return static_cast<std::uint32_t>(b.first[s]) / per + s;
@@ -133,16 +151,7 @@ __device__ inline bool find_group(const Batch& b, std::uint32_t slot, std::uint3
         total = 1;
         g->from = 0;
     } else {
-        std::uint32_t lo = 0, hi = b.seqs;  // the last sequence whose base is not above slot
-        while (hi - lo > 1) {
-            const std::uint32_t mid = (lo + hi) / 2;
-            if (slot_base(b, mid, per) <= slot) {
-                lo = mid;
-            } else {
-                hi = mid;
-            }
-        }
-        s = lo;
+        s = last_not_above(b.seqs, slot, [&](std::uint32_t i) { return slot_base(b, i, per); });
         begin = b.first[s];
         total = b.first[s + 1] - begin;
         const std::uint32_t base = slot_base(b, s, per);
@@ -1066,16 +1075,7 @@ __device__ inline bool find_write(const Append& a, std::uint32_t slot, Write* w)
         const auto base = [&](std::uint32_t i) {
             return static_cast<std::uint32_t>(a.b.first[i]) / t + 2 * i;
         };
-        std::uint32_t lo = 0, hi = a.b.seqs;
-        while (hi - lo > 1) {
-            const std::uint32_t mid = (lo + hi) / 2;
-            if (base(mid) <= slot) {
-                lo = mid;
-            } else {
-                hi = mid;
-            }
-        }
-        s = lo;
+        s = last_not_above(a.b.seqs, slot, base);
         if (slot < base(s)) {
             return false;
         }
@@ -1750,16 +1750,8 @@ __global__ __launch_bounds__(256) void k_kv_pick(Select a)
     const std::uint32_t token = blockIdx.x / a.c.kv_heads;
     std::uint32_t slot = token;
     if (a.b.first != nullptr) {
-        std::uint32_t lo = 0, hi = a.b.seqs;
-        while (hi - lo > 1) {
-            const std::uint32_t mid = (lo + hi) / 2;
-            if (static_cast<std::uint32_t>(a.b.first[mid]) <= token) {
-                lo = mid;
-            } else {
-                hi = mid;
-            }
-        }
-        slot = token + lo;  // slot_base with one token per slot
+        // slot_base with one token per slot
+        slot = token + last_not_above(a.b.seqs, token, [&](std::uint32_t i) { return static_cast<std::uint32_t>(a.b.first[i]); });
     }
     Group g;
     const std::uint32_t nb = find_group(a.b, slot, 1, &g) ? select_blocks(a, g.seen) : 0;
