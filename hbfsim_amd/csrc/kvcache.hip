@@ -366,6 +366,11 @@ __device__ inline float lane_float(float x, int lane)
 // up one tile of the wave's next 64 (block, scales), so the loop itself has no
 // dependent loads; the keys of the pair of tiles after this one are on their
 // way while its softmax runs, the values while the next scores do.
+// It reads the codes once and is bound by HBM: 64 sequences of 1024..32768
+// tokens (2.44 GB) in 424 us, 5.75 TB/s; one of 262,147 (0.54 GB) in 89 us,
+// 6.07 TB/s (a sum over 4 GiB reaches 6.14 here, a copy 4.79 read and
+// written).  16 rows of a product serve 1 to 16 query rows alike, since the
+// matrix units are idle otherwise.
 // kWeigh: each tile's sum of a row's weights is left behind as one logarithm,
 // from which k_kv_weigh makes probabilities once the row's denominator is known.
 // kOnce: no other workgroup reads the same codes, which then pass the caches
@@ -575,6 +580,14 @@ __global__ __launch_bounds__(kWaves * kWave, CH <= 2 ? 4 : CH == 3 ? 2 : 1) void
 // f16 once for all of them and keep in LDS in lane order (a 16-byte read per
 // lane per operand, free of conflicts, two buffers), and each keeps RT tiles of
 // 16 rows in registers, so that an operand read serves RT products.
+// 16 chunks of 2,048 tokens over 16,384 (8.2e12 operations) take 8.2 ms, 1,003
+// TFLOP/s (a large library product reaches 1,420 here); two chunks of about
+// 2,000 over 12,001..16,384 take 1.02-1.15 ms by box, the last round of
+// workgroups partly empty.  The matrix units are busy 38 % of the time, the
+// vector units 58 %: 180 vector instructions a pair of tiles (24 exponentials;
+// scale, maximum, sum and rounding of 24 scores a lane; widening) beside 48
+// products, and vector work runs at half rate while the matrix unit of its
+// SIMD does, so that their sum bounds it more than either.
 template <typename T, int CH, int RT>
 __global__ __launch_bounds__(256, 2) void k_kv_attend_many(Attend a)
 {
@@ -934,7 +947,7 @@ __global__ __launch_bounds__(256) void k_kv_merge(Attend a)
 // weight[block, head] += the probabilities of the unit's rows over the block,
 // from the tiles' sums: one thread per block.  Sums are f32 within a block and
 // joined as integers, so the order in which blocks of shared prefixes are
-// reached does not change them.
+// reached does not change them.  24 sequences of 777..20,001 tokens: 7.5 us.
 __device__ inline void add_weight(const Attend& a, std::size_t bh, float sum)
 {
     if (sum < 1e9f) {  // a sum that is not a number adds nothing
@@ -1165,7 +1178,9 @@ __device__ inline std::uint32_t from_quad(std::uint32_t x)  // lane kLane's of e
 // the block: a lane holds token lane % 16's dims 16 (lane / 16) .. + 15 of
 // every 64 in registers from the one read of the input to its codes.  That is
 // the keys' layout already; values are transposed four tokens by four dims
-// within four lanes.
+// within four lanes.  Bound by memory: 27,600 tokens of 8 kv heads x 128 (170 MB
+// in and out) take 57 us, 3.0 TB/s; 64 tokens 6.4 us, the way from the table
+// through the scale to the row.
 template <typename T, int CH>
 __global__ __launch_bounds__(512) void k_kv_append(Append a)
 {
@@ -1316,7 +1331,7 @@ __global__ __launch_bounds__(512) void k_kv_append(Append a)
 // Blocks back as values: one wave per (entry, kv head, 16 tokens, keys or
 // values).  Keys: a lane widens a token's 16 dims of every 64 and stores them
 // as they are.  Values: four lanes transpose four tokens by four dims first,
-// as append does.
+// as append does.  The blocks of those 27,600 tokens (171 MB) take 37 us, 4.6 TB/s.
 template <typename T>
 __device__ inline void store_16(T* row, int d0, int dim, bool vector, std::uint32_t w0, std::uint32_t w1, std::uint32_t w2,
                                 std::uint32_t w3, float scale)
@@ -1647,7 +1662,10 @@ __device__ void write_choice(const Select& a, const std::uint32_t* keys, std::ui
 }
 
 // Scores and choice of one query token and kv head in one workgroup, the keys
-// in LDS.
+// in LDS.  64 sequences of 1024..32768 tokens (155 MB of bounds) take 66 us: the
+// bounds of a block and head are 256 bytes at random places, which come at
+// about 3 TB/s (42 us of it; in order of address 40, without the scales 47),
+// and the choice takes the rest.
 template <typename T, int CH>
 __global__ __launch_bounds__(kPickThreads) void k_kv_select(Select a)
 {
@@ -1692,7 +1710,9 @@ __global__ __launch_bounds__(kPickThreads) void k_kv_select(Select a)
     write_choice<kPickThreads>(a, s_keys, nb, a.selected + static_cast<std::size_t>(blockIdx.x) * a.count);
 }
 
-// Scores of groups of up to 8 tokens of a sequence, to global memory.
+// Scores of groups of up to 8 tokens of a sequence, to global memory.  1,001
+// tokens of 4 kv heads over 1,001 blocks: 26 us, the codes' preparation and
+// the way through the table more than the bounds; their choice 21 us.
 template <typename T, int CH>
 __global__ __launch_bounds__(256) void k_kv_score(Select a)
 {
@@ -1779,7 +1799,9 @@ struct Evict {
 
 // One workgroup per sequence, the keys in LDS if they fit (kStaged).  A
 // block's key is its summed weight plus 1; a table entry that names no block
-// has key 0 and goes first.
+// has key 0 and goes first.  Latency bounds it: 6.6 us for 3 sequences of up to
+// 313 blocks, 13.6 for 64 of up to 2,048 (5.3 MB), of which each digit's
+// histogram and scan is about 1.5.
 template <bool kStaged>
 __global__ __launch_bounds__(kPickThreads) void k_kv_evict(Evict a)
 {
@@ -1829,8 +1851,8 @@ __global__ __launch_bounds__(kPickThreads) void k_kv_evict(Evict a)
 
 // ---- host -----------------------------------------------------------------
 
-// A launch dimension holds fewer than 2^32 threads.
-constexpr std::size_t kMostGroups = std::size_t{1} << 23;
+// A launch dimension holds fewer than 2^32 threads, a workgroup at most 1024.
+constexpr std::size_t kMostGroups = (std::size_t{1} << 22) - 1;
 
 bool aligned16(const void* p) { return (reinterpret_cast<std::uintptr_t>(p) & 15u) == 0; }
 
@@ -1905,7 +1927,9 @@ struct Cut {
 
 std::size_t up256(std::size_t x) { return (x + 255) & ~std::size_t{255}; }
 
-// Row tiles per wave that fit the registers of two waves per SIMD.
+// Row tiles per wave that fit the registers of two waves per SIMD (16 chunks
+// of 2048 tokens over 16384, D = 64: 6.03 / 5.39 / 5.73 ms with 3 / 4 / 5; 8 of
+// 1024 over 8192, D = 256: 3.62 / 3.35 ms with 1 / 2).
 std::uint32_t many_tiles(std::uint32_t dims) { return dims <= 64 ? 4 : dims <= 128 ? 3 : 2; }
 
 Cut cut_few(const Cache& c, const Batch& b, std::uint32_t heads, std::uint32_t count)
@@ -1918,10 +1942,13 @@ Cut cut_few(const Cache& c, const Batch& b, std::uint32_t heads, std::uint32_t c
     k.units = b.first == nullptr ? b.seqs : b.tokens / k.per + b.seqs;
     const std::uint64_t longest = static_cast<std::uint64_t>(count != 0 ? count : b.width) * c.tokens;
     const std::uint64_t pairs = static_cast<std::uint64_t>(k.units) * c.kv_heads * k.row_tiles;
-    // Splits of 2048 tokens, shorter where they would not fill the card; up to
-    // 768 tokens take one, whose few microseconds a second launch would cost.
+    // Splits of 2048 tokens (64 sequences of 1024..32768 tokens: 464 us, with
+    // 1024 478, with 4096 462 and less to share out), shorter where they would
+    // not fill the card.  Up to 1024 tokens take one and no second launch: one
+    // sequence of 1024 takes 12.0 us in one split, 7.6 + 3.5 and a launch in
+    // four; of 1536, 15.3 against 7.9 + 4.5.
     std::uint64_t split = 2048;
-    while (longest > 768 && split > 256 && pairs * ((longest + split - 1) / split) < 1024) split /= 2;
+    while (longest > 1024 && split > 256 && pairs * ((longest + split - 1) / split) < 1024) split /= 2;
     k.split = static_cast<std::uint32_t>(split);
     k.splits = longest == 0 ? 1 : static_cast<std::uint32_t>((longest + split - 1) / split);
     return k;
@@ -1940,10 +1967,12 @@ Cut cut_many(const Cache& c, const Batch& b, std::uint32_t heads)
     const std::uint64_t longest = static_cast<std::uint64_t>(b.width) * c.tokens;
     const std::uint64_t groups = static_cast<std::uint64_t>(k.units) * c.kv_heads;
     // Two workgroups fit a CU; splits fill the last round of them, each at
-    // the price of its partial sums' round trip.
+    // the price of its partial sums' round trip: two chunks of about 2,000
+    // tokens over 12,001..16,384 take 1,226 us in 1 split, 1,202 in 2, 1,181 in
+    // 3, 1,196 in 4, 1,353 in 10.
     std::uint64_t best = 1;
     double score = 0.0;
-    for (std::uint64_t s = 1; s <= 8 && (s == 1 || longest / s >= 512); ++s) {
+    for (std::uint64_t s = 1; s <= 16 && (s == 1 || longest / s >= 256); ++s) {
         const double rounds = static_cast<double>(groups * s) / 512.0;
         const double whole = static_cast<double>(static_cast<std::uint64_t>((groups * s + 511) / 512));
         const double got = rounds / whole / (1.0 + 0.03 * static_cast<double>(s - 1));
@@ -1961,10 +1990,15 @@ Cut cut_many(const Cache& c, const Batch& b, std::uint32_t heads)
 Cut cut_attend(const Cache& c, const Batch& b, std::uint32_t heads, std::uint32_t count, bool accumulate)
 {
     const std::uint32_t group = heads / c.kv_heads;
-    // Many rows once a sequence's share of the step fills half a workgroup's.
+    // The many-row form once a sequence's share of the step comes near a
+    // workgroup's rows: 16 sequences of 8192 tokens (4 heads a kv head, D = 128)
+    // take 178 us in the few-row form and 224 in this with 32 tokens (128 of
+    // 192 rows), 260 and 229 with 48, 512 and 302 with 96.  One sequence of 4096
+    // tokens, which fills the card with neither: 79 and 55 with 400 tokens, but
+    // 23 and 27 with 48.
     const std::uint64_t room = 4 * many_tiles(c.dims) * 16;
     const bool many = b.first != nullptr && count == 0 && group <= room &&
-                      static_cast<std::uint64_t>(b.tokens) * group * 2 >= room * b.seqs;
+                      static_cast<std::uint64_t>(b.tokens) * group * 5 >= room * b.seqs * 4;
     Cut k = many ? cut_many(c, b, heads) : cut_few(c, b, heads, count);
     if (k.splits > 1) {
         const std::size_t cells = static_cast<std::size_t>(k.units) * c.kv_heads * k.row_tiles * k.splits * k.rows;
@@ -2029,7 +2063,9 @@ bool lds_allowed(const void* kernel, std::size_t bytes)
 }
 
 // One workgroup per row does it all where there are rows enough to fill the
-// card and no other token reads the same bounds.
+// card and no other token reads the same bounds: 64 sequences of 16384..32768
+// tokens and 8 kv heads take 72.5 us in one launch and 63 + 12 in two, 32 take
+// 42 and 35 + 11.5, 16 take 29 and 18 + 11, 8 take 29 and 13 + 10.
 bool select_in_one(const Cache& c, const Batch& b)
 {
     return b.first == nullptr && static_cast<std::uint64_t>(b.tokens) * c.kv_heads >= 128 &&
@@ -2104,7 +2140,8 @@ bool launch_attend(Attend a, const Cut& k, bool accumulate, hipStream_t stream)
         }
         hipLaunchKernelGGL(kernel, dim3(groups, k.splits), dim3(256), lds, stream, a);
     }
-    if (k.splits > 16) {
+    // 24 sequences of 12 / 16 / 32 splits: 5.3 / 5.5 / 6.4 us by rows, 5.3 / 6.2 / 9.9 by quads of dims
+    if (k.splits > 12) {
         hipLaunchKernelGGL((k_kv_merge<T>), dim3(groups, k.rows), dim3(256), 0, stream, a);
     } else if (k.splits > 1) {
         const std::uint32_t at_once = 1024 / a.c.dims;
@@ -2265,7 +2302,8 @@ HBF_API int hbfsim_amd_kv_attend(const hbfsim_amd_kv_cache* cache, const hbfsim_
     }
     const Cut few = cut_few(a.c, a.b, heads, count);
     if (static_cast<std::uint64_t>(k.units) * a.c.kv_heads * k.row_tiles > kMostGroups || k.splits > 65535 ||
-        (accumulate != 0 && static_cast<std::uint64_t>(few.units) * a.c.kv_heads * few.row_tiles > kMostGroups)) {
+        (accumulate != 0 && (static_cast<std::uint64_t>(few.units) * a.c.kv_heads * few.row_tiles > kMostGroups ||
+                             a.b.width > 65535 * 256u))) {
         return HBFSIM_UNSUPPORTED;
     }
     a.q = d_q;
@@ -2336,7 +2374,7 @@ HBF_API int hbfsim_amd_kv_select(const hbfsim_amd_kv_cache* cache, const hbfsim_
         (need != 0 && (d_workspace == nullptr || !aligned16(d_workspace)))) {
         return HBFSIM_INVALID_ARGUMENT;
     }
-    if (static_cast<std::uint64_t>(a.b.tokens) * a.c.kv_heads > kMostGroups / 2) {
+    if (static_cast<std::uint64_t>(a.b.tokens) * a.c.kv_heads > kMostGroups) {
         return HBFSIM_UNSUPPORTED;
     }
     a.q = d_q;
@@ -2373,7 +2411,7 @@ HBF_API int hbfsim_amd_kv_evict(const int64_t* d_weight, uint32_t blocks, uint32
     if (seqs == 0) {
         return HBFSIM_OK;
     }
-    if (seqs > kMostGroups / 2) {
+    if (seqs > kMostGroups) {
         return HBFSIM_UNSUPPORTED;
     }
     const std::size_t need = static_cast<std::size_t>(seqs) * width * sizeof(unsigned long long);

@@ -24,7 +24,8 @@ def filled(rng, kv, dim, t, lens, spread=0.3, spare=1):
 
 @pytest.mark.parametrize("kv,g,dim,t,dtype", [(1, 4, 37, 16, "bf16"), (2, 3, 192, 32, "f16"),
                                               (1, 48, 128, 16, "bf16"), (1, 200, 64, 64, "f16"),
-                                              (2, 1, 256, 128, "bf16"), (1, 130, 256, 16, "f16")])
+                                              (2, 1, 256, 128, "bf16"), (2, 2, 256, 32, "bf16"),
+                                              (1, 130, 256, 16, "f16")])
 def test_many_rows_of_odd_shapes(kv, g, dim, t, dtype):
     """Odd dims and groups that leave rows of a workgroup empty, or need one
     token each; a long and a short sequence, and one whose queries see less
