@@ -1928,9 +1928,10 @@ struct Cut {
 std::size_t up256(std::size_t x) { return (x + 255) & ~std::size_t{255}; }
 
 // Row tiles per wave that fit the registers of two waves per SIMD (16 chunks
-// of 2048 tokens over 16384, D = 64: 6.03 / 5.39 / 5.73 ms with 3 / 4 / 5; 8 of
-// 1024 over 8192, D = 256: 3.62 / 3.35 ms with 1 / 2).
-std::uint32_t many_tiles(std::uint32_t dims) { return dims <= 64 ? 4 : dims <= 128 ? 3 : 2; }
+// of 2048 tokens over 16384, D = 64: 6.03 / 5.39 / 5.73 ms with 3 / 4 / 5, D =
+// 128: 9.25 / 8.5 with 2 / 3; 8 of 1024 over 8192, D = 256: 3.73 / 3.92 with 1 /
+// 2, of which two spill).
+std::uint32_t many_tiles(std::uint32_t dims) { return 5 - dims / 64; }
 
 Cut cut_few(const Cache& c, const Batch& b, std::uint32_t heads, std::uint32_t count)
 {
@@ -1967,15 +1968,17 @@ Cut cut_many(const Cache& c, const Batch& b, std::uint32_t heads)
     const std::uint64_t longest = static_cast<std::uint64_t>(b.width) * c.tokens;
     const std::uint64_t groups = static_cast<std::uint64_t>(k.units) * c.kv_heads;
     // Two workgroups fit a CU; splits fill the last round of them, each at
-    // the price of its partial sums' round trip: two chunks of about 2,000
-    // tokens over 12,001..16,384 take 1,226 us in 1 split, 1,202 in 2, 1,181 in
-    // 3, 1,196 in 4, 1,353 in 10.
+    // the price of its partial sums' round trip.  Chunks of 2,048 tokens over
+    // 16,384 (8 kv heads, D = 128) take, with 1 / 2 / 3 / 4 splits and their
+    // merge, 838 / 726 / 708 / 697 us for one of them (0.7 rounds), 1,303 /
+    // 1,261 / 1,260 / 1,271 for two, 1,927 / 1,776 / 1,767 / 1,775 for three,
+    // 3,350 / 3,278 / 3,321 / 3,384 for six (4.1), 4,086 / 4,283 for eight.
     std::uint64_t best = 1;
     double score = 0.0;
-    for (std::uint64_t s = 1; s <= 16 && (s == 1 || longest / s >= 256); ++s) {
+    for (std::uint64_t s = 1; s <= 16 && (s == 1 || (groups < 2048 && longest / s >= 256)); ++s) {
         const double rounds = static_cast<double>(groups * s) / 512.0;
         const double whole = static_cast<double>(static_cast<std::uint64_t>((groups * s + 511) / 512));
-        const double got = rounds / whole / (1.0 + 0.03 * static_cast<double>(s - 1));
+        const double got = rounds / whole / (s == 1 ? 1.0 : 1.0 + 0.03 * static_cast<double>(s));
         if (got > score * 1.02) {
             score = got;
             best = s;
@@ -2121,7 +2124,7 @@ bool run_select(Select& a, bool one, hipStream_t stream)
 template <typename T, int CH>
 bool launch_attend(Attend a, const Cut& k, bool accumulate, hipStream_t stream)
 {
-    constexpr int RT = CH == 1 ? 4 : CH == 2 ? 3 : 2;
+    constexpr int RT = 5 - CH;
     const std::uint32_t groups = k.units * a.pairs;
     if (k.many != 0) {
         const std::size_t lds = (CH <= 2 ? 32 : 16) * 1024 * CH;
