@@ -1662,10 +1662,11 @@ __device__ void write_choice(const Select& a, const std::uint32_t* keys, std::ui
 }
 
 // Scores and choice of one query token and kv head in one workgroup, the keys
-// in LDS.  64 sequences of 1024..32768 tokens (155 MB of bounds) take 66 us: the
-// bounds of a block and head are 256 bytes at random places, which come at
-// about 3 TB/s (42 us of it; in order of address 40, without the scales 47),
-// and the choice takes the rest.
+// in LDS.  64 sequences of 1024..32768 tokens (155 MB of bounds) take 66 us, 24
+// of them without the bounds and 60 without the choice; 64 of equal length 23.5
+// us at 8192 tokens, 45.7 at 16384 and 80.3 at 32768, so that once running the
+// bounds of a block and head, 256 bytes at random places, come at 3.9 TB/s
+// (about 5 with the cache lines of their scales), and the longest rows end last.
 template <typename T, int CH>
 __global__ __launch_bounds__(kPickThreads) void k_kv_select(Select a)
 {
