@@ -582,8 +582,8 @@ __global__ __launch_bounds__(kWaves * kWave, CH <= 2 ? 4 : CH == 3 ? 2 : 1) void
 // 16 rows in registers, so that an operand read serves RT products.
 // 16 chunks of 2,048 tokens over 16,384 (8.2e12 operations) take 8.2 ms, 1,003
 // TFLOP/s (a large library product reaches 1,420 here); two chunks of about
-// 2,000 over 12,001..16,384 take 1.02-1.15 ms by box, the last round of
-// workgroups partly empty.  The matrix units are busy 43 % of the time, the
+// 2,000 over 12,001..16,384 take 1.01-1.16 ms, the last
+// of two rounds of workgroups partly empty.  The matrix units are busy 43 % of the time, the
 // vector units 59 %: 180 vector instructions a pair of tiles (24 exponentials;
 // scale, maximum, sum and rounding of 24 scores a lane; widening) beside 48
 // products, and vector work runs at half rate while the matrix unit of its
