@@ -212,3 +212,28 @@ def test_evict_first_and_last_alone():
         want = kr.evict(weight, table, [400, 30], keep, 16, first, last)
         for a, b in zip(got, want):
             np.testing.assert_array_equal(a.cpu().numpy(), b)
+
+
+@pytest.mark.parametrize("dim", [64, 128, 192, 256])
+@pytest.mark.parametrize("new", [1, 300])
+def test_weights_far_below_the_largest_still_count(dim, new):
+    """One token 21.5 bits above 30,000 others, whose weights lie below the
+    normal numbers of 16 bits: they are a hundredth of the denominator and all
+    of the second half of the dims.  Their rounding is at most 2^-10 of them,
+    the largest's and the output's 2^-11."""
+    n, t = 30_000, 16
+    k = torch.zeros((n + 1, 1, dim))
+    v = torch.ones((n + 1, 1, dim))
+    k[0, 0, 0] = 21.5 * np.log(2)
+    v[0, 0, dim // 2:] = 0
+    blocks = -(-(n + 1) // t)
+    cache = kvcache.KvCache(blocks, 1, dim, t)
+    table, lens = ints(np.arange(blocks)[None]), ints([n + 1])
+    cache.append(k.cuda(), v.cuda(), table, lens, ints([0, n + 1]))
+    q = torch.zeros((new, 1, dim), dtype=torch.float16)
+    q[:, 0, 0] = 1
+    got = cache.attend(q.cuda(), table, lens, ints([0, new]), scale=1.0)[-1, 0].double().cpu()
+    rest = n * 2.0 ** -21.5
+    want = torch.ones(dim, dtype=torch.float64)
+    want[dim // 2:] = rest / (1 + rest)
+    assert ((got - want).abs() <= 2.0 ** -8 * want).all(), (got - want).abs().max()
