@@ -782,17 +782,10 @@ __global__ __launch_bounds__(256, 2) void k_kv_attend_many(Attend a)
                         x[i] = exp2_fast(s[u][k][i]);
                         w[k][u * 4 + i] = static_cast<_Float16>(x[i]);
                     }
-                    // Two rounded weights and the sum in one instruction: 8 chunks of 1024 tokens
-                    // over 8192 at 256 dims (one row tile) 3.31 ms, with the adds 3.56; at 128
-                    // dims (three) 8.83 and 8.12 for 16 of 2048 over 16384, as registers spill.
-                    float sum;
-                    if constexpr (RT == 1) {
-                        constexpr f16x2 one = {static_cast<_Float16>(1.0f), static_cast<_Float16>(1.0f)};
-                        const f16x2 lo = {w[k][u * 4], w[k][u * 4 + 1]}, hi = {w[k][u * 4 + 2], w[k][u * 4 + 3]};
-                        sum = __builtin_amdgcn_fdot2(hi, one, __builtin_amdgcn_fdot2(lo, one, 0.0f, false), false);
-                    } else {
-                        sum = (x[0] + x[1]) + (x[2] + x[3]);
-                    }
+                    // The f32 weights, not the rounded ones that the products take: in a block
+                    // of a small value scale these lose bits or vanish, and with them the
+                    // block's whole share, since inv_scale brings the sum back up.
+                    const float sum = (x[0] + x[1]) + (x[2] + x[3]);
                     den[k] = fmaf(sum, lane_float(seen_info.inv_scale, tile + u), den[k]);
                 }
             }
