@@ -43,6 +43,12 @@ def _refuse(rc: int, what: str) -> None:
     nat.check(rc, what)
 
 
+def _on_gpu(device: Any) -> None:
+    """Kernels follow the tensors' addresses: only a GPU's may reach them."""
+    if device.type != "cuda":
+        raise ValueError(f"the cache is on {device}, not on a GPU")
+
+
 def _handle(stream: Any, device: Any) -> int:
     """The stream's handle: the device's current one, a torch stream's, or a
     handle already.  (The raw accessor costs a tenth of building a Stream.)"""
@@ -117,6 +123,7 @@ def evict(weight: Any, table: Any, lens: Any, keep: int, block_tokens: int = 16,
         raise ValueError(f"{lens.shape[0]} lengths for {seqs} sequences")
     if min(keep, keep_first, keep_last) < 0:
         raise ValueError("keep, keep_first and keep_last must not be negative")
+    _on_gpu(device)
     stride = table.stride(0) if seqs > 1 else width
     out_table, freed = torch.empty((2, seqs, width), dtype=torch.int32, device=device).unbind()
     out_lens, count = torch.empty((2, seqs), dtype=torch.int32, device=device).unbind()
@@ -230,6 +237,7 @@ class KvCache:
         if self._rows(v, self.kv_heads, "v") != (tokens, self.kv_heads, kind):
             raise ValueError("k and v differ in tokens or type")
         b = _batch(table, lens, first, tokens, self.device)
+        _on_gpu(self.device)
         strides = (ctypes.c_int64 * 4)(k.stride(0), k.stride(1), v.stride(0), v.stride(1))
         _refuse(self._lib.hbfsim_amd_kv_append(self._ref, ctypes.byref(b), k.data_ptr(),
                                                v.data_ptr(), kind, strides,
@@ -242,6 +250,7 @@ class KvCache:
         _ints(blocks, "blocks", self.device, 1)
         if dtype not in _TYPES:
             raise ValueError("dtype must be bfloat16, float16 or float32")
+        _on_gpu(self.device)
         n = blocks.shape[0]
         kv = torch.empty((2, n, self.kv_heads, self.block_tokens, self.head_dim), dtype=dtype,
                          device=self.device)
@@ -277,13 +286,14 @@ class KvCache:
             if accumulate:
                 raise ValueError("weights accumulate over every visible block, not a selection")
             chosen = selected.data_ptr()
+        if out is not None and (tuple(out.shape) != tuple(q.shape) or out.dtype != q.dtype
+                                or out.device != self.device or not out.is_contiguous()):
+            raise ValueError("out must be a contiguous tensor of q's shape and type")
+        _on_gpu(self.device)
         if out is None:
             out = torch.empty((tokens, heads, self.head_dim), dtype=q.dtype, device=self.device)
             if stream is not None:
                 _used_on(stream, out)
-        elif tuple(out.shape) != tuple(q.shape) or out.dtype != q.dtype \
-                or out.device != self.device or not out.is_contiguous():
-            raise ValueError("out must be a contiguous tensor of q's shape and type")
         ref = ctypes.byref(b)
         sizes = (b.seqs, b.table_width, tokens, first is None, heads, count, accumulate)
         need = self._need.get(sizes)
@@ -311,6 +321,7 @@ class KvCache:
         if min(count, keep_first, keep_last) < 0:
             raise ValueError("count, keep_first and keep_last must not be negative")
         b = _batch(table, lens, first, tokens, self.device)
+        _on_gpu(self.device)
         ref = ctypes.byref(b)
         out = torch.empty((tokens, self.kv_heads, count), dtype=torch.int32, device=self.device)
         if stream is not None:
