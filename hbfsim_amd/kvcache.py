@@ -19,6 +19,7 @@ No counterpart in the reference.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import math
 from typing import Any
@@ -43,38 +44,47 @@ def _refuse(rc: int, what: str) -> None:
     nat.check(rc, what)
 
 
-def _on_gpu(device: Any) -> None:
-    """Kernels follow the tensors' addresses: only a GPU's may reach them."""
+_HERE = contextlib.nullcontext()
+
+
+def _queue(device: Any, stream: Any) -> Any:
+    """Context in which a call allocates and queues its work: `stream` (a torch
+    stream or a handle) is current in it, so that scratch and outputs come from
+    its pool.  A block of the current stream's pool may have work queued there
+    that `stream` is not ordered behind.  Kernels follow the tensors'
+    addresses, so the device has to be a GPU."""
     if device.type != "cuda":
         raise ValueError(f"the cache is on {device}, not on a GPU")
-
-
-def _handle(stream: Any, device: Any) -> int:
-    """The stream's handle: the device's current one, a torch stream's, or a
-    handle already.  (The raw accessor costs a tenth of building a Stream.)"""
     if stream is None:
-        return torch._C._cuda_getCurrentRawStream(device.index)
-    return stream.cuda_stream if hasattr(stream, "cuda_stream") else stream
+        return _HERE
+    if not hasattr(stream, "cuda_stream"):
+        stream = torch.cuda.ExternalStream(stream, device=device)
+    return torch.cuda.stream(stream)
 
 
-def _workspace(nbytes: int, device: Any, stream: Any) -> Any:
+def _handle(device: Any) -> int:
+    """The current stream's handle.  (The raw accessor costs a tenth of
+    building a Stream.)"""
+    return torch._C._cuda_getCurrentRawStream(device.index)
+
+
+def _workspace(nbytes: int, device: Any) -> Any:
     """Scratch of one call, handed back to torch's allocator after it: work
     queued later on the same stream is ordered behind the call."""
-    if nbytes == 0:
-        return None
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
-    if stream is not None:
-        _used_on(stream, ws)
-    return ws
+    return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
 
 
-def _used_on(stream: Any, *tensors: Any) -> None:
-    """Tells torch's allocator that a stream other than the current one uses
-    the tensors, so that none of them is handed out again before it has."""
-    if not hasattr(stream, "cuda_stream"):
-        stream = torch.cuda.ExternalStream(stream, device=tensors[0].device)
-    for t in tensors:
-        t.record_stream(stream)
+def _caller(device: Any, stream: Any) -> Any:
+    """The stream that will read a call's outputs, if it is another than theirs."""
+    return None if stream is None else torch.cuda.current_stream(device)
+
+
+def _hand_over(caller: Any, *tensors: Any) -> None:
+    """Tells torch's allocator that the caller's stream uses the tensors, so
+    that none of them is handed out again on its own before that is done."""
+    if caller is not None:
+        for t in tensors:
+            t.record_stream(caller)
 
 
 def _ints(x: Any, name: str, device: Any, dims: int) -> Any:
@@ -123,19 +133,19 @@ def evict(weight: Any, table: Any, lens: Any, keep: int, block_tokens: int = 16,
         raise ValueError(f"{lens.shape[0]} lengths for {seqs} sequences")
     if min(keep, keep_first, keep_last) < 0:
         raise ValueError("keep, keep_first and keep_last must not be negative")
-    _on_gpu(device)
     stride = table.stride(0) if seqs > 1 else width
-    out_table, freed = torch.empty((2, seqs, width), dtype=torch.int32, device=device).unbind()
-    out_lens, count = torch.empty((2, seqs), dtype=torch.int32, device=device).unbind()
-    ws = _workspace(seqs * width * 8, device, stream)
-    if stream is not None:
-        _used_on(stream, out_table, out_lens)
-    _refuse(nat.load().hbfsim_amd_kv_evict(
-        weight.data_ptr(), weight.shape[0], weight.shape[1], block_tokens, table.data_ptr(),
-        lens.data_ptr(), seqs, width, stride, keep, keep_first, keep_last, out_table.data_ptr(),
-        out_lens.data_ptr(), freed.data_ptr(), count.data_ptr(),
-        ws.data_ptr() if ws is not None else None, seqs * width * 8, _handle(stream, device)),
-        "evict")
+    queue, caller = _queue(device, stream), _caller(device, stream)
+    with queue:
+        out_table, freed = torch.empty((2, seqs, width), dtype=torch.int32, device=device).unbind()
+        out_lens, count = torch.empty((2, seqs), dtype=torch.int32, device=device).unbind()
+        _hand_over(caller, out_table, out_lens)
+        ws = _workspace(seqs * width * 8, device)
+        _refuse(nat.load().hbfsim_amd_kv_evict(
+            weight.data_ptr(), weight.shape[0], weight.shape[1], block_tokens, table.data_ptr(),
+            lens.data_ptr(), seqs, width, stride, keep, keep_first, keep_last,
+            out_table.data_ptr(), out_lens.data_ptr(), freed.data_ptr(), count.data_ptr(),
+            ws.data_ptr() if ws is not None else None, seqs * width * 8, _handle(device)),
+            "evict")
     return out_table, out_lens, freed, count
 
 
@@ -237,11 +247,11 @@ class KvCache:
         if self._rows(v, self.kv_heads, "v") != (tokens, self.kv_heads, kind):
             raise ValueError("k and v differ in tokens or type")
         b = _batch(table, lens, first, tokens, self.device)
-        _on_gpu(self.device)
         strides = (ctypes.c_int64 * 4)(k.stride(0), k.stride(1), v.stride(0), v.stride(1))
-        _refuse(self._lib.hbfsim_amd_kv_append(self._ref, ctypes.byref(b), k.data_ptr(),
-                                               v.data_ptr(), kind, strides,
-                                               _handle(stream, self.device)), "append")
+        with _queue(self.device, stream):
+            _refuse(self._lib.hbfsim_amd_kv_append(self._ref, ctypes.byref(b), k.data_ptr(),
+                                                   v.data_ptr(), kind, strides,
+                                                   _handle(self.device)), "append")
 
     def read(self, blocks: Any, dtype: Any = torch.bfloat16, stream: Any = None) -> tuple:
         """The values that the blocks (int32 ids) stand for: keys and values
@@ -250,18 +260,19 @@ class KvCache:
         _ints(blocks, "blocks", self.device, 1)
         if dtype not in _TYPES:
             raise ValueError("dtype must be bfloat16, float16 or float32")
-        _on_gpu(self.device)
         n = blocks.shape[0]
-        kv = torch.empty((2, n, self.kv_heads, self.block_tokens, self.head_dim), dtype=dtype,
-                         device=self.device)
-        ends = torch.empty((2, n, self.kv_heads, self.head_dim), dtype=dtype, device=self.device)
-        k, v = kv.unbind()
-        low, high = ends.unbind()
-        if stream is not None:
-            _used_on(stream, kv, ends)
-        _refuse(self._lib.hbfsim_amd_kv_read(self._ref, blocks.data_ptr(), n, _TYPES[dtype],
-                                             k.data_ptr(), v.data_ptr(), low.data_ptr(),
-                                             high.data_ptr(), _handle(stream, self.device)), "read")
+        queue, caller = _queue(self.device, stream), _caller(self.device, stream)
+        with queue:
+            kv = torch.empty((2, n, self.kv_heads, self.block_tokens, self.head_dim), dtype=dtype,
+                             device=self.device)
+            ends = torch.empty((2, n, self.kv_heads, self.head_dim), dtype=dtype,
+                               device=self.device)
+            _hand_over(caller, kv, ends)
+            k, v = kv.unbind()
+            low, high = ends.unbind()
+            _refuse(self._lib.hbfsim_amd_kv_read(self._ref, blocks.data_ptr(), n, _TYPES[dtype],
+                                                 k.data_ptr(), v.data_ptr(), low.data_ptr(),
+                                                 high.data_ptr(), _handle(self.device)), "read")
         return k, v, low, high
 
     def attend(self, q: Any, table: Any, lens: Any, first: Any = None, selected: Any = None,
@@ -289,11 +300,7 @@ class KvCache:
         if out is not None and (tuple(out.shape) != tuple(q.shape) or out.dtype != q.dtype
                                 or out.device != self.device or not out.is_contiguous()):
             raise ValueError("out must be a contiguous tensor of q's shape and type")
-        _on_gpu(self.device)
-        if out is None:
-            out = torch.empty((tokens, heads, self.head_dim), dtype=q.dtype, device=self.device)
-            if stream is not None:
-                _used_on(stream, out)
+        queue, caller = _queue(self.device, stream), _caller(self.device, stream)
         ref = ctypes.byref(b)
         sizes = (b.seqs, b.table_width, tokens, first is None, heads, count, accumulate)
         need = self._need.get(sizes)
@@ -303,12 +310,17 @@ class KvCache:
                                                              int(accumulate), ctypes.byref(got)),
                     "attend")
             need = self._remember(sizes, got.value)
-        ws = _workspace(need, self.device, stream)
-        _refuse(self._lib.hbfsim_amd_kv_attend(
-            self._ref, ref, q.data_ptr(), kind, heads, q.stride(0), q.stride(1),
-            1.0 / math.sqrt(self.head_dim) if scale is None else scale, chosen, count,
-            int(accumulate), out.data_ptr(), ws.data_ptr() if ws is not None else None,
-            need, _handle(stream, self.device)), "attend")
+        with queue:
+            if out is None:
+                out = torch.empty((tokens, heads, self.head_dim), dtype=q.dtype,
+                                  device=self.device)
+                _hand_over(caller, out)
+            ws = _workspace(need, self.device)
+            _refuse(self._lib.hbfsim_amd_kv_attend(
+                self._ref, ref, q.data_ptr(), kind, heads, q.stride(0), q.stride(1),
+                1.0 / math.sqrt(self.head_dim) if scale is None else scale, chosen, count,
+                int(accumulate), out.data_ptr(), ws.data_ptr() if ws is not None else None,
+                need, _handle(self.device)), "attend")
         return out
 
     def select(self, q: Any, table: Any, lens: Any, count: int, first: Any = None,
@@ -321,11 +333,8 @@ class KvCache:
         if min(count, keep_first, keep_last) < 0:
             raise ValueError("count, keep_first and keep_last must not be negative")
         b = _batch(table, lens, first, tokens, self.device)
-        _on_gpu(self.device)
+        queue, caller = _queue(self.device, stream), _caller(self.device, stream)
         ref = ctypes.byref(b)
-        out = torch.empty((tokens, self.kv_heads, count), dtype=torch.int32, device=self.device)
-        if stream is not None:
-            _used_on(stream, out)
         sizes = (b.seqs, b.table_width, tokens, first is None)
         need = self._need.get(sizes)
         if need is None:
@@ -333,11 +342,15 @@ class KvCache:
             _refuse(self._lib.hbfsim_amd_kv_select_workspace(self._ref, ref, ctypes.byref(got)),
                     "select")
             need = self._remember(sizes, got.value)
-        ws = _workspace(need, self.device, stream)
-        _refuse(self._lib.hbfsim_amd_kv_select(
-            self._ref, ref, q.data_ptr(), kind, heads, q.stride(0), q.stride(1), count, keep_first,
-            keep_last, out.data_ptr(), ws.data_ptr() if ws is not None else None, need,
-            _handle(stream, self.device)), "select")
+        with queue:
+            out = torch.empty((tokens, self.kv_heads, count), dtype=torch.int32,
+                              device=self.device)
+            _hand_over(caller, out)
+            ws = _workspace(need, self.device)
+            _refuse(self._lib.hbfsim_amd_kv_select(
+                self._ref, ref, q.data_ptr(), kind, heads, q.stride(0), q.stride(1), count,
+                keep_first, keep_last, out.data_ptr(), ws.data_ptr() if ws is not None else None,
+                need, _handle(self.device)), "select")
         return out
 
     def evict(self, table: Any, lens: Any, keep: int, keep_first: int = 1, keep_last: int = 1,

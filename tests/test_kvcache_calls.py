@@ -4,6 +4,7 @@ from __future__ import annotations
 
 import pytest
 import torch
+from torch._subclasses.fake_tensor import FakeTensorMode
 
 from hbfsim_amd import _native as nat
 from hbfsim_amd import kvcache
@@ -36,7 +37,7 @@ def every_call(cache, device, **kw):
             ("append", lambda: cache.append(k, k, table, lens, first, **kw)),
             ("read", lambda: cache.read(lens, **kw)),
             ("attend", lambda: cache.attend(q, table, lens, **kw)),
-            ("attend", lambda: cache.attend(q, table, lens, out=torch.zeros_like(q), **kw)),
+            ("attend into", lambda: cache.attend(q, table, lens, out=torch.zeros_like(q), **kw)),
             ("attend", lambda: cache.attend(q, table, lens, first, accumulate=True, **kw)),
             ("attend", lambda: cache.attend(q, table, lens, selected=chosen, **kw)),
             ("select", lambda: cache.select(q, table, lens, 2, **kw)),
@@ -55,3 +56,111 @@ def test_host_memory_reaches_no_kernel(monkeypatch, stream):
         with pytest.raises(ValueError, match="GPU"):
             call()
     assert library.calls == []
+
+
+class Machine:
+    """Two GPUs that are not there: which of them and which stream is current,
+    and what is allocated where.  Streams are named (device, handle)."""
+
+    def __init__(self, patch):
+        self.device, self.stream = 0, {0: 0, 1: 0}
+        self.made, self.recorded = [], []
+        machine = self
+
+        class Stream:
+            def __init__(self, handle, device):
+                self.cuda_stream, self.device = handle, torch.device(device)
+
+        class Device:
+            def __init__(self, device):
+                self.index = torch.device(device).index
+
+            def __enter__(self):
+                self.before, machine.device = machine.device, self.index
+
+            def __exit__(self, *_):
+                machine.device = self.before
+
+        class On(Device):
+            def __init__(self, stream):
+                super().__init__(stream.device)
+                self.handle = stream.cuda_stream
+
+            def __enter__(self):
+                super().__enter__()
+                self.was = machine.stream[self.index]
+                machine.stream[self.index] = self.handle
+
+            def __exit__(self, *_):
+                machine.stream[self.index] = self.was
+                super().__exit__()
+
+        empty = torch.empty
+
+        def make(*args, device, **kw):
+            if torch.device(device).type == "cuda":
+                index = torch.device(device).index
+                self.made.append((index, self.stream[index]))
+            return empty(*args, device=device, **kw)
+
+        self.Stream = Stream
+        patch.setattr(torch.cuda, "ExternalStream", Stream)
+        patch.setattr(torch.cuda, "device", Device)
+        patch.setattr(torch.cuda, "stream", On)
+        patch.setattr(torch.cuda, "current_device", lambda: self.device)
+        patch.setattr(torch.cuda, "current_stream",
+                      lambda device=None: Stream(self.stream[self.index(device)],
+                                                 f"cuda:{self.index(device)}"))
+        patch.setattr(torch._C, "_cuda_getDevice", lambda: self.device, raising=False)
+        patch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda index: self.stream[index],
+                      raising=False)
+        patch.setattr(torch.Tensor, "data_ptr", lambda t: 4096)
+        patch.setattr(torch.Tensor, "record_stream", lambda t, s: self.recorded.append(
+            (s.device.index, s.cuda_stream)))
+        patch.setattr(torch, "empty", make)
+
+    def index(self, device):
+        return self.device if device is None else torch.device(device).index
+
+
+def on_machine(monkeypatch, device, stream):
+    """Every operator of a cache on `device`: (what was current when the
+    library was called, the stream it was given, where it had tensors made,
+    streams that the outputs were recorded on)."""
+    launches = {"append", "read", "attend", "select", "evict"}
+    rows = []
+    with FakeTensorMode(), monkeypatch.context() as patch:
+        machine = Machine(patch)
+
+        def seen(name, args):
+            if name.removeprefix("hbfsim_amd_kv_") in launches:
+                rows.append((machine.device, args[-1], machine.made[:]))
+            elif name.endswith("workspace"):
+                args[-1]._obj.value = 4096
+
+        library = Library(seen)
+        patch.setattr(nat, "load", lambda: library)
+        cache = kvcache.KvCache(4, 2, 64, device=device)
+        got = []
+        for name, call in every_call(cache, device, stream=stream(machine)):
+            rows.clear(), machine.made.clear(), machine.recorded.clear()
+            call()
+            (current, handle, made), = rows
+            got.append((name, current, handle, made, machine.recorded[:]))
+            assert machine.device == 0 and machine.stream == {0: 0, 1: 0}
+    return got
+
+
+@pytest.mark.parametrize("raw", [False, True])
+def test_memory_comes_from_the_pool_of_the_stream_that_writes_it(monkeypatch, raw):
+    """Scratch and outputs of a call on another stream: a block just freed on
+    the current one may have work queued on it that the other is not ordered
+    behind.  The outputs are recorded on the caller's stream, which reads them."""
+    for name, _, handle, made, recorded in on_machine(
+            monkeypatch, "cuda:0", lambda m: 77 if raw else m.Stream(77, "cuda:0")):
+        assert handle == 77
+        assert set(made) <= {(0, 77)} and bool(made) == (name != "append"), (name, made)
+        own = name not in ("append", "attend into")  # outputs that the call makes itself
+        assert set(recorded) <= {(0, 0)} and bool(recorded) == own, (name, recorded)
+    for _, _, handle, made, recorded in on_machine(monkeypatch, "cuda:0", lambda m: None):
+        assert handle == 0 and set(made) <= {(0, 0)} and not recorded
