@@ -48,17 +48,20 @@ _HERE = contextlib.nullcontext()
 
 
 def _queue(device: Any, stream: Any) -> Any:
-    """Context in which a call allocates and queues its work: `stream` (a torch
-    stream or a handle) is current in it, so that scratch and outputs come from
-    its pool.  A block of the current stream's pool may have work queued there
-    that `stream` is not ordered behind.  Kernels follow the tensors'
-    addresses, so the device has to be a GPU."""
-    if device.type != "cuda":
+    """Context in which a call allocates and queues its work.  The cache's GPU
+    is current in it: handle 0 is the current one's default stream, and a
+    kernel runs where it is launched, not where its tensors are.  `stream` (a
+    torch stream or a handle) is current too, so that scratch and outputs come
+    from its pool: a block of the current stream's may have work queued there
+    that `stream` is not ordered behind."""
+    if device.type != "cuda":  # kernels would be handed host addresses
         raise ValueError(f"the cache is on {device}, not on a GPU")
     if stream is None:
-        return _HERE
+        return _HERE if torch._C._cuda_getDevice() == device.index else torch.cuda.device(device)
     if not hasattr(stream, "cuda_stream"):
         stream = torch.cuda.ExternalStream(stream, device=device)
+    elif stream.device != device:
+        raise ValueError(f"stream is of {stream.device}, the cache on {device}")
     return torch.cuda.stream(stream)
 
 

@@ -820,7 +820,8 @@ int hbfsim_amd_probe_bandwidth(void* d_buffer, size_t bytes, unsigned reps, void
  *            units of 2^-32
  * keys, values and bounds are 16-byte aligned.  No call allocates,
  * synchronises or copies to the host: work is queued on `stream`, and a
- * workspace must stay untouched until it is done. */
+ * workspace must stay untouched until it is done.  As with any launch, the
+ * GPU of the arrays and of `stream` is the calling thread's current one. */
 #define HBFSIM_AMD_KV_BF16 0u
 #define HBFSIM_AMD_KV_F16 1u
 #define HBFSIM_AMD_KV_F32 2u

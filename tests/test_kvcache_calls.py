@@ -164,3 +164,19 @@ def test_memory_comes_from_the_pool_of_the_stream_that_writes_it(monkeypatch, ra
         assert set(recorded) <= {(0, 0)} and bool(recorded) == own, (name, recorded)
     for _, _, handle, made, recorded in on_machine(monkeypatch, "cuda:0", lambda m: None):
         assert handle == 0 and set(made) <= {(0, 0)} and not recorded
+
+
+def test_the_cache_s_gpu_is_current_in_its_calls(monkeypatch):
+    """Handle 0 is the current device's default stream: with another GPU
+    current, the launch would go there."""
+    for stream, handle in ((lambda m: None, 0), (lambda m: 0, 0), (lambda m: 77, 77),
+                           (lambda m: m.Stream(77, "cuda:1"), 77)):
+        for name, current, got, made, _ in on_machine(monkeypatch, "cuda:1", stream):
+            assert (current, got) == (1, handle), (name, current, got)
+            assert set(made) <= {(1, handle)}, (name, made)
+
+
+def test_a_stream_of_another_gpu_is_refused(monkeypatch):
+    for device, other in (("cuda:0", "cuda:1"), ("cuda:1", "cuda:0")):
+        with pytest.raises(ValueError, match="stream"):
+            on_machine(monkeypatch, device, lambda m: m.Stream(77, other))
