@@ -227,6 +227,7 @@ struct Attend {
     std::uint32_t row_tiles;       // 16-row tiles per unit (1 unless group > 16)
     std::uint32_t pairs;           // kv heads times row tiles: a unit's workgroups, heads first
     std::uint32_t rows;            // rows of a tile that any unit uses
+    std::uint32_t groups;          // units times pairs; a merge's workgroups beyond clear rows
     float scale;                   // softmax scale times log2(e)
     const std::int32_t* selected;
     std::uint32_t count;
@@ -845,11 +846,45 @@ __global__ __launch_bounds__(256, 2) void k_kv_attend_many(Attend a)
     }
 }
 
+// Zeros in the step's rows that belong to no sequence: before the first one's,
+// from the last one's end on, or of one that ends past the step.  The merge
+// does it in workgroups behind its own, k_kv_clear_rest where there is no merge
+// (2 us of a call).  Within the attention's kernels the same lines cost registers:
+// 3.54 -> 4.44 ms for 8 chunks of 1,024 tokens over 8,192 at 256 dims.
+template <typename T>
+__device__ inline void clear_rest(const Attend& a, std::uint32_t at, std::uint32_t each)
+{
+    const std::int64_t tokens = a.b.tokens;
+    std::int64_t lo = a.b.first[0], hi = a.b.first[a.b.seqs];
+    if (hi > tokens) {
+        hi = a.b.first[last_not_above(a.b.seqs + 1, a.b.tokens, [&](std::uint32_t i) {
+            return static_cast<std::uint32_t>(a.b.first[i]);
+        })];
+    }
+    lo = lo < 0 ? 0 : lo < tokens ? lo : tokens;
+    hi = hi < lo ? lo : hi < tokens ? hi : tokens;
+    const std::int64_t wide = static_cast<std::int64_t>(a.heads) * a.c.dim;
+    for (std::int64_t i = at; i < lo + tokens - hi; i += each) {
+        T* out = static_cast<T*>(a.out) + (i < lo ? i : hi + (i - lo)) * wide;
+        for (std::int64_t e = threadIdx.x; e < wide; e += 256) out[e] = T{};
+    }
+}
+
+template <typename T>
+__global__ __launch_bounds__(256) void k_kv_clear_rest(Attend a)
+{
+    clear_rest<T>(a, blockIdx.x, gridDim.x);
+}
+
 // Joins a unit's splits where there are few of them: a thread takes four dims
 // of a row and goes through the splits, a workgroup as many rows as fit.
 template <typename T>
 __global__ __launch_bounds__(256) void k_kv_merge_few(Attend a)
 {
+    if (blockIdx.x >= a.groups) {
+        if (blockIdx.y == 0) clear_rest<T>(a, blockIdx.x - a.groups, gridDim.x - a.groups);
+        return;
+    }
     const std::uint32_t unit = blockIdx.x / a.pairs, pair = blockIdx.x % a.pairs;
     const std::uint32_t head = pair % a.c.kv_heads, row_tile = pair / a.c.kv_heads;
     const std::uint32_t quads = a.c.dims / 4, groups = 256 / quads;
@@ -890,6 +925,10 @@ __global__ __launch_bounds__(256) void k_kv_merge(Attend a)
     constexpr int kChunk = 256;
     __shared__ float s_factor[kChunk], s_wave[4], s_sum[4];
     __shared__ f32x4 s_part[256];
+    if (blockIdx.x >= a.groups) {
+        if (blockIdx.y == 0) clear_rest<T>(a, blockIdx.x - a.groups, gridDim.x - a.groups);
+        return;
+    }
     const std::uint32_t unit = blockIdx.x / a.pairs, pair = blockIdx.x % a.pairs, row = blockIdx.y;
     const std::uint32_t head = pair % a.c.kv_heads, row_tile = pair / a.c.kv_heads;
     const int P = static_cast<int>(a.c.dims), lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
@@ -1778,7 +1817,7 @@ __global__ __launch_bounds__(256) void k_kv_pick(Select a)
         slot = token + last_not_above(a.b.seqs, token, [&](std::uint32_t i) { return static_cast<std::uint32_t>(a.b.first[i]); });
     }
     Group g;
-    const std::uint32_t nb = find_group(a.b, slot, 1, &g) ? select_blocks(a, g.seen) : 0;
+    const std::uint32_t nb = a.b.seqs != 0 && find_group(a.b, slot, 1, &g) ? select_blocks(a, g.seen) : 0;
     const std::uint32_t* keys = a.keys + static_cast<std::size_t>(blockIdx.x) * a.b.width;
     if (a.staged != 0) {
         for (std::uint32_t i = threadIdx.x; i < nb; i += 256) s_keys[i] = keys[i];
@@ -2097,7 +2136,7 @@ bool launch_select(Select& a, bool one, hipStream_t stream)
         hipLaunchKernelGGL((k_kv_select<T, CH>), dim3(rows), dim3(kPickThreads), keys, stream, a);
         return true;
     }
-    if (a.b.width != 0) {
+    if (a.b.width != 0 && a.b.seqs != 0) {
         a.per = a.b.first == nullptr ? 1 : 8;
         const std::uint32_t slots = a.b.first == nullptr ? a.b.seqs : a.b.tokens / 8 + a.b.seqs;
         a.share = 256;
@@ -2130,6 +2169,12 @@ bool launch_attend(Attend a, const Cut& k, bool accumulate, hipStream_t stream)
 {
     constexpr int RT = 5 - CH;
     const std::uint32_t groups = k.units * a.pairs;
+    const std::uint32_t clearing = a.b.first == nullptr ? 0 : a.b.tokens < 128 ? a.b.tokens : 128;
+    if (a.b.seqs == 0) {
+        hipLaunchKernelGGL((k_kv_clear_rest<T>), dim3(clearing), dim3(256), 0, stream, a);
+        return true;
+    }
+    a.groups = groups;
     if (k.many != 0) {
         const std::size_t lds = (CH <= 2 ? 32 : 16) * 1024 * CH;
         if (!lds_allowed(reinterpret_cast<const void*>(&k_kv_attend_many<T, CH, RT>), lds)) {
@@ -2149,10 +2194,12 @@ bool launch_attend(Attend a, const Cut& k, bool accumulate, hipStream_t stream)
     }
     // 24 sequences of 12 / 16 / 32 splits: 5.3 / 5.5 / 6.4 us by rows, 5.3 / 6.2 / 9.9 by quads of dims
     if (k.splits > 12) {
-        hipLaunchKernelGGL((k_kv_merge<T>), dim3(groups, k.rows), dim3(256), 0, stream, a);
+        hipLaunchKernelGGL((k_kv_merge<T>), dim3(groups + clearing, k.rows), dim3(256), 0, stream, a);
     } else if (k.splits > 1) {
         const std::uint32_t at_once = 1024 / a.c.dims;
-        hipLaunchKernelGGL((k_kv_merge_few<T>), dim3(groups, (k.rows + at_once - 1) / at_once), dim3(256), 0, stream, a);
+        hipLaunchKernelGGL((k_kv_merge_few<T>), dim3(groups + clearing, (k.rows + at_once - 1) / at_once), dim3(256), 0, stream, a);
+    } else if (clearing != 0) {
+        hipLaunchKernelGGL((k_kv_clear_rest<T>), dim3(clearing), dim3(256), 0, stream, a);
     }
     if (!accumulate || a.b.width == 0) {
     } else if (k.many == 0) {
@@ -2299,10 +2346,11 @@ HBF_API int hbfsim_amd_kv_attend(const hbfsim_amd_kv_cache* cache, const hbfsim_
         (accumulate != 0 && count != 0) || static_cast<std::uint64_t>(count) * a.c.tokens > 0x7fffff00u) {
         return HBFSIM_INVALID_ARGUMENT;
     }
-    if (a.b.tokens == 0 || a.b.seqs == 0) {
+    if (a.b.tokens == 0) {
         return HBFSIM_OK;
     }
-    const Cut k = cut_attend(a.c, a.b, heads, count, accumulate != 0);
+    Cut k{};
+    if (a.b.seqs != 0) k = cut_attend(a.c, a.b, heads, count, accumulate != 0);
     if (d_q == nullptr || d_out == nullptr || workspace_bytes < k.bytes ||
         (k.bytes != 0 && (d_workspace == nullptr || !aligned16(d_workspace)))) {
         return HBFSIM_INVALID_ARGUMENT;
@@ -2372,7 +2420,7 @@ HBF_API int hbfsim_amd_kv_select(const hbfsim_amd_kv_cache* cache, const hbfsim_
         count > 0x7fffffffu || static_cast<std::uint64_t>(keep_first) + keep_last > count) {
         return HBFSIM_INVALID_ARGUMENT;
     }
-    if (a.b.tokens == 0 || a.b.seqs == 0) {
+    if (a.b.tokens == 0) {
         return HBFSIM_OK;
     }
     const bool one = select_in_one(a.c, a.b);

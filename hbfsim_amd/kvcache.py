@@ -4,7 +4,8 @@
 `KvCache` owns the device arrays.  A step names its sequences by a block table
 (int32 [seqs, width], -1 for a block that is not there), their lengths after
 the step (int32 [seqs]) and, when a sequence has other than one token in the
-step, the offsets of their rows in the batch (`first`, int32 [seqs + 1]).  All
+step, the offsets of their rows in the batch (`first`, int32 [seqs + 1]).  Rows
+that belong to no sequence store and select nothing and attend to nothing.  All
 tensors are on the cache's GPU; calls queue their work on `stream` (the
 current one by default) and return without waiting for it.
 

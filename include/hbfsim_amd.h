@@ -844,10 +844,13 @@ typedef struct hbfsim_amd_kv_cache {
 /* The sequences of a step.  Sequence s holds d_lens[s] tokens once the
  * step's own are stored, in the blocks d_table[s * table_stride + i]; the
  * step's tokens are its last ones, rows [d_first[s], d_first[s + 1]) of the
- * batch (d_first NULL: one token each, tokens == seqs).  Token i of them
- * sees the sequence up to itself.  Table entries outside [0, blocks) are
- * blocks that are not there: nothing is stored in them and nothing attends
- * to them; so are positions past table_width blocks. */
+ * batch (d_first NULL: one token each, tokens == seqs).  Offsets do not
+ * decrease; rows of no sequence (a batch padded to a fixed size) and those of
+ * one that ends past `tokens` store nothing, attend to nothing and select
+ * nothing.  Token i of a sequence's own sees the sequence up to itself.
+ * Table entries outside [0, blocks) are blocks that are not there: nothing is
+ * stored in them and nothing attends to them; so are positions past
+ * table_width blocks. */
 typedef struct hbfsim_amd_kv_batch {
     uint32_t struct_size;       /* sizeof(hbfsim_amd_kv_batch) */
     uint32_t seqs;
@@ -885,7 +888,7 @@ int hbfsim_amd_kv_read(const hbfsim_amd_kv_cache* cache, const int32_t* d_blocks
  * strides in elements; query heads h * heads / kv_heads .. share kv head h)
  * over the cache: d_out [tokens][heads][head_dim], contiguous, is the
  * softmax of scale * q k over the tokens that the query sees, times v; zeros
- * where it sees none.  With d_selected [tokens][kv_heads][count] (logical
+ * where it sees none, and in rows of no sequence.  With d_selected [tokens][kv_heads][count] (logical
  * blocks, distinct, anything below 0 for none) a query sees those blocks
  * alone.  With `accumulate` (not together with d_selected) d_weight of each
  * block and kv head gains the probabilities of its tokens, summed over the
