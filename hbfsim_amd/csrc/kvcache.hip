@@ -986,13 +986,36 @@ __global__ __launch_bounds__(256) void k_kv_merge(Attend a)
     }
 }
 
+// What a lane's row (m of the unit's row tile) divides its weights by, as a
+// logarithm; infinite for a row that adds none: one that is not there or sees
+// nothing, and those of a token any of whose heads in the group is not a
+// number.  A whole token is left out, whichever rows share its unit or tile.
+// All lanes of a wave call it, m from lane & 15.
+__device__ inline float weigh_lse(const Attend& a, const Group& g, std::uint32_t head, std::uint32_t row_tile)
+{
+    const std::uint32_t m = threadIdx.x & 15, r = row_tile * 16 + m;
+    const float* lse = a.lse + g.row * static_cast<std::int64_t>(a.heads) + head * a.group;
+    const bool there = r < g.count * a.group && m < a.rows;
+    const float l = there ? lse[static_cast<std::int64_t>(r / a.group) * a.heads + r % a.group] : kInf;
+    bool lost;
+    if (a.row_tiles > 1) {  // one token a unit, its heads in several tiles
+        bool bad = false;
+        for (std::uint32_t h = threadIdx.x % kWave; h < a.group; h += kWave) bad |= lse[h] != lse[h];
+        lost = __any(bad);
+    } else {
+        const std::uint32_t votes = static_cast<std::uint32_t>(__ballot(l != l)) & 0xffffu;
+        lost = (votes >> (m / a.group * a.group) & ((1u << a.group) - 1)) != 0;
+    }
+    return lost ? kInf : l;
+}
+
 // weight[block, head] += the probabilities of the unit's rows over the block,
 // from the tiles' sums: one thread per block.  Sums are f32 within a block and
 // joined as integers, so the order in which blocks of shared prefixes are
 // reached does not change them.  24 sequences of 777..20,001 tokens: 7.5 us.
 __device__ inline void add_weight(const Attend& a, std::size_t bh, float sum)
 {
-    if (sum < 1e9f) {  // a sum that is not a number adds nothing
+    if (sum < 1e9f) {  // rows that are not numbers are left out before
         atomicAdd(a.c.weight + bh, static_cast<unsigned long long>(__double2ull_rn(static_cast<double>(sum) * 0x1p32)));
     }
 }
@@ -1010,11 +1033,9 @@ __global__ __launch_bounds__(256) void k_kv_weigh(Attend a)
     if (seen <= 0 || static_cast<std::int64_t>(blockIdx.y) * 256 * a.c.tokens >= seen) {
         return;
     }
-    const std::uint32_t r = row_tile * 16 + threadIdx.x;
-    if (threadIdx.x < a.rows) {
-        s_lse[threadIdx.x] = r < g.count * a.group
-                                 ? a.lse[(g.row + static_cast<std::int64_t>(r / a.group)) * a.heads + head * a.group + r % a.group]
-                                 : kInf;
+    if (threadIdx.x < kWave) {
+        const float l = weigh_lse(a, g, head, row_tile);
+        if (threadIdx.x < a.rows) s_lse[threadIdx.x] = l;
     }
     __syncthreads();
     const std::uint32_t blk = blockIdx.y * 256 + threadIdx.x;
@@ -1054,15 +1075,14 @@ __global__ __launch_bounds__(256) void k_kv_weigh_again(Attend a)
     }
     const std::uint32_t r = row_tile * 16 + m;
     const std::uint32_t row_token = r / a.group, row_head = r % a.group;
-    const bool row_live = row_token < static_cast<std::uint32_t>(g.count) && (a.per > 1 || r < a.group);
+    const float lse = weigh_lse(a, g, head, row_tile);
+    const bool row_live = lse != kInf;
     const std::int64_t limit64 = row_live ? visible(a, g.seen + row_token) : 0;
     const int limit = limit64 > 0 ? static_cast<int>(limit64) : 0;
     const std::int64_t token_row = g.row + static_cast<std::int64_t>(row_token);
-    const std::uint32_t q_head = head * a.group + row_head;
     f16x8 query[CH * 2];
     float factor;
-    load_query<T, CH>(a, token_row, q_head, row_live, quarter, query, &factor);
-    const float lse = row_live ? a.lse[token_row * a.heads + q_head] : kInf;
+    load_query<T, CH>(a, token_row, head * a.group + row_head, row_live, quarter, query, &factor);
     const std::size_t head_bytes = static_cast<std::size_t>(a.c.tokens) * P;
     const std::uint32_t nb = static_cast<std::uint32_t>((seen + a.c.tokens - 1) / a.c.tokens);
     for (std::uint32_t blk = blockIdx.y * 4 + wave; blk < nb; blk += gridDim.y * 4) {

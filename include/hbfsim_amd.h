@@ -892,8 +892,8 @@ int hbfsim_amd_kv_read(const hbfsim_amd_kv_cache* cache, const int32_t* d_blocks
  * blocks, distinct, anything below 0 for none) a query sees those blocks
  * alone.  With `accumulate` (not together with d_selected) d_weight of each
  * block and kv head gains the probabilities of its tokens, summed over the
- * queries and the heads that share it; a sum that is not a number adds
- * nothing.  The workspace call gives the bytes needed for the same sizes. */
+ * queries and the heads that share it; a query token any of whose heads that
+ * share a kv head comes out as not a number adds nothing to its blocks.  The workspace call gives the bytes needed for the same sizes. */
 int hbfsim_amd_kv_attend_workspace(const hbfsim_amd_kv_cache* cache,
                                    const hbfsim_amd_kv_batch* batch, uint32_t heads,
                                    uint32_t count, uint32_t accumulate, size_t* bytes);
