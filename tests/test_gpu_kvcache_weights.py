@@ -65,3 +65,31 @@ def test_tokens_that_see_a_block_of_nan_scale_add_nothing(new, which):
     weight, bound = gains(ref, qn, table, [n], np.array([0, new]), without)
     diff = np.abs(cache.weights().double().cpu().numpy() - weight)
     assert (diff <= bound + 2.0 ** -24 * np.abs(weight)).all(), diff.max()
+
+
+@pytest.mark.parametrize("kv,g,dim,t,dtype", [(2, 1, 64, 16, "f16"), (1, 3, 64, 128, "bf16"),
+                                              (1, 20, 128, 16, "f16"), (2, 3, 100, 128, "bf16"),
+                                              (1, 48, 192, 16, "bf16"), (2, 3, 170, 32, "f16"),
+                                              (1, 1, 256, 128, "bf16"), (2, 20, 256, 16, "f16"),
+                                              (1, 48, 230, 64, "bf16")])
+def test_weights_of_many_rows(kv, g, dim, t, dtype):
+    """The second pass over the keys: every count of dims, both types, groups
+    of one, several and more than 16 heads, blocks of one tile and more, holes,
+    a shared block, a sequence without tokens and a row that is not finite."""
+    rng = np.random.default_rng(dim * g)
+    room = 4 * (5 - -(-dim // 64)) * 16          # rows of a many-row workgroup
+    m = -(-13 * room // (10 * g)) + 3
+    assert 2 * m * g * 5 >= room * 3 * 4         # or the step takes the other form
+    lens, new = [m + 2 * t + 45, m + 5, 0], [m, m, 0]
+    first = np.concatenate([[0], np.cumsum(new)])
+    blocks = sum(-(-n // t) for n in lens) + 1
+    cache, ref = pair(kv, dim, t, blocks)
+    kr.fill(cache, ref, rng, spread=1.0)
+    table = kr.make_table(rng, lens, t, blocks)
+    table[0, 1], table[1, 0] = -1, table[0, 0]
+    q, qn = rows(rng, (2 * m, kv * g, dim), dtype, 1.5)
+    q[m // 2, g - 1, 3] = float("nan")
+    cache.attend(q, ints(table), ints(lens), ints(first), accumulate=True)
+    weight, bound = gains(ref, qn, table, lens, first, {(m // 2, 0)})
+    diff = np.abs(cache.weights().double().cpu().numpy() - weight)
+    assert (diff <= bound + 2.0 ** -24 * weight).all(), diff.max()
