@@ -2079,6 +2079,33 @@ Cut cut_attend(const Cache& c, const Batch& b, std::uint32_t heads, std::uint32_
     return k;
 }
 
+// Whether the output [tokens][heads][dim] at `out` shares memory with the
+// query rows; `same` if it is they, row for row.  Two-byte elements.
+bool overlaps(std::uintptr_t q, std::int64_t token_stride, std::int64_t head_stride, std::uintptr_t out, std::uint32_t tokens,
+              std::uint32_t heads, std::uint32_t dim, bool* same)
+{
+    const std::int64_t row = std::int64_t{2} * dim, whole = row * heads * tokens;
+    const std::int64_t t = 2 * token_stride, h = 2 * head_stride, last_t = (tokens - 1) * t, last_h = (heads - 1) * h;
+    *same = q == out && (tokens == 1 || t == row * heads) && (heads == 1 || h == row);
+    // distances from the output's first byte
+    const std::int64_t at = static_cast<std::int64_t>(q - out);
+    const std::int64_t lo = at + (last_t < 0 ? last_t : 0) + (last_h < 0 ? last_h : 0);
+    const std::int64_t hi = at + (last_t > 0 ? last_t : 0) + (last_h > 0 ? last_h : 0) + row;
+    if (lo >= whole || hi <= 0) {
+        return false;
+    }
+    // within the rows' span: between them, perhaps
+    for (std::uint32_t i = 0; i < tokens; ++i) {
+        for (std::uint32_t j = 0; j < heads; ++j) {
+            const std::int64_t x = at + i * t + j * h;
+            if (x < whole && x + row > 0) {
+                return true;
+            }
+        }
+    }
+    return false;
+}
+
 template <typename T, int CH>
 void launch_append(const Append& a, std::uint32_t slots, hipStream_t stream)
 {
@@ -2373,6 +2400,13 @@ HBF_API int hbfsim_amd_kv_attend(const hbfsim_amd_kv_cache* cache, const hbfsim_
     if (a.b.seqs != 0) k = cut_attend(a.c, a.b, heads, count, accumulate != 0);
     if (d_q == nullptr || d_out == nullptr || workspace_bytes < k.bytes ||
         (k.bytes != 0 && (d_workspace == nullptr || !aligned16(d_workspace)))) {
+        return HBFSIM_INVALID_ARGUMENT;
+    }
+    // weights of several tokens a sequence may read the queries a second time
+    bool same = false;
+    if (overlaps(reinterpret_cast<std::uintptr_t>(d_q), token_stride, head_stride, reinterpret_cast<std::uintptr_t>(d_out),
+                 a.b.tokens, heads, a.c.dim, &same) &&
+        (!same || (accumulate != 0 && a.b.first != nullptr))) {
         return HBFSIM_INVALID_ARGUMENT;
     }
     const Cut few = cut_few(a.c, a.b, heads, count);

@@ -287,7 +287,8 @@ class KvCache:
         `selected` (int32 [tokens, kv_heads, count], logical blocks, negative
         for none) limits it to those blocks; `scale` defaults to
         head_dim ** -0.5.  With `accumulate` the blocks' weights grow by the
-        probabilities.  Returns [tokens, heads, head_dim] in q's type."""
+        probabilities.  `out` may be q itself, but not where weights accumulate
+        with `first`.  Returns [tokens, heads, head_dim] in q's type."""
         tokens, heads, kind = self._queries(q)
         b = _batch(table, lens, first, tokens, self.device)
         count, chosen = 0, None

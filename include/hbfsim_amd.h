@@ -888,12 +888,17 @@ int hbfsim_amd_kv_read(const hbfsim_amd_kv_cache* cache, const int32_t* d_blocks
  * strides in elements; query heads h * heads / kv_heads .. share kv head h)
  * over the cache: d_out [tokens][heads][head_dim], contiguous, is the
  * softmax of scale * q k over the tokens that the query sees, times v; zeros
- * where it sees none, and in rows of no sequence.  With d_selected [tokens][kv_heads][count] (logical
- * blocks, distinct, anything below 0 for none) a query sees those blocks
+ * where it sees none, and in rows of no sequence.  With d_selected
+ * [tokens][kv_heads][count] (logical blocks, distinct, anything below 0 for
+ * none) a query sees those blocks
  * alone.  With `accumulate` (not together with d_selected) d_weight of each
  * block and kv head gains the probabilities of its tokens, summed over the
  * queries and the heads that share it; a query token any of whose heads that
- * share a kv head comes out as not a number adds nothing to its blocks.  The workspace call gives the bytes needed for the same sizes. */
+ * share a kv head comes out as not a number adds nothing to its blocks.
+ * d_out may be d_q itself, row for row, but not with `accumulate` and d_first
+ * together (the queries are read again for the weights); any other overlap of
+ * the two is refused.  The workspace call gives the bytes needed for the same
+ * sizes. */
 int hbfsim_amd_kv_attend_workspace(const hbfsim_amd_kv_cache* cache,
                                    const hbfsim_amd_kv_batch* batch, uint32_t heads,
                                    uint32_t count, uint32_t accumulate, size_t* bytes);

@@ -93,3 +93,29 @@ def test_weights_of_many_rows(kv, g, dim, t, dtype):
     weight, bound = gains(ref, qn, table, lens, first, {(m // 2, 0)})
     diff = np.abs(cache.weights().double().cpu().numpy() - weight)
     assert (diff <= bound + 2.0 ** -24 * weight).all(), diff.max()
+
+
+@pytest.mark.parametrize("new", [1, 5, 90])
+def test_output_in_place_of_the_queries(new):
+    rng = np.random.default_rng(81)
+    kv, g, dim, t, n = 2, 3, 128, 16, 900
+    cache, ref = pair(kv, dim, t, -(-n // t))
+    kr.fill(cache, ref, rng)
+    table, lens = ints(kr.make_table(rng, [n], t, -(-n // t))), ints([n])
+    first = None if new == 1 else ints([0, new])
+    q, _ = rows(rng, (new, kv * g, dim), "bf16", 1.0)
+    want = cache.attend(q, table, lens, first)
+    x = q.clone()
+    assert cache.attend(x, table, lens, first, out=x) is x and torch.equal(x, want)
+    x = q.clone()
+    if first is not None:
+        with pytest.raises(ValueError):
+            cache.attend(x, table, lens, first, accumulate=True, out=x)
+        assert torch.equal(x, q) and not cache.weight.any()
+        with pytest.raises(ValueError):
+            cache.attend(x[1:], table, lens, ints([0, new - 1]), out=x[:-1])
+    else:
+        cache.attend(q, table, lens, accumulate=True)
+        once = cache.weight.clone()
+        assert torch.equal(cache.attend(x, table, lens, accumulate=True, out=x), want)
+        assert torch.equal(cache.weight, 2 * once)

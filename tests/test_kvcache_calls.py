@@ -2,6 +2,8 @@
 in its place."""
 from __future__ import annotations
 
+import ctypes
+
 import pytest
 import torch
 from torch._subclasses.fake_tensor import FakeTensorMode
@@ -180,3 +182,44 @@ def test_a_stream_of_another_gpu_is_refused(monkeypatch):
     for device, other in (("cuda:0", "cuda:1"), ("cuda:1", "cuda:0")):
         with pytest.raises(ValueError, match="stream"):
             on_machine(monkeypatch, device, lambda m: m.Stream(77, other))
+
+
+HERE = 0x7f0000000000  # a device address that no call here reaches
+
+
+def attend_at(q, out, token_stride, head_stride, tokens=3, first=None, acc=0, heads=4, dim=64):
+    """The C call with queries and output at these addresses; what it does not
+    refuse has no GPU to run on."""
+    c = nat.KvCacheArrays(ctypes.sizeof(nat.KvCacheArrays), 8, 2, dim, 16, 0, *[HERE] * 6)
+    b = nat.KvBatch(ctypes.sizeof(nat.KvBatch), 3, 4, 4, tokens, 0, HERE, HERE, first)
+    return nat.load().hbfsim_amd_kv_attend(
+        ctypes.byref(c), ctypes.byref(b), q, nat.KV_BF16, heads, token_stride, head_stride, 0.1,
+        None, 0, acc, out, HERE, 1 << 30, None)
+
+
+@pytest.mark.skipif(torch.cuda.is_available(), reason="its addresses are not a GPU's")
+def test_outputs_over_the_queries():
+    """An output may be the queries themselves, row for row, unless they are
+    read again for the weights; any other overlap would have rows read after
+    they are overwritten."""
+    at, row = HERE + (1 << 20), 4 * 64
+    bad, runs = nat.HBFSIM_INVALID_ARGUMENT, nat.HBFSIM_CUDA_ERROR
+    size = 3 * row * 2
+    for out, strides, kw, want in (
+            (at, (row, 64), {}, runs),                          # in place
+            (at, (row, 64), dict(acc=1), runs),                 # one token each: not read again
+            (at, (row, 64), dict(first=HERE), runs),
+            (at, (row, 64), dict(first=HERE, acc=1), bad),
+            (at + size, (row, 64), dict(first=HERE, acc=1), runs),
+            (at - size, (row, 64), dict(first=HERE, acc=1), runs),
+            (at + 128, (row, 64), {}, bad),                     # a head further
+            (at - 512, (row, 64), {}, bad),                     # a token before
+            (at + size - 2, (row, 64), {}, bad),
+            (at, (2 * row, 64), {}, bad),                       # rows of a wider buffer
+            (at, (row, 0), {}, bad),
+            (at + 2 * row, (10 * row, 64), {}, runs),           # between its rows
+            (at + 2 * row - 2, (10 * row, 64), {}, bad),
+            (at + 2 * row, (4 * row - 2, 64), {}, bad),
+            (at + 20 * row * 2, (10 * row, 64), {}, bad),
+            (at + 2, (row, 64), dict(tokens=3), bad)):
+        assert attend_at(at, out, *strides, **kw) == want, (out - at, strides, kw)
