@@ -2171,6 +2171,9 @@ std::size_t select_bytes(const Cache& c, const Batch& b)
                                : static_cast<std::size_t>(b.tokens) * c.kv_heads * b.width * sizeof(std::uint32_t);
 }
 
+// Groups of up to 8 tokens of the scoring launch.
+std::uint32_t score_slots(const Batch& b) { return b.first == nullptr ? b.seqs : b.tokens / 8 + b.seqs; }
+
 template <typename T, int CH>
 bool launch_select(Select& a, bool one, hipStream_t stream)
 {
@@ -2185,7 +2188,7 @@ bool launch_select(Select& a, bool one, hipStream_t stream)
     }
     if (a.b.width != 0 && a.b.seqs != 0) {
         a.per = a.b.first == nullptr ? 1 : 8;
-        const std::uint32_t slots = a.b.first == nullptr ? a.b.seqs : a.b.tokens / 8 + a.b.seqs;
+        const std::uint32_t slots = score_slots(a.b);
         a.share = 256;
         while (a.share < 4096 && static_cast<std::uint64_t>(slots) * a.c.kv_heads * (a.b.width / a.share) > 4096) a.share *= 2;
         while (a.b.width / a.share > 65534) a.share *= 2;
@@ -2304,10 +2307,11 @@ HBF_API int hbfsim_amd_kv_append(const hbfsim_amd_kv_cache* cache, const hbfsim_
         a.token_stride[i] = strides[2 * i];
         a.head_stride[i] = strides[2 * i + 1];
     }
-    const std::uint32_t slots = a.b.first == nullptr ? a.b.seqs : a.b.tokens / a.c.tokens + 2 * a.b.seqs;
-    if (slots > kMostGroups) {
+    const std::uint64_t blocks = a.b.first == nullptr ? a.b.seqs : a.b.tokens / a.c.tokens + std::uint64_t{2} * a.b.seqs;
+    if (blocks > kMostGroups) {
         return HBFSIM_UNSUPPORTED;
     }
+    const std::uint32_t slots = static_cast<std::uint32_t>(blocks);
     const std::size_t each = type == HBFSIM_AMD_KV_F32 ? 4 : 8;  // elements of 16 bytes
     for (int i = 0; i < 2; ++i) {
         a.vector[i] = aligned16(a.x[i]) && a.token_stride[i] % static_cast<std::int64_t>(each) == 0 &&
@@ -2483,7 +2487,9 @@ HBF_API int hbfsim_amd_kv_select(const hbfsim_amd_kv_cache* cache, const hbfsim_
         (need != 0 && (d_workspace == nullptr || !aligned16(d_workspace)))) {
         return HBFSIM_INVALID_ARGUMENT;
     }
-    if (static_cast<std::uint64_t>(a.b.tokens) * a.c.kv_heads > kMostGroups) {
+    // scores come in workgroups of a quarter of the threads
+    if (static_cast<std::uint64_t>(a.b.tokens) * a.c.kv_heads > kMostGroups ||
+        (!one && static_cast<std::uint64_t>(score_slots(a.b)) * a.c.kv_heads > 4 * kMostGroups)) {
         return HBFSIM_UNSUPPORTED;
     }
     a.q = d_q;

@@ -223,3 +223,20 @@ def test_outputs_over_the_queries():
             (at + 20 * row * 2, (10 * row, 64), {}, bad),
             (at + 2, (row, 64), dict(tokens=3), bad)):
         assert attend_at(at, out, *strides, **kw) == want, (out - at, strides, kw)
+
+
+@pytest.mark.skipif(torch.cuda.is_available(), reason="its addresses are not a GPU's")
+@pytest.mark.parametrize("seqs,tokens", [(0x7fffff00, 0x3000), (1 << 23, 5), (1 << 22, 1 << 21),
+                                         (0x7fffff00, 0x7fffff00)])
+def test_steps_of_more_sequences_than_a_launch_holds(seqs, tokens):
+    """Most of them without a token: the slots are counted in 64 bits."""
+    c = nat.KvCacheArrays(ctypes.sizeof(nat.KvCacheArrays), 8, 2, 64, 16, 0, *[HERE] * 6)
+    b = nat.KvBatch(ctypes.sizeof(nat.KvBatch), seqs, 4, 4, tokens, 0, HERE, HERE, HERE)
+    lib, refs = nat.load(), (ctypes.byref(c), ctypes.byref(b))
+    strides = (ctypes.c_int64 * 4)(128, 64, 128, 64)
+    assert lib.hbfsim_amd_kv_append(*refs, HERE, HERE, 0, strides, None) == nat.HBFSIM_UNSUPPORTED
+    assert lib.hbfsim_amd_kv_select(*refs, HERE, 0, 4, 256, 64, 4, 1, 1, HERE, HERE, 1 << 62,
+                                    None) == nat.HBFSIM_UNSUPPORTED
+    for acc in (0, 1):
+        assert lib.hbfsim_amd_kv_attend(*refs, HERE, 0, 4, 256, 64, 0.1, None, 0, acc, 2 * HERE,
+                                        HERE, 1 << 62, None) == nat.HBFSIM_UNSUPPORTED
