@@ -99,6 +99,12 @@ def _ints(x: Any, name: str, device: Any, dims: int) -> Any:
     return x
 
 
+def _counts(*values: int) -> None:
+    """The library's counts are of 32 bits; ctypes would pass their low half."""
+    if min(values) < 0 or max(values) >> 32:
+        raise ValueError(f"counts must be in 0..2^32 - 1: {values}")
+
+
 def _batch(table: Any, lens: Any, first: Any, tokens: int, device: Any) -> nat.KvBatch:
     _ints(table, "table", device, 2)
     _ints(lens, "lens", device, 1)
@@ -114,6 +120,7 @@ def _batch(table: Any, lens: Any, first: Any, tokens: int, device: Any) -> nat.K
     stride = table.stride(0) if seqs > 1 else width
     if stride < width:
         raise ValueError("table rows overlap")
+    _counts(seqs, width, stride, tokens)
     return nat.KvBatch(ctypes.sizeof(nat.KvBatch), seqs, width, stride, tokens, 0,
                        table.data_ptr(), lens.data_ptr(),
                        first.data_ptr() if first is not None else None)
@@ -138,6 +145,8 @@ def evict(weight: Any, table: Any, lens: Any, keep: int, block_tokens: int = 16,
     if min(keep, keep_first, keep_last) < 0:
         raise ValueError("keep, keep_first and keep_last must not be negative")
     stride = table.stride(0) if seqs > 1 else width
+    keep = min(keep, 2 ** 32 - 1)  # no table has more blocks
+    _counts(*weight.shape, block_tokens, seqs, width, stride, keep_first, keep_last)
     queue, caller = _queue(device, stream), _caller(device, stream)
     with queue:
         out_table, freed = torch.empty((2, seqs, width), dtype=torch.int32, device=device).unbind()
@@ -337,6 +346,7 @@ class KvCache:
         tokens, heads, kind = self._queries(q)
         if min(count, keep_first, keep_last) < 0:
             raise ValueError("count, keep_first and keep_last must not be negative")
+        _counts(count, keep_first, keep_last)
         b = _batch(table, lens, first, tokens, self.device)
         queue, caller = _queue(self.device, stream), _caller(self.device, stream)
         ref = ctypes.byref(b)

@@ -240,3 +240,32 @@ def test_steps_of_more_sequences_than_a_launch_holds(seqs, tokens):
     for acc in (0, 1):
         assert lib.hbfsim_amd_kv_attend(*refs, HERE, 0, 4, 256, 64, 0.1, None, 0, acc, 2 * HERE,
                                         HERE, 1 << 62, None) == nat.HBFSIM_UNSUPPORTED
+
+
+def test_arguments_past_32_bits(monkeypatch):
+    """The library takes 32-bit counts: larger ones do not arrive as their low
+    halves.  To keep more blocks than there can be is to keep all."""
+    with FakeTensorMode(), monkeypatch.context() as patch:
+        Machine(patch)
+        got = []
+        patch.setattr(nat, "load", lambda: Library(lambda name, args: got.append((name, args))))
+        cache = kvcache.KvCache(4, 2, 64, device="cuda:0")
+        table, lens = (torch.zeros(s, dtype=I32, device="cuda:0") for s in ((3, 2), (3,)))
+        q = torch.zeros((3, 4, 64), dtype=torch.bfloat16, device="cuda:0")
+        k = torch.zeros((3, 2, 64), dtype=torch.bfloat16, device="cuda:0")
+        for keep in (2 ** 32, 2 ** 32 + 5, 2 ** 63 - 1, 2 ** 80):
+            cache.evict(table, lens, keep)
+            kvcache.evict(cache.weight, table, lens, keep)
+            assert [args[9] for _, args in got] == [2 ** 32 - 1] * 2
+            got.clear()
+        far = torch.empty_strided((3, 2), (2 ** 32 + 2, 1), dtype=I32, device="cuda:0")
+        for bad in (lambda: cache.evict(table, lens, 2, 2 ** 32),
+                    lambda: cache.evict(table, lens, 2, 0, 2 ** 32 + 1),
+                    lambda: kvcache.evict(cache.weight, table, lens, 2, 2 ** 32 + 16),
+                    lambda: cache.select(q, table, lens, 2, None, 2 ** 32, 1),
+                    lambda: cache.select(q, table, lens, 2, None, 0, 2 ** 32 + 1),
+                    lambda: cache.evict(far, lens, 2), lambda: cache.append(k, k, far, lens),
+                    lambda: cache.select(q, far, lens, 2), lambda: cache.attend(q, far, lens)):
+            with pytest.raises(ValueError):
+                bad()
+        assert got == []
