@@ -374,8 +374,9 @@ __device__ inline float lane_float(float x, int lane)
 // matrix units are idle otherwise.
 // kWeigh: each tile's sum of a row's weights is left behind as one logarithm,
 // from which k_kv_weigh makes probabilities once the row's denominator is known.
-// kOnce: no other workgroup reads the same codes, which then pass the caches
-// as streams do (6.07 against 5.41 TB/s over one sequence of 262,147 tokens).
+// kOnce: a sequence's codes have one unit of rows in the step, whose workgroups
+// read them once, past the caches as streams do (6.07 against 5.41 TB/s over one
+// sequence of 262,147 tokens).
 template <typename T, int CH, int kWaves, bool kWeigh, bool kOnce>
 __global__ __launch_bounds__(kWaves * kWave, CH <= 2 ? 4 : CH == 3 ? 2 : 1) void k_kv_attend(Attend a)
 {
@@ -2233,7 +2234,11 @@ bool launch_attend(Attend a, const Cut& k, bool accumulate, hipStream_t stream)
         hipLaunchKernelGGL((k_kv_attend_many<T, CH, RT>), dim3(groups, k.splits), dim3(256), lds, stream, a);
     } else {
         const std::size_t lds = 4 * k.rows * (CH * 64 + 4) * sizeof(float);
-        const bool once = k.row_tiles == 1 && (a.b.first == nullptr || a.count != 0 || a.b.tokens <= k.per * a.b.seqs);
+        // Codes pass the caches where a workgroup is alone with them: not where several units
+        // of a sequence read the same blocks, of a selection either.  Marked / cached: 2 chunks of
+        // 1,001 tokens (8 kv heads, D = 128) over 64 / 128 / 256 selected blocks 510 / 360, 895 / 645
+        // and 1,545 / 1,170 us; 32 sequences of 4 tokens 49 / 51, 90 / 87 and 171 / 145.
+        const bool once = k.row_tiles == 1 && (a.b.first == nullptr || a.b.tokens <= k.per * a.b.seqs);
         void (*kernel)(Attend) = accumulate ? once ? k_kv_attend<T, CH, 4, true, true> : k_kv_attend<T, CH, 4, true, false>
                                  : once     ? k_kv_attend<T, CH, 4, false, true>
                                             : k_kv_attend<T, CH, 4, false, false>;
