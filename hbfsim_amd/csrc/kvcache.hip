@@ -345,8 +345,11 @@ __device__ inline Tiles load_tiles(const Attend& a, std::uint32_t seq, std::uint
         const std::int64_t pos = logical * a.c.tokens + sub * 16;
         if (id >= 0 && pos < seen) {
             const std::size_t bh = static_cast<std::size_t>(id) * a.c.kv_heads + head;
-            const float vs = a.c.value_scale[bh];
+            float vs = a.c.value_scale[bh];
             const float ks = a.c.key_scale[bh];
+            // scales below the least, of blocks not begun yet, have no
+            // logarithm or inverse to take part with
+            vs = vs < kScaleMin ? kScaleMin : vs;
             // a NaN value scale shows through its logarithm in the rows that
             // see the block, and through nothing in those that do not
             t = Tiles{id, sub, static_cast<std::int32_t>(pos), ks < kScaleMin ? kScaleMin : ks, log2f(vs),

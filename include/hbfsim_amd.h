@@ -813,7 +813,8 @@ int hbfsim_amd_probe_bandwidth(void* d_buffer, size_t bytes, unsigned reps, void
  *            token 16 * tile + [5], dim 64 * chunk + 16 * [4] + [6]
  *   d_values int8 [blocks][kv_heads][block_tokens / 16][dims / 64][4][16][4][4]
  *            token 16 * tile + 4 * [4] + [7], dim 64 * chunk + 16 * [6] + [5]
- *   d_key_scale, d_value_scale float [blocks][kv_heads]
+ *   d_key_scale, d_value_scale float [blocks][kv_heads]; attention takes one
+ *            below 2^-40, as in arrays of zeros, for 2^-40
  *   d_bounds int8 [blocks][kv_heads][2][dims]: the lowest, then the highest
  *            key code of the block's tokens in each dim
  *   d_weight int64 [blocks][kv_heads]: accumulated attention probability in

@@ -60,3 +60,35 @@ def test_value_scales_from_the_least_up(kv, g, dim, t, dtype):
                                      accumulate=True)
     diff = np.abs(cache.weights().double().cpu().numpy() - weight)
     assert (diff <= wbound + 2.0 ** -24 * weight).all()
+
+
+@pytest.mark.parametrize("dim", [64, 256])
+@pytest.mark.parametrize("new", [1, 3, 120])
+def test_blocks_of_scale_zero_hold_zeros(dim, new):
+    """Arrays that a caller made of zeros: a block not begun yet stands for
+    zeros, and what sees it weighs it as that (the oracle's block has codes of
+    zero; 2^-33 is the largest code at the least scale)."""
+    rng = np.random.default_rng(dim + new)
+    kv, g, t, n = 2, 4, 16, 500
+    blocks = -(-n // t)
+    cache, ref = pair(kv, dim, t, blocks)
+    kr.fill(cache, ref, rng)
+    table = kr.make_table(rng, [n], t, blocks)
+    zero = table[0, [0, 3, 4, 17, 31]]
+    scales = [x.clone() for x in (cache.key_scale, cache.value_scale)]
+    for x in scales:
+        x[torch.from_numpy(zero).long().cuda()] = 0
+    for codes in ref.codes:
+        codes[zero] = 0
+    q, qn = rows(rng, (new, kv * g, dim), "f16", 1.0)
+    first = [0, new]
+    want, bound, weight, wbound = ref.attend(qn, table, [n], first)
+    bound = bound + 2.0 ** -33 + 2.0 ** -11 * (np.abs(want) + bound) + 2.0 ** -24
+    cache.key_scale.copy_(scales[0])
+    cache.value_scale.copy_(scales[1])
+    got = cache.attend(q, ints(table), ints([n]), ints(first), accumulate=True)
+    assert (np.abs(got.double().cpu().numpy() - want) <= bound).all()
+    diff = np.abs(cache.weights().double().cpu().numpy() - weight)
+    assert (diff <= wbound + 2.0 ** -24 * weight).all()
+    cache.keys.zero_(), cache.values.zero_(), cache.key_scale.zero_(), cache.value_scale.zero_()
+    assert not cache.attend(q, ints(table), ints([n]), ints(first)).any()
