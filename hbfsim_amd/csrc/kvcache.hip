@@ -623,7 +623,7 @@ __global__ __launch_bounds__(256, 2) void k_kv_attend_many(Attend a)
     f16x8 query[RT][CH * 2];
     float factor[RT], ref[RT], den[RT], over[RT];  // over: how far a score may pass ref
     int limit[RT];
-    int least = 0x7fffffff, most = 0;
+    int least = 0x7fffffff;  // tokens that every row of the wave sees
     f32x4 acc[RT][CH * 4];
 #pragma unroll
     for (int k = 0; k < RT; ++k) {
@@ -633,7 +633,6 @@ __global__ __launch_bounds__(256, 2) void k_kv_attend_many(Attend a)
         const std::int64_t limit64 = row_live ? visible(a, g.seen + row_token) : 0;
         limit[k] = limit64 > 0 ? static_cast<int>(limit64) : 0;
         least = row_live && limit[k] < least ? limit[k] : least;
-        most = limit[k] > most ? limit[k] : most;
         load_query<T, CH>(a, g.row + static_cast<std::int64_t>(row_token), head * a.group + row_head, row_live, quarter,
                           query[k], &factor[k]);
         ref[k] = 0.0f;
@@ -644,12 +643,10 @@ __global__ __launch_bounds__(256, 2) void k_kv_attend_many(Attend a)
     }
 #pragma unroll
     for (int k = 1; k < kWave; k *= 2) {
-        const int x = __shfl_xor(least, k), y = __shfl_xor(most, k);
+        const int x = __shfl_xor(least, k);
         least = x < least ? x : least;
-        most = y > most ? y : most;
     }
     least = __builtin_amdgcn_readfirstlane(least);
-    most = __builtin_amdgcn_readfirstlane(most);
 
     const std::int64_t begin = static_cast<std::int64_t>(split) * a.split;
     const std::int64_t end = begin + a.split < seen ? begin + a.split : seen;
