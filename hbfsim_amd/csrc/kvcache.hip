@@ -378,8 +378,8 @@ __device__ inline float lane_float(float x, int lane)
 // kWeigh: each tile's sum of a row's weights is left behind as one logarithm,
 // from which k_kv_weigh makes probabilities once the row's denominator is known.
 // kOnce: a sequence's codes have one unit of rows in the step, whose workgroups
-// read them once, past the caches as streams do (6.07 against 5.41 TB/s over one
-// sequence of 262,147 tokens).
+// read them once, past the caches as streams do (6.1 against 5.4 TB/s over one
+// sequence of 262,147 tokens; 422 against 467 us over 64 of 1024..32768).
 template <typename T, int CH, int kWaves, bool kWeigh, bool kOnce>
 __global__ __launch_bounds__(kWaves * kWave, CH <= 2 ? 4 : CH == 3 ? 2 : 1) void k_kv_attend(Attend a)
 {
@@ -585,14 +585,16 @@ __global__ __launch_bounds__(kWaves * kWave, CH <= 2 ? 4 : CH == 3 ? 2 : 1) void
 // f16 once for all of them and keep in LDS in lane order (a 16-byte read per
 // lane per operand, free of conflicts, two buffers), and each keeps RT tiles of
 // 16 rows in registers, so that an operand read serves RT products.
-// 16 chunks of 2,048 tokens over 16,384 (8.2e12 operations) take 8.2 ms, 1,003
-// TFLOP/s (a large library product reaches 1,420 here); two chunks of about
-// 2,000 over 12,001..16,384 take 1.01-1.16 ms, the last
-// of two rounds of workgroups partly empty.  The matrix units are busy 43 % of the time, the
-// vector units 59 %: 180 vector instructions a pair of tiles (24 exponentials;
-// scale, maximum, sum and rounding of 24 scores a lane; widening) beside 48
-// products, and vector work runs at half rate while the matrix unit of its
-// SIMD does, so that their sum bounds it more than either.
+// 16 chunks of 2,048 tokens over 16,384 (8.2e12 operations) take 8.1-8.5 ms by
+// card, about 1,000 TFLOP/s (a large library product reaches 1,420 here); two
+// chunks of about 2,000 over 12,001..16,384 take 1.08-1.16 ms, the last of two
+// rounds of workgroups partly empty.  8 of 1,024 over 8,192 take 3.55 ms at 256
+// dims and 1.95 at 192, where accumulators leave room for one and two row tiles
+// and an operand read serves as few products.  At 128 dims the matrix units are
+// busy 43 % of the time, the vector units 59 %: 180 vector instructions a pair
+// of tiles (24 exponentials; scale, maximum, sum and rounding of 24 scores a
+// lane; widening) beside 48 products, and vector work runs at half rate while
+// the matrix unit of its SIMD does, so that their sum bounds it more than either.
 template <typename T, int CH, int RT>
 __global__ __launch_bounds__(256, 2) void k_kv_attend_many(Attend a)
 {
@@ -1057,7 +1059,9 @@ __global__ __launch_bounds__(256) void k_kv_weigh(Attend a)
 }
 
 // The same where the many-row form ran, from the keys again: one wave per
-// block of the sequence; 16 query rows at a time.
+// block of the sequence; 16 query rows at a time, so that every 16 rows widen
+// the keys anew and this takes longer than the attention itself: 2 chunks of
+// 2,048 tokens over 16,384 (8 kv heads, D = 128) 2.33 ms beside 1.13 + 0.04.
 template <typename T, int CH>
 __global__ __launch_bounds__(256) void k_kv_weigh_again(Attend a)
 {
@@ -1992,9 +1996,9 @@ struct Cut {
 std::size_t up256(std::size_t x) { return (x + 255) & ~std::size_t{255}; }
 
 // Row tiles per wave that fit the registers of two waves per SIMD (16 chunks
-// of 2048 tokens over 16384, D = 64: 6.03 / 5.39 / 5.73 ms with 3 / 4 / 5, D =
-// 128: 9.25 / 8.5 with 2 / 3; 8 of 1024 over 8192, D = 256: 3.73 / 3.92 with 1 /
-// 2, of which two spill).
+// of 2048 tokens over 16384, D = 64: 5.84 / 5.14 / 5.38 ms with 3 / 4 / 5, D =
+// 128: 9.06 / 8.53 / 14.2 with 2 / 3 / 4; 8 of 1024 over 8192, D = 192: 2.22 /
+// 1.95 / 6.92 with 1 / 2 / 3, D = 256: 3.59 / 3.95 with 1 / 2: more spill).
 std::uint32_t many_tiles(std::uint32_t dims) { return 5 - dims / 64; }
 
 Cut cut_few(const Cache& c, const Batch& b, std::uint32_t heads, std::uint32_t count)
@@ -2007,11 +2011,11 @@ Cut cut_few(const Cache& c, const Batch& b, std::uint32_t heads, std::uint32_t c
     k.units = b.first == nullptr ? b.seqs : b.tokens / k.per + b.seqs;
     const std::uint64_t longest = static_cast<std::uint64_t>(count != 0 ? count : b.width) * c.tokens;
     const std::uint64_t pairs = static_cast<std::uint64_t>(k.units) * c.kv_heads * k.row_tiles;
-    // Splits of 2048 tokens (64 sequences of 1024..32768 tokens: 464 us, with
-    // 1024 478, with 4096 462 and less to share out), shorter where they would
-    // not fill the card.  Up to 1024 tokens take one and no second launch: one
-    // sequence of 1024 takes 12.0 us in one split, 7.6 + 3.5 and a launch in
-    // four; of 1536, 15.3 against 7.9 + 4.5.
+    // Splits of 2048 tokens (64 sequences of 1024..32768 tokens: 422 us and 7 of
+    // merge, with 1024 442 + 8, with 4096 427 + 5), shorter where they would not
+    // fill the card.  Up to 1024 tokens take one and no second launch: one
+    // sequence of 1024 takes 12.1 us in one split, 7.7 + 3.1 and a launch in
+    // four; of 1536, 15.3 against 7.7 + 3.4.
     std::uint64_t split = 2048;
     while (longest > 1024 && split > 256 && pairs * ((longest + split - 1) / split) < 1024) split /= 2;
     k.split = static_cast<std::uint32_t>(split);
@@ -2034,9 +2038,11 @@ Cut cut_many(const Cache& c, const Batch& b, std::uint32_t heads)
     // Two workgroups fit a CU; splits fill the last round of them, each at
     // the price of its partial sums' round trip.  Chunks of 2,048 tokens over
     // 16,384 (8 kv heads, D = 128) take, with 1 / 2 / 3 / 4 splits and their
-    // merge, 838 / 726 / 708 / 697 us for one of them (0.7 rounds), 1,303 /
-    // 1,261 / 1,260 / 1,271 for two, 1,927 / 1,776 / 1,767 / 1,775 for three,
-    // 3,350 / 3,278 / 3,321 / 3,384 for six (4.1), 4,086 / 4,283 for eight.
+    // merge, 839 / 730 / 719 / 704 us for one of them (0.7 rounds), 1,285 /
+    // 1,245 / 1,264 / 1,253 for two, 1,917 / 1,746 / 1,721 / 1,759 for three,
+    // 3,383 / 3,537 / 3,564 / 3,565 for six (4.1), 4,128 / 4,291 / 4,376 / 4,476
+    // for eight.  The table's width stands for the lengths, which the host does
+    // not know: a table much wider than they are gives splits without work.
     std::uint64_t best = 1;
     double score = 0.0;
     for (std::uint64_t s = 1; s <= 16 && (s == 1 || (groups < 2048 && longest / s >= 256)); ++s) {
@@ -2059,10 +2065,10 @@ Cut cut_attend(const Cache& c, const Batch& b, std::uint32_t heads, std::uint32_
     const std::uint32_t group = heads / c.kv_heads;
     // The many-row form once a sequence's share of the step comes near a
     // workgroup's rows: 16 sequences of 8192 tokens (4 heads a kv head, D = 128)
-    // take 178 us in the few-row form and 224 in this with 32 tokens (128 of
-    // 192 rows), 260 and 229 with 48, 512 and 302 with 96.  One sequence of 4096
-    // tokens, which fills the card with neither: 79 and 55 with 400 tokens, but
-    // 23 and 27 with 48.
+    // take, merge and all, 142 us in the few-row form and 180 in this with 24
+    // tokens (96 of 192 rows), 179 and 171 with 32, 268 and 244 with 48, 514 and
+    // 322 with 96.  One sequence of 4096 tokens, which fills the card with
+    // neither: 84 and 67 with 400 tokens, but 30 and 44 with 48.
     const std::uint64_t room = 4 * many_tiles(c.dims) * 16;
     const bool many = b.first != nullptr && count == 0 && group <= room &&
                       static_cast<std::uint64_t>(b.tokens) * group * 5 >= room * b.seqs * 4;
@@ -2158,8 +2164,8 @@ bool lds_allowed(const void* kernel, std::size_t bytes)
 
 // One workgroup per row does it all where there are rows enough to fill the
 // card and no other token reads the same bounds: 64 sequences of 16384..32768
-// tokens and 8 kv heads take 72.5 us in one launch and 63 + 12 in two, 32 take
-// 42 and 35 + 11.5, 16 take 29 and 18 + 11, 8 take 29 and 13 + 10.
+// tokens and 8 kv heads take 72 us in one launch and 63 + 12 in two, 32 take
+// 43 and 34 + 12, 16 take 29 and 17 + 11, 8 take 29 and 13 + 10.
 bool select_in_one(const Cache& c, const Batch& b)
 {
     return b.first == nullptr && static_cast<std::uint64_t>(b.tokens) * c.kv_heads >= 128 &&
@@ -2247,7 +2253,7 @@ bool launch_attend(Attend a, const Cut& k, bool accumulate, hipStream_t stream)
         }
         hipLaunchKernelGGL(kernel, dim3(groups, k.splits), dim3(256), lds, stream, a);
     }
-    // 24 sequences of 12 / 16 / 32 splits: 5.3 / 5.5 / 6.4 us by rows, 5.3 / 6.2 / 9.9 by quads of dims
+    // 24 sequences of 12 / 16 / 32 splits: 5.5 / 5.6 / 6.3 us by rows, 5.4 / 6.4 / 10.1 by quads of dims
     if (k.splits > 12) {
         hipLaunchKernelGGL((k_kv_merge<T>), dim3(groups + clearing, k.rows), dim3(256), 0, stream, a);
     } else if (k.splits > 1) {
