@@ -20,7 +20,6 @@ No counterpart in the reference.
 """
 from __future__ import annotations
 
-import contextlib
 import ctypes
 import math
 from typing import Any
@@ -45,50 +44,56 @@ def _refuse(rc: int, what: str) -> None:
     nat.check(rc, what)
 
 
-_HERE = contextlib.nullcontext()
+def _gpu(x: Any) -> int | None:
+    """The index of the tensor's GPU, None on another kind of device."""
+    return x.device.index if x.is_cuda else None
 
 
-def _queue(device: Any, stream: Any) -> Any:
-    """Context in which a call allocates and queues its work.  The cache's GPU
-    is current in it: handle 0 is the current one's default stream, and a
-    kernel runs where it is launched, not where its tensors are.  `stream` (a
-    torch stream or a handle) is current too, so that scratch and outputs come
-    from its pool: a block of the current stream's may have work queued there
-    that `stream` is not ordered behind."""
-    if device.type != "cuda":  # kernels would be handed host addresses
-        raise ValueError(f"the cache is on {device}, not on a GPU")
+def _elsewhere(gpu: int | None, stream: Any) -> bool:
+    """Whether a call has to make another GPU or stream current first."""
+    return gpu is not None and (stream is not None or torch._C._cuda_getDevice() != gpu)
+
+
+def _there(device: Any, stream: Any, call: Any, own: bool = True) -> Any:
+    """`call` with the cache's GPU current (handle 0 is the current one's
+    default stream, and a kernel runs where it is launched, not where its
+    tensors are) and `stream`, a torch stream or a handle, current on it, so
+    that scratch and outputs come from its pool: a block of the current
+    stream's may have work queued there that `stream` is not ordered behind.
+    Its outputs, if it makes them itself, are recorded on the caller's stream,
+    which reads them: none is handed out again before that is done."""
     if stream is None:
-        return _HERE if torch._C._cuda_getDevice() == device.index else torch.cuda.device(device)
+        with torch.cuda.device(device):
+            return call()
     if not hasattr(stream, "cuda_stream"):
         stream = torch.cuda.ExternalStream(stream, device=device)
     elif stream.device != device:
         raise ValueError(f"stream is of {stream.device}, the cache on {device}")
-    return torch.cuda.stream(stream)
+    caller = torch.cuda.current_stream(device)
+    with torch.cuda.stream(stream):
+        got = call()
+    if own and got is not None:
+        for t in got if isinstance(got, tuple) else (got,):
+            t.record_stream(caller)
+    return got
 
 
-def _handle(device: Any) -> int:
+def _handle(gpu: int) -> int:
     """The current stream's handle.  (The raw accessor costs a tenth of
     building a Stream.)"""
-    return torch._C._cuda_getCurrentRawStream(device.index)
+    return torch._C._cuda_getCurrentRawStream(gpu)
+
+
+def _on_gpu(gpu: int | None) -> None:
+    """Kernels follow the tensors' addresses: only a GPU's may reach them."""
+    if gpu is None:
+        raise ValueError("the cache is not on a GPU")
 
 
 def _workspace(nbytes: int, device: Any) -> Any:
     """Scratch of one call, handed back to torch's allocator after it: work
     queued later on the same stream is ordered behind the call."""
     return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
-
-
-def _caller(device: Any, stream: Any) -> Any:
-    """The stream that will read a call's outputs, if it is another than theirs."""
-    return None if stream is None else torch.cuda.current_stream(device)
-
-
-def _hand_over(caller: Any, *tensors: Any) -> None:
-    """Tells torch's allocator that the caller's stream uses the tensors, so
-    that none of them is handed out again on its own before that is done."""
-    if caller is not None:
-        for t in tensors:
-            t.record_stream(caller)
 
 
 def _ints(x: Any, name: str, device: Any, dims: int) -> Any:
@@ -99,10 +104,11 @@ def _ints(x: Any, name: str, device: Any, dims: int) -> Any:
     return x
 
 
-def _counts(*values: int) -> None:
-    """The library's counts are of 32 bits; ctypes would pass their low half."""
-    if min(values) < 0 or max(values) >> 32:
-        raise ValueError(f"counts must be in 0..2^32 - 1: {values}")
+def _counts(bits: int) -> None:
+    """The library's counts are of 32 bits; ctypes would pass their low half.
+    `bits` are those of all counts of a call together."""
+    if bits >> 32:
+        raise ValueError("counts and strides must be in 0..2^32 - 1")
 
 
 def _batch(table: Any, lens: Any, first: Any, tokens: int, device: Any) -> nat.KvBatch:
@@ -120,7 +126,7 @@ def _batch(table: Any, lens: Any, first: Any, tokens: int, device: Any) -> nat.K
     stride = table.stride(0) if seqs > 1 else width
     if stride < width:
         raise ValueError("table rows overlap")
-    _counts(seqs, width, stride, tokens)
+    _counts(seqs | width | stride | tokens)
     return nat.KvBatch(ctypes.sizeof(nat.KvBatch), seqs, width, stride, tokens, 0,
                        table.data_ptr(), lens.data_ptr(),
                        first.data_ptr() if first is not None else None)
@@ -135,6 +141,10 @@ def evict(weight: Any, table: Any, lens: Any, keep: int, block_tokens: int = 16,
     tensors: kept blocks in order, the tokens left, and the blocks that left,
     -1 beyond.  ValueError for what the library refuses."""
     device = weight.device
+    gpu = _gpu(weight)
+    if _elsewhere(gpu, stream):
+        return _there(device, stream, lambda: evict(weight, table, lens, keep, block_tokens,
+                                                    keep_first, keep_last))
     _ints(table, "table", device, 2)
     _ints(lens, "lens", device, 1)
     seqs, width = table.shape
@@ -146,19 +156,17 @@ def evict(weight: Any, table: Any, lens: Any, keep: int, block_tokens: int = 16,
         raise ValueError("keep, keep_first and keep_last must not be negative")
     stride = table.stride(0) if seqs > 1 else width
     keep = min(keep, 2 ** 32 - 1)  # no table has more blocks
-    _counts(*weight.shape, block_tokens, seqs, width, stride, keep_first, keep_last)
-    queue, caller = _queue(device, stream), _caller(device, stream)
-    with queue:
-        out_table, freed = torch.empty((2, seqs, width), dtype=torch.int32, device=device).unbind()
-        out_lens, count = torch.empty((2, seqs), dtype=torch.int32, device=device).unbind()
-        _hand_over(caller, out_table, out_lens)
-        ws = _workspace(seqs * width * 8, device)
-        _refuse(nat.load().hbfsim_amd_kv_evict(
-            weight.data_ptr(), weight.shape[0], weight.shape[1], block_tokens, table.data_ptr(),
-            lens.data_ptr(), seqs, width, stride, keep, keep_first, keep_last,
-            out_table.data_ptr(), out_lens.data_ptr(), freed.data_ptr(), count.data_ptr(),
-            ws.data_ptr() if ws is not None else None, seqs * width * 8, _handle(device)),
-            "evict")
+    _counts(weight.shape[0] | weight.shape[1] | block_tokens | seqs | width | stride | keep_first
+            | keep_last)
+    _on_gpu(gpu)
+    out_table, freed = torch.empty((2, seqs, width), dtype=torch.int32, device=device).unbind()
+    out_lens, count = torch.empty((2, seqs), dtype=torch.int32, device=device).unbind()
+    ws = _workspace(seqs * width * 8, device)
+    _refuse(nat.load().hbfsim_amd_kv_evict(
+        weight.data_ptr(), weight.shape[0], weight.shape[1], block_tokens, table.data_ptr(),
+        lens.data_ptr(), seqs, width, stride, keep, keep_first, keep_last, out_table.data_ptr(),
+        out_lens.data_ptr(), freed.data_ptr(), count.data_ptr(),
+        ws.data_ptr() if ws is not None else None, seqs * width * 8, _handle(gpu)), "evict")
     return out_table, out_lens, freed, count
 
 
@@ -214,7 +222,7 @@ class KvCache:
         self.bounds, self.weight = bounds, weight
         self.blocks, self.kv_heads = blocks, kv_heads
         self.head_dim, self.block_tokens = head_dim, tiles * 16
-        self.device = keys.device
+        self.device, self._gpu = keys.device, _gpu(keys)
         self._lib = nat.load()
         self._c = nat.KvCacheArrays(ctypes.sizeof(nat.KvCacheArrays), blocks, kv_heads, head_dim,
                                     tiles * 16, 0, keys.data_ptr(), values.data_ptr(),
@@ -256,36 +264,36 @@ class KvCache:
         """Stores the step's keys and values [tokens, kv_heads, head_dim]
         (bfloat16, float16 or float32, any token and head strides) as the
         sequences' last tokens."""
+        if _elsewhere(self._gpu, stream):
+            return _there(self.device, stream, lambda: self.append(k, v, table, lens, first))
         tokens, _, kind = self._rows(k, self.kv_heads, "k")
         if self._rows(v, self.kv_heads, "v") != (tokens, self.kv_heads, kind):
             raise ValueError("k and v differ in tokens or type")
         b = _batch(table, lens, first, tokens, self.device)
         strides = (ctypes.c_int64 * 4)(k.stride(0), k.stride(1), v.stride(0), v.stride(1))
-        with _queue(self.device, stream):
-            _refuse(self._lib.hbfsim_amd_kv_append(self._ref, ctypes.byref(b), k.data_ptr(),
-                                                   v.data_ptr(), kind, strides,
-                                                   _handle(self.device)), "append")
+        _on_gpu(self._gpu)
+        _refuse(self._lib.hbfsim_amd_kv_append(self._ref, ctypes.byref(b), k.data_ptr(),
+                                               v.data_ptr(), kind, strides,
+                                               _handle(self._gpu)), "append")
 
     def read(self, blocks: Any, dtype: Any = torch.bfloat16, stream: Any = None) -> tuple:
         """The values that the blocks (int32 ids) stand for: keys and values
         [n, kv_heads, block_tokens, head_dim] and the keys' lower and upper
         bounds [n, kv_heads, head_dim]."""
+        if _elsewhere(self._gpu, stream):
+            return _there(self.device, stream, lambda: self.read(blocks, dtype))
         _ints(blocks, "blocks", self.device, 1)
         if dtype not in _TYPES:
             raise ValueError("dtype must be bfloat16, float16 or float32")
+        _on_gpu(self._gpu)
         n = blocks.shape[0]
-        queue, caller = _queue(self.device, stream), _caller(self.device, stream)
-        with queue:
-            kv = torch.empty((2, n, self.kv_heads, self.block_tokens, self.head_dim), dtype=dtype,
-                             device=self.device)
-            ends = torch.empty((2, n, self.kv_heads, self.head_dim), dtype=dtype,
-                               device=self.device)
-            _hand_over(caller, kv, ends)
-            k, v = kv.unbind()
-            low, high = ends.unbind()
-            _refuse(self._lib.hbfsim_amd_kv_read(self._ref, blocks.data_ptr(), n, _TYPES[dtype],
-                                                 k.data_ptr(), v.data_ptr(), low.data_ptr(),
-                                                 high.data_ptr(), _handle(self.device)), "read")
+        k, v = torch.empty((2, n, self.kv_heads, self.block_tokens, self.head_dim), dtype=dtype,
+                           device=self.device).unbind()
+        low, high = torch.empty((2, n, self.kv_heads, self.head_dim), dtype=dtype,
+                                device=self.device).unbind()
+        _refuse(self._lib.hbfsim_amd_kv_read(self._ref, blocks.data_ptr(), n, _TYPES[dtype],
+                                             k.data_ptr(), v.data_ptr(), low.data_ptr(),
+                                             high.data_ptr(), _handle(self._gpu)), "read")
         return k, v, low, high
 
     def attend(self, q: Any, table: Any, lens: Any, first: Any = None, selected: Any = None,
@@ -298,6 +306,9 @@ class KvCache:
         head_dim ** -0.5.  With `accumulate` the blocks' weights grow by the
         probabilities.  `out` may be q itself, but not where weights accumulate
         with `first`.  Returns [tokens, heads, head_dim] in q's type."""
+        if _elsewhere(self._gpu, stream):
+            return _there(self.device, stream, lambda: self.attend(
+                q, table, lens, first, selected, scale, accumulate, out), out is None)
         tokens, heads, kind = self._queries(q)
         b = _batch(table, lens, first, tokens, self.device)
         count, chosen = 0, None
@@ -314,7 +325,7 @@ class KvCache:
         if out is not None and (tuple(out.shape) != tuple(q.shape) or out.dtype != q.dtype
                                 or out.device != self.device or not out.is_contiguous()):
             raise ValueError("out must be a contiguous tensor of q's shape and type")
-        queue, caller = _queue(self.device, stream), _caller(self.device, stream)
+        _on_gpu(self._gpu)
         ref = ctypes.byref(b)
         sizes = (b.seqs, b.table_width, tokens, first is None, heads, count, accumulate)
         need = self._need.get(sizes)
@@ -324,17 +335,14 @@ class KvCache:
                                                              int(accumulate), ctypes.byref(got)),
                     "attend")
             need = self._remember(sizes, got.value)
-        with queue:
-            if out is None:
-                out = torch.empty((tokens, heads, self.head_dim), dtype=q.dtype,
-                                  device=self.device)
-                _hand_over(caller, out)
-            ws = _workspace(need, self.device)
-            _refuse(self._lib.hbfsim_amd_kv_attend(
-                self._ref, ref, q.data_ptr(), kind, heads, q.stride(0), q.stride(1),
-                1.0 / math.sqrt(self.head_dim) if scale is None else scale, chosen, count,
-                int(accumulate), out.data_ptr(), ws.data_ptr() if ws is not None else None,
-                need, _handle(self.device)), "attend")
+        if out is None:
+            out = torch.empty((tokens, heads, self.head_dim), dtype=q.dtype, device=self.device)
+        ws = _workspace(need, self.device)
+        _refuse(self._lib.hbfsim_amd_kv_attend(
+            self._ref, ref, q.data_ptr(), kind, heads, q.stride(0), q.stride(1),
+            1.0 / math.sqrt(self.head_dim) if scale is None else scale, chosen, count,
+            int(accumulate), out.data_ptr(), ws.data_ptr() if ws is not None else None,
+            need, _handle(self._gpu)), "attend")
         return out
 
     def select(self, q: Any, table: Any, lens: Any, count: int, first: Any = None,
@@ -343,12 +351,15 @@ class KvCache:
         int32 [tokens, kv_heads, count], ascending, -1 beyond: the first
         `keep_first` and the last `keep_last` that the token sees, and the
         best by the blocks' key bounds."""
+        if _elsewhere(self._gpu, stream):
+            return _there(self.device, stream, lambda: self.select(
+                q, table, lens, count, first, keep_first, keep_last))
         tokens, heads, kind = self._queries(q)
         if min(count, keep_first, keep_last) < 0:
             raise ValueError("count, keep_first and keep_last must not be negative")
-        _counts(count, keep_first, keep_last)
+        _counts(count | keep_first | keep_last)
         b = _batch(table, lens, first, tokens, self.device)
-        queue, caller = _queue(self.device, stream), _caller(self.device, stream)
+        _on_gpu(self._gpu)
         ref = ctypes.byref(b)
         sizes = (b.seqs, b.table_width, tokens, first is None)
         need = self._need.get(sizes)
@@ -357,15 +368,12 @@ class KvCache:
             _refuse(self._lib.hbfsim_amd_kv_select_workspace(self._ref, ref, ctypes.byref(got)),
                     "select")
             need = self._remember(sizes, got.value)
-        with queue:
-            out = torch.empty((tokens, self.kv_heads, count), dtype=torch.int32,
-                              device=self.device)
-            _hand_over(caller, out)
-            ws = _workspace(need, self.device)
-            _refuse(self._lib.hbfsim_amd_kv_select(
-                self._ref, ref, q.data_ptr(), kind, heads, q.stride(0), q.stride(1), count,
-                keep_first, keep_last, out.data_ptr(), ws.data_ptr() if ws is not None else None,
-                need, _handle(self.device)), "select")
+        out = torch.empty((tokens, self.kv_heads, count), dtype=torch.int32, device=self.device)
+        ws = _workspace(need, self.device)
+        _refuse(self._lib.hbfsim_amd_kv_select(
+            self._ref, ref, q.data_ptr(), kind, heads, q.stride(0), q.stride(1), count, keep_first,
+            keep_last, out.data_ptr(), ws.data_ptr() if ws is not None else None, need,
+            _handle(self._gpu)), "select")
         return out
 
     def evict(self, table: Any, lens: Any, keep: int, keep_first: int = 1, keep_last: int = 1,
