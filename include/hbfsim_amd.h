@@ -846,9 +846,10 @@ typedef struct hbfsim_amd_kv_cache {
  * step's own are stored, in the blocks d_table[s * table_stride + i]; the
  * step's tokens are its last ones, rows [d_first[s], d_first[s + 1]) of the
  * batch (d_first NULL: one token each, tokens == seqs).  Offsets are not
- * negative and do not decrease; rows of no sequence (a batch padded to a fixed size) and those of
- * one that ends past `tokens` store nothing, attend to nothing and select
- * nothing.  Token i of a sequence's own sees the sequence up to itself.
+ * negative and do not decrease; rows of no sequence (a batch padded to a
+ * fixed size) and those of one that ends past `tokens` store nothing, attend
+ * to nothing and select nothing.  Token i of a sequence's own sees the
+ * sequence up to itself.
  * Table entries outside [0, blocks) are blocks that are not there: nothing is
  * stored in them and nothing attends to them; so are positions past
  * table_width blocks. */
