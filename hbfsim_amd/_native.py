@@ -281,6 +281,19 @@ SIGNATURES = {
                                     _SZ, _P]),
     "hbfsim_amd_kv_evict": (_INT, [_P, _U32, _U32, _U32, _P, _P, _U32, _U32, _U32, _U32, _U32,
                                    _U32, _P, _P, _P, _P, _P, _SZ, _P]),
+    "hbfsim_amd_kv_copy_workspace": (_INT, [_P, _SZ, ctypes.POINTER(_SZ)]),
+    "hbfsim_amd_kv_copy": (_INT, [_P, _P, _P, _P, _SZ, _P, _SZ, _P]),
+    "hbfsim_amd_kv_hold": (_INT, [_P, _U32, _P, _U32, _U32, _U32, _P]),
+    "hbfsim_amd_kv_fork": (_INT, [_P, _U32, _P, _P, _U32, _U32, _U32, _P, _U32, _P, _P, _P]),
+    "hbfsim_amd_kv_release": (_INT, [_P, _U32, _U32, _P, _P, _U32, _U32, _U32, _P]),
+    "hbfsim_amd_kv_grow_workspace": (_INT, [_P, _U32, _U32, ctypes.POINTER(_SZ)]),
+    "hbfsim_amd_kv_grow": (_INT, [_P, _P, _P, _P, _P, _U32, _U32, _U32, _U32, _P, _P, _P, _SZ,
+                                  _P]),
+    "hbfsim_amd_kv_compact_workspace": (_INT, [_P, ctypes.POINTER(_SZ)]),
+    "hbfsim_amd_kv_compact": (_INT, [_P, _P, _P, _U32, _U32, _U32, _P, _P, _SZ, _P]),
+    "hbfsim_amd_verify_workspace": (_INT, [_U32, _U32, _U32, ctypes.POINTER(_SZ)]),
+    "hbfsim_amd_verify": (_INT, [_P, _P, _U32, _U32, _I64, _I64, _P, _P, _P, _U32, _U32, _P, _P, _P,
+                                 _P, _P, _SZ, _P]),
 }
 
 _lib = None

@@ -31,15 +31,14 @@
 #include <hip/hip_bf16.h>
 #include <hip/hip_fp16.h>
 
-#include "../../include/hbfsim_amd.h"
+#include "kvcache.hpp"
 
-#include <cstddef>
-#include <cstdint>
 #include <type_traits>
 
 namespace {
 
-constexpr int kWave = 64;
+using namespace hbfamd::kv;
+
 constexpr int kPickThreads = 1024;  // of a workgroup that chooses blocks
 constexpr float kInv127 = 1.0f / 127.0f;
 constexpr float kScaleMin = 0x1p-40f;
@@ -55,21 +54,6 @@ typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef std::int32_t i32x4 __attribute__((ext_vector_type(4)));
-typedef std::uint32_t u32x4 __attribute__((ext_vector_type(4)));
-
-struct Bf16 {
-    std::uint16_t bits;
-};
-struct F16 {
-    std::uint16_t bits;
-};
-
-__device__ inline float to_float(Bf16 x)
-{
-    return __uint_as_float(static_cast<std::uint32_t>(x.bits) << 16);
-}
-__device__ inline float to_float(F16 x) { return static_cast<float>(__builtin_bit_cast(_Float16, x.bits)); }
-__device__ inline float to_float(float x) { return x; }
 
 template <typename T>
 __device__ inline T from_float(float x);
@@ -93,24 +77,6 @@ __device__ inline float from_float<float>(float x)
     return x;
 }
 
-// One call's view of the cache and the batch.
-struct Cache {
-    std::int8_t* keys;
-    std::int8_t* values;
-    float* key_scale;
-    float* value_scale;
-    std::int8_t* bounds;
-    unsigned long long* weight;
-    std::uint32_t blocks, kv_heads, dim, dims;  // dims: dim rounded up to 64
-    std::uint32_t tokens, tile_shift;           // a block's tokens; log2 of its 16-token tiles
-};
-struct Batch {
-    const std::int32_t* table;
-    const std::int32_t* lens;
-    const std::int32_t* first;  // null: one token of the batch per sequence
-    std::uint32_t seqs, width, stride, tokens;
-};
-
 // A group of consecutive tokens of one sequence of the batch.  Sequence s owns
 // the slots from floor(first[s] / per) + s on, at least one and at least
 // ceil(its tokens / per); the host launches floor(tokens / per) + seqs.
@@ -120,24 +86,6 @@ struct Group {
     std::int32_t row;          // batch row of token `from`
     std::int64_t seen;         // tokens of the cache that token `from` attends to
 };
-// The last of n indices whose base (not decreasing) is not above `value`, 0 if
-// there is none.  A wave compares 64 of them at a time, so that up to 64
-// sequences cost one trip to memory and 4096 two; all lanes take part.
-template <typename F>
-__device__ inline std::uint32_t last_not_above(std::uint32_t n, std::uint32_t value, F base)
-{
-    const std::uint32_t lane = threadIdx.x % kWave;
-    std::uint32_t lo = 0;
-    while (n > 1) {
-        const std::uint32_t step = (n + kWave - 1) / kWave;
-        const unsigned long long votes = __ballot(lane * step < n && base(lo + lane * step) <= value);
-        const std::uint32_t at = votes == 0 ? 0 : (63 - static_cast<std::uint32_t>(__clzll(static_cast<long long>(votes)))) * step;
-        lo += at;
-        n = n - at < step ? n - at : step;
-        if (votes == 0) break;
-    }
-    return __builtin_amdgcn_readfirstlane(lo);
-}
 __device__ inline std::uint32_t slot_base(const Batch& b, std::uint32_t s, std::uint32_t per)
 {
     return static_cast<std::uint32_t>(b.first[s]) / per + s;
@@ -174,17 +122,6 @@ __device__ inline bool find_group(const Batch& b, std::uint32_t slot, std::uint3
     g->row = begin + g->from;
     g->seen = static_cast<std::int64_t>(b.lens[s]) - total + g->from + 1;
     return true;
-}
-
-// A physical block, or -1 for an entry that names none of the pool's.
-__device__ inline std::int32_t block_at(const Cache& c, const Batch& b, std::uint32_t seq,
-                                        std::int64_t logical)
-{
-    if (logical < 0 || logical >= static_cast<std::int64_t>(b.width)) {
-        return -1;
-    }
-    const std::int32_t id = b.table[static_cast<std::size_t>(seq) * b.stride + logical];
-    return static_cast<std::uint32_t>(id) < c.blocks ? id : -1;
 }
 
 // 4 codes -> 4 f16, exactly: 0x6400 | (code + 128) is 1024 + 128 + code.
@@ -1919,71 +1856,6 @@ __global__ __launch_bounds__(kPickThreads) void k_kv_evict(Evict a)
 
 // ---- host -----------------------------------------------------------------
 
-// A launch dimension holds fewer than 2^32 threads, a workgroup at most 1024.
-constexpr std::size_t kMostGroups = (std::size_t{1} << 22) - 1;
-
-bool aligned16(const void* p) { return (reinterpret_cast<std::uintptr_t>(p) & 15u) == 0; }
-
-int checked(hipError_t e) { return e == hipSuccess ? HBFSIM_OK : HBFSIM_CUDA_ERROR; }
-
-// The cache's own fields; pools may be asked for or not.
-int take_cache(const hbfsim_amd_kv_cache* in, Cache* out)
-{
-    if (in == nullptr || in->struct_size != sizeof(*in)) {
-        return HBFSIM_INVALID_ARGUMENT;
-    }
-    const bool tokens_ok = in->block_tokens == 16 || in->block_tokens == 32 ||
-                           in->block_tokens == 64 || in->block_tokens == 128;
-    if (in->blocks == 0 || in->blocks > 0x7fffffffu || in->kv_heads == 0 || in->kv_heads > 1024 ||
-        in->head_dim == 0 || in->head_dim > 256 || !tokens_ok) {
-        return HBFSIM_INVALID_ARGUMENT;
-    }
-    if (in->d_keys == nullptr || in->d_values == nullptr || in->d_key_scale == nullptr ||
-        in->d_value_scale == nullptr || in->d_bounds == nullptr || in->d_weight == nullptr ||
-        !aligned16(in->d_keys) || !aligned16(in->d_values) || !aligned16(in->d_bounds)) {
-        return HBFSIM_INVALID_ARGUMENT;
-    }
-    out->keys = in->d_keys;
-    out->values = in->d_values;
-    out->key_scale = in->d_key_scale;
-    out->value_scale = in->d_value_scale;
-    out->bounds = in->d_bounds;
-    out->weight = reinterpret_cast<unsigned long long*>(in->d_weight);
-    out->blocks = in->blocks;
-    out->kv_heads = in->kv_heads;
-    out->dim = in->head_dim;
-    out->dims = (in->head_dim + 63) / 64 * 64;
-    out->tokens = in->block_tokens;
-    out->tile_shift = in->block_tokens == 16 ? 0 : in->block_tokens == 32 ? 1 : in->block_tokens == 64 ? 2 : 3;
-    return HBFSIM_OK;
-}
-
-int take_batch(const hbfsim_amd_kv_batch* in, const Cache& c, Batch* out)
-{
-    if (in == nullptr || in->struct_size != sizeof(*in) || in->table_stride < in->table_width) {
-        return HBFSIM_INVALID_ARGUMENT;
-    }
-    // positions are 32-bit signed, with room for a tile beyond the last
-    if (static_cast<std::uint64_t>(in->table_width) * c.tokens > 0x7fffff00u ||
-        in->tokens > 0x7fffff00u || in->seqs > 0x7fffff00u) {
-        return HBFSIM_INVALID_ARGUMENT;
-    }
-    if (in->d_first == nullptr && in->tokens != in->seqs) {
-        return HBFSIM_INVALID_ARGUMENT;
-    }
-    if (in->seqs != 0 && in->tokens != 0 && (in->d_lens == nullptr || (in->table_width != 0 && in->d_table == nullptr))) {
-        return HBFSIM_INVALID_ARGUMENT;
-    }
-    out->table = in->d_table;
-    out->lens = in->d_lens;
-    out->first = in->d_first;
-    out->seqs = in->seqs;
-    out->width = in->table_width;
-    out->stride = in->table_stride;
-    out->tokens = in->tokens;
-    return HBFSIM_OK;
-}
-
 bool two_byte(std::uint32_t type) { return type == HBFSIM_AMD_KV_BF16 || type == HBFSIM_AMD_KV_F16; }
 
 // How attend cuts its work: from the call's host-side sizes alone.
@@ -1992,8 +1864,6 @@ struct Cut {
     std::uint32_t per, row_tiles, rows, units, split, splits;
     std::size_t partial, stats, lse, tile_sums, bytes;
 };
-
-std::size_t up256(std::size_t x) { return (x + 255) & ~std::size_t{255}; }
 
 // Row tiles per wave that fit the registers of two waves per SIMD (16 chunks
 // of 2048 tokens over 16384, D = 64: 5.84 / 5.14 / 5.38 ms with 3 / 4 / 5, D =

@@ -1,0 +1,97 @@
+"""Drafted tokens: which of a step's stay (hbfsim_amd_verify,
+include/hbfsim_amd.h section 9).
+
+A step of drafts over a paged cache appends and attends to several tokens of
+each sequence at once, the last known one and those that a draft proposes;
+`verify` says from the target's probabilities which of them stay and which
+token follows, and the cache's `release` gives back the blocks of the others.
+
+    step, missing = cache.grow(table, lens, first, tokens)
+    cache.append(k, v, table, step, first)
+    out = cache.attend(q, table, step, first)
+    new, gained, lens = verify(target, tokens, uniform, first, draft=draft, lens=step)
+    cache.release(table, lens)
+
+No counterpart in the reference.
+"""
+from __future__ import annotations
+
+import ctypes
+from typing import Any
+
+import torch
+
+from . import _native as nat
+from .kvcache import (_TYPES, _counts, _elsewhere, _gpu, _handle, _ints, _on_gpu, _refuse, _there,
+                      _workspace)
+
+_need: dict = {}  # workspace bytes by a call's sizes
+
+
+def _probabilities(x: Any, name: str, rows: int | None = None) -> Any:
+    if x.dim() != 2 or x.dtype not in _TYPES or (x.shape[1] > 1 and x.stride(1) != 1):
+        raise ValueError(f"{name} must be [rows, vocab] of bfloat16, float16 or float32, "
+                         "contiguous in its last dimension")
+    return x
+
+
+def verify(target: Any, tokens: Any, uniform: Any, first: Any = None, draft: Any = None,
+           lens: Any = None, stream: Any = None) -> tuple:
+    """Which of a step's drafted tokens stay, and the token behind them.
+
+    Sequence s has rows first[s] .. first[s + 1] - 1 of the batch (`first`
+    int32 [seqs + 1]; one row each without it): `tokens` (int32 [rows]) holds
+    its last token, then the drafted ones; target[r] and draft[r] [rows, vocab]
+    are the probabilities of the token after row r (no `draft`: the drafted
+    tokens were sure).  Draft x after row r stays while
+    uniform[r] * draft[r, x] < target[r, x]; at the first that does not, the
+    next token is drawn from max(target - draft, 0), behind the last one from
+    target, both by the `uniform` (float32 [rows], in [0, 1)) of the sequence's
+    last row.  The drawing is in whole numbers, 2^40 to a probability of one.
+
+    Returns (out, gained, lens): int32 [rows] with each sequence's tokens from
+    its first row on, -1 beyond; how many they are; and, from `lens` (tokens
+    stored with all of the step's), those that remain, None without it."""
+    gpu = _gpu(target)
+    if _elsewhere(gpu, stream):
+        return _there(target.device, stream, lambda: verify(target, tokens, uniform, first, draft,
+                                                            lens))
+    device = target.device
+    rows, vocab = _probabilities(target, "target").shape
+    if draft is not None and (_probabilities(draft, "draft").shape != target.shape
+                              or draft.dtype != target.dtype or draft.device != device):
+        raise ValueError("draft must be of target's shape, type and device")
+    if _ints(tokens, "tokens", device, 1).shape[0] != rows:
+        raise ValueError(f"{tokens.shape[0]} tokens for {rows} rows")
+    if uniform.dtype != torch.float32 or tuple(uniform.shape) != (rows,) \
+            or uniform.device != device or not uniform.is_contiguous():
+        raise ValueError(f"uniform must be a contiguous float32 tensor [{rows}] on {device}")
+    seqs = rows
+    if first is not None:
+        seqs = _ints(first, "first", device, 1).shape[0] - 1
+        if seqs < 0:
+            raise ValueError("first must hold one offset more than there are sequences")
+    if lens is not None and _ints(lens, "lens", device, 1).shape[0] != seqs:
+        raise ValueError(f"{lens.shape[0]} lengths for {seqs} sequences")
+    _counts(rows | seqs | vocab)
+    _on_gpu(gpu)
+    kind = _TYPES[target.dtype]
+    need = _need.get((seqs, vocab, kind))
+    if need is None:
+        got = ctypes.c_size_t()
+        _refuse(nat.load().hbfsim_amd_verify_workspace(seqs, vocab, kind, ctypes.byref(got)),
+                "verify")
+        if len(_need) >= 4096:
+            _need.clear()
+        need = _need[seqs, vocab, kind] = got.value
+    out = torch.empty((rows,), dtype=torch.int32, device=device)
+    gained, left = torch.empty((2, seqs), dtype=torch.int32, device=device).unbind()
+    ws = _workspace(need, device)
+    _refuse(nat.load().hbfsim_amd_verify(
+        target.data_ptr(), draft.data_ptr() if draft is not None else None, kind, vocab,
+        target.stride(0), draft.stride(0) if draft is not None else 0, tokens.data_ptr(),
+        uniform.data_ptr(), first.data_ptr() if first is not None else None, seqs, rows,
+        lens.data_ptr() if lens is not None else None, out.data_ptr(), gained.data_ptr(),
+        left.data_ptr() if lens is not None else None, ws.data_ptr() if ws is not None else None,
+        need, _handle(gpu)), "verify")
+    return out, gained, left if lens is not None else None

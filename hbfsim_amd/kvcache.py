@@ -16,6 +16,21 @@ current one by default) and return without waiting for it.
     out = cache.attend(q, table, lens, accumulate=True)
     table, lens, freed, count = cache.evict(table, lens, keep=512)
 
+Who holds a block may be left to the cache as well (section 8 of the header):
+`refs` (int32 [blocks]) counts the table entries that name each block, and one
+of no reference is free.  Sequences that branch share their blocks.
+
+    table = torch.full((seqs, width), -1, dtype=torch.int32, device="cuda")
+    step, missing = cache.grow(table, lens)       # blocks for the step's tokens
+    cache.append(k, v, table, step)
+    table, lens = cache.fork(table, lens, parents)  # the next batch: branches, beams
+    cache.release(table, lens)                    # blocks past the lengths
+    where = cache.compact(table)                  # blocks in use to the pool's front
+    cache.copy(src, dst, to=other)                # to another pool, or within it
+
+A tensor that a call changes (`refs`, the table of grow, release and compact)
+is changed on the call's stream: other streams wait for it as for any write.
+
 No counterpart in the reference.
 """
 from __future__ import annotations
@@ -74,7 +89,8 @@ def _there(device: Any, stream: Any, call: Any, own: bool = True) -> Any:
         got = call()
     if own and got is not None:
         for t in got if isinstance(got, tuple) else (got,):
-            t.record_stream(caller)
+            if t is not None:
+                t.record_stream(caller)
     return got
 
 
@@ -170,6 +186,84 @@ def evict(weight: Any, table: Any, lens: Any, keep: int, block_tokens: int = 16,
     return out_table, out_lens, freed, count
 
 
+def _references(refs: Any, blocks: int | None = None) -> Any:
+    if refs.dtype != torch.int32 or refs.dim() != 1 or not refs.is_contiguous() \
+            or not refs.shape[0] or blocks not in (None, refs.shape[0]):
+        raise ValueError("refs must be a contiguous int32 tensor [blocks]")
+    return refs
+
+
+def _written(x: Any, name: str) -> Any:
+    """A table that a call changes: its rows must not share memory."""
+    if x.shape[0] > 1 and x.stride(0) < x.shape[1]:
+        raise ValueError(f"{name} rows overlap")
+    return x
+
+
+def _rows_of(table: Any, refs: Any, lens: Any = None) -> tuple[int, int, int]:
+    """(sequences, width, stride) of a table beside its references."""
+    device = refs.device
+    _written(_ints(table, "table", device, 2), "table")
+    seqs, width = table.shape
+    if lens is not None and _ints(lens, "lens", device, 1).shape[0] != seqs:
+        raise ValueError(f"{lens.shape[0]} lengths for {seqs} sequences")
+    stride = table.stride(0) if seqs > 1 else width
+    _counts(refs.shape[0] | seqs | width | stride)
+    return seqs, width, stride
+
+
+def hold(refs: Any, table: Any, stream: Any = None) -> None:
+    """Counts the table's entries (int32 [seqs, width]): one reference each in
+    `refs` (int32 [blocks]).  For tables made by hand; fork, release and grow
+    count what they change themselves."""
+    gpu = _gpu(refs)
+    if _elsewhere(gpu, stream):
+        return _there(refs.device, stream, lambda: hold(refs, table))
+    _references(refs)
+    seqs, width, stride = _rows_of(table, refs)
+    _on_gpu(gpu)
+    _refuse(nat.load().hbfsim_amd_kv_hold(refs.data_ptr(), refs.shape[0], table.data_ptr(), seqs,
+                                          width, stride, _handle(gpu)), "hold")
+
+
+def fork(refs: Any, table: Any, lens: Any, parents: Any, stream: Any = None) -> tuple:
+    """The next batch: row i continues sequence parents[i] (int32 [rows]; any
+    number outside 0..seqs-1 gives an empty row).  Returns (table, lens), new
+    tensors.  The old rows' references go and the new ones' come, so a sequence
+    that no row continues gives its blocks back: the old table is done with."""
+    gpu = _gpu(refs)
+    if _elsewhere(gpu, stream):
+        return _there(refs.device, stream, lambda: fork(refs, table, lens, parents))
+    _references(refs)
+    seqs, width, stride = _rows_of(table, refs, lens)
+    rows = _ints(parents, "parents", refs.device, 1).shape[0]
+    _counts(rows)
+    _on_gpu(gpu)
+    out = torch.empty((rows, width), dtype=torch.int32, device=refs.device)
+    out_lens = torch.empty((rows,), dtype=torch.int32, device=refs.device)
+    _refuse(nat.load().hbfsim_amd_kv_fork(
+        refs.data_ptr(), refs.shape[0], table.data_ptr(), lens.data_ptr(), seqs, width, stride,
+        parents.data_ptr(), rows, out.data_ptr(), out_lens.data_ptr(), _handle(gpu)), "fork")
+    return out, out_lens
+
+
+def release(refs: Any, table: Any, lens: Any = None, block_tokens: int = 16,
+            stream: Any = None) -> None:
+    """Entries of blocks that start at or past the sequences' lengths (all of
+    them without `lens`) leave: they become -1 in `table` itself, and their
+    references go."""
+    gpu = _gpu(refs)
+    if _elsewhere(gpu, stream):
+        return _there(refs.device, stream, lambda: release(refs, table, lens, block_tokens))
+    _references(refs)
+    seqs, width, stride = _rows_of(table, refs, lens)
+    _counts(block_tokens)
+    _on_gpu(gpu)
+    _refuse(nat.load().hbfsim_amd_kv_release(
+        refs.data_ptr(), refs.shape[0], block_tokens, table.data_ptr(),
+        lens.data_ptr() if lens is not None else None, seqs, width, stride, _handle(gpu)), "release")
+
+
 class KvCache:
     """A pool of blocks of `block_tokens` tokens of every kv head."""
 
@@ -188,18 +282,19 @@ class KvCache:
                    torch.ones((blocks, kv_heads), dtype=torch.float32, **new),
                    torch.ones((blocks, kv_heads), dtype=torch.float32, **new),
                    torch.zeros((blocks, kv_heads, 2, dims), dtype=torch.int8, **new),
-                   torch.zeros((blocks, kv_heads), dtype=torch.int64, **new), head_dim)
+                   torch.zeros((blocks, kv_heads), dtype=torch.int64, **new), head_dim, None)
 
     @classmethod
     def from_tensors(cls, keys: Any, values: Any, key_scale: Any, value_scale: Any, bounds: Any,
-                     weight: Any, head_dim: int) -> "KvCache":
+                     weight: Any, head_dim: int, refs: Any = None) -> "KvCache":
         """A cache over arrays the caller keeps, in the library's layout (the
-        tensors' shapes as the constructor makes them)."""
+        tensors' shapes as the constructor makes them); without `refs` every
+        block is free."""
         self = cls.__new__(cls)
-        self._take(keys, values, key_scale, value_scale, bounds, weight, head_dim)
+        self._take(keys, values, key_scale, value_scale, bounds, weight, head_dim, refs)
         return self
 
-    def _take(self, keys, values, key_scale, value_scale, bounds, weight, head_dim):
+    def _take(self, keys, values, key_scale, value_scale, bounds, weight, head_dim, refs):
         if keys.dim() != 7 or not 0 < head_dim <= 256:
             raise ValueError("keys must have 7 dimensions and head_dim be in 1..256")
         blocks, kv_heads, tiles, chunks = keys.shape[:4]
@@ -217,7 +312,11 @@ class KvCache:
                 raise ValueError(f"{name} must be a contiguous {dtype} tensor of shape {want}")
             if x.device != keys.device:
                 raise ValueError(f"{name} is on {x.device}, keys on {keys.device}")
-        self.keys, self.values = keys, values
+        if refs is None:
+            refs = torch.zeros((blocks,), dtype=torch.int32, device=keys.device)
+        elif _references(refs, blocks).device != keys.device:
+            raise ValueError(f"refs is on {refs.device}, keys on {keys.device}")
+        self.keys, self.values, self.refs = keys, values, refs
         self.key_scale, self.value_scale = key_scale, value_scale
         self.bounds, self.weight = bounds, weight
         self.blocks, self.kv_heads = blocks, kv_heads
@@ -381,6 +480,102 @@ class KvCache:
         """`evict` by this cache's weights."""
         return evict(self.weight, table, lens, keep, self.block_tokens, keep_first, keep_last,
                      stream)
+
+    def copy(self, src: Any, dst: Any, to: "KvCache | None" = None, stream: Any = None) -> None:
+        """Blocks `src` (int32 ids) become blocks `dst` of the same cache or of
+        `to`, another one of the same heads, dim and block tokens: codes,
+        scales, bounds and weight (references stay with their tables).  Ids
+        outside a pool copy nothing; of pairs with the same destination the
+        first copies; within one cache a block that is a destination of the
+        call is no source."""
+        if _elsewhere(self._gpu, stream):
+            return _there(self.device, stream, lambda: self.copy(src, dst, to))
+        to = self if to is None else to
+        _ints(src, "src", self.device, 1)
+        n = _ints(dst, "dst", self.device, 1).shape[0]
+        if src.shape[0] != n:
+            raise ValueError(f"{src.shape[0]} sources for {n} destinations")
+        if to.device != self.device:
+            raise ValueError(f"to is on {to.device}, the cache on {self.device}")
+        _on_gpu(self._gpu)
+        need = to.blocks * 4 if n else 0
+        ws = _workspace(need, self.device)
+        _refuse(self._lib.hbfsim_amd_kv_copy(
+            self._ref, to._ref, src.data_ptr(), dst.data_ptr(), n,
+            ws.data_ptr() if ws is not None else None, need, _handle(self._gpu)), "copy")
+
+    def hold(self, table: Any, stream: Any = None) -> None:
+        """`hold` in this cache's references."""
+        hold(self.refs, table, stream)
+
+    def fork(self, table: Any, lens: Any, parents: Any, stream: Any = None) -> tuple:
+        """`fork` in this cache's references."""
+        return fork(self.refs, table, lens, parents, stream)
+
+    def release(self, table: Any, lens: Any = None, stream: Any = None) -> None:
+        """`release` in this cache's references."""
+        release(self.refs, table, lens, self.block_tokens, stream)
+
+    def grow(self, table: Any, lens: Any, first: Any = None, tokens: int | None = None,
+             stream: Any = None) -> tuple:
+        """Blocks for a step's tokens before they are appended: `lens` and
+        `first` are the append's, `tokens` its rows where `first` is given.  The
+        table is changed: a row gets a new block where it names none, and one
+        of its own, with the content, where the step writes to a shared one.
+        Returns (lens, missing): the step's lengths, 0 for a sequence that lacks
+        blocks (its row stays as it is), and how many such a sequence needs."""
+        if _elsewhere(self._gpu, stream):
+            return _there(self.device, stream, lambda: self.grow(table, lens, first, tokens))
+        refs = _references(self.refs, self.blocks)
+        seqs, width, stride = _rows_of(table, refs, lens)
+        if first is None:
+            if tokens not in (None, seqs):
+                raise ValueError(f"{tokens} tokens for {seqs} sequences of one token each")
+            tokens = seqs
+        else:
+            if _ints(first, "first", self.device, 1).shape[0] != seqs + 1:
+                raise ValueError("first must hold one offset more than there are sequences")
+            if tokens is None or tokens < 0:
+                raise ValueError("tokens must say how many rows the batch of `first` has")
+        _counts(tokens)
+        _on_gpu(self._gpu)
+        sizes = ("grow", seqs, tokens)
+        need = self._need.get(sizes)
+        if need is None:
+            got = ctypes.c_size_t()
+            _refuse(self._lib.hbfsim_amd_kv_grow_workspace(self._ref, seqs, tokens,
+                                                           ctypes.byref(got)), "grow")
+            need = self._remember(sizes, got.value)
+        out, missing = torch.empty((2, seqs), dtype=torch.int32, device=self.device).unbind()
+        ws = _workspace(need, self.device)
+        _refuse(self._lib.hbfsim_amd_kv_grow(
+            self._ref, refs.data_ptr(), table.data_ptr(), lens.data_ptr(),
+            first.data_ptr() if first is not None else None, seqs, tokens, width, stride,
+            out.data_ptr(), missing.data_ptr(), ws.data_ptr() if ws is not None else None, need,
+            _handle(self._gpu)), "grow")
+        return out, missing
+
+    def compact(self, table: Any, stream: Any = None) -> Any:
+        """Blocks in use move to the front of the pool, and the table's entries
+        with them.  Returns where each block went (int32 [blocks], -1 for a
+        free one), by which other tables of this cache can follow."""
+        if _elsewhere(self._gpu, stream):
+            return _there(self.device, stream, lambda: self.compact(table))
+        refs = _references(self.refs, self.blocks)
+        seqs, width, stride = _rows_of(table, refs)
+        _on_gpu(self._gpu)
+        need = self._need.get("compact")
+        if need is None:
+            got = ctypes.c_size_t()
+            _refuse(self._lib.hbfsim_amd_kv_compact_workspace(self._ref, ctypes.byref(got)),
+                    "compact")
+            need = self._remember("compact", got.value)
+        where = torch.empty((self.blocks,), dtype=torch.int32, device=self.device)
+        ws = _workspace(need, self.device)
+        _refuse(self._lib.hbfsim_amd_kv_compact(
+            self._ref, refs.data_ptr(), table.data_ptr(), seqs, width, stride, where.data_ptr(),
+            ws.data_ptr(), need, _handle(self._gpu)), "compact")
+        return where
 
     def weights(self) -> Any:
         """The accumulated weights as float32 probabilities."""

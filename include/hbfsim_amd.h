@@ -943,6 +943,121 @@ int hbfsim_amd_kv_evict(const int64_t* d_weight, uint32_t blocks, uint32_t kv_he
                         int32_t* d_out_lens, int32_t* d_freed, int32_t* d_freed_count,
                         void* d_workspace, size_t workspace_bytes, void* stream);
 
+/* ===== 8. Blocks of branching sequences ================================
+ *
+ * No counterpart in the reference.  Who holds the blocks of a paged cache:
+ * d_refs int32 [blocks] counts the table entries that name each block, and a
+ * block of no reference (0 or below) is free.  Sequences that continue the
+ * same tokens share blocks; every entry in [0, blocks) of a live row is one
+ * reference, whether its sequence's length reaches it or not.  As above, work
+ * is queued on `stream` and nothing is allocated or copied to the host; calls
+ * on one d_refs follow one another.  Counts change by whole numbers, so
+ * results do not depend on an order of atomics.  Tables are
+ * [seqs][width] with `stride` entries from one row to the next (at least
+ * width, also where there is one row); HBFSIM_INVALID_ARGUMENT for sizes
+ * outside section 7's limits. */
+
+/* Blocks d_src[i] of `from` become blocks d_dst[i] of `to`, i in [0, n):
+ * codes, scales, bounds and weight.  `to` may be `from`, or another cache of
+ * the same kv heads, dim and block tokens whose arrays do not overlap its.
+ * Pairs with an id outside its pool count for nothing.  Of those that name the
+ * same destination the first copies; within one cache, a pair whose source is
+ * any pair's destination copies nothing.  The workspace call gives the bytes
+ * needed. */
+int hbfsim_amd_kv_copy_workspace(const hbfsim_amd_kv_cache* to, size_t n, size_t* bytes);
+int hbfsim_amd_kv_copy(const hbfsim_amd_kv_cache* from, const hbfsim_amd_kv_cache* to,
+                       const int32_t* d_src, const int32_t* d_dst, size_t n, void* d_workspace,
+                       size_t workspace_bytes, void* stream);
+
+/* The table's entries are counted: one reference each. */
+int hbfsim_amd_kv_hold(int32_t* d_refs, uint32_t blocks, const int32_t* d_table, uint32_t seqs,
+                       uint32_t width, uint32_t stride, void* stream);
+
+/* The next batch: row i of d_out_table [rows][width] and d_out_lens [rows]
+ * continues sequence d_parents[i] of this one (a row of -1 and length 0 where
+ * that is outside [0, seqs)).  The old rows' references go and the new ones'
+ * come: a sequence of c children changes its blocks' counts by c - 1.  The
+ * outputs overlap no input. */
+int hbfsim_amd_kv_fork(int32_t* d_refs, uint32_t blocks, const int32_t* d_table,
+                       const int32_t* d_lens, uint32_t seqs, uint32_t width, uint32_t stride,
+                       const int32_t* d_parents, uint32_t rows, int32_t* d_out_table,
+                       int32_t* d_out_lens, void* stream);
+
+/* Entries that start at or past d_lens[s] tokens (all of them where d_lens is
+ * NULL) leave: their references go and they become -1. */
+int hbfsim_amd_kv_release(int32_t* d_refs, uint32_t blocks, uint32_t block_tokens,
+                          int32_t* d_table, const int32_t* d_lens, uint32_t seqs, uint32_t width,
+                          uint32_t stride, void* stream);
+
+/* Blocks for a step's tokens, before they are appended: the batch is the
+ * append's (`tokens` rows, d_first as there), its table is changed.  A block
+ * that the step writes to becomes a new one where the row names none or a
+ * free one, and where it is shared: then its content is copied if it holds
+ * tokens of the sequence already, and its count falls by one.  Where all of a
+ * block's references are entries that the step writes to, the last of them
+ * (by sequence, then by place) keeps it.  New blocks are the free ones in
+ * ascending order, by sequence and place.  A block begun before the step that
+ * the row does not name stays away; one that it names though it is free leaves
+ * the row (-1).
+ * Where there are fewer free blocks than that needs, no shared block is kept
+ * and sequences are served in order for as long as the blocks last; one that
+ * needs more than are left after those before it, or whose tokens reach past
+ * the table, gets none and keeps its row.  d_missing[s] is then the number of
+ * blocks that it needs, and d_out_lens[s], otherwise d_lens[s], is 0, with
+ * which the step neither stores nor attends for it.  d_out_lens may be
+ * d_lens. */
+int hbfsim_amd_kv_grow_workspace(const hbfsim_amd_kv_cache* cache, uint32_t seqs, uint32_t tokens,
+                                 size_t* bytes);
+int hbfsim_amd_kv_grow(const hbfsim_amd_kv_cache* cache, int32_t* d_refs, int32_t* d_table,
+                       const int32_t* d_lens, const int32_t* d_first, uint32_t seqs,
+                       uint32_t tokens, uint32_t width, uint32_t stride, int32_t* d_out_lens,
+                       int32_t* d_missing, void* d_workspace, size_t workspace_bytes,
+                       void* stream);
+
+/* The cache's blocks in use move to the front of the pool: with L of them, the
+ * j-th (by id) at or past L moves to the j-th free one below L.  d_where
+ * [blocks] receives each block's new id, -1 for a free one; entries of the
+ * table (width or seqs may be 0) become the new ids, -1 where they name no
+ * block in use.  d_refs moves too. */
+int hbfsim_amd_kv_compact_workspace(const hbfsim_amd_kv_cache* cache, size_t* bytes);
+int hbfsim_amd_kv_compact(const hbfsim_amd_kv_cache* cache, int32_t* d_refs, int32_t* d_table,
+                          uint32_t seqs, uint32_t width, uint32_t stride, int32_t* d_where,
+                          void* d_workspace, size_t workspace_bytes, void* stream);
+
+/* ===== 9. Drafted tokens ===============================================
+ *
+ * No counterpart in the reference.  Which of a step's drafted tokens stay.
+ * Sequence s has rows [d_first[s], d_first[s + 1]) of the batch (d_first NULL:
+ * one each): d_tokens holds its last token (not read), then the drafted ones.
+ * d_target[r] and d_draft[r] (`vocab` probabilities of `type`, the KV types,
+ * with strides in elements) are what the target and the draft give for the
+ * token after row r; the draft's last row of a sequence is not read, and
+ * d_draft NULL stands for a draft that was sure of its tokens.  Probabilities
+ * are taken into [0, 1], what is not a number as 0.
+ *   Draft x after row r stays while  u[r] q(x) < p(x),  exactly (64 bits).
+ *   At the first that does not, the next token is drawn from max(P - Q, 0)
+ *   (without a draft: P but for x), where no whole number is left of that, and
+ *   behind the last draft, from P;  P = 2^40 p, rounded to nearest even.
+ *   A drafted token outside the vocabulary ends its sequence's drafts; what
+ *   follows is drawn from P.
+ *   Drawn is the first token whose running sum is above
+ *   floor(floor(2^31 u) T / 2^31), u of the sequence's last row within [0, 1)
+ *   and T the sum: whole numbers, so that no order of sums matters.  -1 where T
+ *   is 0.
+ * d_out [tokens] holds a sequence's tokens from its first row on, those that
+ * stay and the drawn one, -1 beyond and in rows of no sequence; d_gained [seqs]
+ * how many they are (0 for a sequence of no rows or with rows past `tokens`).
+ * With d_lens, the tokens stored for each sequence with all of its rows,
+ * d_out_lens (which may be d_lens) is what remains of them: less by the rows
+ * whose tokens did not stay.  d_out overlaps no input.  vocab is at most 2^22. */
+int hbfsim_amd_verify_workspace(uint32_t seqs, uint32_t vocab, uint32_t type, size_t* bytes);
+int hbfsim_amd_verify(const void* d_target, const void* d_draft, uint32_t type, uint32_t vocab,
+                      int64_t target_stride, int64_t draft_stride, const int32_t* d_tokens,
+                      const float* d_uniform, const int32_t* d_first, uint32_t seqs,
+                      uint32_t tokens, const int32_t* d_lens, int32_t* d_out, int32_t* d_gained,
+                      int32_t* d_out_lens, void* d_workspace, size_t workspace_bytes,
+                      void* stream);
+
 #ifdef __cplusplus
 }
 #endif
