@@ -66,6 +66,7 @@ struct Copy {
     std::int32_t* owner;  // [to.blocks]: the first pair that names the block as its destination
 };
 constexpr std::int32_t kNobody = 0x7fffffff;
+constexpr std::uint32_t kFewPairs = 1024;
 
 __device__ inline bool pair_at(const Copy& a, std::uint32_t i, std::int32_t* src, std::int32_t* dst)
 {
@@ -88,8 +89,7 @@ __global__ __launch_bounds__(kThreads) void k_kv_copy_claim(Copy a)
     std::int32_t src, dst;
     if (i < a.n && pair_at(a, i, &src, &dst)) atomicMin(&a.owner[dst], static_cast<std::int32_t>(i));
 }
-// A destination that an invalid pair names is claimed by nobody: pairs count
-// only where both ids are of their pools.
+// Pairs count only where both ids are of their pools.
 __global__ __launch_bounds__(kThreads) void k_kv_copy(Copy a)
 {
     const std::uint32_t i = blockIdx.x / a.p.parts, part = blockIdx.x % a.p.parts;
@@ -99,6 +99,19 @@ __global__ __launch_bounds__(kThreads) void k_kv_copy(Copy a)
         return;
     }
     copy_part(a.from, a.to, a.p, src, dst, part);
+}
+// Every workgroup looks through the pairs itself: one launch instead of three.
+__global__ __launch_bounds__(kThreads) void k_kv_copy_few(Copy a)
+{
+    const std::uint32_t i = blockIdx.x / a.p.parts, part = blockIdx.x % a.p.parts;
+    std::int32_t src, dst;
+    const bool counts = pair_at(a, i, &src, &dst);
+    bool taken = !counts;
+    for (std::uint32_t j = threadIdx.x; j < a.n; j += kThreads) {
+        std::int32_t s, d;
+        if (pair_at(a, j, &s, &d)) taken |= (d == dst && j < i) || (a.same != 0 && d == src);
+    }
+    if (__syncthreads_or(taken) == 0) copy_part(a.from, a.to, a.p, src, dst, part);
 }
 
 // ---- counts and tables --------------------------------------------------------
@@ -201,6 +214,7 @@ struct Grow {
     const std::int32_t* lens;
     const std::int32_t* first;
     std::uint32_t seqs, tokens, width, stride, slots;
+    std::uint32_t vector;  // counts may be loaded 16 bytes at a time
     std::int32_t* out_lens;
     std::int32_t* missing;
     // workspace
@@ -240,12 +254,8 @@ __device__ inline std::uint32_t base_of(const Grow& a, std::uint32_t s)
     const std::uint64_t at = static_cast<std::uint32_t>(a.first[s]) / a.c.tokens + std::uint64_t{2} * s;
     return at < a.slots ? static_cast<std::uint32_t>(at) : a.slots;
 }
+// Atomics' results as they are now.
 __device__ inline std::int32_t now(const std::int32_t* p) { return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
-__device__ inline void settled()  // what the workgroup stored is seen by all of it
-{
-    __threadfence();
-    __syncthreads();
-}
 
 // Sums before each thread's `x`, and of all; all threads call it.
 __device__ inline std::int32_t before(std::int32_t x, std::int32_t* all)
@@ -285,14 +295,77 @@ __device__ inline std::int32_t count_needs(const Grow& a, F fresh)
         total += all;
     }
     if (threadIdx.x == 0) a.need[a.slots] = total;
-    settled();
+    __syncthreads();
     return total;
 }
 
+// Bits of a thread's 8 blocks from id0 on that are free.
+__device__ inline std::uint32_t free_of_8(const Grow& a, std::uint64_t id0)
+{
+    std::int32_t r[8];
+    if (a.vector != 0 && id0 + 8 <= a.c.blocks) {
+        *reinterpret_cast<int4*>(r) = *reinterpret_cast<const int4*>(a.refs + id0);
+        *reinterpret_cast<int4*>(r + 4) = *reinterpret_cast<const int4*>(a.refs + id0 + 4);
+    } else {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) r[k] = id0 + k < a.c.blocks ? a.refs[id0 + k] : 1;
+    }
+    std::uint32_t bits = 0;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) bits |= r[k] <= 0 ? 1u << k : 0u;
+    return bits;
+}
+// Sums of numbers below 2^kBits before each thread's, and of all.
+template <int kBits>
+__device__ inline std::int32_t before_small(std::uint32_t x, std::int32_t* all)
+{
+    __shared__ std::int32_t s_wave[kPlanWaves];
+    const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
+    const unsigned long long below = (1ull << lane) - 1;
+    std::int32_t mine = 0, sum = 0;
+#pragma unroll
+    for (int b = 0; b < kBits; ++b) {
+        const unsigned long long votes = __ballot((x >> b & 1u) != 0);
+        mine += __popcll(votes & below) << b;
+        sum += __popcll(votes) << b;
+    }
+    __syncthreads();
+    if (lane == 0) s_wave[wave] = sum;
+    __syncthreads();
+    sum = 0;
+#pragma unroll
+    for (int i = 0; i < kPlanWaves; ++i) {
+        mine += i < wave ? s_wave[i] : 0;
+        sum += s_wave[i];
+    }
+    *all = sum;
+    return mine;
+}
+
+// One workgroup plans: what each slot writes to, who keeps a shared block, how
+// many blocks are wanted, the first free ones, who gets them.
 __global__ __launch_bounds__(kPlan) void k_kv_grow(Grow a)
 {
+    constexpr std::uint32_t kHeld = 4096;  // sequences whose parts lie in LDS
+    __shared__ std::int32_t s_base[kHeld + 1];
+    __shared__ int2 s_part[kHeld];
     const std::uint32_t t = a.c.tokens;
-    // what each slot writes to
+    const bool held = a.seqs <= kHeld;
+    for (std::uint32_t s = threadIdx.x; s < a.seqs; s += kPlan) {
+        a.pair[s] = int2{-1, -1};
+        if (held) {
+            const Part part = part_of(a, s);
+            s_part[s] = int2{static_cast<int>(part.from), static_cast<int>(part.to)};
+            s_base[s] = static_cast<std::int32_t>(base_of(a, s));
+        }
+    }
+    if (held && threadIdx.x == 0) s_base[a.seqs] = static_cast<std::int32_t>(a.slots);
+    std::uint32_t tile = free_of_8(a, std::uint64_t{8} * threadIdx.x);
+    __syncthreads();
+    const auto base = [&](std::uint32_t s) {
+        return held ? static_cast<std::uint32_t>(s_base[s]) : s < a.seqs ? base_of(a, s) : a.slots;
+    };
+    const auto parts = [&](std::uint32_t s) { return held ? Part{s_part[s].x, s_part[s].y} : part_of(a, s); };
     bool shared = false;
     for (std::uint32_t i = threadIdx.x; i < a.slots; i += kPlan) {
         std::uint32_t s = i;
@@ -300,15 +373,14 @@ __global__ __launch_bounds__(kPlan) void k_kv_grow(Grow a)
             std::uint32_t lo = 0, hi = a.seqs;  // the last sequence whose slots begin at or before i
             while (hi - lo > 1) {
                 const std::uint32_t mid = lo + (hi - lo) / 2;
-                if (base_of(a, mid) <= i) lo = mid; else hi = mid;
+                if (base(mid) <= i) lo = mid; else hi = mid;
             }
             s = lo;
         }
         int4 slot = {static_cast<int>(s), 0, kIdle, 0};
-        const Part part = part_of(a, s);
-        const std::uint32_t base = base_of(a, s);
-        const std::int64_t place = part.from / t + (static_cast<std::int64_t>(i) - base);
-        if (i >= base && place * t < part.to && (part.to - 1) / t < static_cast<std::int64_t>(a.width)) {
+        const Part part = parts(s);
+        const std::int64_t place = part.from / t + (static_cast<std::int64_t>(i) - base(s));
+        if (i >= base(s) && place * t < part.to && (part.to - 1) / t < static_cast<std::int64_t>(a.width)) {
             const std::int32_t id = a.table[static_cast<std::size_t>(s) * a.stride + place];
             const bool named = inside(id, a.c.blocks), begun = place * t < part.from;
             const std::int32_t refs = named ? a.refs[id] : 0;
@@ -327,10 +399,7 @@ __global__ __launch_bounds__(kPlan) void k_kv_grow(Grow a)
         }
         a.slot[i] = slot;
     }
-    for (std::uint32_t s = threadIdx.x; s < a.seqs; s += kPlan) a.pair[s] = int2{-1, -1};
-    const bool any = __syncthreads_or(shared);
-    if (any) {
-        settled();
+    if (__syncthreads_or(shared)) {
         for (std::uint32_t i = threadIdx.x; i < a.slots; i += kPlan) {
             const int4 slot = a.slot[i];
             if (slot.z >= 0 && slot.w > 1) {
@@ -338,67 +407,194 @@ __global__ __launch_bounds__(kPlan) void k_kv_grow(Grow a)
                 atomicMax(&a.last[slot.z], static_cast<std::int32_t>(i));
             }
         }
+        __syncthreads();
     }
-    settled();
-    const auto keeps = [&](std::uint32_t i) {
-        const int4 slot = a.slot[i];
-        return slot.w <= 1 || (now(&a.writers[slot.z]) >= slot.w && now(&a.last[slot.z]) == static_cast<std::int32_t>(i));
-    };
     const auto fresh = [&](std::uint32_t i) {
-        const int z = a.slot[i].z;
-        return z == kNew || (z >= 0 && !keeps(i));
+        const int4 slot = a.slot[i];
+        if (slot.z < 0 || slot.w <= 1) return slot.z == kNew;
+        return now(&a.writers[slot.z]) < slot.w || now(&a.last[slot.z]) != static_cast<std::int32_t>(i);
     };
     const auto fresh_alone = [&](std::uint32_t i) {  // no shared block is kept
         const int4 slot = a.slot[i];
         return slot.z == kNew || (slot.z >= 0 && slot.w > 1);
     };
     std::int32_t want = count_needs(a, fresh);
-    // free blocks, as many as are wanted
     std::int32_t free = 0;
-    for (std::uint64_t at = 0; at < a.c.blocks && free < want; at += kPlan) {
-        const std::uint64_t id = at + threadIdx.x;
-        const bool is = id < a.c.blocks && a.refs[id] <= 0;
+    for (std::uint64_t from = 0; free < want && from < a.c.blocks; from += 8 * kPlan) {
+        const std::uint64_t id0 = from + std::uint64_t{8} * threadIdx.x;
+        const std::uint32_t next = from + 8 * kPlan < a.c.blocks ? free_of_8(a, id0 + 8 * kPlan) : 0;
         std::int32_t all;
-        const std::int32_t rank = free + before(is ? 1 : 0, &all);
-        if (is && rank < want) a.found[rank] = static_cast<std::int32_t>(id);
+        std::int32_t rank = free + before_small<4>(__popc(tile), &all);
+        for (std::uint32_t bits = tile; bits != 0 && rank < want; bits &= bits - 1) {
+            a.found[rank++] = static_cast<std::int32_t>(id0) + __ffs(bits) - 1;
+        }
         free += all;
+        tile = next;
     }
     const bool enough = free >= want;
     if (!enough) want = count_needs(a, fresh_alone);
-    settled();
-    const auto granted = [&](std::uint32_t s) {
-        const Part part = part_of(a, s);
+    __syncthreads();
+    const auto granted = [&](std::uint32_t s, const Part& part) {
         if (part.to > 0 && (part.to - 1) / t >= static_cast<std::int64_t>(a.width)) return false;
-        const std::int32_t from = a.need[base_of(a, s)], to = a.need[s + 1 < a.seqs ? base_of(a, s + 1) : a.slots];
+        const std::int32_t from = a.need[base(s)], to = a.need[base(s + 1)];
         return enough || to == from || to <= free;
     };
     for (std::uint32_t i = threadIdx.x; i < a.slots; i += kPlan) {
         const int4 slot = a.slot[i];
-        if (slot.z == kIdle || !granted(slot.x)) continue;
+        if (slot.z == kIdle) continue;
+        const Part part = parts(slot.x);
+        const bool gets = enough ? fresh(i) : fresh_alone(i);
+        if ((!gets && slot.z != kStale) || !granted(slot.x, part)) continue;
         std::int32_t* entry = a.table + static_cast<std::size_t>(slot.x) * a.stride + slot.y;
-        if (slot.z == kStale) {
+        if (!gets) {
             *entry = -1;
-        } else if (enough ? fresh(i) : fresh_alone(i)) {
-            const std::int32_t id = a.found[a.need[i]];
-            *entry = id;
-            a.refs[id] = 1;
-            if (slot.z >= 0) {
-                atomicSub(&a.refs[slot.z], 1);
-                if (static_cast<std::int64_t>(slot.y) * t < part_of(a, slot.x).from) a.pair[slot.x] = int2{slot.z, id};
-            }
+            continue;
+        }
+        const std::int32_t id = a.found[a.need[i]];
+        *entry = id;
+        a.refs[id] = 1;
+        if (slot.z >= 0) {
+            atomicSub(&a.refs[slot.z], 1);
+            if (static_cast<std::int64_t>(slot.y) * t < part.from) a.pair[slot.x] = int2{slot.z, id};
         }
     }
     __syncthreads();  // the lengths may become the new ones
     for (std::uint32_t s = threadIdx.x; s < a.seqs; s += kPlan) {
-        const Part part = part_of(a, s);
+        const Part part = parts(s);
         std::int32_t lacks = 0;
-        if (!granted(s)) {
+        if (!granted(s, part)) {
             const std::int64_t from = part.from / t, to = (part.to - 1) / t + 1, width = a.width;
-            lacks = to > width ? static_cast<std::int32_t>(to - (from > width ? from : width))
-                               : a.need[s + 1 < a.seqs ? base_of(a, s + 1) : a.slots] - a.need[base_of(a, s)];
+            lacks = to > width ? static_cast<std::int32_t>(to - (from > width ? from : width)) : a.need[base(s + 1)] - a.need[base(s)];
         }
         a.missing[s] = lacks;
         a.out_lens[s] = lacks != 0 ? 0 : a.lens[s];
+    }
+}
+
+// The same for at most kPlan slots, a thread each: what the slots share lies in
+// LDS, and the first free blocks are looked for while the rows come in.
+constexpr int kShared = 2 * kPlan;  // of the table of shared blocks
+
+__global__ __launch_bounds__(kPlan) void k_kv_grow_few(Grow a)
+{
+    __shared__ std::int32_t s_base[kPlan + 1], s_need[kPlan + 1], s_found[kPlan];
+    __shared__ int2 s_part[kPlan], s_pair[kPlan];
+    __shared__ std::int32_t s_id[kShared], s_writers[kShared], s_last[kShared];
+    const int i = threadIdx.x;
+    const std::int64_t width = a.width;
+    const std::uint32_t shift = 4 + a.c.tile_shift;
+    std::int32_t len = 0;
+    Part own{0, 0};
+    if (i < static_cast<int>(a.seqs)) {
+        len = a.lens[i];
+        own = part_of(a, i);
+        s_part[i] = int2{static_cast<int>(own.from), static_cast<int>(own.to)};
+        s_base[i] = static_cast<std::int32_t>(base_of(a, i));
+        s_pair[i] = int2{-1, -1};
+    }
+    if (i == 0) s_base[a.seqs] = static_cast<std::int32_t>(a.slots);
+#pragma unroll
+    for (int k = 0; k < kShared; k += kPlan) {
+        s_id[k + i] = -1;
+        s_writers[k + i] = 0;
+        s_last[k + i] = -1;
+    }
+    std::uint32_t tile = free_of_8(a, std::uint64_t{8} * i);
+    __syncthreads();
+    std::uint32_t s = i;
+    int z = kIdle;
+    std::int32_t refs = 0;
+    std::int64_t place = 0;
+    bool begun = false;
+    if (i < static_cast<int>(a.slots)) {
+        if (a.first != nullptr) {
+            std::uint32_t lo = 0, hi = a.seqs;
+            while (hi - lo > 1) {
+                const std::uint32_t mid = lo + (hi - lo) / 2;
+                if (s_base[mid] <= i) lo = mid; else hi = mid;
+            }
+            s = lo;
+        }
+        const int2 part = s_part[s];
+        place = (part.x >> shift) + static_cast<std::int64_t>(i - s_base[s]);
+        if (i >= s_base[s] && place << shift < part.y && (part.y - 1) >> shift < width) {
+            const std::int32_t id = a.table[static_cast<std::size_t>(s) * a.stride + place];
+            const bool named = inside(id, a.c.blocks);
+            refs = named ? a.refs[id] : 0;
+            begun = place << shift < part.x;
+            z = refs > 0 ? id : !begun ? kNew : named ? kStale : kIdle;
+        }
+    }
+    const bool shared = z >= 0 && refs > 1;
+    bool keeps = !shared;
+    if (__syncthreads_or(shared)) {
+        std::uint32_t h = 0;
+        if (shared) {
+            h = static_cast<std::uint32_t>(z) * 2654435761u >> 21;
+            for (;;) {  // at most half of the places are taken
+                const std::int32_t was = atomicCAS(&s_id[h], -1, z);
+                if (was == -1 || was == z) break;
+                h = (h + 1) % kShared;
+            }
+            atomicAdd(&s_writers[h], 1);
+            atomicMax(&s_last[h], i);
+        }
+        __syncthreads();
+        if (shared) keeps = s_writers[h] >= refs && s_last[h] == i;
+    }
+    bool fresh = z == kNew || (z >= 0 && !keeps);
+    std::int32_t want;
+    std::int32_t at = before_small<1>(fresh ? 1 : 0, &want);
+    std::int32_t free = 0;
+    for (std::uint64_t from = 0; free < want && from < a.c.blocks; from += 8 * kPlan) {
+        const std::uint64_t id0 = from + std::uint64_t{8} * i;
+        const std::uint32_t next = from + 8 * kPlan < a.c.blocks ? free_of_8(a, id0 + 8 * kPlan) : 0;
+        std::int32_t all;
+        std::int32_t rank = free + before_small<4>(__popc(tile), &all);
+        for (std::uint32_t bits = tile; bits != 0 && rank < want; bits &= bits - 1) {
+            s_found[rank++] = static_cast<std::int32_t>(id0) + __ffs(bits) - 1;
+        }
+        free += all;
+        tile = next;
+    }
+    const bool enough = free >= want;
+    if (!enough) {  // no shared block is kept
+        fresh = z == kNew || shared;
+        at = before_small<1>(fresh ? 1 : 0, &want);
+    }
+    s_need[i] = at;
+    if (i == 0) s_need[kPlan] = want;
+    __syncthreads();
+    const auto needs = [&](std::uint32_t q) { return int2{s_need[s_base[q]], s_need[s_base[q + 1]]}; };
+    const auto granted = [&](std::uint32_t q, const int2& part) {
+        const int2 need = needs(q);
+        return !(part.y > 0 && (part.y - 1) >> shift >= width) && (enough || need.x == need.y || need.y <= free);
+    };
+    if ((fresh || z == kStale) && granted(s, s_part[s])) {
+        std::int32_t* entry = a.table + static_cast<std::size_t>(s) * a.stride + place;
+        if (!fresh) {
+            *entry = -1;
+        } else {
+            const std::int32_t id = s_found[at];
+            *entry = id;
+            a.refs[id] = 1;
+            if (z >= 0) {
+                atomicSub(&a.refs[z], 1);
+                if (begun) s_pair[s] = int2{z, id};
+            }
+        }
+    }
+    __syncthreads();
+    if (i < static_cast<int>(a.seqs)) {
+        std::int32_t lacks = 0;
+        if (!granted(i, s_part[i])) {
+            const std::int64_t from = own.from >> shift, to = ((own.to - 1) >> shift) + 1;
+            const int2 need = needs(i);
+            lacks = to > width ? static_cast<std::int32_t>(to - (from > width ? from : width)) : need.y - need.x;
+        }
+        a.missing[i] = lacks;
+        a.out_lens[i] = lacks != 0 ? 0 : len;
+        a.pair[i] = s_pair[i];
     }
 }
 
@@ -418,6 +614,7 @@ struct Compact {
     Table t;
     std::int32_t* where;
     std::uint32_t chunks;
+    std::uint32_t vector;  // counts and `where` may be moved 16 bytes at a time
     std::uint32_t* count;  // [chunks]: blocks in use
     std::uint32_t* moves;  // how many
     std::int32_t* source;  // [blocks / 2]: the j-th block in use past the front
@@ -505,6 +702,99 @@ __global__ __launch_bounds__(kThreads) void k_kv_compact_plan(Compact a)
         at += used[k];
     }
     if (blockIdx.x == 0 && threadIdx.x == 0) *a.moves = live - front;
+}
+
+// Both steps in one workgroup, for pools of up to kOne blocks: a wave takes a
+// run of them, 256 at a time, and keeps which are in use as bits.
+constexpr std::uint32_t kOne = kPlanWaves * 16 * 256;
+constexpr std::uint32_t kFewBlocks = 16384;
+static_assert(kFewBlocks <= kOne, "bits of a thread");
+
+__global__ __launch_bounds__(kPlan) void k_kv_compact_plan_one(Compact a)
+{
+    __shared__ std::uint32_t s_live[kPlanWaves], s_front[kPlanWaves];
+    const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
+    const std::uint32_t run = (a.c.blocks + kPlanWaves * 256 - 1) / (kPlanWaves * 256) * 256;
+    const std::uint32_t first = wave * run + lane * 4;
+    unsigned long long used = 0;
+#pragma unroll
+    for (int n = 0; n < 16; ++n) {
+        const std::uint32_t id = first + n * 256;
+        if (n * 256 < static_cast<int>(run)) {
+            std::int32_t r[4] = {0, 0, 0, 0};
+            if (a.vector != 0 && id + 4 <= a.c.blocks) {
+                *reinterpret_cast<int4*>(r) = *reinterpret_cast<const int4*>(a.t.refs + id);
+            } else {
+#pragma unroll
+                for (int k = 0; k < 4; ++k) r[k] = id + k < a.c.blocks ? a.t.refs[id + k] : 0;
+            }
+#pragma unroll
+            for (int k = 0; k < 4; ++k) used |= r[k] > 0 ? 1ull << (4 * n + k) : 0ull;
+        }
+    }
+    const auto wave_total = [&](std::uint32_t x) {
+#pragma unroll
+        for (int k = 1; k < kWave; k *= 2) x += __shfl_xor(x, k);
+        return x;
+    };
+    const std::uint32_t mine = wave_total(__popcll(used));
+    if (lane == 0) s_live[wave] = mine;
+    __syncthreads();
+    std::uint32_t at = 0, live = 0;
+#pragma unroll
+    for (int i = 0; i < kPlanWaves; ++i) {
+        at += i < wave ? s_live[i] : 0;
+        live += s_live[i];
+    }
+    std::uint32_t front = 0;  // blocks in use before the front's end
+#pragma unroll
+    for (int n = 0; n < 16; ++n) {
+        const std::uint32_t id = first + n * 256;
+        const std::uint32_t ahead = id >= live ? 0 : live - id < 4 ? live - id : 4;
+        front += __popcll(used >> (4 * n) & ((1ull << ahead) - 1));
+    }
+    front = wave_total(front);
+    if (lane == 0) s_front[wave] = front;
+    __syncthreads();
+    front = 0;
+#pragma unroll
+    for (int i = 0; i < kPlanWaves; ++i) front += s_front[i];
+    const unsigned long long below = (1ull << lane) - 1;
+    for (std::uint32_t n = 0; n * 256 < run; ++n) {
+        const std::uint32_t id0 = first + n * 256, four = static_cast<std::uint32_t>(used >> (4 * n)) & 15u;
+        std::uint32_t rank = at;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const unsigned long long votes = __ballot((four >> k & 1u) != 0);
+            rank += __popcll(votes & below);
+            at += __popcll(votes);
+        }
+        std::int32_t to[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const std::uint32_t id = id0 + k;
+            to[k] = -1;
+            if ((four >> k & 1u) != 0) {
+                to[k] = static_cast<std::int32_t>(id);
+                if (id >= live) {
+                    a.source[rank - front] = static_cast<std::int32_t>(id);
+                    to[k] = kMoves - static_cast<std::int32_t>(rank - front);
+                }
+                ++rank;
+            } else if (id < live) {
+                a.hole[id - rank] = static_cast<std::int32_t>(id);
+            }
+        }
+        if (a.vector != 0 && id0 + 4 <= a.c.blocks) {
+            *reinterpret_cast<int4*>(a.where + id0) = *reinterpret_cast<const int4*>(to);
+        } else {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                if (id0 + k < a.c.blocks) a.where[id0 + k] = to[k];
+            }
+        }
+    }
+    if (threadIdx.x == 0) *a.moves = live - front;
 }
 
 // The first workgroups move blocks, those from `movers` on the table's entries.
@@ -677,10 +967,15 @@ HBF_API int hbfsim_amd_kv_copy(const hbfsim_amd_kv_cache* from, const hbfsim_amd
     a.n = static_cast<std::uint32_t>(n);
     a.owner = static_cast<std::int32_t*>(d_workspace);
     const hipStream_t s = static_cast<hipStream_t>(stream);
-    const dim3 few((a.n + kThreads - 1) / kThreads);
-    hipLaunchKernelGGL(k_kv_copy_clear, few, dim3(kThreads), 0, s, a);
-    hipLaunchKernelGGL(k_kv_copy_claim, few, dim3(kThreads), 0, s, a);
-    hipLaunchKernelGGL(k_kv_copy, dim3(a.n * a.p.parts), dim3(kThreads), 0, s, a);
+    const dim3 every(a.n * a.p.parts);
+    if (a.n <= kFewPairs) {
+        hipLaunchKernelGGL(k_kv_copy_few, every, dim3(kThreads), 0, s, a);
+    } else {
+        const dim3 pairs((a.n + kThreads - 1) / kThreads);
+        hipLaunchKernelGGL(k_kv_copy_clear, pairs, dim3(kThreads), 0, s, a);
+        hipLaunchKernelGGL(k_kv_copy_claim, pairs, dim3(kThreads), 0, s, a);
+        hipLaunchKernelGGL(k_kv_copy, every, dim3(kThreads), 0, s, a);
+    }
     return checked(hipGetLastError());
 }
 
@@ -799,6 +1094,7 @@ HBF_API int hbfsim_amd_kv_grow(const hbfsim_amd_kv_cache* cache, int32_t* d_refs
     a.width = width;
     a.stride = stride;
     a.slots = static_cast<std::uint32_t>(slots);
+    a.vector = aligned16(d_refs) ? 1 : 0;
     a.out_lens = d_out_lens;
     a.missing = d_missing;
     unsigned char* ws = static_cast<unsigned char*>(d_workspace);
@@ -809,7 +1105,11 @@ HBF_API int hbfsim_amd_kv_grow(const hbfsim_amd_kv_cache* cache, int32_t* d_refs
     a.writers = reinterpret_cast<std::int32_t*>(ws + g.writers);
     a.last = reinterpret_cast<std::int32_t*>(ws + g.last);
     const hipStream_t s = static_cast<hipStream_t>(stream);
-    hipLaunchKernelGGL(k_kv_grow, dim3(1), dim3(kPlan), 0, s, a);
+    if (a.slots <= kPlan) {
+        hipLaunchKernelGGL(k_kv_grow_few, dim3(1), dim3(kPlan), 0, s, a);
+    } else {
+        hipLaunchKernelGGL(k_kv_grow, dim3(1), dim3(kPlan), 0, s, a);
+    }
     hipLaunchKernelGGL(k_kv_grow_copy, dim3(seqs * a.p.parts), dim3(kThreads), 0, s, a);
     return checked(hipGetLastError());
 }
@@ -850,6 +1150,7 @@ HBF_API int hbfsim_amd_kv_compact(const hbfsim_amd_kv_cache* cache, int32_t* d_r
         return HBFSIM_UNSUPPORTED;
     }
     a.where = d_where;
+    a.vector = aligned16(d_refs) && aligned16(d_where) ? 1 : 0;
     a.chunks = k.chunks;
     unsigned char* ws = static_cast<unsigned char*>(d_workspace);
     a.moves = reinterpret_cast<std::uint32_t*>(ws + k.moves);
@@ -857,8 +1158,12 @@ HBF_API int hbfsim_amd_kv_compact(const hbfsim_amd_kv_cache* cache, int32_t* d_r
     a.source = reinterpret_cast<std::int32_t*>(ws + k.source);
     a.hole = reinterpret_cast<std::int32_t*>(ws + k.hole);
     const hipStream_t s = static_cast<hipStream_t>(stream);
-    hipLaunchKernelGGL(k_kv_compact_count, dim3(k.chunks), dim3(kThreads), 0, s, a);
-    hipLaunchKernelGGL(k_kv_compact_plan, dim3(k.chunks), dim3(kThreads), 0, s, a);
+    if (a.c.blocks <= kFewBlocks) {
+        hipLaunchKernelGGL(k_kv_compact_plan_one, dim3(1), dim3(kPlan), 0, s, a);
+    } else {
+        hipLaunchKernelGGL(k_kv_compact_count, dim3(k.chunks), dim3(kThreads), 0, s, a);
+        hipLaunchKernelGGL(k_kv_compact_plan, dim3(k.chunks), dim3(kThreads), 0, s, a);
+    }
     if (groups != 0) {
         hipLaunchKernelGGL(k_kv_compact, dim3(static_cast<std::uint32_t>(groups)), dim3(kThreads), 0, s, a, movers);
     }

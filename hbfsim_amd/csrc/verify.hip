@@ -18,7 +18,6 @@ namespace {
 using namespace hbfamd::kv;
 
 constexpr int kThreads = 256;
-constexpr int kWaves = kThreads / kWave;
 constexpr double kUnit = 0x1p40;
 constexpr double kWhole = 0x1.8p52;  // whole numbers above it are its bits plus themselves
 
@@ -32,13 +31,13 @@ struct Verify {
     const float* uniform;
     const std::int32_t* first;
     const std::int32_t* lens;
-    std::uint32_t seqs, rows, vocab, chunks;
+    std::uint32_t seqs, rows, vocab, regions;
     std::uint32_t vector;  // rows of both may be loaded 16 bytes at a time
     std::int32_t* out;
     std::int32_t* gained;
     std::int32_t* out_lens;
     int4* state;  // [seqs]: accepted, whether a draft was refused, that draft
-    u64* sums;    // [seqs][chunks][2]: of what is drawn from, and of P alone
+    ulonglong2* sums;  // [seqs][regions]: of what is drawn from, and of P alone
 };
 
 // A sequence's rows, none if they do not describe the batch.
@@ -65,44 +64,95 @@ __device__ inline u64 whole(float x)
            static_cast<u64>(__double_as_longlong(kWhole));
 }
 
-// Elements e .. e + kEach - 1 of a row as whole numbers, 0 past its end.
-template <typename T, int kEach>
-__device__ inline void load_whole(const T* row, std::uint32_t e, std::uint32_t vocab, bool vector, u64 (&x)[kEach])
+// A wave's part of a row: kSteps consecutive KiB, 16 bytes a lane each, zeros
+// past the row's end.
+template <typename T, int kSteps>
+__device__ inline void load_region(const T* row, std::uint32_t region, std::uint32_t vocab, bool vector, u32x4 (&x)[kSteps])
 {
-    if (vector && e + kEach <= vocab) {
+    constexpr int kEach = 16 / sizeof(T);
+    const std::uint32_t from = region * kSteps * kWave * kEach, mine = from + threadIdx.x % kWave * kEach;
+    if (vector && from + kSteps * kWave * kEach <= vocab) {  // all of the loads at once
+#pragma unroll
+        for (int i = 0; i < kSteps; ++i) x[i] = *reinterpret_cast<const u32x4*>(row + mine + i * kWave * kEach);
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < kSteps; ++i) {
+        const std::uint32_t e = mine + i * kWave * kEach;
         union {
             u32x4 v;
             T t[kEach];
         } u;
-        u.v = *reinterpret_cast<const u32x4*>(row + e);
+        u.v = u32x4{0u, 0u, 0u, 0u};
+        if (vector && e + kEach <= vocab) {
+            u.v = *reinterpret_cast<const u32x4*>(row + e);
+        } else {
 #pragma unroll
-        for (int i = 0; i < kEach; ++i) x[i] = whole(to_float(u.t[i]));
-    } else {
-#pragma unroll
-        for (int i = 0; i < kEach; ++i) {
-            const float f = to_float(row[e + i < vocab ? e + i : 0]);
-            x[i] = e + i < vocab ? whole(f) : 0;
+            for (int k = 0; k < kEach; ++k) {
+                if (e + k < vocab) u.t[k] = row[e + k];
+            }
         }
+        x[i] = u.v;
     }
 }
 
 // What the next token is drawn from: P where no draft was refused, otherwise
 // max(P - Q, 0), or P but for the refused token.
-template <typename T, int kEach>
-__device__ inline void load_drawn(const Verify& a, std::int64_t row, const int4& state, std::uint32_t e, u64 (&full)[kEach],
-                                  u64 (&less)[kEach])
-{
-    load_whole<T, kEach>(static_cast<const T*>(a.target) + row * a.target_stride, e, a.vocab, a.vector != 0, full);
-    if (state.y != 0 && a.draft != nullptr) {
-        u64 q[kEach];
-        load_whole<T, kEach>(static_cast<const T*>(a.draft) + row * a.draft_stride, e, a.vocab, a.vector != 0, q);
+template <typename T, int kSteps>
+struct Region {
+    static constexpr int kEach = 16 / sizeof(T);
+    u32x4 p[kSteps], q[kSteps];
+    std::uint32_t mine, skip;  // index of the lane's first element; the element to leave out
+
+    __device__ inline void load(const Verify& a, std::int64_t row, const int4& state, std::uint32_t region)
+    {
+        mine = region * kSteps * kWave * kEach + threadIdx.x % kWave * kEach;
+        skip = state.y != 0 && a.draft == nullptr ? static_cast<std::uint32_t>(state.z) : ~0u;
+        load_region<T, kSteps>(static_cast<const T*>(a.target) + row * a.target_stride, region, a.vocab, a.vector != 0, p);
+        if (state.y != 0 && a.draft != nullptr) {
+            load_region<T, kSteps>(static_cast<const T*>(a.draft) + row * a.draft_stride, region, a.vocab, a.vector != 0, q);
+        } else {
 #pragma unroll
-        for (int i = 0; i < kEach; ++i) less[i] = full[i] > q[i] ? full[i] - q[i] : 0;
-    } else {
-#pragma unroll
-        for (int i = 0; i < kEach; ++i) less[i] = state.y != 0 && e + i == static_cast<std::uint32_t>(state.z) ? 0 : full[i];
+            for (int i = 0; i < kSteps; ++i) q[i] = u32x4{0u, 0u, 0u, 0u};
+        }
     }
-}
+    __device__ inline u64 full(int i, int j) const { return whole(element(p[i], j)); }
+    __device__ inline u64 less(int i, int j) const
+    {
+        const u64 x = full(i, j), y = whole(element(q[i], j));
+        return x > y && mine + i * kWave * kEach + j != skip ? x - y : 0;
+    }
+    // A step's weights are computed from here on, and none kept from before:
+    // without this the compiler holds those of all steps, more than there are
+    // registers for.
+    __device__ inline void begin(int i) { asm volatile("" : "+v"(p[i]), "+v"(q[i])); }
+    static __device__ inline void done(u64& x) { asm volatile("" : "+v"(x)); }
+    __device__ inline void add(u64* drawn, u64* all)
+    {
+#pragma unroll
+        for (int i = 0; i < kSteps; ++i) {
+            begin(i);
+#pragma unroll
+            for (int j = 0; j < kEach; ++j) {
+                *drawn += less(i, j);
+                *all += full(i, j);
+            }
+            done(*drawn);
+            done(*all);
+        }
+    }
+
+private:
+    static __device__ inline float element(const u32x4& v, int j)
+    {
+        union {
+            u32x4 v;
+            T t[kEach];
+        } u;
+        u.v = v;
+        return to_float(u.t[j]);
+    }
+};
 
 __device__ inline u64 wave_sum(u64 x)
 {
@@ -148,199 +198,281 @@ __device__ inline int4 accept(const Verify& a, const Rows& r)
     return int4{drafts, 0, 0, 0};
 }
 
-// One workgroup per (sequence, chunk of kSteps * 256 16-byte loads).
-template <typename T, int kSteps>
-__global__ __launch_bounds__(kThreads) void k_verify_sum(Verify a)
+// The number that is drawn, of `sum` whole numbers.
+__device__ inline u64 drawn_of(float uniform, u64 sum)
 {
-    constexpr int kEach = 16 / sizeof(T);
-    __shared__ int4 s_state;
-    __shared__ u64 s_sum[2][kWaves];
-    const std::uint32_t s = blockIdx.x / a.chunks, chunk = blockIdx.x % a.chunks;
-    const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
-    const Rows r = rows_of(a, s);
-    if (r.count == 0) {
-        return;
-    }
-    if (wave == 0) {
-        const int4 got = accept<T>(a, r);
-        if (lane == 0) s_state = got;
-    }
-    __syncthreads();
-    const int4 state = s_state;
-    if (chunk == 0 && threadIdx.x == 0) a.state[s] = state;
-    u64 drawn = 0, all = 0;
-#pragma unroll
-    for (int i = 0; i < kSteps; ++i) {
-        const std::uint32_t e = ((chunk * kSteps + i) * kThreads + threadIdx.x) * kEach;
-        u64 full[kEach], less[kEach];
-        if (e < a.vocab) {
-            load_drawn<T, kEach>(a, r.begin + state.x, state, e, full, less);
-#pragma unroll
-            for (int j = 0; j < kEach; ++j) {
-                drawn += less[j];
-                all += full[j];
-            }
-        }
-    }
-    drawn = wave_sum(drawn);
-    all = wave_sum(all);
-    if (lane == 0) {
-        s_sum[0][wave] = drawn;
-        s_sum[1][wave] = all;
-    }
-    __syncthreads();
-    if (threadIdx.x < 2) {
-        u64 sum = 0;
-#pragma unroll
-        for (int i = 0; i < kWaves; ++i) sum += s_sum[threadIdx.x][i];
-        a.sums[(static_cast<std::size_t>(s) * a.chunks + chunk) * 2 + threadIdx.x] = sum;
-    }
+    const float u = share(uniform) * 0x1p31f;
+    const u64 k31 = u >= 0x1p31f ? 0x7fffffffull : static_cast<u64>(u);
+    return k31 * (sum >> 31) + ((k31 * (sum & 0x7fffffffull)) >> 31);
 }
 
-// One workgroup per sequence: the chunk, then the step, the wave, the lane and
-// the element whose running sum passes the drawn number.  The last workgroup
-// clears the rows of no sequence.
+// The element of a wave's region whose running sum passes `left`: the step,
+// then the lane, then the element.  Weights are computed again rather than
+// kept: 8 steps of them would be 64 registers and more.
 template <typename T, int kSteps>
-__global__ __launch_bounds__(kThreads) void k_verify_find(Verify a)
+__device__ inline std::int32_t walk(Region<T, kSteps>& x, std::uint32_t region, u64 left, bool full_only)
 {
-    constexpr int kEach = 16 / sizeof(T);
-    __shared__ u64 s_sum[2][kWaves];
-    __shared__ u64 s_step[kSteps][kWaves];
-    __shared__ u64 s_left;
-    __shared__ std::uint32_t s_chunk;
-    __shared__ std::int32_t s_token;
-    const std::uint32_t s = blockIdx.x;
-    const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
-    if (s == a.seqs) {
-        const std::int64_t from = a.first == nullptr || a.seqs == 0 ? 0 : a.first[0];
-        const std::int64_t to = a.seqs == 0 ? 0 : a.first == nullptr ? a.seqs : a.first[a.seqs];
-        for (std::int64_t i = threadIdx.x; i < a.rows; i += kThreads) {
-            if (i < from || i >= to) a.out[i] = -1;
-        }
-        return;
-    }
-    const Rows r = rows_of(a, s);
-    if (r.count == 0) {
-        if (a.first != nullptr) {  // rows that end past the batch
-            for (std::int64_t i = a.first[s] + static_cast<std::int64_t>(threadIdx.x); i < a.first[s + 1] && i < a.rows; i += kThreads) {
-                if (i >= 0) a.out[i] = -1;
-            }
-        }
-        if (threadIdx.x == 0) {
-            a.gained[s] = 0;
-            if (a.lens != nullptr) a.out_lens[s] = a.lens[s] - (a.first[s + 1] - a.first[s]);
-        }
-        return;
-    }
-    const int4 state = a.state[s];
-    const u64* sums = a.sums + static_cast<std::size_t>(s) * a.chunks * 2;
-    const std::uint32_t each = (a.chunks + kThreads - 1) / kThreads;
-    const std::uint32_t begin = threadIdx.x * each < a.chunks ? threadIdx.x * each : a.chunks;
-    const std::uint32_t end = begin + each < a.chunks ? begin + each : a.chunks;
-    u64 mine[2] = {0, 0};
-    for (std::uint32_t i = begin; i < end; ++i) {
-        mine[0] += sums[2 * i];
-        mine[1] += sums[2 * i + 1];
-    }
-    u64 upto[2] = {wave_upto(mine[0]), wave_upto(mine[1])};
-    if (lane == kWave - 1) {
-        s_sum[0][wave] = upto[0];
-        s_sum[1][wave] = upto[1];
-    }
-    __syncthreads();
-    u64 total[2] = {0, 0};
+    constexpr int kEach = Region<T, kSteps>::kEach;
+    u64 to[kSteps];
 #pragma unroll
-    for (int w = 0; w < 2; ++w) {
+    for (int i = 0; i < kSteps; ++i) {
+        x.begin(i);
+        to[i] = 0;
 #pragma unroll
-        for (int i = 0; i < kWaves; ++i) {
-            upto[w] += i < wave ? s_sum[w][i] : 0;
-            total[w] += s_sum[w][i];
-        }
+        for (int j = 0; j < kEach; ++j) to[i] += full_only ? x.full(i, j) : x.less(i, j);
+        x.done(to[i]);
     }
-    const int which = total[0] != 0 ? 0 : 1;  // nothing left: from P
-    const u64 sum = total[which];
-    std::int32_t token = -1;
-    if (sum != 0) {
-        const float u = share(a.uniform[r.begin + r.count - 1]) * 0x1p31f;
-        const u64 k31 = u >= 0x1p31f ? 0x7fffffffull : static_cast<u64>(u);
-        const u64 k = k31 * (sum >> 31) + ((k31 * (sum & 0x7fffffffull)) >> 31);
-        u64 before = upto[which] - mine[which];
-        if (k >= before && k < upto[which]) {
-            for (std::uint32_t i = begin; i < end; ++i) {
-                const u64 c = sums[2 * i + which];
-                if (k < before + c) {
-                    s_chunk = i;
-                    s_left = k - before;
-                    break;
-                }
-                before += c;
-            }
+#pragma unroll
+    for (int i = 0; i < kSteps; ++i) to[i] = wave_upto(to[i]);
+    Region<T, 1> one;
+    int step = -1;
+    u64 upto = 0;
+#pragma unroll
+    for (int i = 0; i < kSteps; ++i) {
+        const u64 all = __shfl(to[i], kWave - 1);
+        if (step < 0 && left < all) {
+            step = i;
+            upto = to[i];
+            one.p[0] = x.p[i];
+            one.q[0] = x.q[i];
         }
-        __syncthreads();
-        const std::uint32_t chunk = s_chunk;
-        const u64 left = s_left;
-        u64 lane_sum[kSteps];
-#pragma unroll
-        for (int i = 0; i < kSteps; ++i) {
-            const std::uint32_t e = ((chunk * kSteps + i) * kThreads + threadIdx.x) * kEach;
-            lane_sum[i] = 0;
-            if (e < a.vocab) {
-                u64 full[kEach], less[kEach];
-                load_drawn<T, kEach>(a, r.begin + state.x, state, e, full, less);
-#pragma unroll
-                for (int j = 0; j < kEach; ++j) lane_sum[i] += which == 0 ? less[j] : full[j];
-            }
-            const u64 got = wave_sum(lane_sum[i]);
-            if (lane == 0) s_step[i][wave] = got;
-        }
-        __syncthreads();
-        u64 at = 0;
-        for (int i = 0; i < kSteps; ++i) {
-            for (int w = 0; w < kWaves; ++w) {
-                const u64 c = s_step[i][w];
-                if (left >= at && left < at + c && w == wave) {
-                    u64 own = 0;
-#pragma unroll
-                    for (int n = 0; n < kSteps; ++n) own = n == i ? lane_sum[n] : own;
-                    const u64 sofar = at + wave_upto(own);
-                    if (left < sofar && left >= sofar - own) {
-                        const std::uint32_t e = ((chunk * kSteps + i) * kThreads + threadIdx.x) * kEach;
-                        u64 full[kEach], less[kEach], walk = sofar - own;
-                        load_drawn<T, kEach>(a, r.begin + state.x, state, e, full, less);
-                        int found = -1;
-#pragma unroll
-                        for (int j = 0; j < kEach; ++j) {
-                            walk += which == 0 ? less[j] : full[j];
-                            if (found < 0 && left < walk) found = static_cast<int>(e) + j;
-                        }
-                        s_token = found;
-                    }
-                }
-                at += c;
-            }
-        }
-        __syncthreads();
-        token = s_token;
+        left -= step < 0 ? all : 0;
     }
-    for (int i = threadIdx.x; i < r.count; i += kThreads) {
-        a.out[r.begin + i] = i < state.x ? a.tokens[r.begin + i + 1] : i == state.x ? token : -1;
+    if (step < 0) {
+        return -1;
     }
-    if (threadIdx.x == 0) {
+    one.mine = x.mine + step * kWave * kEach;
+    one.skip = x.skip;
+    one.begin(0);
+    u64 weight[kEach], sofar = upto;
+#pragma unroll
+    for (int j = 0; j < kEach; ++j) {
+        weight[j] = full_only ? one.full(0, j) : one.less(0, j);
+        sofar -= weight[j];
+    }
+    int at = 0;  // elements whose running sum does not pass it
+#pragma unroll
+    for (int j = 0; j < kEach; ++j) {
+        sofar += weight[j];
+        at += sofar <= left ? 1 : 0;
+    }
+    const int lane = __ffsll(__ballot(upto > left)) - 1;
+    return static_cast<std::int32_t>(((region * kSteps + step) * kWave + lane) * kEach) + __shfl(at, lane);
+}
+
+// One wave writes what a sequence gains; `mine` is the drafted token after row
+// `lane` of it.
+__device__ inline void give(const Verify& a, std::uint32_t s, const Rows& r, const int4& state, std::int32_t mine, std::int32_t token)
+{
+    const int lane = threadIdx.x % kWave;
+    for (int i = lane; i < r.count; i += kWave) {
+        const std::int32_t x = i == lane ? mine : i < state.x ? a.tokens[r.begin + i + 1] : 0;
+        a.out[r.begin + i] = i < state.x ? x : i == state.x ? token : -1;
+    }
+    if (lane == 0) {
         a.gained[s] = state.x + 1;
         if (a.lens != nullptr) a.out_lens[s] = a.lens[s] - (r.count - 1 - state.x);
     }
+}
+__device__ inline std::int32_t drafted(const Verify& a, const Rows& r)
+{
+    const int lane = threadIdx.x % kWave;
+    return lane + 1 < r.count ? a.tokens[r.begin + lane + 1] : 0;
+}
+// One wave for a sequence without rows, or (s == seqs) for rows of no sequence.
+__device__ inline void give_nothing(const Verify& a, std::uint32_t s)
+{
+    const int lane = threadIdx.x % kWave;
+    if (s == a.seqs) {
+        const std::int64_t from = a.first == nullptr || a.seqs == 0 ? 0 : a.first[0];
+        const std::int64_t to = a.seqs == 0 ? 0 : a.first == nullptr ? a.seqs : a.first[a.seqs];
+        for (std::int64_t i = lane; i < from && i < a.rows; i += kWave) a.out[i] = -1;
+        for (std::int64_t i = (to > 0 ? to : 0) + lane; i < a.rows; i += kWave) a.out[i] = -1;
+        return;
+    }
+    for (std::int64_t i = a.first[s] + static_cast<std::int64_t>(lane); i < a.first[s + 1] && i < a.rows; i += kWave) {
+        if (i >= 0) a.out[i] = -1;  // rows that end past the batch
+    }
+    if (lane == 0) {
+        a.gained[s] = 0;
+        if (a.lens != nullptr) a.out_lens[s] = a.lens[s] - (a.first[s + 1] - a.first[s]);
+    }
+}
+
+// A region is kSteps consecutive KiB of a row.  One wave sums one, and finds
+// how far the drafts stay by itself first: the same few loads for all of a
+// sequence's waves, cheaper than a launch or a barrier.  Sums of whole numbers
+// need no order, so nothing is shared between waves.
+template <typename T, int kSteps>
+__global__ __launch_bounds__(kThreads) void k_verify_sum(Verify a)
+{
+    const std::uint32_t groups = (a.regions + kThreads / kWave - 1) / (kThreads / kWave);
+    const std::uint32_t s = blockIdx.x / groups;
+    const std::uint32_t region = __builtin_amdgcn_readfirstlane(blockIdx.x % groups * (kThreads / kWave) + threadIdx.x / kWave);
+    const Rows r = rows_of(a, s);
+    if (r.count == 0 || region >= a.regions) {
+        return;
+    }
+    const int4 state = accept<T>(a, r);
+    const bool first = threadIdx.x % kWave == 0;
+    if (region == 0 && first) a.state[s] = state;
+    Region<T, kSteps> x;
+    x.load(a, r.begin + state.x, state, region);
+    u64 drawn = 0, all = 0;
+    x.add(&drawn, &all);
+    drawn = wave_sum(drawn);
+    all = wave_sum(all);
+    if (first) a.sums[static_cast<std::size_t>(s) * a.regions + region] = ulonglong2{drawn, all};
+}
+
+// One wave per sequence: the region whose running sum passes the drawn number,
+// and the element in it.  The last wave clears the rows of no sequence.
+template <typename T, int kSteps>
+__global__ __launch_bounds__(kWave) void k_verify_find(Verify a)
+{
+    constexpr int kHeld = 4;  // regions of a lane that stay in registers
+    const std::uint32_t s = blockIdx.x;
+    const int lane = threadIdx.x;
+    Rows r{0, 0};
+    if (s < a.seqs) r = rows_of(a, s);
+    if (r.count == 0) {
+        give_nothing(a, s);
+        return;
+    }
+    const float uniform = a.uniform[r.begin + r.count - 1];
+    const std::int32_t mine = drafted(a, r);
+    const int4 state = a.state[s];
+    const ulonglong2* sums = a.sums + static_cast<std::size_t>(s) * a.regions;
+    const std::uint32_t each = (a.regions + kWave - 1) / kWave;
+    const std::uint32_t begin = lane * each < a.regions ? lane * each : a.regions;
+    const std::uint32_t end = begin + each < a.regions ? begin + each : a.regions;
+    ulonglong2 held[kHeld];
+    u64 drawn = 0, all = 0;
+#pragma unroll
+    for (int i = 0; i < kHeld; ++i) held[i] = begin + i < end ? sums[begin + i] : ulonglong2{0, 0};
+#pragma unroll
+    for (int i = 0; i < kHeld; ++i) {
+        drawn += held[i].x;
+        all += held[i].y;
+    }
+    for (std::uint32_t i = begin + kHeld; i < end; ++i) {
+        const ulonglong2 x = sums[i];
+        drawn += x.x;
+        all += x.y;
+    }
+    u64 upto = wave_upto(drawn), sum = __shfl(upto, kWave - 1);
+    const bool full_only = sum == 0;  // nothing left: from P
+    if (full_only) {
+        upto = wave_upto(all);
+        sum = __shfl(upto, kWave - 1);
+    }
+    std::int32_t token = -1;
+    if (sum != 0) {
+        const u64 k = drawn_of(uniform, sum);
+        const int owner = __ffsll(__ballot(upto > k)) - 1;
+        // what is left of k in the owner's regions, and the one that it is in
+        u64 left = k - (upto - (full_only ? all : drawn));
+        std::uint32_t region = begin;
+        bool found = false;
+#pragma unroll
+        for (int i = 0; i < kHeld; ++i) {
+            const u64 c = full_only ? held[i].y : held[i].x;
+            found |= left < c;
+            left -= found ? 0 : c;
+            region += found ? 0 : 1;
+        }
+        if (lane == owner && !found) {
+            for (; region < end; ++region) {
+                const ulonglong2 x = sums[region];
+                const u64 c = full_only ? x.y : x.x;
+                if (left < c) break;
+                left -= c;
+            }
+        }
+        region = __builtin_amdgcn_readfirstlane(__shfl(region, owner));
+        left = __shfl(left, owner);
+        Region<T, kSteps> x;
+        x.load(a, r.begin + state.x, state, region);
+        token = walk<T, kSteps>(x, region, left, full_only);
+    }
+    give(a, s, r, state, mine, token);
+}
+
+// All of it in one workgroup per sequence, for rows that its registers hold:
+// the row is read once and one barrier passed.  The last workgroup clears the
+// rows of no sequence.
+template <typename T, int kSteps>
+__global__ __launch_bounds__(1024) void k_verify_one(Verify a)
+{
+    __shared__ ulonglong2 s_sum[16];
+    const std::uint32_t s = blockIdx.x;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), waves = static_cast<int>(blockDim.x) / kWave;
+    Rows r{0, 0};
+    if (s < a.seqs) r = rows_of(a, s);
+    if (r.count == 0) {
+        if (wave == 0) give_nothing(a, s);
+        return;
+    }
+    const float uniform = a.uniform[r.begin + r.count - 1];
+    const std::int32_t mine = drafted(a, r);
+    const int4 state = accept<T>(a, r);
+    Region<T, kSteps> x;
+    x.load(a, r.begin + state.x, state, wave);
+    u64 drawn = 0, all = 0;
+    x.add(&drawn, &all);
+    drawn = wave_sum(drawn);
+    all = wave_sum(all);
+    if (threadIdx.x % kWave == 0) s_sum[wave] = ulonglong2{drawn, all};
+    __syncthreads();
+    u64 sum = 0, full = 0;
+    for (int i = 0; i < waves; ++i) {
+        sum += s_sum[i].x;
+        full += s_sum[i].y;
+    }
+    const bool full_only = sum == 0;
+    sum = full_only ? full : sum;
+    if (sum == 0) {
+        if (wave == 0) give(a, s, r, state, mine, -1);
+        return;
+    }
+    u64 left = drawn_of(uniform, sum);
+    for (int i = 0; i < wave; ++i) {  // another wave's, if it lies before this one's
+        const u64 c = full_only ? s_sum[i].y : s_sum[i].x;
+        if (left < c) return;
+        left -= c;
+    }
+    if (left < (full_only ? all : drawn)) give(a, s, r, state, mine, walk<T, kSteps>(x, wave, left, full_only));
 }
 
 // ---- host -----------------------------------------------------------------
 
 constexpr std::uint32_t kMostVocab = 1u << 22;
-constexpr int kSteps = 8;  // of f32, half as many of the two-byte types
 
-std::uint32_t chunks_of(std::uint32_t vocab) { return (vocab + kThreads * 4 * kSteps - 1) / (kThreads * 4 * kSteps); }
-
-std::size_t bytes_of(std::uint32_t seqs, std::uint32_t vocab)
+// How a call is cut: from its sizes alone.
+struct Cut {
+    bool one;  // a workgroup per sequence
+    int steps;
+    std::uint32_t regions;
+    std::size_t sums, bytes;
+};
+Cut cut_of(std::uint32_t seqs, std::uint32_t vocab, std::uint32_t type)
 {
-    return up256(static_cast<std::size_t>(seqs) * sizeof(int4)) + static_cast<std::size_t>(seqs) * chunks_of(vocab) * 2 * sizeof(u64);
+    const std::uint32_t each = type == HBFSIM_AMD_KV_F32 ? 256 : 512;  // elements of a step
+    Cut k{};
+    k.one = vocab <= 16 * 8 * each;
+    if (k.one) {
+        k.steps = vocab <= 16 * 2 * each ? 2 : 8;
+    } else {
+        const std::uint64_t waves = static_cast<std::uint64_t>(seqs) * ((vocab + 4 * each - 1) / (4 * each));
+        k.steps = waves < 4096 ? 1 : 4;
+    }
+    const std::uint32_t region = static_cast<std::uint32_t>(k.steps) * each;
+    k.regions = (vocab + region - 1) / region;
+    if (!k.one) {
+        k.sums = up256(static_cast<std::size_t>(seqs) * sizeof(int4));
+        k.bytes = k.sums + static_cast<std::size_t>(seqs) * k.regions * sizeof(ulonglong2);
+    }
+    return k;
 }
 
 bool sizes_ok(std::uint32_t seqs, std::uint32_t vocab, std::uint32_t type)
@@ -348,14 +480,30 @@ bool sizes_ok(std::uint32_t seqs, std::uint32_t vocab, std::uint32_t type)
     return vocab != 0 && vocab <= kMostVocab && type <= HBFSIM_AMD_KV_F32 && seqs <= 0x7fffff00u;
 }
 
-template <typename T>
-void launch(const Verify& a, hipStream_t s)
+template <typename T, int kSteps>
+void launch_two(const Verify& a, hipStream_t s)
 {
-    constexpr int kOf = sizeof(T) == 4 ? kSteps : kSteps / 2;
+    constexpr std::uint32_t kWaves = kThreads / kWave;
     if (a.seqs != 0) {
-        hipLaunchKernelGGL((k_verify_sum<T, kOf>), dim3(a.seqs * a.chunks), dim3(kThreads), 0, s, a);
+        hipLaunchKernelGGL((k_verify_sum<T, kSteps>), dim3(a.seqs * ((a.regions + kWaves - 1) / kWaves)), dim3(kThreads), 0, s, a);
     }
-    hipLaunchKernelGGL((k_verify_find<T, kOf>), dim3(a.seqs + 1), dim3(kThreads), 0, s, a);
+    hipLaunchKernelGGL((k_verify_find<T, kSteps>), dim3(a.seqs + 1), dim3(kWave), 0, s, a);
+}
+template <typename T>
+void launch(const Verify& a, const Cut& k, hipStream_t s)
+{
+    if (k.one) {
+        const dim3 waves(k.regions * kWave);
+        if (k.steps == 2) {
+            hipLaunchKernelGGL((k_verify_one<T, 2>), dim3(a.seqs + 1), waves, 0, s, a);
+        } else {
+            hipLaunchKernelGGL((k_verify_one<T, 8>), dim3(a.seqs + 1), waves, 0, s, a);
+        }
+    } else if (k.steps == 1) {
+        launch_two<T, 1>(a, s);
+    } else {
+        launch_two<T, 4>(a, s);
+    }
 }
 
 // Whether [p, p + n) and [q, q + m) have a byte in common.
@@ -374,7 +522,7 @@ HBF_API int hbfsim_amd_verify_workspace(uint32_t seqs, uint32_t vocab, uint32_t 
     if (!sizes_ok(seqs, vocab, type) || bytes == nullptr) {
         return HBFSIM_INVALID_ARGUMENT;
     }
-    *bytes = seqs == 0 ? 0 : bytes_of(seqs, vocab);
+    *bytes = seqs == 0 ? 0 : cut_of(seqs, vocab, type).bytes;
     return HBFSIM_OK;
 }
 
@@ -390,9 +538,10 @@ HBF_API int hbfsim_amd_verify(const void* d_target, const void* d_draft, uint32_
     if (seqs == 0 && tokens == 0) {
         return HBFSIM_OK;
     }
-    const std::size_t need = seqs == 0 ? 0 : bytes_of(seqs, vocab);
+    const Cut k = cut_of(seqs, vocab, type);
     if ((tokens != 0 && d_out == nullptr) ||
-        (seqs != 0 && (d_gained == nullptr || workspace_bytes < need || d_workspace == nullptr || !aligned16(d_workspace))) ||
+        (seqs != 0 && d_gained == nullptr) ||
+        (seqs != 0 && k.bytes != 0 && (workspace_bytes < k.bytes || d_workspace == nullptr || !aligned16(d_workspace))) ||
         (d_lens == nullptr) != (d_out_lens == nullptr)) {
         return HBFSIM_INVALID_ARGUMENT;
     }
@@ -407,8 +556,8 @@ HBF_API int hbfsim_amd_verify(const void* d_target, const void* d_draft, uint32_
         return HBFSIM_INVALID_ARGUMENT;
     }
     Verify a{};
-    a.chunks = chunks_of(vocab);
-    if (static_cast<std::uint64_t>(seqs) * a.chunks > 4 * kMostGroups || seqs >= 4 * kMostGroups) {
+    a.regions = k.regions;
+    if (static_cast<std::uint64_t>(seqs) * ((k.regions + 3) / 4) > (k.one ? kMostGroups : 4 * kMostGroups)) {
         return HBFSIM_UNSUPPORTED;
     }
     const std::int64_t each = type == HBFSIM_AMD_KV_F32 ? 4 : 8;
@@ -432,14 +581,14 @@ HBF_API int hbfsim_amd_verify(const void* d_target, const void* d_draft, uint32_
     a.out_lens = d_out_lens;
     unsigned char* ws = static_cast<unsigned char*>(d_workspace);
     a.state = reinterpret_cast<int4*>(ws);
-    a.sums = seqs == 0 ? nullptr : reinterpret_cast<u64*>(ws + up256(static_cast<std::size_t>(seqs) * sizeof(int4)));
+    a.sums = k.one || seqs == 0 ? nullptr : reinterpret_cast<ulonglong2*>(ws + k.sums);
     const hipStream_t s = static_cast<hipStream_t>(stream);
     if (type == HBFSIM_AMD_KV_BF16) {
-        launch<Bf16>(a, s);
+        launch<Bf16>(a, k, s);
     } else if (type == HBFSIM_AMD_KV_F16) {
-        launch<F16>(a, s);
+        launch<F16>(a, k, s);
     } else {
-        launch<float>(a, s);
+        launch<float>(a, k, s);
     }
     return checked(hipGetLastError());
 }

@@ -22,8 +22,7 @@ from typing import Any
 import torch
 
 from . import _native as nat
-from .kvcache import (_TYPES, _counts, _elsewhere, _gpu, _handle, _ints, _on_gpu, _refuse, _there,
-                      _workspace)
+from .kvcache import (_TYPES, _counts, _elsewhere, _gpu, _handle, _ints, _on_gpu, _refuse, _there)
 
 _need: dict = {}  # workspace bytes by a call's sizes
 
@@ -84,14 +83,15 @@ def verify(target: Any, tokens: Any, uniform: Any, first: Any = None, draft: Any
         if len(_need) >= 4096:
             _need.clear()
         need = _need[seqs, vocab, kind] = got.value
-    out = torch.empty((rows,), dtype=torch.int32, device=device)
-    gained, left = torch.empty((2, seqs), dtype=torch.int32, device=device).unbind()
-    ws = _workspace(need, device)
+    # outputs and scratch are parts of one allocation, scratch first (it is aligned)
+    ws, out, gained, left = torch.empty((need // 4 + rows + 2 * seqs,), dtype=torch.int32,
+                                        device=device).split_with_sizes(
+        (need // 4, rows, seqs, seqs))
     _refuse(nat.load().hbfsim_amd_verify(
         target.data_ptr(), draft.data_ptr() if draft is not None else None, kind, vocab,
         target.stride(0), draft.stride(0) if draft is not None else 0, tokens.data_ptr(),
         uniform.data_ptr(), first.data_ptr() if first is not None else None, seqs, rows,
         lens.data_ptr() if lens is not None else None, out.data_ptr(), gained.data_ptr(),
-        left.data_ptr() if lens is not None else None, ws.data_ptr() if ws is not None else None,
-        need, _handle(gpu)), "verify")
+        left.data_ptr() if lens is not None else None, ws.data_ptr() if need else None, need,
+        _handle(gpu)), "verify")
     return out, gained, left if lens is not None else None

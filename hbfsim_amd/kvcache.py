@@ -115,7 +115,7 @@ def _workspace(nbytes: int, device: Any) -> Any:
 def _ints(x: Any, name: str, device: Any, dims: int) -> Any:
     if x.dtype != torch.int32 or x.dim() != dims or x.device != device:
         raise ValueError(f"{name} must be an int32 tensor of {dims} dimension(s) on {device}")
-    if x.shape[-1] > 1 and x.stride(-1) != 1:
+    if not x.is_contiguous() and x.shape[-1] > 1 and x.stride(-1) != 1:
         raise ValueError(f"{name} must be contiguous in its last dimension")
     return x
 

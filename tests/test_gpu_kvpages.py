@@ -295,6 +295,24 @@ def test_grow_of_what_a_batch_may_not_say():
     assert missing.tolist() == [1, 0, 1]
 
 
+@pytest.mark.parametrize("seqs,start", [(1024, 0), (1025, 0), (512, 1), (513, 3), (2000, 1),
+                                        (4096, 0), (4097, 0)])
+def test_grow_on_both_sides_of_a_thread_a_slot(seqs, start):
+    """One token each, and two each with offsets; counts at any address."""
+    rng = np.random.default_rng(seqs)
+    for new in (1, 2):
+        blocks = 3 * seqs
+        table, n = batch(rng, seqs, 3, blocks, 2 * seqs)
+        cache, was = filled(blocks, 1, 64, 16, 6)
+        buffer = torch.zeros(start + blocks, dtype=torch.int32, device="cuda")
+        cache.refs = buffer[start:]
+        cache.refs.copy_(dev(pr.count(table, blocks)))
+        lens = np.minimum(np.maximum(0, n * 16 - rng.integers(0, 16, seqs)) + new, 48)
+        first = None if new == 1 else 2 * np.arange(seqs + 1)
+        _, pairs = grow_both(cache, was, table, lens, first, None if new == 1 else 2 * seqs)
+        assert pairs
+
+
 def test_grow_in_a_large_pool():
     """Free blocks far apart and behind many that are held."""
     rng = np.random.default_rng(8)
@@ -349,6 +367,33 @@ def test_compact(kv, dim, t, blocks, seqs, width):
     cache.compact(got_table)  # nothing is left to move
     np.testing.assert_array_equal(got_table.cpu(), table)
     same(cache, moved(was, pairs))
+
+
+@pytest.mark.parametrize("blocks", [65536, 65537, 150_001])
+@pytest.mark.parametrize("start", [0, 1])
+def test_compact_of_large_pools(blocks, start):
+    """On both sides of what one workgroup plans; counts at any address."""
+    rng = np.random.default_rng(blocks)
+    refs = rng.integers(-1, 3, blocks).astype(np.int32)
+    cache = kvcache.KvCache(blocks, 1, 64)
+    buffer = torch.zeros(start + blocks, dtype=torch.int32, device="cuda")
+    cache.refs = buffer[start:]
+    cache.refs.copy_(dev(refs))
+    cache.weight.copy_(torch.arange(blocks, device="cuda")[:, None])
+    cache.values.view(blocks, -1)[:] = (torch.arange(blocks, device="cuda")[:, None] % 127).to(torch.int8)
+    weight = np.arange(blocks)
+    table = rng.integers(-1, blocks + 1, (40, 700)).astype(np.int32)
+    got = dev(table)
+    where = cache.compact(got)
+    want, pairs = pr.compact(refs, table)
+    for src, dst in pairs:
+        weight[dst] = src
+    np.testing.assert_array_equal(where.cpu(), want)
+    np.testing.assert_array_equal(got.cpu(), table)
+    np.testing.assert_array_equal(cache.refs.cpu(), refs)
+    np.testing.assert_array_equal(cache.weight.cpu()[:, 0], weight)
+    values = cache.values.view(blocks, -1).cpu().numpy()
+    assert (values == (weight % 127)[:, None]).all()
 
 
 @pytest.mark.parametrize("used", ["none", "all", "front", "back", "every other"])

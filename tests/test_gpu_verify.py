@@ -54,7 +54,8 @@ def check(p, q, tokens, u, first, lens=True, padded=0):
 @pytest.mark.parametrize("sure", [False, True])
 @pytest.mark.parametrize("vocab,seqs,rows", [(1, 3, 3), (2, 9, 2), (5, 40, 6), (257, 6, 9),
                                              (2048, 2, 3), (8192, 2, 2), (8193, 2, 3),
-                                             (20011, 3, 4), (32000, 1, 5)])
+                                             (20011, 3, 4), (32000, 1, 5), (32768, 1, 2),
+                                             (32769, 2, 2), (65536, 1, 2), (65541, 2, 2)])
 def test_verify(dtype, sure, vocab, seqs, rows):
     rng = np.random.default_rng(vocab + seqs)
     counts = rng.integers(0, rows + 1, seqs)
@@ -74,7 +75,7 @@ def test_one_row_each_draws_from_the_target(vocab):
 def test_every_place_can_be_drawn():
     """A uniform target over sizes that end inside every tile: the drawn token
     is the one whose share of [0, 1) holds the number."""
-    for vocab in (4, 1000, 1024, 4095, 12288, 33001):
+    for vocab in (4, 1000, 1024, 4095, 12288, 33001, 100_003):
         at = np.unique(np.concatenate([np.arange(min(vocab, 40)), vocab - 1 - np.arange(min(vocab, 40)),
                                        np.linspace(0, vocab - 1, 60).astype(int)]))
         w = pr.whole(np.float32(1.0 / vocab))

@@ -161,7 +161,8 @@ def test_verify_refuses():
     assert verify(seqs=0, rows=0, first=None, out=None, gained=None, ws=None) == OK
     assert verify(seqs=0, gained=None, ws=None, nbytes=0) == RUNS  # rows of no sequence
     for kw in (dict(target=None), dict(tokens=None), dict(uniform=None), dict(out=None),
-               dict(gained=None), dict(ws=None), dict(ws=HERE + 4), dict(nbytes=63), dict(kind=3),
+               dict(gained=None), dict(vocab=70_000, ws=None), dict(vocab=70_000, ws=HERE + 4),
+               dict(vocab=70_000, nbytes=63), dict(kind=3),
                dict(vocab=0), dict(vocab=(1 << 22) + 1), dict(first=None), dict(lens=None),
                dict(out_lens=None), dict(rows=0x7fffff01), dict(seqs=0x7fffff01),
                dict(out=HERE + FAR + 16), dict(out=HERE + 2 * FAR - 4), dict(out=HERE + 3 * FAR + 8),
@@ -172,7 +173,10 @@ def test_verify_refuses():
     for seqs, vocab, kind in ((2, 100, 2), (70, 50_000, 0), (3, 1 << 22, 1)):
         assert nat.load().hbfsim_amd_verify_workspace(seqs, vocab, kind, ctypes.byref(need)) == OK
         assert verify(seqs=seqs, vocab=vocab, kind=kind, nbytes=need.value) == RUNS
-        assert verify(seqs=seqs, vocab=vocab, kind=kind, nbytes=need.value - 1) == BAD
+        if need.value:  # short rows need none
+            assert verify(seqs=seqs, vocab=vocab, kind=kind, nbytes=need.value - 1) == BAD
+        else:
+            assert verify(seqs=seqs, vocab=vocab, kind=kind, ws=None, nbytes=0) == RUNS
     for bad in ((3, 0, 0), (3, 5, 3), (3, (1 << 22) + 1, 0)):
         assert nat.load().hbfsim_amd_verify_workspace(*bad, ctypes.byref(need)) == BAD
 
