@@ -18,8 +18,6 @@ namespace {
 using namespace hbfamd::kv;
 
 constexpr int kThreads = 256;
-constexpr double kUnit = 0x1p40;
-constexpr double kWhole = 0x1.8p52;  // whole numbers above it are its bits plus themselves
 
 typedef unsigned long long u64;
 
@@ -37,7 +35,7 @@ struct Verify {
     std::int32_t* gained;
     std::int32_t* out_lens;
     int4* state;  // [seqs]: accepted, whether a draft was refused, that draft
-    ulonglong2* sums;  // [seqs][regions]: of what is drawn from, and of P alone
+    u64* sums;    // [seqs][regions]: of what is drawn from
 };
 
 // A sequence's rows, none if they do not describe the batch.
@@ -58,11 +56,21 @@ __device__ inline Rows rows_of(const Verify& a, std::uint32_t s)
 }
 
 __device__ inline float share(float x) { return fminf(fmaxf(x, 0.0f), 1.0f); }
-__device__ inline u64 whole(float x)
+// rint(2^40 x) = 2^20 a + b in 32-bit arithmetic: 2^20 x has 24 bits, so its
+// whole part a and its fraction are exact, and one fused step rounds 2^20 of
+// the fraction to a whole number above 2^23 (to even: 2^20 a is even).  Five
+// instructions of full rate, where 64-bit floats took one workgroup 13.4 us for
+// two rows of 32,000.
+struct Parts {
+    std::int32_t a, b;
+};
+__device__ inline Parts parts_of(float x)
 {
-    return static_cast<u64>(__double_as_longlong(__fma_rn(static_cast<double>(share(x)), kUnit, kWhole))) -
-           static_cast<u64>(__double_as_longlong(kWhole));
+    const float t = x * 0x1p20f;
+    return Parts{static_cast<std::int32_t>(t),
+                 static_cast<std::int32_t>(__float_as_uint(__builtin_fmaf(__builtin_amdgcn_fractf(t), 0x1p20f, 0x1p23f)) - 0x4b000000u)};
 }
+__device__ inline u64 joined(const Parts& x) { return static_cast<u64>((static_cast<std::int64_t>(x.a) << 20) + x.b); }
 
 // A wave's part of a row: kSteps consecutive KiB, 16 bytes a lane each, zeros
 // past the row's end.
@@ -98,48 +106,83 @@ __device__ inline void load_region(const T* row, std::uint32_t region, std::uint
 
 // What the next token is drawn from: P where no draft was refused, otherwise
 // max(P - Q, 0), or P but for the refused token.
+enum class From { kTarget, kRest, kOthers };
+__device__ inline From from_of(const Verify& a, const int4& state)
+{
+    return state.y == 0 ? From::kTarget : a.draft != nullptr ? From::kRest : From::kOthers;
+}
+
 template <typename T, int kSteps>
 struct Region {
     static constexpr int kEach = 16 / sizeof(T);
-    u32x4 p[kSteps], q[kSteps];
-    std::uint32_t mine, skip;  // index of the lane's first element; the element to leave out
+    u32x4 p[kSteps], q[kSteps];  // q only where the draft's row is taken off
+    std::uint32_t mine;          // index of the lane's first element
 
-    __device__ inline void load(const Verify& a, std::int64_t row, const int4& state, std::uint32_t region)
+    __device__ inline void load(const Verify& a, std::int64_t row, From from, std::uint32_t region)
     {
         mine = region * kSteps * kWave * kEach + threadIdx.x % kWave * kEach;
-        skip = state.y != 0 && a.draft == nullptr ? static_cast<std::uint32_t>(state.z) : ~0u;
         load_region<T, kSteps>(static_cast<const T*>(a.target) + row * a.target_stride, region, a.vocab, a.vector != 0, p);
-        if (state.y != 0 && a.draft != nullptr) {
+        if (from == From::kRest) {
             load_region<T, kSteps>(static_cast<const T*>(a.draft) + row * a.draft_stride, region, a.vocab, a.vector != 0, q);
+        }
+    }
+    // Element j of step i, without token `out`.  Where q is not below p, neither
+    // is its whole number.
+    __device__ inline Parts weight(int i, int j, From from, std::uint32_t out) const
+    {
+        const float x = element(p[i], j);
+        Parts w = parts_of(x);
+        if (from == From::kRest) {
+            const float y = element(q[i], j);
+            const Parts v = parts_of(y);
+            w.a = x > y ? w.a - v.a : 0;
+            w.b = x > y ? w.b - v.b : 0;
+        } else if (from == From::kOthers) {
+            const bool stays = mine + i * kWave * kEach + j != out;
+            w.a = stays ? w.a : 0;
+            w.b = stays ? w.b : 0;
+        }
+        return w;
+    }
+    // Sum of a step's elements.  They are computed here and none is kept from
+    // before or for later: without this the compiler holds those of all steps,
+    // more than there are registers for.
+    __device__ inline Parts sum(int i, From from, std::uint32_t out)
+    {
+        if (from == From::kRest) {
+            asm volatile("" : "+v"(p[i]), "+v"(q[i]));
         } else {
-#pragma unroll
-            for (int i = 0; i < kSteps; ++i) q[i] = u32x4{0u, 0u, 0u, 0u};
+            asm volatile("" : "+v"(p[i]));
         }
-    }
-    __device__ inline u64 full(int i, int j) const { return whole(element(p[i], j)); }
-    __device__ inline u64 less(int i, int j) const
-    {
-        const u64 x = full(i, j), y = whole(element(q[i], j));
-        return x > y && mine + i * kWave * kEach + j != skip ? x - y : 0;
-    }
-    // A step's weights are computed from here on, and none kept from before:
-    // without this the compiler holds those of all steps, more than there are
-    // registers for.
-    __device__ inline void begin(int i) { asm volatile("" : "+v"(p[i]), "+v"(q[i])); }
-    static __device__ inline void done(u64& x) { asm volatile("" : "+v"(x)); }
-    __device__ inline void add(u64* drawn, u64* all)
-    {
+        Parts s{0, 0};
 #pragma unroll
-        for (int i = 0; i < kSteps; ++i) {
-            begin(i);
+        for (int j = 0; j < kEach; ++j) {
+            const Parts w = weight(i, j, from, out);
+            s.a += w.a;
+            s.b += w.b;
+        }
+        asm volatile("" : "+v"(s.a), "+v"(s.b));
+        return s;
+    }
+    __device__ inline u64 sum(From from, std::uint32_t out)
+    {
+        Parts s{0, 0};
+        const auto add = [&](From f) {
 #pragma unroll
-            for (int j = 0; j < kEach; ++j) {
-                *drawn += less(i, j);
-                *all += full(i, j);
+            for (int i = 0; i < kSteps; ++i) {
+                const Parts x = sum(i, f, out);
+                s.a += x.a;
+                s.b += x.b;
             }
-            done(*drawn);
-            done(*all);
+        };
+        if (from == From::kRest) {
+            add(From::kRest);
+        } else if (from == From::kOthers) {
+            add(From::kOthers);
+        } else {
+            add(From::kTarget);
         }
+        return joined(s);
     }
 
 private:
@@ -150,7 +193,7 @@ private:
             T t[kEach];
         } u;
         u.v = v;
-        return to_float(u.t[j]);
+        return share(to_float(u.t[j]));
     }
 };
 
@@ -207,21 +250,14 @@ __device__ inline u64 drawn_of(float uniform, u64 sum)
 }
 
 // The element of a wave's region whose running sum passes `left`: the step,
-// then the lane, then the element.  Weights are computed again rather than
-// kept: 8 steps of them would be 64 registers and more.
+// then the lane, then the element.
 template <typename T, int kSteps>
-__device__ inline std::int32_t walk(Region<T, kSteps>& x, std::uint32_t region, u64 left, bool full_only)
+__device__ inline std::int32_t walk(Region<T, kSteps>& x, std::uint32_t region, u64 left, From from, std::uint32_t out)
 {
     constexpr int kEach = Region<T, kSteps>::kEach;
     u64 to[kSteps];
 #pragma unroll
-    for (int i = 0; i < kSteps; ++i) {
-        x.begin(i);
-        to[i] = 0;
-#pragma unroll
-        for (int j = 0; j < kEach; ++j) to[i] += full_only ? x.full(i, j) : x.less(i, j);
-        x.done(to[i]);
-    }
+    for (int i = 0; i < kSteps; ++i) to[i] = joined(x.sum(i, from, out));
 #pragma unroll
     for (int i = 0; i < kSteps; ++i) to[i] = wave_upto(to[i]);
     Region<T, 1> one;
@@ -234,7 +270,7 @@ __device__ inline std::int32_t walk(Region<T, kSteps>& x, std::uint32_t region, 
             step = i;
             upto = to[i];
             one.p[0] = x.p[i];
-            one.q[0] = x.q[i];
+            if (from == From::kRest) one.q[0] = x.q[i];
         }
         left -= step < 0 ? all : 0;
     }
@@ -242,12 +278,10 @@ __device__ inline std::int32_t walk(Region<T, kSteps>& x, std::uint32_t region, 
         return -1;
     }
     one.mine = x.mine + step * kWave * kEach;
-    one.skip = x.skip;
-    one.begin(0);
     u64 weight[kEach], sofar = upto;
 #pragma unroll
     for (int j = 0; j < kEach; ++j) {
-        weight[j] = full_only ? one.full(0, j) : one.less(0, j);
+        weight[j] = joined(one.weight(0, j, from, out));
         sofar -= weight[j];
     }
     int at = 0;  // elements whose running sum does not pass it
@@ -258,6 +292,33 @@ __device__ inline std::int32_t walk(Region<T, kSteps>& x, std::uint32_t region, 
     }
     const int lane = __ffsll(__ballot(upto > left)) - 1;
     return static_cast<std::int32_t>(((region * kSteps + step) * kWave + lane) * kEach) + __shfl(at, lane);
+}
+
+// One wave draws from P alone, a row at a time: where nothing is left of it
+// without the draft's, which only rows that are no distributions bring about.
+template <typename T>
+__device__ std::int32_t draw_full(const Verify& a, std::int64_t row, float uniform)
+{
+    constexpr std::uint32_t kStep = kWave * 16 / sizeof(T);
+    const std::uint32_t regions = (a.vocab + kStep - 1) / kStep;
+    u64 sum = 0, left = 0;
+    for (int pass = 0; pass < 2; ++pass) {
+        for (std::uint32_t i = 0; i < regions; ++i) {
+            Region<T, 1> x;
+            x.load(a, row, From::kTarget, i);
+            const u64 c = wave_sum(x.sum(From::kTarget, 0));
+            if (pass == 0) {
+                sum += c;
+            } else if (left < c) {
+                return walk<T, 1>(x, i, left, From::kTarget, 0);
+            } else {
+                left -= c;
+            }
+        }
+        if (sum == 0) break;
+        left = drawn_of(uniform, sum);
+    }
+    return -1;
 }
 
 // One wave writes what a sequence gains; `mine` is the drafted token after row
@@ -317,12 +378,9 @@ __global__ __launch_bounds__(kThreads) void k_verify_sum(Verify a)
     const bool first = threadIdx.x % kWave == 0;
     if (region == 0 && first) a.state[s] = state;
     Region<T, kSteps> x;
-    x.load(a, r.begin + state.x, state, region);
-    u64 drawn = 0, all = 0;
-    x.add(&drawn, &all);
-    drawn = wave_sum(drawn);
-    all = wave_sum(all);
-    if (first) a.sums[static_cast<std::size_t>(s) * a.regions + region] = ulonglong2{drawn, all};
+    x.load(a, r.begin + state.x, from_of(a, state), region);
+    const u64 sum = wave_sum(x.sum(from_of(a, state), state.z));
+    if (first) a.sums[static_cast<std::size_t>(s) * a.regions + region] = sum;
 }
 
 // One wave per sequence: the region whose running sum passes the drawn number,
@@ -342,58 +400,42 @@ __global__ __launch_bounds__(kWave) void k_verify_find(Verify a)
     const float uniform = a.uniform[r.begin + r.count - 1];
     const std::int32_t mine = drafted(a, r);
     const int4 state = a.state[s];
-    const ulonglong2* sums = a.sums + static_cast<std::size_t>(s) * a.regions;
+    const From from = from_of(a, state);
+    const u64* sums = a.sums + static_cast<std::size_t>(s) * a.regions;
     const std::uint32_t each = (a.regions + kWave - 1) / kWave;
     const std::uint32_t begin = lane * each < a.regions ? lane * each : a.regions;
     const std::uint32_t end = begin + each < a.regions ? begin + each : a.regions;
-    ulonglong2 held[kHeld];
-    u64 drawn = 0, all = 0;
+    u64 held[kHeld], own = 0;
 #pragma unroll
-    for (int i = 0; i < kHeld; ++i) held[i] = begin + i < end ? sums[begin + i] : ulonglong2{0, 0};
+    for (int i = 0; i < kHeld; ++i) held[i] = begin + i < end ? sums[begin + i] : 0;
 #pragma unroll
-    for (int i = 0; i < kHeld; ++i) {
-        drawn += held[i].x;
-        all += held[i].y;
-    }
-    for (std::uint32_t i = begin + kHeld; i < end; ++i) {
-        const ulonglong2 x = sums[i];
-        drawn += x.x;
-        all += x.y;
-    }
-    u64 upto = wave_upto(drawn), sum = __shfl(upto, kWave - 1);
-    const bool full_only = sum == 0;  // nothing left: from P
-    if (full_only) {
-        upto = wave_upto(all);
-        sum = __shfl(upto, kWave - 1);
-    }
+    for (int i = 0; i < kHeld; ++i) own += held[i];
+    for (std::uint32_t i = begin + kHeld; i < end; ++i) own += sums[i];
+    const u64 upto = wave_upto(own), sum = __shfl(upto, kWave - 1);
     std::int32_t token = -1;
     if (sum != 0) {
         const u64 k = drawn_of(uniform, sum);
         const int owner = __ffsll(__ballot(upto > k)) - 1;
         // what is left of k in the owner's regions, and the one that it is in
-        u64 left = k - (upto - (full_only ? all : drawn));
+        u64 left = k - (upto - own);
         std::uint32_t region = begin;
         bool found = false;
 #pragma unroll
         for (int i = 0; i < kHeld; ++i) {
-            const u64 c = full_only ? held[i].y : held[i].x;
-            found |= left < c;
-            left -= found ? 0 : c;
+            found |= left < held[i];
+            left -= found ? 0 : held[i];
             region += found ? 0 : 1;
         }
         if (lane == owner && !found) {
-            for (; region < end; ++region) {
-                const ulonglong2 x = sums[region];
-                const u64 c = full_only ? x.y : x.x;
-                if (left < c) break;
-                left -= c;
-            }
+            for (; region < end && left >= sums[region]; ++region) left -= sums[region];
         }
         region = __builtin_amdgcn_readfirstlane(__shfl(region, owner));
         left = __shfl(left, owner);
         Region<T, kSteps> x;
-        x.load(a, r.begin + state.x, state, region);
-        token = walk<T, kSteps>(x, region, left, full_only);
+        x.load(a, r.begin + state.x, from, region);
+        token = walk<T, kSteps>(x, region, left, from, state.z);
+    } else {
+        token = draw_full<T>(a, r.begin + state.x, uniform);
     }
     give(a, s, r, state, mine, token);
 }
@@ -404,7 +446,7 @@ __global__ __launch_bounds__(kWave) void k_verify_find(Verify a)
 template <typename T, int kSteps>
 __global__ __launch_bounds__(1024) void k_verify_one(Verify a)
 {
-    __shared__ ulonglong2 s_sum[16];
+    __shared__ u64 s_sum[16];
     const std::uint32_t s = blockIdx.x;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), waves = static_cast<int>(blockDim.x) / kWave;
     Rows r{0, 0};
@@ -416,32 +458,24 @@ __global__ __launch_bounds__(1024) void k_verify_one(Verify a)
     const float uniform = a.uniform[r.begin + r.count - 1];
     const std::int32_t mine = drafted(a, r);
     const int4 state = accept<T>(a, r);
+    const From from = from_of(a, state);
     Region<T, kSteps> x;
-    x.load(a, r.begin + state.x, state, wave);
-    u64 drawn = 0, all = 0;
-    x.add(&drawn, &all);
-    drawn = wave_sum(drawn);
-    all = wave_sum(all);
-    if (threadIdx.x % kWave == 0) s_sum[wave] = ulonglong2{drawn, all};
+    x.load(a, r.begin + state.x, from, wave);
+    const u64 own = wave_sum(x.sum(from, state.z));
+    if (threadIdx.x % kWave == 0) s_sum[wave] = own;
     __syncthreads();
-    u64 sum = 0, full = 0;
-    for (int i = 0; i < waves; ++i) {
-        sum += s_sum[i].x;
-        full += s_sum[i].y;
-    }
-    const bool full_only = sum == 0;
-    sum = full_only ? full : sum;
+    u64 sum = 0;
+    for (int i = 0; i < waves; ++i) sum += s_sum[i];
     if (sum == 0) {
-        if (wave == 0) give(a, s, r, state, mine, -1);
+        if (wave == 0) give(a, s, r, state, mine, draw_full<T>(a, r.begin + state.x, uniform));
         return;
     }
     u64 left = drawn_of(uniform, sum);
     for (int i = 0; i < wave; ++i) {  // another wave's, if it lies before this one's
-        const u64 c = full_only ? s_sum[i].y : s_sum[i].x;
-        if (left < c) return;
-        left -= c;
+        if (left < s_sum[i]) return;
+        left -= s_sum[i];
     }
-    if (left < (full_only ? all : drawn)) give(a, s, r, state, mine, walk<T, kSteps>(x, wave, left, full_only));
+    if (left < own) give(a, s, r, state, mine, walk<T, kSteps>(x, wave, left, from, state.z));
 }
 
 // ---- host -----------------------------------------------------------------
@@ -459,9 +493,9 @@ Cut cut_of(std::uint32_t seqs, std::uint32_t vocab, std::uint32_t type)
 {
     const std::uint32_t each = type == HBFSIM_AMD_KV_F32 ? 256 : 512;  // elements of a step
     Cut k{};
-    k.one = vocab <= 16 * 8 * each;
+    k.one = vocab <= 16 * 2 * each;
     if (k.one) {
-        k.steps = vocab <= 16 * 2 * each ? 2 : 8;
+        k.steps = 2;
     } else {
         const std::uint64_t waves = static_cast<std::uint64_t>(seqs) * ((vocab + 4 * each - 1) / (4 * each));
         k.steps = waves < 4096 ? 1 : 4;
@@ -470,7 +504,7 @@ Cut cut_of(std::uint32_t seqs, std::uint32_t vocab, std::uint32_t type)
     k.regions = (vocab + region - 1) / region;
     if (!k.one) {
         k.sums = up256(static_cast<std::size_t>(seqs) * sizeof(int4));
-        k.bytes = k.sums + static_cast<std::size_t>(seqs) * k.regions * sizeof(ulonglong2);
+        k.bytes = k.sums + static_cast<std::size_t>(seqs) * k.regions * sizeof(u64);
     }
     return k;
 }
@@ -493,12 +527,7 @@ template <typename T>
 void launch(const Verify& a, const Cut& k, hipStream_t s)
 {
     if (k.one) {
-        const dim3 waves(k.regions * kWave);
-        if (k.steps == 2) {
-            hipLaunchKernelGGL((k_verify_one<T, 2>), dim3(a.seqs + 1), waves, 0, s, a);
-        } else {
-            hipLaunchKernelGGL((k_verify_one<T, 8>), dim3(a.seqs + 1), waves, 0, s, a);
-        }
+        hipLaunchKernelGGL((k_verify_one<T, 2>), dim3(a.seqs + 1), dim3(k.regions * kWave), 0, s, a);
     } else if (k.steps == 1) {
         launch_two<T, 1>(a, s);
     } else {
@@ -581,7 +610,7 @@ HBF_API int hbfsim_amd_verify(const void* d_target, const void* d_draft, uint32_
     a.out_lens = d_out_lens;
     unsigned char* ws = static_cast<unsigned char*>(d_workspace);
     a.state = reinterpret_cast<int4*>(ws);
-    a.sums = k.one || seqs == 0 ? nullptr : reinterpret_cast<ulonglong2*>(ws + k.sums);
+    a.sums = k.one || seqs == 0 ? nullptr : reinterpret_cast<u64*>(ws + k.sums);
     const hipStream_t s = static_cast<hipStream_t>(stream);
     if (type == HBFSIM_AMD_KV_BF16) {
         launch<Bf16>(a, k, s);

@@ -45,6 +45,7 @@ from . import _native as nat
 
 BLOCK_TOKENS = (16, 32, 64, 128)
 WEIGHT_UNIT = 2.0 ** -32
+_I32 = torch.int32
 _TYPES = {torch.bfloat16: nat.KV_BF16, torch.float16: nat.KV_F16, torch.float32: nat.KV_F32}
 
 
@@ -113,7 +114,7 @@ def _workspace(nbytes: int, device: Any) -> Any:
 
 
 def _ints(x: Any, name: str, device: Any, dims: int) -> Any:
-    if x.dtype != torch.int32 or x.dim() != dims or x.device != device:
+    if x.dtype is not _I32 or x.dim() != dims or x.device != device:
         raise ValueError(f"{name} must be an int32 tensor of {dims} dimension(s) on {device}")
     if not x.is_contiguous() and x.shape[-1] > 1 and x.stride(-1) != 1:
         raise ValueError(f"{name} must be contiguous in its last dimension")
@@ -187,29 +188,24 @@ def evict(weight: Any, table: Any, lens: Any, keep: int, block_tokens: int = 16,
 
 
 def _references(refs: Any, blocks: int | None = None) -> Any:
-    if refs.dtype != torch.int32 or refs.dim() != 1 or not refs.is_contiguous() \
-            or not refs.shape[0] or blocks not in (None, refs.shape[0]):
+    if refs.dtype is not _I32 or refs.dim() != 1 or not refs.is_contiguous() \
+            or refs.shape[0] == 0 or (blocks is not None and refs.shape[0] != blocks):
         raise ValueError("refs must be a contiguous int32 tensor [blocks]")
     return refs
 
 
-def _written(x: Any, name: str) -> Any:
-    """A table that a call changes: its rows must not share memory."""
-    if x.shape[0] > 1 and x.stride(0) < x.shape[1]:
-        raise ValueError(f"{name} rows overlap")
-    return x
-
-
-def _rows_of(table: Any, refs: Any, lens: Any = None) -> tuple[int, int, int]:
-    """(sequences, width, stride) of a table beside its references."""
+def _rows_of(table: Any, refs: Any, lens: Any = None) -> tuple[int, int, int, int]:
+    """(blocks, sequences, width, stride) of a table beside its references."""
     device = refs.device
-    _written(_ints(table, "table", device, 2), "table")
-    seqs, width = table.shape
+    seqs, width = _ints(table, "table", device, 2).shape
     if lens is not None and _ints(lens, "lens", device, 1).shape[0] != seqs:
         raise ValueError(f"{lens.shape[0]} lengths for {seqs} sequences")
     stride = table.stride(0) if seqs > 1 else width
-    _counts(refs.shape[0] | seqs | width | stride)
-    return seqs, width, stride
+    if stride < width:
+        raise ValueError("table rows overlap")
+    blocks = refs.shape[0]
+    _counts(blocks | seqs | width | stride)
+    return blocks, seqs, width, stride
 
 
 def hold(refs: Any, table: Any, stream: Any = None) -> None:
@@ -220,10 +216,10 @@ def hold(refs: Any, table: Any, stream: Any = None) -> None:
     if _elsewhere(gpu, stream):
         return _there(refs.device, stream, lambda: hold(refs, table))
     _references(refs)
-    seqs, width, stride = _rows_of(table, refs)
+    blocks, seqs, width, stride = _rows_of(table, refs)
     _on_gpu(gpu)
-    _refuse(nat.load().hbfsim_amd_kv_hold(refs.data_ptr(), refs.shape[0], table.data_ptr(), seqs,
-                                          width, stride, _handle(gpu)), "hold")
+    _refuse(nat.load().hbfsim_amd_kv_hold(refs.data_ptr(), blocks, table.data_ptr(), seqs, width,
+                                          stride, _handle(gpu)), "hold")
 
 
 def fork(refs: Any, table: Any, lens: Any, parents: Any, stream: Any = None) -> tuple:
@@ -235,14 +231,14 @@ def fork(refs: Any, table: Any, lens: Any, parents: Any, stream: Any = None) -> 
     if _elsewhere(gpu, stream):
         return _there(refs.device, stream, lambda: fork(refs, table, lens, parents))
     _references(refs)
-    seqs, width, stride = _rows_of(table, refs, lens)
+    blocks, seqs, width, stride = _rows_of(table, refs, lens)
     rows = _ints(parents, "parents", refs.device, 1).shape[0]
     _counts(rows)
     _on_gpu(gpu)
     out = torch.empty((rows, width), dtype=torch.int32, device=refs.device)
     out_lens = torch.empty((rows,), dtype=torch.int32, device=refs.device)
     _refuse(nat.load().hbfsim_amd_kv_fork(
-        refs.data_ptr(), refs.shape[0], table.data_ptr(), lens.data_ptr(), seqs, width, stride,
+        refs.data_ptr(), blocks, table.data_ptr(), lens.data_ptr(), seqs, width, stride,
         parents.data_ptr(), rows, out.data_ptr(), out_lens.data_ptr(), _handle(gpu)), "fork")
     return out, out_lens
 
@@ -256,11 +252,11 @@ def release(refs: Any, table: Any, lens: Any = None, block_tokens: int = 16,
     if _elsewhere(gpu, stream):
         return _there(refs.device, stream, lambda: release(refs, table, lens, block_tokens))
     _references(refs)
-    seqs, width, stride = _rows_of(table, refs, lens)
+    blocks, seqs, width, stride = _rows_of(table, refs, lens)
     _counts(block_tokens)
     _on_gpu(gpu)
     _refuse(nat.load().hbfsim_amd_kv_release(
-        refs.data_ptr(), refs.shape[0], block_tokens, table.data_ptr(),
+        refs.data_ptr(), blocks, block_tokens, table.data_ptr(),
         lens.data_ptr() if lens is not None else None, seqs, width, stride, _handle(gpu)), "release")
 
 
@@ -527,7 +523,7 @@ class KvCache:
         if _elsewhere(self._gpu, stream):
             return _there(self.device, stream, lambda: self.grow(table, lens, first, tokens))
         refs = _references(self.refs, self.blocks)
-        seqs, width, stride = _rows_of(table, refs, lens)
+        _, seqs, width, stride = _rows_of(table, refs, lens)
         if first is None:
             if tokens not in (None, seqs):
                 raise ValueError(f"{tokens} tokens for {seqs} sequences of one token each")
@@ -546,12 +542,17 @@ class KvCache:
             _refuse(self._lib.hbfsim_amd_kv_grow_workspace(self._ref, seqs, tokens,
                                                            ctypes.byref(got)), "grow")
             need = self._remember(sizes, got.value)
-        out, missing = torch.empty((2, seqs), dtype=torch.int32, device=self.device).unbind()
-        ws = _workspace(need, self.device)
+        if need <= 65536:  # outputs and scratch in one allocation, scratch first (it is aligned)
+            ws, out, missing = torch.empty((need // 4 + 2 * seqs,), dtype=_I32,
+                                           device=self.device).split_with_sizes(
+                (need // 4, seqs, seqs))
+        else:
+            out, missing = torch.empty((2, seqs), dtype=_I32, device=self.device).unbind()
+            ws = _workspace(need, self.device)
         _refuse(self._lib.hbfsim_amd_kv_grow(
             self._ref, refs.data_ptr(), table.data_ptr(), lens.data_ptr(),
             first.data_ptr() if first is not None else None, seqs, tokens, width, stride,
-            out.data_ptr(), missing.data_ptr(), ws.data_ptr() if ws is not None else None, need,
+            out.data_ptr(), missing.data_ptr(), ws.data_ptr() if need else None, need,
             _handle(self._gpu)), "grow")
         return out, missing
 
@@ -562,7 +563,7 @@ class KvCache:
         if _elsewhere(self._gpu, stream):
             return _there(self.device, stream, lambda: self.compact(table))
         refs = _references(self.refs, self.blocks)
-        seqs, width, stride = _rows_of(table, refs)
+        _, seqs, width, stride = _rows_of(table, refs)
         _on_gpu(self._gpu)
         need = self._need.get("compact")
         if need is None:
