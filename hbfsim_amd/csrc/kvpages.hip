@@ -106,6 +106,8 @@ __global__ __launch_bounds__(kThreads) void k_kv_copy(Copy a)
     copy_part(a.from, a.to, a.p, src, dst, part);
 }
 // Every workgroup looks through the pairs itself: one launch instead of three.
+// 4 pairs take 3.1 us against 6.2, 256 of 35 KB 5.3 against 8.8, 1,024 18.0
+// against 20.7; 4,096 take 75 against 64.
 __global__ __launch_bounds__(kThreads) void k_kv_copy_few(Copy a)
 {
     const std::uint32_t i = blockIdx.x / a.p.parts, part = blockIdx.x % a.p.parts;
@@ -229,6 +231,7 @@ struct Grow {
     std::int32_t* writers;  // [blocks]: slots that write to a shared block, and the last of them
     std::int32_t* last;
     int2* pair;             // [seqs]: content to copy, source and destination
+    std::int32_t* count;    // [tiles] of the pool: free blocks; or null
 };
 constexpr std::int32_t kNew = -1;    // no block of its own: a new one
 constexpr std::int32_t kIdle = -2;   // nothing to do
@@ -347,6 +350,67 @@ __device__ inline std::int32_t before_small(std::uint32_t x, std::int32_t* all)
     return mine;
 }
 
+// Free blocks of every tile, a workgroup each: for pools that one compute unit
+// would look through for longer than a launch takes.
+constexpr std::uint32_t kTile = 8 * kPlan;  // blocks
+__global__ __launch_bounds__(kPlan) void k_kv_grow_count(Grow a)
+{
+    std::int32_t all;
+    before_small<4>(__popc(free_of_8(a, std::uint64_t{blockIdx.x} * kTile + std::uint64_t{8} * threadIdx.x)), &all);
+    if (threadIdx.x == 0) a.count[blockIdx.x] = all;
+}
+
+// The first `want` free blocks, in order, to put(rank, id); returns how many
+// there are, all of them where they are fewer.  `tile` holds a thread's of the
+// first tile, and each tile is on its way while the one before is counted; with
+// counts, tiles without a free block are left out.
+// A compute unit reads 33 GB/s so, a tile in 1.03 us: a step of 64 sequences
+// takes 5 us where the first tile has their blocks, and without counts 14 where
+// the first half of 131,072 blocks is in use, 21 where nearly all are; with
+// them 9 wherever the free ones lie, also of 500,000 (71 without).
+template <typename F>
+__device__ inline std::int32_t first_free(const Grow& a, std::uint32_t tile, std::int32_t want, F put)
+{
+    __shared__ int2 s_tile[kPlan];  // index, free blocks before it
+    const auto take = [&](std::uint32_t bits, std::int32_t rank, std::uint64_t id0) {
+        for (; bits != 0 && rank < want; bits &= bits - 1) put(rank++, static_cast<std::int32_t>(id0) + __ffs(bits) - 1);
+    };
+    const std::uint64_t mine = std::uint64_t{8} * threadIdx.x;
+    std::int32_t free = 0, all;
+    if (a.count == nullptr) {
+        for (std::uint64_t from = 0; free < want && from < a.c.blocks; from += kTile) {
+            const std::uint32_t next = from + kTile < a.c.blocks ? free_of_8(a, from + kTile + mine) : 0;
+            const std::int32_t rank = free + before_small<4>(__popc(tile), &all);
+            take(tile, rank, from + mine);
+            free += all;
+            tile = next;
+        }
+        return free;
+    }
+    const std::uint32_t tiles = (a.c.blocks + kTile - 1) / kTile;
+    for (std::uint32_t group = 0; free < want && group < tiles; group += kPlan) {
+        const std::int32_t count = group + threadIdx.x < tiles ? a.count[group + threadIdx.x] : 0;
+        std::int32_t used;
+        const std::int32_t rank = free + before(count, &all);
+        const bool use = count > 0 && rank < want;
+        const std::int32_t at = before_small<1>(use ? 1 : 0, &used);
+        if (use) s_tile[at] = int2{static_cast<int>(group + threadIdx.x), rank};
+        __syncthreads();
+        const auto from = [&](int i) { return static_cast<std::uint64_t>(s_tile[i].x) * kTile + mine; };
+        std::uint32_t bits = used > 0 ? free_of_8(a, from(0)) : 0;
+        for (int i = 0; i < used; ++i) {
+            const std::uint32_t next = i + 1 < used ? free_of_8(a, from(i + 1)) : 0;
+            std::int32_t here;
+            const std::int32_t first = before_small<4>(__popc(bits), &here);
+            take(bits, s_tile[i].y + first, from(i));
+            bits = next;
+        }
+        __syncthreads();
+        free += all;
+    }
+    return free;
+}
+
 // One workgroup plans: what each slot writes to, who keeps a shared block, how
 // many blocks are wanted, the first free ones, who gets them.
 __global__ __launch_bounds__(kPlan) void k_kv_grow(Grow a)
@@ -424,18 +488,7 @@ __global__ __launch_bounds__(kPlan) void k_kv_grow(Grow a)
         return slot.z == kNew || (slot.z >= 0 && slot.w > 1);
     };
     std::int32_t want = count_needs(a, fresh);
-    std::int32_t free = 0;
-    for (std::uint64_t from = 0; free < want && from < a.c.blocks; from += 8 * kPlan) {
-        const std::uint64_t id0 = from + std::uint64_t{8} * threadIdx.x;
-        const std::uint32_t next = from + 8 * kPlan < a.c.blocks ? free_of_8(a, id0 + 8 * kPlan) : 0;
-        std::int32_t all;
-        std::int32_t rank = free + before_small<4>(__popc(tile), &all);
-        for (std::uint32_t bits = tile; bits != 0 && rank < want; bits &= bits - 1) {
-            a.found[rank++] = static_cast<std::int32_t>(id0) + __ffs(bits) - 1;
-        }
-        free += all;
-        tile = next;
-    }
+    const std::int32_t free = first_free(a, tile, want, [&](std::int32_t rank, std::int32_t id) { a.found[rank] = id; });
     const bool enough = free >= want;
     if (!enough) want = count_needs(a, fresh_alone);
     __syncthreads();
@@ -550,18 +603,7 @@ __global__ __launch_bounds__(kPlan) void k_kv_grow_few(Grow a)
     bool fresh = z == kNew || (z >= 0 && !keeps);
     std::int32_t want;
     std::int32_t at = before_small<1>(fresh ? 1 : 0, &want);
-    std::int32_t free = 0;
-    for (std::uint64_t from = 0; free < want && from < a.c.blocks; from += 8 * kPlan) {
-        const std::uint64_t id0 = from + std::uint64_t{8} * i;
-        const std::uint32_t next = from + 8 * kPlan < a.c.blocks ? free_of_8(a, id0 + 8 * kPlan) : 0;
-        std::int32_t all;
-        std::int32_t rank = free + before_small<4>(__popc(tile), &all);
-        for (std::uint32_t bits = tile; bits != 0 && rank < want; bits &= bits - 1) {
-            s_found[rank++] = static_cast<std::int32_t>(id0) + __ffs(bits) - 1;
-        }
-        free += all;
-        tile = next;
-    }
+    const std::int32_t free = first_free(a, tile, want, [&](std::int32_t rank, std::int32_t id) { s_found[rank] = id; });
     const bool enough = free >= want;
     if (!enough) {  // no shared block is kept
         fresh = z == kNew || shared;
@@ -709,11 +751,12 @@ __global__ __launch_bounds__(kThreads) void k_kv_compact_plan(Compact a)
     if (blockIdx.x == 0 && threadIdx.x == 0) *a.moves = live - front;
 }
 
-// Both steps in one workgroup, for pools of up to kOne blocks: a wave takes a
-// run of them, 256 at a time, and keeps which are in use as bits.
-constexpr std::uint32_t kOne = kPlanWaves * 16 * 256;
-constexpr std::uint32_t kFewBlocks = 16384;
-static_assert(kFewBlocks <= kOne, "bits of a thread");
+// Both steps in one workgroup, for pools of up to kFewBlocks: a wave takes a run
+// of them, 256 at a time, and keeps which are in use as bits.
+// (4,000 blocks: 10.1 us against 13.1 in two launches; 8,000: 12.1 and 13.4;
+// 16,000: 14.8 and 14.2, and 65,000: 32.8 and 19.5.)
+constexpr int kRounds = 2;
+constexpr std::uint32_t kFewBlocks = kPlanWaves * kRounds * 256;
 
 __global__ __launch_bounds__(kPlan) void k_kv_compact_plan_one(Compact a)
 {
@@ -721,9 +764,9 @@ __global__ __launch_bounds__(kPlan) void k_kv_compact_plan_one(Compact a)
     const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
     const std::uint32_t run = (a.c.blocks + kPlanWaves * 256 - 1) / (kPlanWaves * 256) * 256;
     const std::uint32_t first = wave * run + lane * 4;
-    unsigned long long used = 0;
+    std::uint32_t used = 0;
 #pragma unroll
-    for (int n = 0; n < 16; ++n) {
+    for (int n = 0; n < kRounds; ++n) {
         const std::uint32_t id = first + n * 256;
         if (n * 256 < static_cast<int>(run)) {
             std::int32_t r[4] = {0, 0, 0, 0};
@@ -734,7 +777,7 @@ __global__ __launch_bounds__(kPlan) void k_kv_compact_plan_one(Compact a)
                 for (int k = 0; k < 4; ++k) r[k] = id + k < a.c.blocks ? a.t.refs[id + k] : 0;
             }
 #pragma unroll
-            for (int k = 0; k < 4; ++k) used |= r[k] > 0 ? 1ull << (4 * n + k) : 0ull;
+            for (int k = 0; k < 4; ++k) used |= r[k] > 0 ? 1u << (4 * n + k) : 0u;
         }
     }
     const auto wave_total = [&](std::uint32_t x) {
@@ -742,7 +785,7 @@ __global__ __launch_bounds__(kPlan) void k_kv_compact_plan_one(Compact a)
         for (int k = 1; k < kWave; k *= 2) x += __shfl_xor(x, k);
         return x;
     };
-    const std::uint32_t mine = wave_total(__popcll(used));
+    const std::uint32_t mine = wave_total(__popc(used));
     if (lane == 0) s_live[wave] = mine;
     __syncthreads();
     std::uint32_t at = 0, live = 0;
@@ -753,10 +796,10 @@ __global__ __launch_bounds__(kPlan) void k_kv_compact_plan_one(Compact a)
     }
     std::uint32_t front = 0;  // blocks in use before the front's end
 #pragma unroll
-    for (int n = 0; n < 16; ++n) {
+    for (int n = 0; n < kRounds; ++n) {
         const std::uint32_t id = first + n * 256;
         const std::uint32_t ahead = id >= live ? 0 : live - id < 4 ? live - id : 4;
-        front += __popcll(used >> (4 * n) & ((1ull << ahead) - 1));
+        front += __popc(used >> (4 * n) & ((1u << ahead) - 1));
     }
     front = wave_total(front);
     if (lane == 0) s_front[wave] = front;
@@ -765,8 +808,10 @@ __global__ __launch_bounds__(kPlan) void k_kv_compact_plan_one(Compact a)
 #pragma unroll
     for (int i = 0; i < kPlanWaves; ++i) front += s_front[i];
     const unsigned long long below = (1ull << lane) - 1;
-    for (std::uint32_t n = 0; n * 256 < run; ++n) {
-        const std::uint32_t id0 = first + n * 256, four = static_cast<std::uint32_t>(used >> (4 * n)) & 15u;
+#pragma unroll
+    for (std::uint32_t n = 0; n < kRounds; ++n) {
+        if (n * 256 >= run) break;
+        const std::uint32_t id0 = first + n * 256, four = used >> (4 * n) & 15u;
         std::uint32_t rank = at;
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
@@ -883,12 +928,16 @@ int take_table(std::int32_t* refs, std::uint32_t blocks, std::uint32_t tokens, s
 bool tokens_ok(std::uint32_t n) { return n == 16 || n == 32 || n == 64 || n == 128; }
 
 struct GrowSpace {
-    std::size_t need, slot, found, writers, last, pair, bytes;
+    std::size_t need, slot, found, writers, last, pair, count, bytes;
 };
 std::uint64_t slots_of(const Cache& c, std::uint32_t seqs, std::uint32_t tokens, bool offsets)
 {
     return offsets ? tokens / c.tokens + std::uint64_t{2} * seqs : seqs;
 }
+// Blocks up to which the planning workgroup looks for free ones without counts:
+// 60,000 cost it 1 to 7 us more than the first tile, by where the free ones lie,
+// and counts 4.
+constexpr std::uint32_t kScanned = 65536;
 // Where a thread takes a slot, the plan lies in LDS and only the pairs in memory.
 GrowSpace grow_space(const Cache& c, std::uint32_t seqs, std::uint64_t slots)
 {
@@ -900,6 +949,7 @@ GrowSpace grow_space(const Cache& c, std::uint32_t seqs, std::uint64_t slots)
         return here;
     };
     g.pair = take(seqs * sizeof(int2));
+    if (c.blocks > kScanned) g.count = take((static_cast<std::size_t>(c.blocks) + kTile - 1) / kTile * 4);
     if (slots > kPlan) {
         g.slot = take(slots * sizeof(int4));
         g.need = take((slots + 1) * 4);
@@ -1113,6 +1163,10 @@ HBF_API int hbfsim_amd_kv_grow(const hbfsim_amd_kv_cache* cache, int32_t* d_refs
     a.writers = reinterpret_cast<std::int32_t*>(ws + g.writers);
     a.last = reinterpret_cast<std::int32_t*>(ws + g.last);
     const hipStream_t s = static_cast<hipStream_t>(stream);
+    if (a.c.blocks > kScanned) {
+        a.count = reinterpret_cast<std::int32_t*>(ws + g.count);
+        hipLaunchKernelGGL(k_kv_grow_count, dim3((a.c.blocks + kTile - 1) / kTile), dim3(kPlan), 0, s, a);
+    }
     if (a.slots <= kPlan) {
         hipLaunchKernelGGL(k_kv_grow_few, dim3(1), dim3(kPlan), 0, s, a);
     } else {

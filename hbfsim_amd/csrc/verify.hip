@@ -482,7 +482,16 @@ __global__ __launch_bounds__(1024) void k_verify_one(Verify a)
 
 constexpr std::uint32_t kMostVocab = 1u << 22;
 
-// How a call is cut: from its sizes alone.
+// How a call is cut: from its sizes alone (floats, by graph replays; two-byte
+// types take within 2 us of the same).
+// A workgroup per sequence where 16 waves of two loads each hold the row: 1 and
+// 256 sequences over 4,000 tokens take 5.8 and 6.2 us against 6.4 and 7.6 in two
+// launches, over 8,000 6.7 and 7.9 against 6.1 and 8.9, and one launch less costs
+// the host 3 us less.  Eight loads a wave would hold 32,000, but one compute unit
+// then reads for 12 us what two launches are done with in 6.
+// Two launches otherwise, of regions of one load where few waves would be left:
+// 64 sequences over 32,000 take 8.9 us with one load and 10.0 with four (2,000
+// waves), over 60,000 12.2 and 11.4 (3,800), over 151,936 22.4 and 18.9.
 struct Cut {
     bool one;  // a workgroup per sequence
     int steps;
@@ -498,7 +507,7 @@ Cut cut_of(std::uint32_t seqs, std::uint32_t vocab, std::uint32_t type)
         k.steps = 2;
     } else {
         const std::uint64_t waves = static_cast<std::uint64_t>(seqs) * ((vocab + 4 * each - 1) / (4 * each));
-        k.steps = waves < 4096 ? 1 : 4;
+        k.steps = waves < 3000 ? 1 : 4;
     }
     const std::uint32_t region = static_cast<std::uint32_t>(k.steps) * each;
     k.regions = (vocab + region - 1) / region;

@@ -187,10 +187,12 @@ def evict(weight: Any, table: Any, lens: Any, keep: int, block_tokens: int = 16,
     return out_table, out_lens, freed, count
 
 
-def _references(refs: Any, blocks: int | None = None) -> Any:
+def _references(refs: Any, cache: "KvCache | None" = None) -> Any:
     if refs.dtype is not _I32 or refs.dim() != 1 or not refs.is_contiguous() \
-            or refs.shape[0] == 0 or (blocks is not None and refs.shape[0] != blocks):
+            or refs.shape[0] == 0 or (cache is not None and refs.shape[0] != cache.blocks):
         raise ValueError("refs must be a contiguous int32 tensor [blocks]")
+    if cache is not None and refs.device != cache.device:
+        raise ValueError(f"refs is on {refs.device}, the cache on {cache.device}")
     return refs
 
 
@@ -308,16 +310,15 @@ class KvCache:
                 raise ValueError(f"{name} must be a contiguous {dtype} tensor of shape {want}")
             if x.device != keys.device:
                 raise ValueError(f"{name} is on {x.device}, keys on {keys.device}")
-        if refs is None:
-            refs = torch.zeros((blocks,), dtype=torch.int32, device=keys.device)
-        elif _references(refs, blocks).device != keys.device:
-            raise ValueError(f"refs is on {refs.device}, keys on {keys.device}")
-        self.keys, self.values, self.refs = keys, values, refs
+        self.keys, self.values = keys, values
         self.key_scale, self.value_scale = key_scale, value_scale
         self.bounds, self.weight = bounds, weight
         self.blocks, self.kv_heads = blocks, kv_heads
         self.head_dim, self.block_tokens = head_dim, tiles * 16
         self.device, self._gpu = keys.device, _gpu(keys)
+        if refs is None:
+            refs = torch.zeros((blocks,), dtype=torch.int32, device=keys.device)
+        self.refs = _references(refs, self)
         self._lib = nat.load()
         self._c = nat.KvCacheArrays(ctypes.sizeof(nat.KvCacheArrays), blocks, kv_heads, head_dim,
                                     tiles * 16, 0, keys.data_ptr(), values.data_ptr(),
@@ -522,7 +523,7 @@ class KvCache:
         blocks (its row stays as it is), and how many such a sequence needs."""
         if _elsewhere(self._gpu, stream):
             return _there(self.device, stream, lambda: self.grow(table, lens, first, tokens))
-        refs = _references(self.refs, self.blocks)
+        refs = _references(self.refs, self)
         _, seqs, width, stride = _rows_of(table, refs, lens)
         if first is None:
             if tokens not in (None, seqs):
@@ -562,7 +563,7 @@ class KvCache:
         free one), by which other tables of this cache can follow."""
         if _elsewhere(self._gpu, stream):
             return _there(self.device, stream, lambda: self.compact(table))
-        refs = _references(self.refs, self.blocks)
+        refs = _references(self.refs, self)
         _, seqs, width, stride = _rows_of(table, refs)
         _on_gpu(self._gpu)
         need = self._need.get("compact")

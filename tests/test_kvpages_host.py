@@ -236,3 +236,9 @@ def test_references_that_do_not_fit():
     for bad in (refs[:7], refs.long(), refs.view(2, 4), torch.zeros(16, dtype=I32)[::2]):
         with pytest.raises(ValueError, match="refs"):
             kvcache.KvCache.from_tensors(*own, head_dim=64, refs=bad)
+    # a cache's references may be replaced, but not by ones elsewhere
+    table, lens = (torch.zeros(n, dtype=I32, device="meta") for n in ((3, 2), (3,)))
+    c.refs = torch.zeros(8, dtype=I32, device="meta")
+    for bad in (lambda: c.grow(table, lens), lambda: c.compact(table)):
+        with pytest.raises(ValueError, match="refs is on meta"):
+            bad()
