@@ -173,9 +173,11 @@ struct Fork {
     std::uint32_t rows;
     std::int32_t* out;
     std::int32_t* out_lens;
+    bool net;
 };
 // The first rows * chunks workgroups write the new rows, the others change the
-// old rows' counts by their children less one.
+// old rows' counts: by their children less one, which each finds among the
+// parents, or by one down where the new rows count one up themselves.
 __global__ __launch_bounds__(kThreads) void k_kv_fork(Fork a)
 {
     const std::uint32_t r = blockIdx.x / a.t.chunks, chunk = blockIdx.x % a.t.chunks;
@@ -183,23 +185,29 @@ __global__ __launch_bounds__(kThreads) void k_kv_fork(Fork a)
         const std::int32_t p = a.parents[r];
         const bool there = inside(p, a.t.seqs);
         const std::int32_t* row = a.t.table + static_cast<std::size_t>(there ? p : 0) * a.t.stride;
-        each_entry(a.t, chunk, [&](std::uint32_t i) { a.out[static_cast<std::size_t>(r) * a.t.width + i] = there ? row[i] : -1; });
+        each_entry(a.t, chunk, [&](std::uint32_t i) {
+            const std::int32_t id = there ? row[i] : -1;
+            a.out[static_cast<std::size_t>(r) * a.t.width + i] = id;
+            if (!a.net && inside(id, a.t.blocks)) atomicAdd(&a.t.refs[id], 1);
+        });
         if (chunk == 0 && threadIdx.x == 0) a.out_lens[r] = there ? a.t.lens[p] : 0;
         return;
     }
     const std::uint32_t s = r - a.rows;
     __shared__ std::int32_t s_count[kThreads / kWave];
     std::int32_t children = 0;
-    for (std::uint32_t i = threadIdx.x; i < a.rows; i += kThreads) children += a.parents[i] == static_cast<std::int32_t>(s);
+    if (a.net) {
+        for (std::uint32_t i = threadIdx.x; i < a.rows; i += kThreads) children += a.parents[i] == static_cast<std::int32_t>(s);
 #pragma unroll
-    for (int k = 1; k < kWave; k *= 2) children += __shfl_xor(children, k);
-    if (threadIdx.x % kWave == 0) s_count[threadIdx.x / kWave] = children;
-    __syncthreads();
-    children = 0;
+        for (int k = 1; k < kWave; k *= 2) children += __shfl_xor(children, k);
+        if (threadIdx.x % kWave == 0) s_count[threadIdx.x / kWave] = children;
+        __syncthreads();
+        children = 0;
 #pragma unroll
-    for (int i = 0; i < kThreads / kWave; ++i) children += s_count[i];
-    if (children == 1) {
-        return;
+        for (int i = 0; i < kThreads / kWave; ++i) children += s_count[i];
+        if (children == 1) {
+            return;
+        }
     }
     const std::int32_t* row = a.t.table + static_cast<std::size_t>(s) * a.t.stride;
     each_entry(a.t, chunk, [&](std::uint32_t i) {
@@ -1094,6 +1102,11 @@ HBF_API int hbfsim_amd_kv_fork(int32_t* d_refs, uint32_t blocks, const int32_t* 
     a.t.lens = d_lens;
     a.parents = d_parents;
     a.rows = rows;
+    // Children are looked for among all rows in each old row's workgroups; counts
+    // of their own cost each entry two atomics instead.  1,024 rows of 2,048
+    // entries: 57 us against 160, 16,384 of 256: 134 and 315, of 16: 88 and 24,
+    // 1,024 of 16: 5.7 and 5.5.
+    a.net = rows <= 1024 || rows <= std::uint64_t{128} * width;
     a.out = d_out_table;
     a.out_lens = d_out_lens;
     hipLaunchKernelGGL(k_kv_fork, dim3(static_cast<std::uint32_t>(groups)), dim3(kThreads), 0,

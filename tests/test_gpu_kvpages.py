@@ -82,7 +82,8 @@ def batch(rng, seqs, width, blocks, most=None, holes=True):
 
 @pytest.mark.parametrize("seqs,width,rows,extra", [(1, 1, 1, 0), (5, 40, 9, 3), (64, 130, 64, 0),
                                                    (3, 1025, 700, 1), (300, 7, 2, 0), (4, 2500, 5, 8),
-                                                   (6, 9, 0, 0), (2, 0, 3, 0), (0, 4, 3, 0)])
+                                                   (6, 9, 0, 0), (2, 0, 3, 0), (0, 4, 3, 0),
+                                                   (1500, 2, 1600, 1), (40, 8, 1025, 0)])
 def test_hold_and_fork(seqs, width, rows, extra):
     rng = np.random.default_rng(seqs * 7 + width)
     blocks = max(3, seqs * width)
@@ -135,10 +136,10 @@ def test_what_evict_frees_is_released():
     kept, left, freed, gone = cache.evict(table, lens, keep=11)
     cache.release(freed)
     assert int((freed >= 0).sum()) == 0 and int(gone.sum()) > 0
-    used = np.array(kept.cpu())
+    used = kept.cpu().numpy()
     cache_refs = cache.refs.cpu().numpy()
     # evict's table names the blocks of its lengths; those past them were never in it
-    past = np.array(table.cpu())
+    past = table.cpu().numpy().copy()
     for s, n in enumerate(lens.tolist()):
         past[s, :-(-n // 16)] = -1
     np.testing.assert_array_equal(cache_refs, pr.count(used, 200) + pr.count(past, 200))
@@ -411,6 +412,92 @@ def test_compact_of_one_kind(used):
     np.testing.assert_array_equal(got.cpu(), table)
     np.testing.assert_array_equal(cache.refs.cpu(), refs)
     same(cache, moved(was, pairs))
+
+
+# ---- lengths in place, two calls at once --------------------------------------
+
+
+@pytest.mark.parametrize("seqs", [5, 1300])
+def test_grow_writes_the_step_s_lengths_over_the_lengths(seqs):
+    """As the C call may: both forms read every length before they write one."""
+    import ctypes
+
+    from hbfsim_amd import _native as nat
+
+    rng = np.random.default_rng(seqs)
+    blocks = 2 * seqs
+    table, n = batch(rng, seqs, 4, blocks, blocks - 3)
+    cache, _ = filled(blocks, refs=pr.count(table, blocks))
+    refs = cache.refs.cpu().numpy().copy()
+    lens = np.maximum(1, n * 16 - rng.integers(0, 16, seqs)) + rng.integers(0, 30, seqs)
+    first = np.concatenate([[0], np.cumsum(rng.integers(0, 30, seqs))])
+    got, at, offsets = dev(table), dev(lens), dev(first)
+    need, missing = ctypes.c_size_t(), torch.empty(seqs, dtype=torch.int32, device="cuda")
+    lib, tokens = nat.load(), int(first[-1])
+    assert lib.hbfsim_amd_kv_grow_workspace(cache._ref, seqs, tokens, ctypes.byref(need)) == 0
+    ws = torch.empty(need.value, dtype=torch.uint8, device="cuda")
+    assert lib.hbfsim_amd_kv_grow(
+        cache._ref, cache.refs.data_ptr(), got.data_ptr(), at.data_ptr(), offsets.data_ptr(), seqs,
+        tokens, 4, 4, at.data_ptr(), missing.data_ptr(), ws.data_ptr(), need.value,
+        torch.cuda.current_stream().cuda_stream) == 0
+    out, short, _ = pr.grow(refs, table, lens, 16, first, tokens)
+    np.testing.assert_array_equal(at.cpu(), out)
+    np.testing.assert_array_equal(missing.cpu(), short)
+    np.testing.assert_array_equal(got.cpu(), table)
+    np.testing.assert_array_equal(cache.refs.cpu(), refs)
+    assert short.any() or seqs == 5  # of the five none lacks a block
+
+
+def test_two_streams_at_once():
+    """Calls on two caches side by side share nothing."""
+    rng = np.random.default_rng(21)
+    runs = []
+    for i in range(2):
+        table, n = batch(rng, 300, 20, 4000, 3500)
+        cache, was = filled(4000, seed=30 + i, refs=pr.count(table, 4000))
+        runs.append((cache, was, table, (n * 16 + 1).astype(np.int32), torch.cuda.Stream()))
+    args = [(dev(t), dev(n), dev(rng.integers(-1, 300, 280)), dev(rng.permutation(4000)[:1500]))
+            for _, _, t, n, _ in runs]
+    torch.cuda.synchronize()
+    got = []
+    for (cache, _, _, _, s), (table, lens, parents, ids) in zip(runs, args):
+        got.append((cache.grow(table, lens, stream=s)[0], cache.copy(ids, ids.flip(0), stream=s),
+                    cache.fork(table, lens, parents, stream=s)))
+    for (cache, _, _, _, s), (_, _, (table, _)) in zip(runs, got):
+        cache.compact(table, stream=s)
+    torch.cuda.synchronize()
+    for (cache, was, table, lens, _), (_, _, parents, ids), (out, _, (new, _)) in zip(runs, args, got):
+        refs = pr.count(table, 4000)
+        want, _, pairs = pr.grow(refs, table, lens, 16)
+        was = moved(was, pairs)
+        ids = ids.cpu().numpy()
+        was = moved(was, pr.copy_pairs(ids, ids[::-1], 4000, 4000, True))
+        table, _ = pr.fork(refs, table, lens, parents.cpu().numpy())
+        _, pairs = pr.compact(refs, table)
+        np.testing.assert_array_equal(out.cpu(), want)
+        np.testing.assert_array_equal(new.cpu(), table)
+        np.testing.assert_array_equal(cache.refs.cpu(), refs)
+        same(cache, moved(was, pairs))
+
+
+@pytest.mark.parametrize("n", [40, 1500])
+def test_a_captured_copy_replays(n):
+    """With other ids each time, in one launch and in three."""
+    rng = np.random.default_rng(n)
+    cache, was = filled(2 * n, 1, 64, 16, 9)
+    src, dst = dev([-1] * n), dev([-1] * n)
+    cache.copy(src, dst)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        cache.copy(src, dst)
+    for _ in range(6):
+        a, b = rng.integers(-1, 2 * n, n), rng.integers(0, 2 * n, n)
+        src.copy_(dev(a)), dst.copy_(dev(b))
+        graph.replay()
+        torch.cuda.synchronize()
+        was = moved(was, pr.copy_pairs(a, b, 2 * n, 2 * n, True))
+        same(cache, was)
 
 
 # ---- other devices' ways: streams and graphs ------------------------------------

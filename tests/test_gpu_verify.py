@@ -214,12 +214,13 @@ def test_shares_of_many_draws():
     assert abs(kept - a) < 6 * np.sqrt(a * (1 - a) / n)
 
 
-def test_on_another_stream_and_in_a_graph():
+@pytest.mark.parametrize("vocab", [5000, 20_001])
+def test_on_another_stream_and_in_a_graph(vocab):
     rng = np.random.default_rng(6)
     counts = [3, 1, 5, 2]
-    runs = [steps(rng, counts, 5000, "f32") for _ in range(4)]
+    runs = [steps(rng, counts, vocab, "f32") for _ in range(4)]
     first = dev(runs[0][4])
-    p, q = (torch.zeros((11, 5000), device="cuda") for _ in range(2))
+    p, q = (torch.zeros((11, vocab), device="cuda") for _ in range(2))
     tokens, u, lens = dev(np.zeros(11)), dev(np.zeros(11), np.float32), dev([9, 8, 7, 6])
     stream = torch.cuda.Stream()
     stream.wait_stream(torch.cuda.current_stream())
@@ -239,3 +240,38 @@ def test_on_another_stream_and_in_a_graph():
         for got in (captured, eager):
             for a, b in zip(got, want):
                 np.testing.assert_array_equal(a.cpu(), b)
+
+
+def test_two_streams_at_once_and_lengths_in_place():
+    """Two calls side by side share nothing; the C call may write the lengths
+    that remain over the lengths."""
+    import ctypes
+
+    from hbfsim_amd import _native as nat
+
+    rng = np.random.default_rng(7)
+    runs = [steps(rng, rng.integers(0, 6, 40), 9000 + i, "bf16") for i in range(2)]
+    args = [(p.cuda(), q.cuda(), dev(t), dev(u, np.float32), dev(f)) for p, q, t, u, f in runs]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    got = [[drafts.verify(p, t, u, f, draft=q, stream=s) for _ in range(5)]
+           for s, (p, q, t, u, f) in zip(streams, args)]
+    torch.cuda.synchronize()
+    lens = np.arange(40, dtype=np.int32) + 50
+    for (p, q, t, u, f), results, (gp, gq, gt, gu, gf) in zip(runs, got, args):
+        want = pr.verify(p.float().numpy(), t, u, f, q.float().numpy(), lens)
+        for out, gained, _ in results:
+            np.testing.assert_array_equal(out.cpu(), want[0])
+            np.testing.assert_array_equal(gained.cpu(), want[1])
+        need, at = ctypes.c_size_t(), dev(lens)
+        assert nat.load().hbfsim_amd_verify_workspace(40, p.shape[1], nat.KV_BF16,
+                                                      ctypes.byref(need)) == 0
+        ws = torch.empty(max(16, need.value), dtype=torch.uint8, device="cuda")
+        out, gained = dev(np.zeros(len(t))), dev(np.zeros(40))
+        assert nat.load().hbfsim_amd_verify(
+            gp.data_ptr(), gq.data_ptr(), nat.KV_BF16, p.shape[1], p.shape[1], p.shape[1],
+            gt.data_ptr(), gu.data_ptr(), gf.data_ptr(), 40, len(t), at.data_ptr(), out.data_ptr(),
+            gained.data_ptr(), at.data_ptr(), ws.data_ptr(), need.value,
+            torch.cuda.current_stream().cuda_stream) == 0
+        np.testing.assert_array_equal(out.cpu(), want[0])
+        np.testing.assert_array_equal(at.cpu(), want[2])
