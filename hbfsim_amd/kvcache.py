@@ -259,7 +259,8 @@ def release(refs: Any, table: Any, lens: Any = None, block_tokens: int = 16,
     _on_gpu(gpu)
     _refuse(nat.load().hbfsim_amd_kv_release(
         refs.data_ptr(), blocks, block_tokens, table.data_ptr(),
-        lens.data_ptr() if lens is not None else None, seqs, width, stride, _handle(gpu)), "release")
+        lens.data_ptr() if lens is not None else None, seqs, width, stride, _handle(gpu)),
+        "release")
 
 
 class KvCache:
@@ -495,7 +496,11 @@ class KvCache:
         if to.device != self.device:
             raise ValueError(f"to is on {to.device}, the cache on {self.device}")
         _on_gpu(self._gpu)
-        need = to.blocks * 4 if n else 0
+        need = to._need.get(("copy", n))
+        if need is None:
+            got = ctypes.c_size_t()
+            _refuse(self._lib.hbfsim_amd_kv_copy_workspace(to._ref, n, ctypes.byref(got)), "copy")
+            need = to._remember(("copy", n), got.value)
         ws = _workspace(need, self.device)
         _refuse(self._lib.hbfsim_amd_kv_copy(
             self._ref, to._ref, src.data_ptr(), dst.data_ptr(), n,
@@ -519,8 +524,10 @@ class KvCache:
         `first` are the append's, `tokens` its rows where `first` is given.  The
         table is changed: a row gets a new block where it names none, and one
         of its own, with the content, where the step writes to a shared one.
-        Returns (lens, missing): the step's lengths, 0 for a sequence that lacks
-        blocks (its row stays as it is), and how many such a sequence needs."""
+        Blocks of no reference are handed out, so tables made by hand are to be
+        held first.  Returns (lens, missing): the step's lengths, 0 for a
+        sequence that lacks blocks (its row stays as it is), and how many such a
+        sequence needs."""
         if _elsewhere(self._gpu, stream):
             return _there(self.device, stream, lambda: self.grow(table, lens, first, tokens))
         refs = _references(self.refs, self)

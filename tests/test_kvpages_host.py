@@ -39,8 +39,9 @@ def test_copy_refuses():
     assert copy() == RUNS
     assert copy(b=arrays(HERE + 8 * FAR)) == RUNS
     assert copy(n=0, src=None, dst=None, ws=None, nbytes=0) == OK
-    for kw in (dict(src=None), dict(dst=None), dict(ws=None), dict(ws=HERE + 4), dict(nbytes=31),
-               dict(a=arrays(struct_size=3)), dict(a=arrays(blocks=0)), dict(a=arrays(kv_heads=0)),
+    assert copy(ws=None, nbytes=0) == RUNS  # few pairs need none
+    for kw in (dict(src=None), dict(dst=None), dict(n=5000, ws=None), dict(n=5000, ws=HERE + 4),
+               dict(n=5000, nbytes=31), dict(a=arrays(struct_size=3)), dict(a=arrays(blocks=0)), dict(a=arrays(kv_heads=0)),
                dict(a=arrays(d_keys=None)), dict(a=arrays(d_bounds=HERE + 8)),
                dict(b=arrays(HERE + 8 * FAR, kv_heads=4)), dict(b=arrays(HERE + 8 * FAR, head_dim=65)),
                dict(b=arrays(HERE + 8 * FAR, block_tokens=32)),
@@ -51,9 +52,10 @@ def test_copy_refuses():
     assert copy(n=1 << 40, nbytes=1 << 50) == NO
     need = ctypes.c_size_t()
     assert nat.load().hbfsim_amd_kv_copy_workspace(ctypes.byref(arrays()), 3, None) == BAD
-    assert nat.load().hbfsim_amd_kv_copy_workspace(ctypes.byref(arrays()), 3,
-                                                   ctypes.byref(need)) == OK
-    assert need.value == 32
+    for n, want in ((0, 0), (3, 0), (5000, 32)):
+        assert nat.load().hbfsim_amd_kv_copy_workspace(ctypes.byref(arrays()), n,
+                                                       ctypes.byref(need)) == OK
+        assert need.value == want
 
 
 def hold(refs=HERE, blocks=8, table=HERE, seqs=3, width=4, stride=4):
