@@ -383,9 +383,9 @@ __global__ __launch_bounds__(kPlan) void k_kv_grow_count(Grow a)
 // first tile, and each tile is on its way while the one before is counted; with
 // counts, tiles without a free block are left out.
 // A compute unit reads 33 GB/s so, a tile in 1.03 us: a step of 64 sequences
-// takes 5 us where the first tile has their blocks, and without counts 14 where
-// the first half of 131,072 blocks is in use, 21 where nearly all are; with
-// them 9 wherever the free ones lie, also of 500,000 (71 without).
+// takes 6 us where the first tile has their blocks, and without counts 15 where
+// the first half of 131,072 blocks is in use, 22 where nearly all are; with
+// them 10 wherever the free ones lie, also of 500,000 (70 without).
 template <typename F>
 __device__ inline std::int32_t first_free(const Grow& a, std::uint32_t tile, std::int32_t want, F put)
 {
@@ -433,7 +433,7 @@ __device__ inline std::int32_t first_free(const Grow& a, std::uint32_t tile, std
 // many blocks are wanted, the first free ones, who gets them.  A slot is a block
 // that a sequence may write to, as in append.  Every step needs the one before
 // of all slots, so it is a chain of trips to memory and barriers, no work to
-// spread: 11.2 us for 17 chunks of 35,769 tokens (1,151 slots), 24 for 4,000
+// spread: 11.2 us for 17 chunks of 35,769 tokens (1,151 slots), 25 for 4,000
 // sequences of one token.  (Steps side by side in several workgroups would need
 // a launch between each two.)
 __global__ __launch_bounds__(kPlan) void k_kv_grow(Grow a)
@@ -556,7 +556,7 @@ __global__ __launch_bounds__(kPlan) void k_kv_grow(Grow a)
 // The same for at most kPlan slots, a thread each: what the slots share lies in
 // LDS, and the first free blocks are looked for while the rows come in: 5.4 us
 // for 64 sequences of one token, a microsecond more for 1,024; the form above
-// takes six more for 1,500.
+// takes five more for 1,500.
 constexpr int kShared = 2 * kPlan;  // of the table of shared blocks
 
 __global__ __launch_bounds__(kPlan) void k_kv_grow_few(Grow a)
@@ -967,8 +967,8 @@ std::uint64_t slots_of(const Cache& c, std::uint32_t seqs, std::uint32_t tokens,
     return offsets ? tokens / c.tokens + std::uint64_t{2} * seqs : seqs;
 }
 // Blocks up to which the planning workgroup looks for free ones without counts:
-// 60,000 cost it 1 to 7 us more than the first tile, by where the free ones lie,
-// and counts 4.
+// 60,000 cost it up to 6 us more than the first tile, by where the free ones
+// lie, and counts 3.5.
 constexpr std::uint32_t kScanned = 65536;
 // Where a thread takes a slot, the plan lies in LDS and only the pairs in memory.
 GrowSpace grow_space(const Cache& c, std::uint32_t seqs, std::uint64_t slots)
