@@ -145,6 +145,13 @@ inline int take_batch(const hbfsim_amd_kv_batch* in, const Cache& c, Batch* out)
     return HBFSIM_OK;
 }
 
+// Whether [p, p + n) and [q, q + m) have a byte in common.
+inline bool meet(const void* p, std::size_t n, const void* q, std::size_t m)
+{
+    const std::uintptr_t a = reinterpret_cast<std::uintptr_t>(p), b = reinterpret_cast<std::uintptr_t>(q);
+    return p != nullptr && q != nullptr && n != 0 && m != 0 && a < b + m && b < a + n;
+}
+
 inline std::size_t up256(std::size_t x) { return (x + 255) & ~std::size_t{255}; }
 
 }  // namespace kv

@@ -924,13 +924,6 @@ Piece piece_of(const Cache& c)
 std::size_t copy_bytes(const Cache& to, std::size_t n) { return n <= kFewPairs ? 0 : static_cast<std::size_t>(to.blocks) * 4; }
 std::size_t block_bytes(const Cache& c) { return static_cast<std::size_t>(c.kv_heads) * c.tokens * c.dims; }
 
-// Whether [p, p + n) and [q, q + m) have a byte in common.
-bool meet(const void* p, std::size_t n, const void* q, std::size_t m)
-{
-    const std::uintptr_t a = reinterpret_cast<std::uintptr_t>(p), b = reinterpret_cast<std::uintptr_t>(q);
-    return n != 0 && m != 0 && a < b + m && b < a + n;
-}
-
 // Two caches share nothing.
 bool apart(const Cache& x, const Cache& y)
 {

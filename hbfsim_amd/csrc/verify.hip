@@ -356,9 +356,8 @@ __device__ inline void give_nothing(const Verify& a, std::uint32_t s)
         for (std::int64_t i = (to > 0 ? to : 0) + lane; i < a.rows; i += kWave) a.out[i] = -1;
         return;
     }
-    for (std::int64_t i = a.first[s] + static_cast<std::int64_t>(lane); i < a.first[s + 1] && i < a.rows; i += kWave) {
-        if (i >= 0) a.out[i] = -1;  // rows that end past the batch
-    }
+    const std::int64_t begin = a.first[s] > 0 ? a.first[s] : 0;
+    for (std::int64_t i = begin + lane; i < a.first[s + 1] && i < a.rows; i += kWave) a.out[i] = -1;  // past the batch
     if (lane == 0) {
         a.gained[s] = 0;
         if (a.lens != nullptr) a.out_lens[s] = a.lens[s] - (a.first[s + 1] - a.first[s]);
@@ -552,13 +551,6 @@ void launch(const Verify& a, const Cut& k, hipStream_t s)
     } else {
         launch_two<T, 4>(a, s);
     }
-}
-
-// Whether [p, p + n) and [q, q + m) have a byte in common.
-bool meet(const void* p, std::size_t n, const void* q, std::size_t m)
-{
-    const std::uintptr_t a = reinterpret_cast<std::uintptr_t>(p), b = reinterpret_cast<std::uintptr_t>(q);
-    return p != nullptr && q != nullptr && n != 0 && m != 0 && a < b + m && b < a + n;
 }
 
 }  // namespace
