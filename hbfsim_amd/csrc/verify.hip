@@ -24,6 +24,13 @@ constexpr int kThreads = 256;
 
 typedef unsigned long long u64;
 
+// What the second launch needs of a sequence, so that it need not look it up.
+struct alignas(16) State {
+    int4 drafts;                // accepted, whether a draft was refused, that draft
+    std::int32_t begin, count;  // its rows
+    float uniform;              // of the last one
+};
+
 struct Verify {
     const void* target;
     const void* draft;  // or null
@@ -37,8 +44,8 @@ struct Verify {
     std::int32_t* out;
     std::int32_t* gained;
     std::int32_t* out_lens;
-    int4* state;  // [seqs]: accepted, whether a draft was refused, that draft
-    u64* sums;    // [seqs][regions]: of what is drawn from
+    State* state;  // [seqs]
+    u64* sums;     // [seqs][regions]: of what is drawn from
 };
 
 // A sequence's rows, none if they do not describe the batch.
@@ -167,16 +174,11 @@ struct Region {
         asm volatile("" : "+v"(s.a), "+v"(s.b));
         return s;
     }
-    __device__ inline u64 sum(From from, std::uint32_t out)
+    __device__ inline void sums(From from, std::uint32_t out, u64 (&to)[kSteps])
     {
-        Parts s{0, 0};
         const auto add = [&](From f) {
 #pragma unroll
-            for (int i = 0; i < kSteps; ++i) {
-                const Parts x = sum(i, f, out);
-                s.a += x.a;
-                s.b += x.b;
-            }
+            for (int i = 0; i < kSteps; ++i) to[i] = joined(sum(i, f, out));
         };
         if (from == From::kRest) {
             add(From::kRest);
@@ -185,7 +187,6 @@ struct Region {
         } else {
             add(From::kTarget);
         }
-        return joined(s);
     }
 
 private:
@@ -205,6 +206,22 @@ __device__ inline u64 wave_sum(u64 x)
 #pragma unroll
     for (int k = 1; k < kWave; k *= 2) x += __shfl_xor(x, k);
     return x;
+}
+// Sums of 1 or 4 numbers over the wave: a quarter of it ends up with each.  At
+// the first two steps a lane passes on the half that is not its quarter's, so
+// that four cost seven exchanges and not 24.
+__device__ inline u64 wave_sums(const u64 (&x)[1]) { return wave_sum(x[0]); }
+__device__ inline u64 wave_sums(const u64 (&x)[4])
+{
+    const int lane = threadIdx.x % kWave;
+    const bool upper = (lane & 32) != 0, odd = (lane & 16) != 0;
+    u64 a = upper ? x[2] : x[0], b = upper ? x[3] : x[1];
+    a += __shfl_xor(upper ? x[0] : x[2], 32);
+    b += __shfl_xor(upper ? x[1] : x[3], 32);
+    u64 s = (odd ? b : a) + __shfl_xor(odd ? a : b, 16);
+#pragma unroll
+    for (int k = 1; k < 16; k *= 2) s += __shfl_xor(s, k);
+    return s;
 }
 __device__ inline u64 wave_upto(u64 x)
 {
@@ -310,7 +327,7 @@ __device__ std::int32_t draw_full(const Verify& a, std::int64_t row, float unifo
         for (std::uint32_t i = 0; i < regions; ++i) {
             Region<T, 1> x;
             x.load(a, row, From::kTarget, i);
-            const u64 c = wave_sum(x.sum(From::kTarget, 0));
+            const u64 c = wave_sum(joined(x.sum(0, From::kTarget, 0)));
             if (pass == 0) {
                 sum += c;
             } else if (left < c) {
@@ -364,50 +381,59 @@ __device__ inline void give_nothing(const Verify& a, std::uint32_t s)
     }
 }
 
-// A region is kSteps consecutive KiB of a row.  One wave sums one, and finds
-// how far the drafts stay by itself first: the same few loads for all of a
+// One wave sums kSteps consecutive KiB of a row, a region each, and finds how
+// far the drafts stay by itself first: the same few loads for all of a
 // sequence's waves, cheaper than a launch or a barrier.  Sums of whole numbers
 // need no order, so nothing is shared between waves.  64 sequences over 151,936
-// tokens in f32 (69 MB, as some keep all drafts and need no q) take 14.2 us, 4.8
+// tokens in f32 (69 MB, as some keep all drafts and need no q) take 14.0 us, 4.9
 // TB/s; a single one over 32,000 3.5, the trips to its offsets, its tokens, their
 // probabilities and the row.
 template <typename T, int kSteps>
 __global__ __launch_bounds__(kThreads) void k_verify_sum(Verify a)
 {
-    const std::uint32_t groups = (a.regions + kThreads / kWave - 1) / (kThreads / kWave);
+    constexpr std::uint32_t kRegions = kThreads / kWave * kSteps;  // of a workgroup
+    const std::uint32_t groups = (a.regions + kRegions - 1) / kRegions;
     const std::uint32_t s = blockIdx.x / groups;
-    const std::uint32_t region = __builtin_amdgcn_readfirstlane(blockIdx.x % groups * (kThreads / kWave) + threadIdx.x / kWave);
+    const std::uint32_t part = __builtin_amdgcn_readfirstlane(blockIdx.x % groups * (kThreads / kWave) + threadIdx.x / kWave);
     const Rows r = rows_of(a, s);
-    if (r.count == 0 || region >= a.regions) {
-        return;
-    }
-    const int4 state = accept<T>(a, r);
     const bool first = threadIdx.x % kWave == 0;
-    if (region == 0 && first) a.state[s] = state;
-    Region<T, kSteps> x;
-    x.load(a, r.begin + state.x, from_of(a, state), region);
-    const u64 sum = wave_sum(x.sum(from_of(a, state), state.z));
-    if (first) a.sums[static_cast<std::size_t>(s) * a.regions + region] = sum;
-}
-
-// One wave per sequence: the region whose running sum passes the drawn number,
-// and the element in it.  The last wave clears the rows of no sequence.  5.4 us
-// for those 64, 3.3 for the one: trips to the sums and to the region, and scans.
-template <typename T, int kSteps>
-__global__ __launch_bounds__(kWave) void k_verify_find(Verify a)
-{
-    constexpr int kHeld = 4;  // regions of a lane that stay in registers
-    const std::uint32_t s = blockIdx.x;
-    const int lane = threadIdx.x;
-    Rows r{0, 0};
-    if (s < a.seqs) r = rows_of(a, s);
-    if (r.count == 0) {
-        give_nothing(a, s);
+    if (r.count == 0 || part * kSteps >= a.regions) {
+        if (part == 0 && first) a.state[s].count = 0;
         return;
     }
     const float uniform = a.uniform[r.begin + r.count - 1];
+    const int4 state = accept<T>(a, r);
+    if (part == 0 && first) a.state[s] = State{state, static_cast<std::int32_t>(r.begin), r.count, uniform};
+    Region<T, kSteps> x;
+    x.load(a, r.begin + state.x, from_of(a, state), part);
+    u64 sum[kSteps];
+    x.sums(from_of(a, state), state.z, sum);
+    const u64 mine = wave_sums(sum);
+    const std::uint32_t region = part * kSteps + threadIdx.x % kWave / (kWave / kSteps);
+    if (threadIdx.x % (kWave / kSteps) == 0 && region < a.regions) {
+        a.sums[static_cast<std::size_t>(s) * a.regions + region] = mine;
+    }
+}
+
+// One wave per sequence: the region whose running sum passes the drawn number,
+// and the element in it.  The last wave clears the rows of no sequence.  4.3 us
+// for those 64, 3.4 for the one: trips to the sums and to the region, and scans.
+template <typename T>
+__global__ __launch_bounds__(kWave) void k_verify_find(Verify a)
+{
+    constexpr int kHeld = 12;  // regions of a lane that stay in registers
+    const std::uint32_t s = blockIdx.x;
+    const int lane = threadIdx.x;
+    State own_state{};
+    if (s < a.seqs) own_state = a.state[s];
+    if (own_state.count == 0) {
+        give_nothing(a, s);
+        return;
+    }
+    const Rows r{own_state.begin, own_state.count};
+    const float uniform = own_state.uniform;
+    const int4 state = own_state.drafts;
     const std::int32_t mine = drafted(a, r);
-    const int4 state = a.state[s];
     const From from = from_of(a, state);
     const u64* sums = a.sums + static_cast<std::size_t>(s) * a.regions;
     const std::uint32_t each = (a.regions + kWave - 1) / kWave;
@@ -415,9 +441,16 @@ __global__ __launch_bounds__(kWave) void k_verify_find(Verify a)
     const std::uint32_t end = begin + each < a.regions ? begin + each : a.regions;
     u64 held[kHeld], own = 0;
 #pragma unroll
-    for (int i = 0; i < kHeld; ++i) held[i] = begin + i < end ? sums[begin + i] : 0;
+    for (int i = 0; i < 4; ++i) held[i] = begin + i < end ? sums[begin + i] : 0;
+#pragma unroll
+    for (int i = 4; i < kHeld; ++i) held[i] = 0;
+    if (each > 4) {
+#pragma unroll
+        for (int i = 4; i < kHeld; ++i) held[i] = begin + i < end ? sums[begin + i] : 0;
+    }
 #pragma unroll
     for (int i = 0; i < kHeld; ++i) own += held[i];
+#pragma unroll 4
     for (std::uint32_t i = begin + kHeld; i < end; ++i) own += sums[i];
     const u64 upto = wave_upto(own), sum = __shfl(upto, kWave - 1);
     std::int32_t token = -1;
@@ -439,9 +472,9 @@ __global__ __launch_bounds__(kWave) void k_verify_find(Verify a)
         }
         region = __builtin_amdgcn_readfirstlane(__shfl(region, owner));
         left = __shfl(left, owner);
-        Region<T, kSteps> x;
+        Region<T, 1> x;
         x.load(a, r.begin + state.x, from, region);
-        token = walk<T, kSteps>(x, region, left, from, state.z);
+        token = walk<T, 1>(x, region, left, from, state.z);
     } else {
         token = draw_full<T>(a, r.begin + state.x, uniform);
     }
@@ -469,7 +502,11 @@ __global__ __launch_bounds__(1024) void k_verify_one(Verify a)
     const From from = from_of(a, state);
     Region<T, kSteps> x;
     x.load(a, r.begin + state.x, from, wave);
-    const u64 own = wave_sum(x.sum(from, state.z));
+    u64 step[kSteps], own = 0;
+    x.sums(from, state.z, step);
+#pragma unroll
+    for (int i = 0; i < kSteps; ++i) own += step[i];
+    own = wave_sum(own);
     if (threadIdx.x % kWave == 0) s_sum[wave] = own;
     __syncthreads();
     u64 sum = 0;
@@ -493,16 +530,17 @@ constexpr std::uint32_t kMostVocab = 1u << 22;
 // How a call is cut: from its sizes alone (floats, by graph replays; two-byte
 // types take within 2 us of the same).
 // A workgroup per sequence where 16 waves of two loads each hold the row: 1 and
-// 256 sequences over 4,000 tokens take 5.8 and 6.2 us against 6.4 and 7.6 in two
-// launches, over 8,000 6.7 and 7.9 against 6.1 and 8.9, and one launch less costs
+// 256 sequences over 4,000 tokens take 5.1 and 6.3 us against 6.8 and 8.2 in two
+// launches, over 8,000 7.3 and 8.0 against 6.8 and 8.7, and one launch less costs
 // the host 3 us less.  Eight loads a wave would hold 32,000, but one compute unit
 // then reads for 12 us what two launches are done with in 6.
-// Two launches otherwise, of regions of one load where few waves would be left:
-// 64 sequences over 32,000 take 8.9 us with one load and 10.0 with four (2,000
-// waves), over 60,000 12.2 and 11.4 (3,800), over 151,936 22.4 and 18.9.
+// Two launches otherwise, a load a wave where few waves would be left: 64
+// sequences over 16,000 take 8.1 us with one load and 8.4 with four (1,000
+// waves), over 32,000 9.4 and 8.9, over 60,000 13.0 and 10.4, over 151,936 22.1
+// and 17.6-18.5.
 struct Cut {
-    bool one;  // a workgroup per sequence
-    int steps;
+    bool one;   // a workgroup per sequence
+    int steps;  // regions of a wave
     std::uint32_t regions;
     std::size_t sums, bytes;
 };
@@ -515,12 +553,11 @@ Cut cut_of(std::uint32_t seqs, std::uint32_t vocab, std::uint32_t type)
         k.steps = 2;
     } else {
         const std::uint64_t waves = static_cast<std::uint64_t>(seqs) * ((vocab + 4 * each - 1) / (4 * each));
-        k.steps = waves < 3000 ? 1 : 4;
+        k.steps = waves < 1500 ? 1 : 4;
     }
-    const std::uint32_t region = static_cast<std::uint32_t>(k.steps) * each;
-    k.regions = (vocab + region - 1) / region;
+    k.regions = (vocab + each - 1) / each;
     if (!k.one) {
-        k.sums = up256(static_cast<std::size_t>(seqs) * sizeof(int4));
+        k.sums = up256(static_cast<std::size_t>(seqs) * sizeof(State));
         k.bytes = k.sums + static_cast<std::size_t>(seqs) * k.regions * sizeof(u64);
     }
     return k;
@@ -536,16 +573,16 @@ void launch_two(const Verify& a, hipStream_t s)
 {
     constexpr std::uint32_t kWaves = kThreads / kWave;
     if (a.seqs != 0) {
-        const dim3 groups(a.seqs * ((a.regions + kWaves - 1) / kWaves));
+        const dim3 groups(a.seqs * ((a.regions + kWaves * kSteps - 1) / (kWaves * kSteps)));
         hipLaunchKernelGGL((k_verify_sum<T, kSteps>), groups, dim3(kThreads), 0, s, a);
     }
-    hipLaunchKernelGGL((k_verify_find<T, kSteps>), dim3(a.seqs + 1), dim3(kWave), 0, s, a);
+    hipLaunchKernelGGL(k_verify_find<T>, dim3(a.seqs + 1), dim3(kWave), 0, s, a);
 }
 template <typename T>
 void launch(const Verify& a, const Cut& k, hipStream_t s)
 {
     if (k.one) {
-        hipLaunchKernelGGL((k_verify_one<T, 2>), dim3(a.seqs + 1), dim3(k.regions * kWave), 0, s, a);
+        hipLaunchKernelGGL((k_verify_one<T, 2>), dim3(a.seqs + 1), dim3((k.regions + 1) / 2 * kWave), 0, s, a);
     } else if (k.steps == 1) {
         launch_two<T, 1>(a, s);
     } else {
@@ -597,7 +634,8 @@ HBF_API int hbfsim_amd_verify(const void* d_target, const void* d_draft, uint32_
     }
     Verify a{};
     a.regions = k.regions;
-    if (static_cast<std::uint64_t>(seqs) * ((k.regions + 3) / 4) > (k.one ? kMostGroups : 4 * kMostGroups)) {
+    const std::uint64_t part = 4 * static_cast<std::uint64_t>(k.steps);
+    if (seqs * ((k.regions + part - 1) / part) > (k.one ? kMostGroups : 4 * kMostGroups)) {
         return HBFSIM_UNSUPPORTED;
     }
     const std::int64_t each = type == HBFSIM_AMD_KV_F32 ? 4 : 8;
@@ -620,7 +658,7 @@ HBF_API int hbfsim_amd_verify(const void* d_target, const void* d_draft, uint32_
     a.gained = d_gained;
     a.out_lens = d_out_lens;
     unsigned char* ws = static_cast<unsigned char*>(d_workspace);
-    a.state = reinterpret_cast<int4*>(ws);
+    a.state = reinterpret_cast<State*>(ws);
     a.sums = k.one || seqs == 0 ? nullptr : reinterpret_cast<u64*>(ws + k.sums);
     const hipStream_t s = static_cast<hipStream_t>(stream);
     if (type == HBFSIM_AMD_KV_BF16) {

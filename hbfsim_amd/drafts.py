@@ -22,12 +22,12 @@ from typing import Any
 import torch
 
 from . import _native as nat
-from .kvcache import (_TYPES, _counts, _elsewhere, _gpu, _handle, _ints, _on_gpu, _refuse, _there)
+from .kvcache import _TYPES, _counts, _elsewhere, _flat, _gpu, _handle, _on_gpu, _refuse, _there
 
 _need: dict = {}  # workspace bytes by a call's sizes
 
 
-def _probabilities(x: Any, name: str, rows: int | None = None) -> Any:
+def _probabilities(x: Any, name: str) -> Any:
     if x.dim() != 2 or x.dtype not in _TYPES or (x.shape[1] > 1 and x.stride(1) != 1):
         raise ValueError(f"{name} must be [rows, vocab] of bfloat16, float16 or float32, "
                          "contiguous in its last dimension")
@@ -58,19 +58,20 @@ def verify(target: Any, tokens: Any, uniform: Any, first: Any = None, draft: Any
     device = target.device
     rows, vocab = _probabilities(target, "target").shape
     if draft is not None and (_probabilities(draft, "draft").shape != target.shape
-                              or draft.dtype != target.dtype or draft.device != device):
+                              or draft.dtype is not target.dtype
+                              or draft.get_device() != target.get_device()):
         raise ValueError("draft must be of target's shape, type and device")
-    if _ints(tokens, "tokens", device, 1).shape[0] != rows:
+    if _flat(tokens, "tokens", target) != rows:
         raise ValueError(f"{tokens.shape[0]} tokens for {rows} rows")
-    if uniform.dtype != torch.float32 or tuple(uniform.shape) != (rows,) \
-            or uniform.device != device or not uniform.is_contiguous():
+    if uniform.dtype is not torch.float32 or uniform.dim() != 1 or uniform.shape[0] != rows \
+            or uniform.get_device() != target.get_device() or not uniform.is_contiguous():
         raise ValueError(f"uniform must be a contiguous float32 tensor [{rows}] on {device}")
     seqs = rows
     if first is not None:
-        seqs = _ints(first, "first", device, 1).shape[0] - 1
+        seqs = _flat(first, "first", target) - 1
         if seqs < 0:
             raise ValueError("first must hold one offset more than there are sequences")
-    if lens is not None and _ints(lens, "lens", device, 1).shape[0] != seqs:
+    if lens is not None and _flat(lens, "lens", target) != seqs:
         raise ValueError(f"{lens.shape[0]} lengths for {seqs} sequences")
     _counts(rows | seqs | vocab)
     _on_gpu(gpu)

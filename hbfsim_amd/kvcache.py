@@ -55,6 +55,8 @@ def padded_dim(head_dim: int) -> int:
 
 
 def _refuse(rc: int, what: str) -> None:
+    if rc == nat.HBFSIM_OK:
+        return
     if rc in (nat.HBFSIM_INVALID_ARGUMENT, nat.HBFSIM_UNSUPPORTED):
         raise ValueError(f"{what} refused: {nat.status_name(rc)} ({rc})")
     nat.check(rc, what)
@@ -62,7 +64,7 @@ def _refuse(rc: int, what: str) -> None:
 
 def _gpu(x: Any) -> int | None:
     """The index of the tensor's GPU, None on another kind of device."""
-    return x.device.index if x.is_cuda else None
+    return x.get_device() if x.is_cuda else None
 
 
 def _elsewhere(gpu: int | None, stream: Any) -> bool:
@@ -187,6 +189,16 @@ def evict(weight: Any, table: Any, lens: Any, keep: int, block_tokens: int = 16,
     return out_table, out_lens, freed, count
 
 
+def _flat(x: Any, name: str, like: Any) -> int:
+    """How many there are of an int32 vector beside `like`.  (The checks below
+    are the common case's, a quarter of a microsecond; `_ints` says what is
+    wrong, or lets pass what they are too strict for.)"""
+    if x.dtype is not _I32 or x.dim() != 1 or x.get_device() != like.get_device() \
+            or not x.is_contiguous():
+        _ints(x, name, like.device, 1)
+    return x.shape[0]
+
+
 def _references(refs: Any, cache: "KvCache | None" = None) -> Any:
     if refs.dtype is not _I32 or refs.dim() != 1 or not refs.is_contiguous() \
             or refs.shape[0] == 0 or (cache is not None and refs.shape[0] != cache.blocks):
@@ -198,13 +210,17 @@ def _references(refs: Any, cache: "KvCache | None" = None) -> Any:
 
 def _rows_of(table: Any, refs: Any, lens: Any = None) -> tuple[int, int, int, int]:
     """(blocks, sequences, width, stride) of a table beside its references."""
-    device = refs.device
-    seqs, width = _ints(table, "table", device, 2).shape
-    if lens is not None and _ints(lens, "lens", device, 1).shape[0] != seqs:
+    if table.dtype is _I32 and table.dim() == 2 and table.get_device() == refs.get_device() \
+            and table.is_contiguous():
+        seqs, width = table.shape
+        stride = width
+    else:
+        seqs, width = _ints(table, "table", refs.device, 2).shape
+        stride = table.stride(0) if seqs > 1 else width
+        if stride < width:
+            raise ValueError("table rows overlap")
+    if lens is not None and _flat(lens, "lens", refs) != seqs:
         raise ValueError(f"{lens.shape[0]} lengths for {seqs} sequences")
-    stride = table.stride(0) if seqs > 1 else width
-    if stride < width:
-        raise ValueError("table rows overlap")
     blocks = refs.shape[0]
     _counts(blocks | seqs | width | stride)
     return blocks, seqs, width, stride
@@ -234,11 +250,12 @@ def fork(refs: Any, table: Any, lens: Any, parents: Any, stream: Any = None) -> 
         return _there(refs.device, stream, lambda: fork(refs, table, lens, parents))
     _references(refs)
     blocks, seqs, width, stride = _rows_of(table, refs, lens)
-    rows = _ints(parents, "parents", refs.device, 1).shape[0]
+    rows = _flat(parents, "parents", refs)
     _counts(rows)
     _on_gpu(gpu)
-    out = torch.empty((rows, width), dtype=torch.int32, device=refs.device)
-    out_lens = torch.empty((rows,), dtype=torch.int32, device=refs.device)
+    device = refs.device
+    out = torch.empty((rows, width), dtype=_I32, device=device)
+    out_lens = torch.empty((rows,), dtype=_I32, device=device)
     _refuse(nat.load().hbfsim_amd_kv_fork(
         refs.data_ptr(), blocks, table.data_ptr(), lens.data_ptr(), seqs, width, stride,
         parents.data_ptr(), rows, out.data_ptr(), out_lens.data_ptr(), _handle(gpu)), "fork")
@@ -489,9 +506,8 @@ class KvCache:
         if _elsewhere(self._gpu, stream):
             return _there(self.device, stream, lambda: self.copy(src, dst, to))
         to = self if to is None else to
-        _ints(src, "src", self.device, 1)
-        n = _ints(dst, "dst", self.device, 1).shape[0]
-        if src.shape[0] != n:
+        n = _flat(dst, "dst", self.keys)
+        if _flat(src, "src", self.keys) != n:
             raise ValueError(f"{src.shape[0]} sources for {n} destinations")
         if to.device != self.device:
             raise ValueError(f"to is on {to.device}, the cache on {self.device}")
@@ -537,7 +553,7 @@ class KvCache:
                 raise ValueError(f"{tokens} tokens for {seqs} sequences of one token each")
             tokens = seqs
         else:
-            if _ints(first, "first", self.device, 1).shape[0] != seqs + 1:
+            if _flat(first, "first", refs) != seqs + 1:
                 raise ValueError("first must hold one offset more than there are sequences")
             if tokens is None or tokens < 0:
                 raise ValueError("tokens must say how many rows the batch of `first` has")
@@ -579,7 +595,7 @@ class KvCache:
             _refuse(self._lib.hbfsim_amd_kv_compact_workspace(self._ref, ctypes.byref(got)),
                     "compact")
             need = self._remember("compact", got.value)
-        where = torch.empty((self.blocks,), dtype=torch.int32, device=self.device)
+        where = torch.empty((self.blocks,), dtype=_I32, device=self.device)
         ws = _workspace(need, self.device)
         _refuse(self._lib.hbfsim_amd_kv_compact(
             self._ref, refs.data_ptr(), table.data_ptr(), seqs, width, stride, where.data_ptr(),

@@ -1,6 +1,6 @@
 """The operators on a paged cache's blocks and the verification of drafted
-tokens from their definitions, on the CPU: one entry, one block, one token at a
-time, in whole numbers of any size.
+tokens from their definitions, on the CPU: one entry, one block, one sequence at
+a time, in whole numbers.
 """
 from __future__ import annotations
 
@@ -165,10 +165,10 @@ def share(x):
 
 
 def whole(x):
-    """2^40 x to the nearest whole number, ties to even."""
-    f = Fraction(share(x)) * 2 ** 40
-    n, half = f.numerator // f.denominator, f - f.numerator // f.denominator
-    return n + (half > Fraction(1, 2) or (half == Fraction(1, 2) and n % 2 == 1))
+    """2^40 x to the nearest whole number, ties to even; x of 24 bits, so that
+    the product is exact in float64."""
+    x = np.clip(np.nan_to_num(np.asarray(x, np.float64), nan=0.0), 0.0, 1.0)
+    return np.rint(x * 2.0 ** 40).astype(np.int64)
 
 
 def verify(target, tokens, uniform, first=None, draft=None, lens=None):
@@ -198,21 +198,18 @@ def verify(target, tokens, uniform, first=None, draft=None, lens=None):
                 break
             stays += 1
         r = begin + stays
-        full = [whole(x) for x in target[r]]
-        weight = full
-        if refused is not None:
-            weight = ([0 if v == refused else w for v, w in enumerate(full)] if draft is None else
-                      [max(0, w - whole(x)) for w, x in zip(full, draft[r])])
-        if not sum(weight):
+        full = whole(target[r])
+        weight = full.copy()
+        if refused is not None and draft is None:
+            weight[refused] = 0
+        elif refused is not None:
+            weight = np.maximum(0, full - whole(draft[r]))
+        if not weight.any():
             weight = full
+        upto = np.cumsum(weight)  # below 2^63
         k = min(int(Fraction(share(uniform[begin + n - 1])) * 2 ** 31), 2 ** 31 - 1)
-        k = k * sum(weight) >> 31
-        token, total = -1, 0
-        for v, w in enumerate(weight):
-            total += w
-            if total > k:
-                token = v
-                break
+        k = k * int(upto[-1]) >> 31
+        token = int(np.argmax(upto > k)) if upto[-1] else -1
         out[begin:begin + stays] = tokens[begin + 1:begin + 1 + stays]
         out[r] = token
         gained[s] = stays + 1

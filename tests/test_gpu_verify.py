@@ -55,7 +55,8 @@ def check(p, q, tokens, u, first, lens=True, padded=0):
 @pytest.mark.parametrize("vocab,seqs,rows", [(1, 3, 3), (2, 9, 2), (5, 40, 6), (257, 6, 9),
                                              (2048, 2, 3), (8192, 2, 2), (8193, 2, 3),
                                              (20011, 3, 4), (32000, 1, 5), (32768, 1, 2),
-                                             (32769, 2, 2), (65536, 1, 2), (65541, 2, 2)])
+                                             (32769, 2, 2), (65536, 1, 2), (65541, 2, 2),
+                                             (40_001, 80, 3)])
 def test_verify(dtype, sure, vocab, seqs, rows):
     rng = np.random.default_rng(vocab + seqs)
     counts = rng.integers(0, rows + 1, seqs)
@@ -78,7 +79,7 @@ def test_every_place_can_be_drawn():
     for vocab in (4, 1000, 1024, 4095, 12288, 33001, 100_003):
         at = np.unique(np.concatenate([np.arange(min(vocab, 40)), vocab - 1 - np.arange(min(vocab, 40)),
                                        np.linspace(0, vocab - 1, 60).astype(int)]))
-        w = pr.whole(np.float32(1.0 / vocab))
+        w = int(pr.whole(np.float32(1.0 / vocab)))
         u = ((at + 0.5) / vocab).astype(np.float32)
         want = [(int(float(x) * 2 ** 31) * w * vocab >> 31) // w for x in u]
         p = torch.full((len(at), vocab), 1.0 / vocab, device="cuda")
