@@ -227,7 +227,7 @@ def grow_both(cache, was, table, lens, first=None, tokens=None, extra=0):
 
 @pytest.mark.parametrize("kv,dim,t", [(2, 64, 16), (1, 100, 128), (3, 128, 32)])
 @pytest.mark.parametrize("seqs,width,new", [(1, 3, 1), (9, 6, 1), (70, 5, 9), (40, 12, 200),
-                                            (1500, 3, 1), (2, 90, 3000 // 2), (600, 4, 40)])
+                                            (1500, 3, 1), (2, 90, 1500), (600, 4, 40)])
 @pytest.mark.parametrize("spare", [0.02, 0.4, 3.0])
 def test_grow(kv, dim, t, seqs, width, new, spare):
     """One token and chunks of tokens each, rows that share prefixes, pools
