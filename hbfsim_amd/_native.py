@@ -294,6 +294,8 @@ SIGNATURES = {
     "hbfsim_amd_verify_workspace": (_INT, [_U32, _U32, _U32, ctypes.POINTER(_SZ)]),
     "hbfsim_amd_verify": (_INT, [_P, _P, _U32, _U32, _I64, _I64, _P, _P, _P, _U32, _U32, _P, _P, _P,
                                  _P, _P, _SZ, _P]),
+    "hbfsim_amd_verify_step": (_INT, [_P, _P, _U32, _U32, _I64, _I64, _P, _P, _P, _U32, _U32, _P, _P,
+                                      _P, _P, _P, _P, _SZ, _P]),
 }
 
 _lib = None

@@ -1,4 +1,4 @@
-"""Drafted tokens: which of a step's stay (hbfsim_amd_verify,
+"""Drafted tokens: which of a step's stay (hbfsim_amd_verify_step,
 include/hbfsim_amd.h section 9).
 
 A step of drafts over a paged cache appends and attends to several tokens of
@@ -6,11 +6,14 @@ each sequence at once, the last known one and those that a draft proposes;
 `verify` says from the target's probabilities which of them stay and which
 token follows, and the cache's `release` gives back the blocks of the others.
 
-    step, missing = cache.grow(table, lens, first, tokens)
+    step, missing = cache.grow(table, lens + rows, first, tokens)  # rows of each sequence
     cache.append(k, v, table, step, first)
     out = cache.attend(q, table, step, first)
-    new, gained, lens = verify(target, tokens, uniform, first, draft=draft, lens=step)
+    new, gained, lens = verify(target, tokens, uniform, first, draft=draft, lens=step, stored=lens)
     cache.release(table, lens)
+
+A sequence that lacks blocks has length 0 in `step`; by `stored` it keeps the
+length that it had, and so its row, and can go on in a later step.
 
 No counterpart in the reference.
 """
@@ -35,7 +38,7 @@ def _probabilities(x: Any, name: str) -> Any:
 
 
 def verify(target: Any, tokens: Any, uniform: Any, first: Any = None, draft: Any = None,
-           lens: Any = None, stream: Any = None) -> tuple:
+           lens: Any = None, stream: Any = None, stored: Any = None) -> tuple:
     """Which of a step's drafted tokens stay, and the token behind them.
 
     Sequence s has rows first[s] .. first[s + 1] - 1 of the batch (`first`
@@ -50,11 +53,15 @@ def verify(target: Any, tokens: Any, uniform: Any, first: Any = None, draft: Any
 
     Returns (out, gained, lens): int32 [rows] with each sequence's tokens from
     its first row on, -1 beyond; how many they are; and, from `lens` (tokens
-    stored with all of the step's), those that remain, None without it."""
+    stored with all of the step's), those that remain, None without it.  A
+    sequence whose `lens` is below its rows was left out of the step: it gains
+    nothing and remains as `lens` says, or as `stored` does (int32 [seqs], the
+    lengths before the step), which a step that `grow` has given lengths needs
+    before blocks are released by them."""
     gpu = _gpu(target)
     if _elsewhere(gpu, stream):
         return _there(target.device, stream, lambda: verify(target, tokens, uniform, first, draft,
-                                                            lens))
+                                                            lens, stored=stored))
     device = target.device
     rows, vocab = _probabilities(target, "target").shape
     if draft is not None and (_probabilities(draft, "draft").shape != target.shape
@@ -73,6 +80,11 @@ def verify(target: Any, tokens: Any, uniform: Any, first: Any = None, draft: Any
             raise ValueError("first must hold one offset more than there are sequences")
     if lens is not None and _flat(lens, "lens", target) != seqs:
         raise ValueError(f"{lens.shape[0]} lengths for {seqs} sequences")
+    if stored is not None:
+        if lens is None:
+            raise ValueError("stored lengths without the step's")
+        if _flat(stored, "stored", target) != seqs:
+            raise ValueError(f"{stored.shape[0]} stored lengths for {seqs} sequences")
     _counts(rows | seqs | vocab)
     _on_gpu(gpu)
     kind = _TYPES[target.dtype]
@@ -88,11 +100,12 @@ def verify(target: Any, tokens: Any, uniform: Any, first: Any = None, draft: Any
     ws, out, gained, left = torch.empty((need // 4 + rows + 2 * seqs,), dtype=torch.int32,
                                         device=device).split_with_sizes(
         (need // 4, rows, seqs, seqs))
-    _refuse(nat.load().hbfsim_amd_verify(
+    _refuse(nat.load().hbfsim_amd_verify_step(
         target.data_ptr(), draft.data_ptr() if draft is not None else None, kind, vocab,
         target.stride(0), draft.stride(0) if draft is not None else 0, tokens.data_ptr(),
         uniform.data_ptr(), first.data_ptr() if first is not None else None, seqs, rows,
-        lens.data_ptr() if lens is not None else None, out.data_ptr(), gained.data_ptr(),
+        lens.data_ptr() if lens is not None else None,
+        stored.data_ptr() if stored is not None else None, out.data_ptr(), gained.data_ptr(),
         left.data_ptr() if lens is not None else None, ws.data_ptr() if need else None, need,
         _handle(gpu)), "verify")
     return out, gained, left if lens is not None else None

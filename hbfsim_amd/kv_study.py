@@ -203,8 +203,10 @@ def run_drafts(seqs: int = 8, tokens: int = 8192, steps: int = 24, branches: int
                 "ms_after": packed["ms"]}
             rows = table.shape[0]
         first = torch.arange(rows + 1, dtype=torch.int32, device=dev) * m
-        want, n = rows * m, lens.cpu().numpy()
+        want = rows * m
         step_lens, missing = cache.grow(table, lens + m, first, want)
+        # a sequence that lacks blocks reads nothing
+        n = torch.where(missing == 0, lens, 0).cpu().numpy()
         result["missing"] += int((missing != 0).sum())
         k, v = (normal(want, kv_heads, head_dim).bfloat16() for _ in range(2))
         cache.append(k, v, table, step_lens, first)
@@ -215,9 +217,10 @@ def run_drafts(seqs: int = 8, tokens: int = 8192, steps: int = 24, branches: int
         said = torch.zeros(want, dtype=torch.int32, device=dev)
         said[1:] = (draft / torch.empty_like(draft).exponential_(generator=gen)).argmax(1)[:-1]
         u = torch.rand((want,), generator=gen, device=dev)
-        _, count, lens = drafted.verify(target, said, u, first, draft=draft, lens=step_lens)
+        _, count, lens = drafted.verify(target, said, u, first, draft=draft, lens=step_lens,
+                                        stored=lens)
         cache.release(table, lens)
-        left, ids = lens.cpu().numpy(), table.cpu().numpy()
+        left, ids = torch.where(missing == 0, lens, 0).cpu().numpy(), table.cpu().numpy()
         done = [ids[s, n[s] // t:left[s] // t] for s in range(rows)]  # filled by this step
         parts[now].append(flash_step(engine, cache, reads(n, ids), np.concatenate(done)))
         gained[now].append(float(count.float().mean()))

@@ -1049,7 +1049,13 @@ int hbfsim_amd_kv_compact(const hbfsim_amd_kv_cache* cache, int32_t* d_refs, int
  * how many they are (0 for a sequence of no rows or with rows past `tokens`).
  * With d_lens, the tokens stored for each sequence with all of its rows,
  * d_out_lens (which may be d_lens) is what remains of them: less by the rows
- * whose tokens did not stay.  d_out overlaps no input.  vocab is at most 2^22. */
+ * whose tokens did not stay.  A sequence whose length is below its rows was
+ * left out of the step, as section 8's grow leaves one out that lacks blocks:
+ * it gains nothing, its rows of d_out are -1, and its length stays d_lens[s],
+ * or becomes d_stored[s], what it held before the step (for grow's length of 0
+ * the one with which release keeps its row), where verify_step is given
+ * d_stored [seqs] (NULL as without; not without d_lens; d_out_lens may be
+ * d_stored).  d_out overlaps no input.  vocab is at most 2^22. */
 int hbfsim_amd_verify_workspace(uint32_t seqs, uint32_t vocab, uint32_t type, size_t* bytes);
 int hbfsim_amd_verify(const void* d_target, const void* d_draft, uint32_t type, uint32_t vocab,
                       int64_t target_stride, int64_t draft_stride, const int32_t* d_tokens,
@@ -1057,6 +1063,13 @@ int hbfsim_amd_verify(const void* d_target, const void* d_draft, uint32_t type, 
                       uint32_t tokens, const int32_t* d_lens, int32_t* d_out, int32_t* d_gained,
                       int32_t* d_out_lens, void* d_workspace, size_t workspace_bytes,
                       void* stream);
+int hbfsim_amd_verify_step(const void* d_target, const void* d_draft, uint32_t type,
+                           uint32_t vocab, int64_t target_stride, int64_t draft_stride,
+                           const int32_t* d_tokens, const float* d_uniform, const int32_t* d_first,
+                           uint32_t seqs, uint32_t tokens, const int32_t* d_lens,
+                           const int32_t* d_stored, int32_t* d_out, int32_t* d_gained,
+                           int32_t* d_out_lens, void* d_workspace, size_t workspace_bytes,
+                           void* stream);
 
 #ifdef __cplusplus
 }
