@@ -21,8 +21,9 @@ Who holds a block may be left to the cache as well (section 8 of the header):
 of no reference is free.  Sequences that branch share their blocks.
 
     table = torch.full((seqs, width), -1, dtype=torch.int32, device="cuda")
-    step, missing = cache.grow(table, lens)       # blocks for the step's tokens
+    step, missing = cache.grow(table, lens + 1)   # blocks for a token of each sequence
     cache.append(k, v, table, step)
+    lens = torch.where(missing == 0, step, lens)  # one that lacks blocks is left out of `step`
     table, lens = cache.fork(table, lens, parents)  # the next batch: branches, beams
     cache.release(table, lens)                    # blocks past the lengths
     where = cache.compact(table)                  # blocks in use to the pool's front

@@ -185,3 +185,46 @@ def test_a_study_whose_pool_runs_short(monkeypatch):
                               kv_heads=2, head_dim=64, seed=1)
     assert got["missing"] > 0
     assert got["compaction"]["named_by_rows"] - got["compaction"]["blocks"] == 32
+
+
+@pytest.mark.parametrize("blocks", [40, 9])
+def test_branches_continue_what_the_step_appended(blocks):
+    """Decode, branch, decode again, with room for all and without: the tokens
+    of the step before the branch are attended to after it."""
+    gen = torch.Generator(device="cuda").manual_seed(blocks)
+    kv, heads, dim, seqs, width = 2, 4, 64, 3, 4
+    cache, alone = kvcache.KvCache(blocks, kv, dim), kvcache.KvCache(2 * seqs * width, kv, dim)
+    own = torch.arange(2 * seqs * width, dtype=torch.int32, device="cuda").view(2 * seqs, width)
+    table = torch.full((seqs, width), -1, dtype=torch.int32, device="cuda")
+
+    def normal(*shape):
+        return torch.randn(shape, generator=gen, device="cuda").bfloat16()
+
+    first = dev([0, 16, 31, 63])
+    lens, missing = cache.grow(table, dev([16, 15, 32]), first, 63)
+    assert not missing.any()
+    k, v = normal(63, kv, dim), normal(63, kv, dim)
+    cache.append(k, v, table, lens, first)
+    alone.append(k, v, own[:seqs], lens, first)
+    short = 0
+    for step in range(9):
+        now, missing = cache.grow(table, lens + 1)
+        short += int((missing != 0).sum())
+        n = len(table)
+        k, v, q = normal(n, kv, dim), normal(n, kv, dim), normal(n, heads, dim)
+        cache.append(k, v, table, now)
+        alone.append(k, v, own[:n], now)
+        assert torch.equal(cache.attend(q, table, now), alone.attend(q, own[:n], now))
+        before, lens = lens, torch.where(missing == 0, now, lens)
+        assert torch.equal(lens, before + (missing == 0))
+        # all of it is there to be attended to
+        assert torch.equal(cache.attend(q, table, lens), alone.attend(q, own[:n], lens))
+        if step in (1, 4):
+            parents = dev([2, 0, 1, 0, 2, 0][:6 if step == 1 else 4])
+            held = lens
+            table, lens = cache.fork(table, lens, parents)
+            assert torch.equal(lens, held[parents.long()])
+            extra = kvcache.KvCache(2 * seqs * width, kv, dim)
+            alone.copy(own[parents.long()].reshape(-1), own[:len(parents)].reshape(-1), to=extra)
+            alone = extra
+    assert int(lens.max()) > 32 and (short == 0) == (blocks == 40)
