@@ -25,7 +25,9 @@ of no reference is free.  Sequences that branch share their blocks.
     cache.append(k, v, table, step)
     lens = torch.where(missing == 0, step, lens)  # one that lacks blocks is left out of `step`
     table, lens = cache.fork(table, lens, parents)  # the next batch: branches, beams
-    cache.release(table, lens)                    # blocks past the lengths
+    cache.release(table, lens)                    # blocks past the lengths: also before an evict
+    table, lens, freed, count = cache.evict(table, lens, keep=512)
+    cache.release(freed)                          # and its freed ones after
     where = cache.compact(table)                  # blocks in use to the pool's front
     cache.copy(src, dst, to=other)                # to another pool, or within it
 
@@ -159,7 +161,9 @@ def evict(weight: Any, table: Any, lens: Any, keep: int, block_tokens: int = 16,
     `keep_first`, its last `keep_last` and the others of the largest weight
     summed over kv heads.  Returns (table, lens, freed, freed_count), new
     tensors: kept blocks in order, the tokens left, and the blocks that left,
-    -1 beyond.  ValueError for what the library refuses."""
+    -1 beyond.  Entries past a sequence's length are in neither: where
+    references are counted, `release` them before.  ValueError for what the
+    library refuses."""
     device = weight.device
     gpu = _gpu(weight)
     if _elsewhere(gpu, stream):

@@ -949,7 +949,10 @@ int hbfsim_amd_kv_evict(const int64_t* d_weight, uint32_t blocks, uint32_t kv_he
  * d_refs int32 [blocks] counts the table entries that name each block, and a
  * block of no reference (0 or below) is free.  Sequences that continue the
  * same tokens share blocks; every entry in [0, blocks) of a live row is one
- * reference, whether its sequence's length reaches it or not.  As above, work
+ * reference, whether its sequence's length reaches it or not.  (Section 7's
+ * evict hands back the blocks below the lengths alone: a table whose entries
+ * are counted is released to its lengths before, d_freed as a table after.)
+ * As above, work
  * is queued on `stream` and nothing is allocated or copied to the host; calls
  * on one d_refs follow one another.  Counts change by whole numbers, so
  * results do not depend on an order of atomics.  Tables are

@@ -228,3 +228,25 @@ def test_branches_continue_what_the_step_appended(blocks):
             alone.copy(own[parents.long()].reshape(-1), own[:len(parents)].reshape(-1), to=extra)
             alone = extra
     assert int(lens.max()) > 32 and (short == 0) == (blocks == 40)
+
+
+def test_an_eviction_leaves_no_reference_behind():
+    """Rows that name blocks past their lengths (grown for drafts that did not
+    stay), some of them shared: released to the lengths, evicted, and what is
+    freed released, they hold what they name and no block more."""
+    rng = np.random.default_rng(9)
+    blocks, seqs, width = 300, 8, 30
+    cache = kvcache.KvCache(blocks, 2, 64)
+    cache.weight.random_(0, 1 << 40)
+    rows = rng.permutation(blocks)[:seqs * width].reshape(seqs, width).astype(np.int32)
+    rows[1, :12] = rows[0, :12]
+    table, lens = dev(rows), dev([480, 470, 465, 16, 0, 300, 177, 176])
+    cache.hold(table)
+    cache.release(table, lens)
+    table, lens, freed, gone = cache.evict(table, lens, keep=11)
+    assert int(gone.sum()) > 0
+    cache.release(freed)
+    np.testing.assert_array_equal(cache.refs.cpu(), pr.count(table.cpu().numpy(), blocks))
+    assert (table >= 0).sum(1).tolist() == [11, 11, 11, 1, 0, 11, 11, 11]
+    cache.release(table)
+    assert not cache.refs.any()
