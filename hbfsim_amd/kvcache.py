@@ -588,7 +588,8 @@ class KvCache:
     def compact(self, table: Any, stream: Any = None) -> Any:
         """Blocks in use move to the front of the pool, and the table's entries
         with them.  Returns where each block went (int32 [blocks], -1 for a
-        free one), by which other tables of this cache can follow."""
+        free one), by which other tables of this cache can follow: their
+        entries in the pool, as -1 would pick the last block's place."""
         if _elsewhere(self._gpu, stream):
             return _there(self.device, stream, lambda: self.compact(table))
         refs = _references(self.refs, self)

@@ -250,3 +250,26 @@ def test_an_eviction_leaves_no_reference_behind():
     assert (table >= 0).sum(1).tolist() == [11, 11, 11, 1, 0, 11, 11, 11]
     cache.release(table)
     assert not cache.refs.any()
+
+
+def test_other_tables_follow_a_compaction():
+    """As the guide has it: entries that name no block stay -1, also where the
+    pool's last block is in use."""
+    rng = np.random.default_rng(10)
+    blocks = 90
+    ids = rng.permutation(blocks - 1)[:36].astype(np.int32)
+    ids[0] = blocks - 1
+    one, two = np.full((3, 9), -1, np.int32), np.full((2, 11), -1, np.int32)
+    one[:, :6], two[:, :9] = ids[:18].reshape(3, 6), ids[18:].reshape(2, 9)
+    refs = pr.count(one, blocks)
+    pr.hold(refs, two)
+    cache = kvcache.KvCache(blocks, 1, 64)
+    cache.refs.copy_(dev(refs))
+    cache.weight.copy_(torch.arange(blocks, device="cuda")[:, None])
+    table, other = dev(one), dev(two)
+    where = cache.compact(table)
+    other = torch.where(other >= 0, where[other.clamp(min=0).long()], -1)
+    for got, was in ((table, one), (other, two)):
+        assert torch.equal(got >= 0, dev(was) >= 0) and int(got.max()) < 36
+        named = torch.where(got >= 0, cache.weight[got.clamp(min=0).long(), 0], -1)
+        np.testing.assert_array_equal(named.cpu(), was)
