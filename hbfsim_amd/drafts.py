@@ -25,7 +25,8 @@ from typing import Any
 import torch
 
 from . import _native as nat
-from .kvcache import _TYPES, _counts, _elsewhere, _flat, _gpu, _handle, _on_gpu, _refuse, _there
+from .kvcache import (_TYPES, _counts, _elsewhere, _flat, _gpu, _handle, _on_gpu, _refuse, _there,
+                      _workspace)
 
 _need: dict = {}  # workspace bytes by a call's sizes
 
@@ -96,10 +97,13 @@ def verify(target: Any, tokens: Any, uniform: Any, first: Any = None, draft: Any
         if len(_need) >= 4096:
             _need.clear()
         need = _need[seqs, vocab, kind] = got.value
-    # outputs and scratch are parts of one allocation, scratch first (it is aligned)
-    ws, out, gained, left = torch.empty((need // 4 + rows + 2 * seqs,), dtype=torch.int32,
-                                        device=device).split_with_sizes(
-        (need // 4, rows, seqs, seqs))
+    # Outputs and scratch are parts of one allocation, scratch first (it is
+    # aligned), if the scratch is small: whoever keeps an output keeps all of it.
+    held = need // 4 if need <= 65536 else 0
+    ws, out, gained, left = torch.empty((held + rows + 2 * seqs,), dtype=torch.int32,
+                                        device=device).split_with_sizes((held, rows, seqs, seqs))
+    if need > 4 * held:
+        ws = _workspace(need, device)
     _refuse(nat.load().hbfsim_amd_verify_step(
         target.data_ptr(), draft.data_ptr() if draft is not None else None, kind, vocab,
         target.stride(0), draft.stride(0) if draft is not None else 0, tokens.data_ptr(),

@@ -273,3 +273,19 @@ def test_other_tables_follow_a_compaction():
         assert torch.equal(got >= 0, dev(was) >= 0) and int(got.max()) < 36
         named = torch.where(got >= 0, cache.weight[got.clamp(min=0).long(), 0], -1)
         np.testing.assert_array_equal(named.cpu(), was)
+
+
+@pytest.mark.parametrize("vocab,seqs", [(151_936, 64), (40_000, 3), (500, 64)])
+def test_what_verify_returns_keeps_no_scratch_alive(vocab, seqs):
+    """A program that collects each step's tokens holds those and 64 KiB at
+    most beside them."""
+    p = torch.full((seqs, vocab), 1.0 / vocab, device="cuda")
+    lens = dev(np.arange(seqs) + 1)
+    got = drafts.verify(p, dev(np.zeros(seqs)), torch.full((seqs,), 0.5, device="cuda"), lens=lens)
+    assert all(x.untyped_storage().nbytes() <= 65536 + 4 * 3 * seqs for x in got)
+    torch.cuda.synchronize()
+    del p
+    before = torch.cuda.memory_allocated()
+    del got
+    torch.cuda.synchronize()
+    assert before - torch.cuda.memory_allocated() <= 65536 + 4 * 3 * seqs + 512
