@@ -650,10 +650,19 @@ HBF_API int hbfsim_amd_verify_step(const void* d_target, const void* d_draft, ui
         (d_target == nullptr || d_uniform == nullptr || (d_first != nullptr && d_tokens == nullptr))) {
         return HBFSIM_INVALID_ARGUMENT;
     }
-    if (meet(d_out, out, d_tokens, out) || meet(d_out, out, d_uniform, out) ||
-        meet(d_out, out, d_first, d_first != nullptr ? (static_cast<std::size_t>(seqs) + 1) * 4 : 0) ||
-        meet(d_out, out, d_lens, static_cast<std::size_t>(seqs) * 4) ||
-        meet(d_out, out, d_stored, static_cast<std::size_t>(seqs) * 4)) {
+    const std::size_t each_seq = static_cast<std::size_t>(seqs) * 4;
+    const auto meets_input = [&](const std::int32_t* p, std::size_t n) {
+        return meet(p, n, d_tokens, out) || meet(p, n, d_uniform, out) || meet(p, n, d_first, each_seq + 4);
+    };
+    const auto meets_lengths = [&](const std::int32_t* p, std::size_t n) {
+        return meet(p, n, d_lens, each_seq) || meet(p, n, d_stored, each_seq);
+    };
+    // the lengths that remain may be written over either of the given ones, place for place
+    const auto over = [&](const std::int32_t* q) { return d_out_lens != q && meet(d_out_lens, each_seq, q, each_seq); };
+    if (meets_input(d_out, out) || meets_lengths(d_out, out) || meets_input(d_gained, each_seq) ||
+        meets_lengths(d_gained, each_seq) || meets_input(d_out_lens, each_seq) || over(d_lens) || over(d_stored) ||
+        meet(d_out, out, d_gained, each_seq) || meet(d_out, out, d_out_lens, each_seq) ||
+        meet(d_gained, each_seq, d_out_lens, each_seq)) {
         return HBFSIM_INVALID_ARGUMENT;
     }
     Verify a{};

@@ -1008,7 +1008,8 @@ int hbfsim_amd_kv_release(int32_t* d_refs, uint32_t blocks, uint32_t block_token
  * the table, gets none and keeps its row.  d_missing[s] is then the number of
  * blocks that it needs, and d_out_lens[s], otherwise d_lens[s], is 0, with
  * which the step neither stores nor attends for it.  d_out_lens may be
- * d_lens. */
+ * d_lens itself; beyond that neither it nor d_missing overlaps another array
+ * of the call. */
 int hbfsim_amd_kv_grow_workspace(const hbfsim_amd_kv_cache* cache, uint32_t seqs, uint32_t tokens,
                                  size_t* bytes);
 int hbfsim_amd_kv_grow(const hbfsim_amd_kv_cache* cache, int32_t* d_refs, int32_t* d_table,
@@ -1021,7 +1022,8 @@ int hbfsim_amd_kv_grow(const hbfsim_amd_kv_cache* cache, int32_t* d_refs, int32_
  * j-th (by id) at or past L moves to the j-th free one below L.  d_where
  * [blocks] receives each block's new id, -1 for a free one; entries of the
  * table (width or seqs may be 0) become the new ids, -1 where they name no
- * block in use.  d_refs moves too. */
+ * block in use.  d_refs moves too.  d_where overlaps no other array of the
+ * call. */
 int hbfsim_amd_kv_compact_workspace(const hbfsim_amd_kv_cache* cache, size_t* bytes);
 int hbfsim_amd_kv_compact(const hbfsim_amd_kv_cache* cache, int32_t* d_refs, int32_t* d_table,
                           uint32_t seqs, uint32_t width, uint32_t stride, int32_t* d_where,
@@ -1058,7 +1060,9 @@ int hbfsim_amd_kv_compact(const hbfsim_amd_kv_cache* cache, int32_t* d_refs, int
  * or becomes d_stored[s], what it held before the step (for grow's length of 0
  * the one with which release keeps its row), where verify_step is given
  * d_stored [seqs] (NULL as without; not without d_lens; d_out_lens may be
- * d_stored).  d_out overlaps no input.  vocab is at most 2^22. */
+ * d_stored).  Beyond that the outputs overlap neither an input nor one another
+ * (HBFSIM_INVALID_ARGUMENT where they overlap the tokens, the numbers, the
+ * offsets, the lengths or one another).  vocab is at most 2^22. */
 int hbfsim_amd_verify_workspace(uint32_t seqs, uint32_t vocab, uint32_t type, size_t* bytes);
 int hbfsim_amd_verify(const void* d_target, const void* d_draft, uint32_t type, uint32_t vocab,
                       int64_t target_stride, int64_t draft_stride, const int32_t* d_tokens,
