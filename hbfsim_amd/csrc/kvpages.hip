@@ -30,6 +30,8 @@ struct Piece {
 // Past the caches, as a block that moves is rarely read again soon: 8,003
 // blocks of 35 KB (560 MB in and out) take 112 us, 5.0 TB/s, with non-temporal
 // loads and stores, and a call 118, 121 with such stores alone, 124 with neither.
+// (Measured on copies of a pool.  grow's few copies are read again in the same
+// step and go the same way.)
 constexpr int kUnits = 4;  // of a thread
 __device__ inline void copy_part(const Cache& from, const Cache& to, const Piece& p, std::int32_t src, std::int32_t dst,
                                  std::uint32_t part)
@@ -110,7 +112,9 @@ __global__ __launch_bounds__(kThreads) void k_kv_copy(Copy a)
 }
 // Every workgroup looks through the pairs itself: one launch instead of three.
 // 4 pairs take 3.1 us against 6.2, 256 of 35 KB 5.3 against 8.8, 1,024 18.0
-// against 20.7; 4,096 take 75 against 64.
+// against 20.7, 2,048 33.3 against 35.0; 4,096 take 75 against 64.  Every part of
+// a block repeats the look, three of them here, 33 where a block has 0.5 MB, which
+// is not measured: the border stays on the low side.
 __global__ __launch_bounds__(kThreads) void k_kv_copy_few(Copy a)
 {
     const std::uint32_t i = blockIdx.x / a.p.parts, part = blockIdx.x % a.p.parts;
@@ -147,8 +151,11 @@ __device__ inline void each_entry(const Table& a, std::uint32_t chunk, F f)
 }
 
 // Tables are walked by workgroups of 1,024 entries.  Bound by the launch, and for
-// large tables by the atomics: 256 rows of 193,000 entries, of which 65,000
-// leave, take 6.8 us, 64 rows of which few do 3.5.
+// large tables by the atomics: hold takes 2.7 us for 8 rows of 512 entries, 6.5 for
+// 64 of 2,048 and 20.7 for 256 of them where every entry names another block, and
+// 131 for 64 of 2,048 that name 100 blocks (1,300 atomics on one address);
+// release 6.7 for 256 rows of 193,000 entries, of which 65,000 leave, and 3.1 for 64
+// rows of which few do.
 __global__ __launch_bounds__(kThreads) void k_kv_hold(Table a)
 {
     const std::uint32_t s = blockIdx.x / a.chunks;
@@ -184,7 +191,7 @@ struct Fork {
 // The first rows * chunks workgroups write the new rows, the others change the
 // old rows' counts: by their children less one, which each finds among the
 // parents, or by one down where the new rows count one up themselves.  64 rows
-// of up to 2,048 entries continued by 256 take 6.4 us, 8 rows 3.3.
+// of up to 2,048 entries continued by 256 take 6.5 us, 8 rows 3.0.
 __global__ __launch_bounds__(kThreads) void k_kv_fork(Fork a)
 {
     const std::uint32_t r = blockIdx.x / a.t.chunks, chunk = blockIdx.x % a.t.chunks;
@@ -433,9 +440,9 @@ __device__ inline std::int32_t first_free(const Grow& a, std::uint32_t tile, std
 // many blocks are wanted, the first free ones, who gets them.  A slot is a block
 // that a sequence may write to, as in append.  Every step needs the one before
 // of all slots, so it is a chain of trips to memory and barriers, no work to
-// spread: 11.2 us for 17 chunks of 35,769 tokens (1,151 slots), 25 for 4,000
-// sequences of one token.  (Steps side by side in several workgroups would need
-// a launch between each two.)
+// spread: 11.4 us for 17 chunks of 35,769 tokens (1,151 slots), 25 for 4,000
+// sequences of one token.  Slots go through global memory between the barriers;
+// a few a thread would fit the LDS as well, as one does below.
 __global__ __launch_bounds__(kPlan) void k_kv_grow(Grow a)
 {
     constexpr std::uint32_t kHeld = 4096;  // sequences whose parts lie in LDS
@@ -672,7 +679,7 @@ __global__ __launch_bounds__(kPlan) void k_kv_grow_few(Grow a)
 }
 
 // The planned copies, at most kCopiers workgroups for all sequences' parts, as
-// most steps have few; 3.3 us for 64 sequences of which a third part with a
+// most steps have few; 3.2 us for 64 sequences of which a third part with a
 // block, 2.0 where none does.  For 4,000 sequences and blocks of 34 parts a
 // workgroup each cost 4 us more of such a step, and where all are copied (0.53
 // GB of blocks of 128 tokens for 1,000) 93 us against 98.
@@ -965,9 +972,11 @@ std::uint64_t slots_of(const Cache& c, std::uint32_t seqs, std::uint32_t tokens,
 {
     return offsets ? tokens / c.tokens + std::uint64_t{2} * seqs : seqs;
 }
-// Blocks up to which the planning workgroup looks for free ones without counts:
-// 60,000 cost it up to 6 us more than the first tile, by where the free ones
-// lie, and counts 3.5.
+// Blocks up to which the planning workgroup looks for free ones without counts,
+// which cost 3.5 us: a step of 64 sequences in a pool of 60,000 takes 6 us where
+// the first tile has their blocks, 12 where only the last ones do, as in a pool
+// that hands out the lowest and is nearly full, and with counts 9.5 wherever they
+// lie.  (From about 28,000 blocks on counts are the shorter way to the last ones.)
 constexpr std::uint32_t kScanned = 65536;
 // Where a thread takes a slot, the plan lies in LDS and only the pairs in memory.
 GrowSpace grow_space(const Cache& c, std::uint32_t seqs, std::uint64_t slots)

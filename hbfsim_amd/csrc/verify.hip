@@ -8,9 +8,11 @@
 // does not, the next token is drawn from max(p - q, 0), so that what a sequence
 // gains is distributed as the target alone would have it; behind the last draft
 // it is drawn from p.  Probabilities become whole numbers P = 2^40 p (f32 holds
-// 24 bits, so a p above 2^-17 keeps all of them; the rounding below that, at
-// most 2^-41 of the whole, is the price of sums that do not depend on their
-// order) and are summed in 64 bits: vocabularies up to 2^22 fit.
+// 24 bits, so a p above 2^-17 keeps all of them; below that a weight is off by
+// at most 2^-41, one of p - q by 2^-40, and the sum by as much times the
+// vocabulary: the price of sums that do not depend on their order) and are
+// summed in 64 bits: vocabularies up to 2^22 fit.  What draws is a float: one of
+// 24 bits tells 2^-24 of the sum apart.
 //
 // Bound by memory where rows are long: one row of p a sequence, and one of q
 // where a draft was refused, are read; of the other rows one element each.
@@ -399,10 +401,12 @@ __device__ inline void give_nothing(const Verify& a, std::uint32_t s)
 // One wave sums kSteps consecutive KiB of a row, a region each, and finds how
 // far the drafts stay by itself first: the same few loads for all of a
 // sequence's waves, cheaper than a launch or a barrier.  Sums of whole numbers
-// need no order, so nothing is shared between waves.  64 sequences over 151,936
-// tokens in f32 (69 MB, as some keep all drafts and need no q) take 14.0 us, 4.9
-// TB/s; a single one over 32,000 3.5, the trips to its offsets, its tokens, their
-// probabilities and the row.
+// need no order, so nothing is shared between waves.  64 sequences of 4 drafts over
+// 151,936 tokens in f32 (69 MB, as some keep all drafts and need no q) take 14.4
+// us, 4.8 TB/s, on rows that the last-level cache holds, 17.1 on others, and 29.3
+// just after 256 MB of writes, which then leave it; in bf16 11.2, 13.0 and 17.3, of half
+// the waves behind the same trips; a single one over 32,000 3.5, the trips to its
+// offsets, its tokens, their probabilities and the row.
 template <typename T, int kSteps>
 __global__ __launch_bounds__(kThreads) void k_verify_sum(Verify a)
 {
@@ -435,7 +439,7 @@ __global__ __launch_bounds__(kThreads) void k_verify_sum(Verify a)
 
 // One wave per sequence: the region whose running sum passes the drawn number,
 // and the element in it.  The last wave clears the rows of no sequence.  4.3 us
-// for those 64, 3.4 for the one: trips to the sums and to the region, and scans.
+// for those 64, 3.5 for the one: trips to the sums and to the region, and scans.
 template <typename T>
 __global__ __launch_bounds__(kWave) void k_verify_find(Verify a)
 {
@@ -550,8 +554,8 @@ __global__ __launch_bounds__(1024) void k_verify_one(Verify a)
 
 constexpr std::uint32_t kMostVocab = 1u << 22;
 
-// How a call is cut: from its sizes alone (floats, by graph replays; two-byte
-// types take within 2 us of the same).
+// How a call is cut: from its sizes alone (by graph replays, floats unless it
+// says bf16).
 // A workgroup per sequence where 16 waves of two loads each hold the row: 1 and
 // 256 sequences over 4,000 tokens take 5.1 and 6.3 us against 6.8 and 8.2 in two
 // launches, over 8,000 7.3 and 8.0 against 6.8 and 8.7, and one launch less costs
@@ -561,6 +565,11 @@ constexpr std::uint32_t kMostVocab = 1u << 22;
 // sequences over 16,000 take 8.1 us with one load and 8.4 with four (1,000
 // waves), over 32,000 9.4 and 8.9, over 60,000 13.0 and 10.4, over 151,936 22.1
 // and 17.6-18.5.
+// In bf16 a workgroup each takes 7.5 us for 64 over 4,000 against 8.4 in two
+// launches, 8.0 and 8.4 over 8,000, but 9.8 and 8.6 over 16,000 (1 over 16,000:
+// 8.1 and 7.4), where the host's call is still the shorter, 12 us and 14.5; a
+// load a wave and four: 64 over 32,000 8.9 and 9.7, over 60,000 10.8 and 10.3, over
+// 151,936 17.1 and 15.4.
 struct Cut {
     bool one;   // a workgroup per sequence
     int steps;  // regions of a wave
