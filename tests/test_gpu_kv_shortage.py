@@ -104,6 +104,35 @@ def test_lengths_in_place(vocab, dtype, sure, one_each, over):
             np.testing.assert_array_equal(a.cpu(), b)
 
 
+@pytest.mark.parametrize("vocab,dtype,sure,one_each", CASES[2:6])
+def test_left_out_on_another_stream_and_in_a_graph(vocab, dtype, sure, one_each):
+    """One captured call serves steps that leave out other sequences each time."""
+    p, q, tokens, u, first, lens, stored = case(vocab, dtype, sure, one_each)
+    rng = np.random.default_rng(1)
+    host = (p.float().numpy(), tokens, u, first, None if q is None else q.float().numpy())
+    at, before = dev(lens), dev(stored)
+    args = (p.cuda(), dev(tokens), dev(u, np.float32), None if first is None else dev(first),
+            None if q is None else q.cuda(), at)
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        drafts.verify(*args, stored=before)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = drafts.verify(*args, stored=before)
+    for _ in range(5):
+        n, m = np.where(rng.random(len(lens)) < 0.5, 0, lens), rng.integers(0, 99, len(lens))
+        at.copy_(dev(n)), before.copy_(dev(m))
+        torch.cuda.synchronize()
+        graph.replay()
+        eager = drafts.verify(*args, stored=before, stream=stream)
+        torch.cuda.synchronize()
+        for got in (captured, eager):
+            for a, b in zip(got, verify(*host, n, m)):
+                np.testing.assert_array_equal(a.cpu(), b)
+
+
 def test_a_pool_that_runs_short():
     """Drafted steps of six sequences that share a prompt over a pool that
     cannot hold them all, beside a cache in which each has blocks of its own:
